@@ -9,6 +9,7 @@
 #include <mutex>
 
 #include "../../include/qmatmul.h"
+#include "qm_fp8.h"
 #include "qm_gguf.h"
 #include "qm_launch.h"
 
@@ -17,6 +18,12 @@ struct qm_weight {
   uint8_t* base;
   size_t bytes;
   qm::WView view;
+};
+
+struct qm_fp8_weight {
+  int rows, K, device;
+  uint8_t* base;
+  qm::Fp8View view;
 };
 
 namespace {
@@ -745,6 +752,263 @@ int qmatmul_moe_grouped(const qm_weight* gate, const qm_weight* up, const qm_wei
 struct qm_gguf {
   std::unique_ptr<qm::Gguf> g;
 };
+
+// ---- 8-bit floating point products
+
+static bool dtype_ok(int t) { return t == QM_F32 || t == QM_F16 || t == QM_BF16; }
+static size_t dtype_size(int t) { return t == QM_F32 ? 4 : 2; }
+static int padded_128(int K) { return (K + 127) / 128 * 128; }
+
+static size_t fp8_payload_bytes(int rows, int K) { return (size_t)((rows + 63) / 64) * 64 * ((size_t)(K + 127) / 128 * 128); }
+static size_t fp8_scale_count(int rows, int K) { return (size_t)((rows + 127) / 128) * ((K + 127) / 128); }
+// (rows and K rounded up stay ints)
+static bool fp8_shape_ok(int rows, int K) { return rows >= 1 && K >= 1 && rows <= 0x7fffff00 && K <= 0x7fffff00; }
+
+size_t qmatmul_fp8_weight_bytes(int rows, int K) {
+  if (!fp8_shape_ok(rows, K)) return 0;
+  return align256(fp8_payload_bytes(rows, K)) + fp8_scale_count(rows, K) * sizeof(float);
+}
+
+int qmatmul_prepare_fp8(const void* w8, const float* wsc, int on_device, int rows, int K, void* stream,
+                        qm_fp8_weight** out) {
+  if (!out || !w8 || !wsc) return fail(QM_ERR_ARG, "qmatmul_prepare_fp8: null pointer");
+  *out = nullptr;
+  if (!fp8_shape_ok(rows, K)) return fail(QM_ERR_SHAPE, "qmatmul_prepare_fp8: rows %d, K %d", rows, K);
+  if (!aligned(wsc, 4)) return fail(QM_ERR_ARG, "qmatmul_prepare_fp8: the scales must be 4-byte aligned");
+  QM_CHECK_INIT();
+  hipStream_t s = (hipStream_t)stream;
+  const size_t raw = (size_t)rows * K, scb = fp8_scale_count(rows, K) * sizeof(float);
+  const size_t at = align256(fp8_payload_bytes(rows, K)), total = at + scb;
+  qm_fp8_weight* w = new (std::nothrow) qm_fp8_weight();
+  if (!w) return fail(QM_ERR_NOMEM, "qmatmul_prepare_fp8: host allocation");
+  hipError_t e = hipGetDevice(&w->device);
+  if (e != hipSuccess) {
+    delete w;
+    return hip_fail(e, "qmatmul_prepare_fp8: hipGetDevice");
+  }
+  e = device_alloc((void**)&w->base, total);
+  if (e != hipSuccess) {
+    delete w;
+    return fail(QM_ERR_NOMEM, "qmatmul_prepare_fp8: hipMalloc(%zu): %s", total, hipGetErrorString(e));
+  }
+  const uint8_t* src = (const uint8_t*)w8;
+  uint8_t* staged = nullptr;
+  if (!on_device) {
+    e = device_alloc((void**)&staged, raw);
+    if (e == hipSuccess) e = hipMemcpyAsync(staged, w8, raw, hipMemcpyHostToDevice, s);
+    src = staged;
+  }
+  if (e == hipSuccess)
+    e = hipMemcpyAsync(w->base + at, wsc, scb, on_device ? hipMemcpyDeviceToDevice : hipMemcpyHostToDevice, s);
+  if (e == hipSuccess) e = qm::launch_fp8_repack(src, rows, K, w->base, s);
+  if (!on_device) {
+    // (whatever was queued has ended before the host's bytes and the staged copy go)
+    const hipError_t e2 = hipStreamSynchronize(s);
+    if (e == hipSuccess) e = e2;
+    if (staged) (void)hipFree(staged);
+  }
+  if (e != hipSuccess) {
+    (void)hipFree(w->base);
+    delete w;
+    return hip_fail(e, "qmatmul_prepare_fp8");
+  }
+  w->rows = rows;
+  w->K = K;
+  w->view.q = w->base;
+  w->view.sc = (const float*)(w->base + at);
+  w->view.rows = rows;
+  w->view.kb = padded_128(K) / 128;
+  *out = w;
+  return QM_OK;
+}
+
+int qmatmul_release_fp8(qm_fp8_weight* w) {
+  if (!w) return fail(QM_ERR_ARG, "qmatmul_release_fp8: null weight");
+  const hipError_t e = hipFree(w->base);
+  delete w;
+  return e == hipSuccess ? QM_OK : hip_fail(e, "qmatmul_release_fp8: hipFree");
+}
+
+int qmatmul_fp8_info(const qm_fp8_weight* w, int* rows, int* K, int* Kp) {
+  if (!w) return fail(QM_ERR_ARG, "qmatmul_fp8_info: null weight");
+  if (rows) *rows = w->rows;
+  if (K) *K = w->K;
+  if (Kp) *Kp = 128 * w->view.kb;
+  return QM_OK;
+}
+
+// what the three producers share: input rows of `width` elements, outputs of K values
+static int check_fp8_rows(const char* fn, const void* x, int xtype, int ldx, long long width, int M, int M_stride, int K,
+                          const uint8_t* a8, const float* asc) {
+  if (!x || !a8 || !asc) return fail(QM_ERR_ARG, "%s: null pointer", fn);
+  if (!dtype_ok(xtype)) return fail(QM_ERR_TYPE, "%s: input type %d (QM_F32, QM_F16 or QM_BF16)", fn, xtype);
+  if (K < 1 || K > 0x3fffff00 || M < 0 || M_stride < 1 || M > M_stride || ldx < width)
+    return fail(QM_ERR_SHAPE, "%s: M %d, M_stride %d, K %d, row stride %d", fn, M, M_stride, K, ldx);
+  if (!aligned(x, dtype_size(xtype)) || !aligned(a8, 16) || !aligned(asc, 4))
+    return fail(QM_ERR_ARG, "%s: the input must be aligned to its type, a8 to 16 bytes, asc to 4", fn);
+  return QM_OK;
+}
+
+int qmatmul_quantize_fp8(const void* x, int xtype, int ldx, int M, int M_stride, int K, uint8_t* a8, float* asc,
+                         void* stream) {
+  if (int st = check_fp8_rows("qmatmul_quantize_fp8", x, xtype, ldx, K, M, M_stride, K, a8, asc)) return st;
+  QM_CHECK_INIT();
+  const hipError_t e = qm::launch_quantize_fp8(x, xtype, ldx, M, M_stride, K, a8, asc, (hipStream_t)stream);
+  return e == hipSuccess ? QM_OK : hip_fail(e, "qmatmul_quantize_fp8");
+}
+
+int qmatmul_rmsnorm_fp8(const void* x, int xtype, int ldx, const float* w, int K, int M, int M_stride, float eps,
+                        uint8_t* a8, float* asc, float* h, int ldh, void* stream) {
+  if (int st = check_fp8_rows("qmatmul_rmsnorm_fp8", x, xtype, ldx, K, M, M_stride, K, a8, asc)) return st;
+  if (!w) return fail(QM_ERR_ARG, "qmatmul_rmsnorm_fp8: null weight");
+  if (!aligned(w, 4) || (h && !aligned(h, 4))) return fail(QM_ERR_ARG, "qmatmul_rmsnorm_fp8: w and h must be 4-byte aligned");
+  if (h && ldh < K) return fail(QM_ERR_SHAPE, "qmatmul_rmsnorm_fp8: ldh %d < K %d", ldh, K);
+  QM_CHECK_INIT();
+  const hipError_t e = qm::launch_rmsnorm_fp8(x, xtype, ldx, w, K, M, M_stride, eps, a8, asc, h, ldh, (hipStream_t)stream);
+  return e == hipSuccess ? QM_OK : hip_fail(e, "qmatmul_rmsnorm_fp8");
+}
+
+int qmatmul_swiglu_fp8(const void* gu, int xtype, int ldg, int F, int M, int M_stride, int gelu, uint8_t* a8, float* asc,
+                       void* stream) {
+  if (int st = check_fp8_rows("qmatmul_swiglu_fp8", gu, xtype, ldg, 2LL * F, M, M_stride, F, a8, asc)) return st;
+  QM_CHECK_INIT();
+  const hipError_t e = qm::launch_swiglu_fp8(gu, xtype, ldg, F, M, M_stride, gelu ? 1 : 0, a8, asc, (hipStream_t)stream);
+  return e == hipSuccess ? QM_OK : hip_fail(e, "qmatmul_swiglu_fp8");
+}
+
+size_t qmatmul_gemm_fp8_workspace_size(const qm_fp8_weight* w, int M) {
+  return w && M >= 1 ? qm::fp8_workspace_bytes(M, w->rows, w->view.kb) : 0;
+}
+
+int qmatmul_gemm_fp8(const qm_fp8_weight* w, const uint8_t* a8, const float* asc, int M, int M_stride, void* C, int ctype,
+                     int ldc, int c_off, int accumulate, void* ws, size_t ws_bytes, void* stream) {
+  const char* fn = "qmatmul_gemm_fp8";
+  if (!w) return fail(QM_ERR_ARG, "%s: null weight", fn);
+  if (!dtype_ok(ctype)) return fail(QM_ERR_TYPE, "%s: output type %d (QM_F32, QM_F16 or QM_BF16)", fn, ctype);
+  if (accumulate < 0 || accumulate > 2) return fail(QM_ERR_ARG, "%s: accumulate %d (0..2)", fn, accumulate);
+  if (M < 0 || M_stride < M || c_off < 0 || ldc < (long long)c_off + w->rows)
+    return fail(QM_ERR_SHAPE, "%s: M %d, M_stride %d, ldc %d, c_off %d, rows %d", fn, M, M_stride, ldc, c_off, w->rows);
+  if (M == 0) return QM_OK;
+  if (!a8 || !asc || !C) return fail(QM_ERR_ARG, "%s: null pointer", fn);
+  if (!aligned(a8, 16) || !aligned(asc, 4) || !aligned(C, dtype_size(ctype)))
+    return fail(QM_ERR_ARG, "%s: a8 must be 16-byte aligned, asc and C to their types", fn);
+  if (ws && !aligned(ws, 256)) return fail(QM_ERR_ARG, "%s: the workspace must be 256-byte aligned", fn);
+  QM_CHECK_INIT();
+  int dev = -1;
+  const hipError_t ed = hipGetDevice(&dev);
+  if (ed != hipSuccess) return hip_fail(ed, fn);
+  if (dev != w->device) return fail(QM_ERR_ARG, "%s: the weight is on device %d, the current device is %d", fn, w->device, dev);
+  qm::Fp8GemmArgs a{};
+  a.w = w->view;
+  a.a8 = a8;
+  a.asc = asc;
+  a.M = M;
+  a.M_stride = M_stride;
+  a.C = C;
+  a.ctype = ctype;
+  a.ldc = ldc;
+  a.c_off = c_off;
+  a.accumulate = accumulate;
+  const size_t need = qm::fp8_workspace_bytes(M, w->rows, w->view.kb);
+  a.part = need && ws && ws_bytes >= need ? (float*)ws : nullptr;
+  const hipError_t e = qm::launch_gemm_fp8(a, (hipStream_t)stream);
+  return e == hipSuccess ? QM_OK : hip_fail(e, fn);
+}
+
+// ---- query and key heads
+
+// Rows in memory: T of them, each `heads` runs of D elements `hs` apart, rows `ld` apart (elements of `size` bytes)
+struct HeadRows {
+  const void* p;
+  long long T, D, heads, hs, ld, size;
+  uintptr_t first() const { return (uintptr_t)p; }
+  uintptr_t width() const { return (uintptr_t)(((heads - 1) * hs + D) * size); }
+  uintptr_t last() const { return first() + (uintptr_t)((T - 1) * ld * size) + width(); }
+};
+
+// Whether two such sets share a byte, or may: rows of one stride are compared within it (the heads' runs taken whole)
+static bool rows_overlap(const HeadRows& a, const HeadRows& b) {
+  if (!a.heads || !b.heads || !a.T) return false;
+  if (a.last() <= b.first() || b.last() <= a.first()) return false;
+  const uintptr_t ld = (uintptr_t)(a.ld * a.size);
+  if (ld != (uintptr_t)(b.ld * b.size)) return true;
+  const uintptr_t d = b.first() >= a.first() ? (b.first() - a.first()) % ld : (ld - (a.first() - b.first()) % ld) % ld;
+  return d < a.width() || d + b.width() > ld;
+}
+
+int qmatmul_qk_norm_rope(const void* x, int xtype, int ldx, int T, int D, int q_off, int q_hs, int HQ, int k_off, int k_hs,
+                         int HK, const float* wq, const float* wk, float eps, const qm_rope* rope, const int32_t* pos,
+                         int pos_stride, const float* inv_freq, void* q, void* k, int otype, int ldq, int ldk,
+                         void* stream) {
+  const char* fn = "qmatmul_qk_norm_rope";
+  if (!rope) return fail(QM_ERR_ARG, "%s: null rotation", fn);
+  if (!dtype_ok(xtype) || !dtype_ok(otype))
+    return fail(QM_ERR_TYPE, "%s: types %d -> %d (QM_F32, QM_F16 or QM_BF16)", fn, xtype, otype);
+  if (T < 0 || D < 2 || D > 512 || D % 2 || HQ < 0 || HK < 0 || HQ > 65536 || HK > 65536)
+    return fail(QM_ERR_SHAPE, "%s: T %d, D %d (even, 2..512), HQ %d, HK %d", fn, T, D, HQ, HK);
+  if (rope->rot < 0 || rope->rot > D || rope->rot % 2 || rope->axes < 1 || rope->axes > 4)
+    return fail(QM_ERR_SHAPE, "%s: rot %d (even, 0..D %d), axes %d (1..4)", fn, rope->rot, D, rope->axes);
+  if (rope->axes > 1) {
+    long long sum = 0;
+    for (int i = 0; i < rope->axes; ++i) {
+      if (rope->sections[i] < 0) return fail(QM_ERR_SHAPE, "%s: sections[%d] = %d", fn, i, rope->sections[i]);
+      sum += rope->sections[i];
+    }
+    if (sum != rope->rot / 2) return fail(QM_ERR_SHAPE, "%s: sections sum to %lld, rot / 2 is %d", fn, sum, rope->rot / 2);
+  }
+  const long long qw = (long long)(HQ - 1) * q_hs + D, kw = (long long)(HK - 1) * k_hs + D;
+  if ((HQ && (q_off < 0 || q_hs < (HQ > 1 ? D : 0) || q_off + qw > ldx || ldq < (long long)HQ * D)) ||
+      (HK && (k_off < 0 || k_hs < (HK > 1 ? D : 0) || k_off + kw > ldx || ldk < (long long)HK * D)))
+    return fail(QM_ERR_SHAPE, "%s: D %d; q: offset %d, %d heads of stride %d, ldq %d; k: offset %d, %d heads of stride %d, "
+                "ldk %d; ldx %d", fn, D, q_off, HQ, q_hs, ldq, k_off, HK, k_hs, ldk, ldx);
+  if (rope->axes > 1 && pos_stride < T) return fail(QM_ERR_SHAPE, "%s: pos_stride %d < T %d", fn, pos_stride, T);
+  if (T == 0 || HQ + HK == 0) return QM_OK;
+  if (!x || (HQ && !q) || (HK && !k) || (rope->rot && (!pos || !inv_freq))) return fail(QM_ERR_ARG, "%s: null pointer", fn);
+  const size_t si = dtype_size(xtype), so = dtype_size(otype);
+  if (!aligned(x, si) || (HQ && !aligned(q, so)) || (HK && !aligned(k, so)) || !aligned(pos, 4) || !aligned(inv_freq, 4) ||
+      !aligned(wq, 4) || !aligned(wk, 4))
+    return fail(QM_ERR_ARG, "%s: every pointer must be aligned to its type", fn);
+  const HeadRows xq{(const char*)x + (size_t)q_off * si, T, D, HQ, q_hs, ldx, (long long)si};
+  const HeadRows xk{(const char*)x + (size_t)k_off * si, T, D, HK, k_hs, ldx, (long long)si};
+  const HeadRows oq{q, T, D, HQ, D, ldq, (long long)so}, ok{k, T, D, HK, D, ldk, (long long)so};
+  const bool q_in = HQ && q == xq.p && si == so && xtype == otype && ldq == ldx && (q_hs == D || HQ == 1);
+  const bool k_in = HK && k == xk.p && si == so && xtype == otype && ldk == ldx && (k_hs == D || HK == 1);
+  if (rows_overlap(oq, ok) || (!q_in && rows_overlap(oq, xq)) || rows_overlap(oq, xk) || (!k_in && rows_overlap(ok, xk)) ||
+      rows_overlap(ok, xq))
+    return fail(QM_ERR_ARG, "%s: an output overlaps the input or the other output", fn);
+  QM_CHECK_INIT();
+  qm::RopeArgs a{};
+  a.x = x;
+  a.xtype = xtype;
+  a.ldx = ldx;
+  a.T = T;
+  a.D = D;
+  a.q_off = HQ ? q_off : 0;
+  a.q_hs = q_hs;
+  a.HQ = HQ;
+  a.k_off = HK ? k_off : 0;
+  a.k_hs = k_hs;
+  a.HK = HK;
+  a.wq = wq;
+  a.wk = wk;
+  a.eps = eps;
+  a.rot = rope->rot;
+  a.adjacent = rope->adjacent ? 1 : 0;
+  a.axes = rope->axes;
+  a.turns = rope->turns ? 1 : 0;
+  for (int i = 0; i < 4; ++i) a.sections[i] = rope->sections[i];
+  a.scale = rope->scale;
+  a.pos = pos;
+  a.pos_stride = pos_stride;
+  a.inv_freq = inv_freq;
+  a.q = q;
+  a.k = k;
+  a.otype = otype;
+  a.ldq = ldq;
+  a.ldk = ldk;
+  const hipError_t e = qm::launch_qk_norm_rope(a, (hipStream_t)stream);
+  return e == hipSuccess ? QM_OK : hip_fail(e, fn);
+}
 
 int qmatmul_gguf_open(const char* path, qm_gguf** out) {
   if (!path || !out) return fail(QM_ERR_ARG, "qmatmul_gguf_open: null pointer");

@@ -47,6 +47,17 @@ SIGNATURES = [
     ("qmatmul_rmsnorm_quant_ex", _I, [_P, _I, _P, _I, _I, _I, _c.c_float, _I, _P, _P, _P, _P, _I, _P]),
     ("qmatmul_swiglu_quant_ex", _I, [_P, _I, _I, _I, _I, _I, _I, _I, _P, _P, _P, _P]),
     ("qmatmul_add_norm_quant_ex", _I, [_P, _P, _P, _I, _c.c_float, _c.c_float, _P, _I, _I, _I, _P, _P, _P, _P]),
+    ("qmatmul_fp8_weight_bytes", _Z, [_I, _I]),
+    ("qmatmul_prepare_fp8", _I, [_P, _P, _I, _I, _I, _P, _c.POINTER(_P)]),
+    ("qmatmul_release_fp8", _I, [_P]),
+    ("qmatmul_fp8_info", _I, [_P, _c.POINTER(_I), _c.POINTER(_I), _c.POINTER(_I)]),
+    ("qmatmul_quantize_fp8", _I, [_P, _I, _I, _I, _I, _I, _P, _P, _P]),
+    ("qmatmul_rmsnorm_fp8", _I, [_P, _I, _I, _P, _I, _I, _I, _c.c_float, _P, _P, _P, _I, _P]),
+    ("qmatmul_swiglu_fp8", _I, [_P, _I, _I, _I, _I, _I, _I, _P, _P, _P]),
+    ("qmatmul_gemm_fp8_workspace_size", _Z, [_P, _I]),
+    ("qmatmul_gemm_fp8", _I, [_P, _P, _P, _I, _I, _P, _I, _I, _I, _I, _P, _Z, _P]),
+    ("qmatmul_qk_norm_rope", _I, [_P, _I, _I, _I, _I, _I, _I, _I, _I, _I, _I, _P, _P, _c.c_float, _P, _P, _I, _P, _P, _P,
+                                  _I, _I, _I, _P]),
     ("qmatmul_gguf_open", _I, [_c.c_char_p, _c.POINTER(_P)]),
     ("qmatmul_gguf_close", _I, [_P]),
     ("qmatmul_gguf_tensor_count", _I, [_P, _c.POINTER(_I)]),
@@ -315,6 +326,214 @@ def add_norm_quant(x, t, w, eps, s, w2=None, M_stride=None, stream=None, act32=T
     _call("qmatmul_add_norm_quant_ex", _ptr(x), _ptr(t), _ptr(w), K, float(eps), float(s), _ptr(w2), M, Ms,
           int(act32), _ptr(aq), _ptr(asc), _ptr(absum), _stream(stream))
     return aq, asc, absum
+
+
+# ---- 8-bit floating point products, query and key heads --------------------------------------------------------------
+_DTYPES = {}  # torch dtype -> qm_dtype (filled on first use: torch is imported late)
+
+
+def _dtype(t):
+    if not _DTYPES:
+        import torch
+        _DTYPES.update({torch.float32: 0, torch.float16: 1, torch.bfloat16: 30})
+    try:
+        return _DTYPES[t]
+    except KeyError:
+        raise QMatmulError("dtype", 3, f"{t}: float32, float16 or bfloat16 rows") from None
+
+
+def _check(fn, ok, what):
+    if not ok:
+        raise QMatmulError(fn, 1, what)
+
+
+def _check_rows(fn, dim, **tensors):
+    """Every tensor (None passes) is on the current GPU, of `dim` dimensions where dim is given, its last one contiguous."""
+    import torch
+    dev = torch.cuda.current_device()
+    for name, t in tensors.items():
+        if t is None:
+            continue
+        _check(fn, t.is_cuda and t.device.index == dev, f"{name} is not on the current GPU")
+        _check(fn, dim is None or t.dim() == dim, f"{name} has {t.dim()} dimensions, not {dim}")
+        _check(fn, t.numel() == 0 or t.shape[-1] == 1 or t.stride(-1) == 1, f"the last dimension of {name} is not contiguous")
+
+
+def _row_stride(t):
+    """The row stride of a matrix in elements (of a single row, whose stride says nothing: its length)."""
+    return t.stride(0) if t.shape[0] > 1 else max(t.shape[1], t.stride(0))
+
+
+class Fp8Weight:
+    """A prepared e4m3 weight (qm_fp8_weight*): w8 torch.float8_e4m3fn (or its bytes as uint8) [rows, K], scales float32
+    [ceil(rows / 128), ceil(K / 128)], both on the current GPU or both on the CPU. Kp: the activations' row length."""
+
+    def __init__(self, w8, scales, stream=None):
+        import torch
+        fn = "qmatmul_prepare_fp8"
+        self.handle = None
+        _check(fn, w8.dtype in (torch.float8_e4m3fn, torch.uint8), f"w8 is {w8.dtype}: float8_e4m3fn (or its bytes)")
+        _check(fn, w8.dim() == 2 and w8.is_contiguous(), "w8 must be a contiguous matrix")
+        self.rows, self.K = w8.shape
+        self.Kp = (self.K + 127) // 128 * 128
+        _check(fn, scales.dtype == torch.float32 and scales.is_contiguous()
+               and tuple(scales.shape) == ((self.rows + 127) // 128, self.Kp // 128),
+               f"scales {tuple(scales.shape)} {scales.dtype}: contiguous float32, one for each 128 x 128 block")
+        _check(fn, w8.device == scales.device, "w8 and scales are on different devices")
+        if w8.is_cuda:
+            _check_rows(fn, 2, w8=w8)
+        h = ctypes.c_void_p()
+        _call(fn, _ptr(w8), _ptr(scales), 1 if w8.is_cuda else 0, self.rows, self.K, _stream(stream), ctypes.byref(h))
+        self.handle = h
+
+    @property
+    def nbytes(self):
+        return load_library().qmatmul_fp8_weight_bytes(self.rows, self.K)
+
+    def release(self):
+        if self.handle:
+            h, self.handle = self.handle, None
+            _call("qmatmul_release_fp8", h)
+
+    def __del__(self):
+        try:
+            if self.handle and _lib is not None:
+                _lib.qmatmul_release_fp8(self.handle)
+                self.handle = None
+        except Exception:
+            pass
+
+
+def _out_fp8(fn, x, K, M_stride):
+    import torch
+    M = x.shape[0]
+    Ms = M if M_stride is None else M_stride
+    Kp = (K + 127) // 128 * 128
+    return (Ms, torch.empty((Ms, Kp), dtype=torch.float8_e4m3fn, device=x.device),
+            torch.empty((Kp // 128, Ms), dtype=torch.float32, device=x.device))
+
+
+def quantize_fp8(x, M_stride=None, stream=None):
+    """x [M, K] (float32, float16 or bfloat16, rows of any stride) -> (a8 float8_e4m3fn [M_stride, Kp], asc float32
+    [Kp / 128, M_stride]), Kp = K rounded up to 128."""
+    fn = "qmatmul_quantize_fp8"
+    _check_rows(fn, 2, x=x)
+    Ms, a8, asc = _out_fp8(fn, x, x.shape[1], M_stride)
+    _call(fn, x.data_ptr(), _dtype(x.dtype), _row_stride(x), x.shape[0], Ms, x.shape[1], a8.data_ptr(), asc.data_ptr(),
+          _stream(stream))
+    return a8, asc
+
+
+def rmsnorm_fp8(x, w, eps, M_stride=None, want_h=False, stream=None):
+    """x [M, K], w float32 [K] -> (a8, asc, h float32 [M, K] or None)."""
+    import torch
+    fn = "qmatmul_rmsnorm_fp8"
+    _check_rows(fn, 2, x=x)
+    _check_rows(fn, 1, w=w)
+    M, K = x.shape
+    _check(fn, w.dtype == torch.float32 and w.numel() == K, "w: float32, one for each column")
+    Ms, a8, asc = _out_fp8(fn, x, K, M_stride)
+    h = torch.empty((M, K), dtype=torch.float32, device=x.device) if want_h else None
+    _call(fn, x.data_ptr(), _dtype(x.dtype), _row_stride(x), w.data_ptr(), K, M, Ms, eps, a8.data_ptr(), asc.data_ptr(),
+          h.data_ptr() if want_h and M else None, K, _stream(stream))
+    return a8, asc, h
+
+
+def swiglu_fp8(gu, F, gelu=False, M_stride=None, stream=None):
+    """gu [M, 2 F] (gate then up) -> (a8, asc) of silu(gate) * up, or gelu_tanh(gate) * up."""
+    fn = "qmatmul_swiglu_fp8"
+    _check_rows(fn, 2, gu=gu)
+    _check(fn, gu.shape[1] >= 2 * F, f"rows of {gu.shape[1]} elements hold no gate and up of {F}")
+    Ms, a8, asc = _out_fp8(fn, gu, F, M_stride)
+    _call(fn, gu.data_ptr(), _dtype(gu.dtype), _row_stride(gu), F, gu.shape[0], Ms, 1 if gelu else 0, a8.data_ptr(),
+          asc.data_ptr(), _stream(stream))
+    return a8, asc
+
+
+def gemm_fp8_workspace(w, M):
+    """A workspace for products of M tokens with w (None where they need none)."""
+    import torch
+    n = load_library().qmatmul_gemm_fp8_workspace_size(w.handle, M)
+    return torch.empty((n,), dtype=torch.uint8, device="cuda") if n else None
+
+
+def gemm_fp8(w, a8, asc, M=None, C=None, ldc=None, c_off=0, accumulate=0, out=None, ws=None, stream=None):
+    """C [M, rows] (op)= the product of activations (a8, asc) with an Fp8Weight. out: the type of a new C (float32 unless
+    given). C: a matrix of that stride unless ldc is given."""
+    import torch
+    fn = "qmatmul_gemm_fp8"
+    _check_rows(fn, 2, a8=a8, asc=asc, C=C)
+    Ms, Kp = a8.shape
+    M = Ms if M is None else M
+    _check(fn, w.handle is not None, "the weight was released")
+    _check(fn, a8.is_contiguous() and a8.element_size() == 1 and Kp == w.Kp, f"a8 {tuple(a8.shape)}: contiguous e4m3 rows of {w.Kp}")
+    _check(fn, asc.is_contiguous() and asc.dtype == torch.float32 and tuple(asc.shape) == (Kp // 128, Ms),
+           f"asc {tuple(asc.shape)}: contiguous float32 [{Kp // 128}, {Ms}]")
+    if C is None:
+        _check(fn, accumulate == 0 and c_off == 0 and ldc is None, "accumulate, c_off and ldc need a C")
+        C = torch.empty((M, w.rows), dtype=torch.float32 if out is None else out, device=a8.device)
+        ld = w.rows
+    else:
+        _check(fn, out is None or out == C.dtype, "out is not C's type")
+        ld = _row_stride(C) if ldc is None else ldc
+        _check(fn, M == 0 or (M - 1) * ld + c_off + w.rows <= (C.shape[0] - 1) * C.stride(0) + C.shape[1], "C is too small")
+    _call(fn, w.handle, a8.data_ptr(), asc.data_ptr(), M, Ms, C.data_ptr(), _dtype(C.dtype), ld, c_off, accumulate,
+          None if ws is None else ws.data_ptr(), 0 if ws is None else ws.numel(), _stream(stream))
+    return C
+
+
+class QmRope(ctypes.Structure):
+    _fields_ = [("rot", _I), ("adjacent", _I), ("axes", _I), ("turns", _I), ("sections", _I * 4), ("scale", _c.c_float)]
+
+
+def qk_norm_rope(x, HQ, HK, D, pos, inv_freq, wq=None, wk=None, eps=1e-6, adjacent=False, sections=None, turns=False,
+                 scale=1.0, q_off=0, q_hs=None, k_off=None, k_hs=None, q=None, k=None, out=None, stream=None):
+    """RMS norm (wq, wk float32 [D]; None: no norm) and rotation of the query and key heads in rows x [T, ldx]: query head h at
+    column q_off + h * q_hs (D unless given), key head h at k_off + h * k_hs (k_off: behind the query heads unless given).
+    pos int32 [T], or [axes, T] with sections (pairs of each axis, behind one another or in turns); inv_freq float32
+    [rot / 2]: its length says how many elements of a head turn. Returns (q [T, HQ, D], k [T, HK, D]) of type out (x's
+    unless given), or writes the q and k given (matrices [T, HQ * D] or [T, HQ, D] of any row stride; views of x for in place)."""
+    import torch
+    fn = "qmatmul_qk_norm_rope"
+    _check_rows(fn, 2, x=x)
+    _check_rows(fn, 1, inv_freq=inv_freq, wq=wq, wk=wk)
+    T = x.shape[0]
+    p = pos if pos.dim() == 2 else pos[None]
+    _check_rows(fn, 2, pos=p)
+    _check(fn, pos.dtype == torch.int32 and p.shape[1] == T, f"pos {tuple(pos.shape)} {pos.dtype}: int32, one column for each of {T} tokens")
+    _check(fn, inv_freq.dtype == torch.float32, "inv_freq: float32")
+    for w in (wq, wk):
+        _check(fn, w is None or (w.dtype == torch.float32 and w.numel() == D), "wq and wk: float32 [D]")
+    axes, half = p.shape[0], inv_freq.numel()
+    sec = [half] if sections is None else [int(n) for n in sections]
+    _check(fn, len(sec) == axes and axes <= 4 and sum(sec) == half, f"sections {sec}: one for each of {axes} axes, their sum {half}")
+    q_hs = D if q_hs is None else q_hs
+    k_hs = D if k_hs is None else k_hs
+    k_off = q_off + HQ * q_hs if k_off is None else k_off
+    ldx = _row_stride(x)
+    _check(fn, T == 0 or x.shape[1] >= max(q_off + (HQ - 1) * q_hs + D if HQ else 0, k_off + (HK - 1) * k_hs + D if HK else 0),
+           f"rows of {x.shape[1]} elements do not hold the heads")
+    otype = out if out is not None else q.dtype if q is not None else k.dtype if k is not None else x.dtype
+    res, ptrs, lds = [], [], []
+    for t, H in ((q, HQ), (k, HK)):
+        if t is None:
+            t = torch.empty((T, H, D), dtype=otype, device=x.device)
+            ld = H * D
+        else:
+            _check_rows(fn, None, output=t)
+            _check(fn, t.dtype == otype and t.dim() in (2, 3) and t.shape[0] == T
+                   and (t.shape[1] == H * D if t.dim() == 2 else tuple(t.shape[1:]) == (H, D) and (H < 2 or t.stride(1) == D)),
+                   f"output {tuple(t.shape)} {t.dtype}: [T, {H} * {D}] of {otype}")
+            ld = t.stride(0) if T > 1 else max(H * D, t.stride(0))
+        res.append(t)
+        ptrs.append(t.data_ptr() if t.numel() else None)
+        lds.append(ld)
+    rope = QmRope(2 * half, 1 if adjacent else 0, axes, 1 if turns else 0, (_I * 4)(*sec), scale)
+    _call(fn, x.data_ptr(), _dtype(x.dtype), ldx, T, D, q_off, q_hs, HQ, k_off, k_hs, HK,
+          None if wq is None else wq.data_ptr(), None if wk is None else wk.data_ptr(), eps, ctypes.byref(rope),
+          p.data_ptr(), p.stride(0) if axes > 1 else T, inv_freq.data_ptr(), ptrs[0], ptrs[1], _dtype(otype), lds[0], lds[1],
+          _stream(stream))
+    return res[0], res[1]
 
 
 class GgufTensor:

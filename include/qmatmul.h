@@ -248,6 +248,92 @@ int qmatmul_gemv_blocksums(const qm_weight* w, const int8_t* aq, const int16_t* 
                            int32_t* isum, int32_t* msum, void* stream);
 int qmatmul_gemm_blocksums(const qm_weight* w, const int8_t* aq, int M, int M_stride, int32_t* isum, void* stream);
 
+/* ---- 8-bit floating point products -------------------------------------------------------------------------------
+ * For checkpoints held in e4m3 (OCP: 1 sign, 4 exponent, 3 mantissa bits, largest value 448, 0x7F / 0xFF are NaN) with an
+ * f32 scale for each 128 x 128 block of the weight. No counterpart in the reference (whose weights are GGUF blocks);
+ * the entry points follow the GGUF products' manner.
+ *
+ * Activations: a8 e4m3 [M_stride][Kp] row-major, one row per token, Kp = K rounded up to 128 (the padding zeros); asc
+ * float [Kp/128][M_stride], the scale of each 128 values, token fastest; rows M..M_stride-1 of a padded batch zero. */
+
+/* Element types of rows that are not quantized (GGML ids) */
+typedef enum { QM_F32 = 0, QM_F16 = 1, QM_BF16 = 30 } qm_dtype;
+
+typedef struct qm_fp8_weight qm_fp8_weight; /* opaque: a prepared e4m3 weight matrix */
+
+/* Device bytes a prepared weight takes: rows rounded up to 64 times K rounded up to 128, and the block scales. */
+size_t qmatmul_fp8_weight_bytes(int rows, int K);
+
+/* Prepares a weight: w8 e4m3 [rows][K] row-major and wsc float [ceil(rows/128)][ceil(K/128)], the scale each block is
+ * multiplied by (the last blocks of a row or column may be cut: any rows >= 1, K >= 1). Both are device pointers if
+ * on_device, else host pointers (the call then waits for the copy). The layout is this library's own; the sources may be
+ * freed once the stream has passed the call. The weight belongs to the current device. */
+int qmatmul_prepare_fp8(const void* w8, const float* wsc, int on_device, int rows, int K, void* stream,
+                        qm_fp8_weight** out);
+/* Frees a prepared weight (waits for the device). */
+int qmatmul_release_fp8(qm_fp8_weight* w);
+/* Rows and K of a prepared weight as given, and the activation rows' length Kp (any output pointer may be NULL). */
+int qmatmul_fp8_info(const qm_fp8_weight* w, int* rows, int* K, int* Kp);
+
+/* Producers of e4m3 activations (layout above) from rows of xtype (qm_dtype), row stride ldx in elements, any K >= 1:
+ * per 128 values y: amax = max |y|; asc = amax / 448; q = y * (448 / amax) rounded to the nearest e4m3, ties to even. A
+ * block whose amax is below 2^-100 is zeros with scale 0. A NaN becomes e4m3's NaN (amax is that of the others); a block with
+ * an infinity has the scale infinity: both make every product of their token NaN.
+ * qmatmul_quantize_fp8: y = x.   qmatmul_rmsnorm_fp8: y = x * w / sqrt(mean(x^2) + eps); h (optional, f32, row stride
+ * ldh, rows < M) receives y.   qmatmul_swiglu_fp8: y = silu(gate) * up (gelu_tanh(gate) * up with gelu) from rows
+ * [gate(F) | up(F)]. y is computed in f32. Rows that are 16-byte aligned (base and stride) and of a K % 8 == 0 are read 16 bytes
+ * at a time, others by the element. */
+int qmatmul_quantize_fp8(const void* x, int xtype, int ldx, int M, int M_stride, int K, uint8_t* a8, float* asc,
+                         void* stream);
+int qmatmul_rmsnorm_fp8(const void* x, int xtype, int ldx, const float* w, int K, int M, int M_stride, float eps,
+                        uint8_t* a8, float* asc, float* h, int ldh, void* stream);
+int qmatmul_swiglu_fp8(const void* gu, int xtype, int ldg, int F, int M, int M_stride, int gelu, uint8_t* a8, float* asc,
+                       void* stream);
+
+/* The product, from one token to long prompts (M = 0 does nothing):
+ *   C[m*ldc + c_off + n] (op)= sum over blocks b of asc[b][m] * wsc[n/128][b] * sum_{k in b} a8[m][k] * w8[n][k]
+ * C of ctype (qm_dtype); op by accumulate (0 store, 1 add, 2 C = silu(C) * result), computed in f32 and rounded once. With a
+ * C of f32 the products are exact and every sum is f32. With a C of 16 bits the products run on the fp8 matrix pipe, twice as
+ * fast, which drops from the sum of each eight neighbouring products what lies 2^-13 below the largest of them (1.3e-5 of the
+ * result for normal values, far below C's rounding); the sums of eights and of blocks are f32. a8 is 16-byte aligned.
+ * ws: device workspace, 256-byte aligned, of qmatmul_gemm_fp8_workspace_size(w, M) bytes (0 for many calls; NULL or too
+ * small: the call runs without, slower); calls that may overlap need different workspaces. No allocation, no host
+ * synchronisation; the call can be captured into a graph. The weight's device must be the current one. */
+size_t qmatmul_gemm_fp8_workspace_size(const qm_fp8_weight* w, int M);
+int qmatmul_gemm_fp8(const qm_fp8_weight* w, const uint8_t* a8, const float* asc, int M, int M_stride, void* C, int ctype,
+                     int ldc, int c_off, int accumulate, void* ws, size_t ws_bytes, void* stream);
+
+/* ---- Query and key heads ------------------------------------------------------------------------------------------
+ * The step after the QKV product: RMS norm of each query and key head and the rotation by the token's position, in one
+ * pass (attention itself is not part of this library).
+ *
+ * Rotation: the first rot elements of a head (rot even, <= D) are rot/2 pairs, the rest pass. Pair i is elements
+ * (i, i + rot/2), or (2i, 2i + 1) with adjacent, and turns by pos[axis(i)][t] * inv_freq[i]:
+ *   (u, v) -> scale * (u cos - v sin, v cos + u sin)
+ * One axis: plain text positions. Several (up to 4; time, height, width of images and video): axis a has sections[a] of
+ * the pairs (their sum is rot/2), either one axis' pairs behind the other's, or with turns in turns: axis(i) = i % axes
+ * where that is 0 or i < axes * sections[i % axes], else 0. The angle and its reduction to one turn are computed in f64, so
+ * positions may be any int32. */
+typedef struct {
+  int rot;         /* elements turned: even, 0..D */
+  int adjacent;    /* 0: pairs (i, i + rot/2); 1: pairs (2i, 2i + 1) */
+  int axes;        /* 1..4 */
+  int turns;       /* 0: sections one behind the other; 1: in turns */
+  int sections[4]; /* pairs of each axis (read when axes > 1) */
+  float scale;     /* of the cosines and sines (1, or a long-context scaling's factor) */
+} qm_rope;
+
+/* T tokens (0 does nothing): x of xtype, row stride ldx; query head h of token t is D elements (even, <= 512) at
+ * t*ldx + q_off + h*q_hs, key head h at t*ldx + k_off + h*k_hs (HQ, HK >= 0: none of a kind is allowed). wq, wk [D] (f32):
+ * y = x * w / sqrt(mean over D of x^2 + eps); NULL: no norm for that kind. pos int32 [axes][pos_stride], inv_freq f32
+ * [rot/2]. Results of otype: q at t*ldq + h*D, k at t*ldk + h*D. Computed in f32, rounded once. q (k) may be the input
+ * itself (same address, type and strides); any other overlap of an output with the input or the other output is refused.
+ * Rows, offsets and strides of 4 elements' alignment are read and written 4 elements at a time, others by the element. */
+int qmatmul_qk_norm_rope(const void* x, int xtype, int ldx, int T, int D, int q_off, int q_hs, int HQ, int k_off, int k_hs,
+                         int HK, const float* wq, const float* wk, float eps, const qm_rope* rope, const int32_t* pos,
+                         int pos_stride, const float* inv_freq, void* q, void* k, int otype, int ldq, int ldk,
+                         void* stream);
+
 /* GGUF files (host side). Maps a GGUF v2/v3 file read-only and indexes its metadata and tensors, so a weight can
  * go to qmatmul_prepare_weight straight from the mapping (raw_on_device = 0; rows = dims[1] * dims[2] * ..., K =
  * dims[0]). Replaces the reference's GgufFile (src/gguf.h:85-305; Win32 mapping there, POSIX here). A split model

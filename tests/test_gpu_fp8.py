@@ -1,0 +1,274 @@
+"""The e4m3 products and their producers on the GPU against 64-bit forms (tests/fp8_plain.py). A product's tolerance is
+the worst case of its f32 additions (gemm_bound) and the rounding to C's type; the producers' rows are the quantizer's exact
+f32 result where the values it met are known, else e4m3 roundings of the 64-bit values."""
+import numpy as np
+import pytest
+import torch
+
+from tests import fp8_plain as P
+
+pytestmark = pytest.mark.gpu
+
+F32, F16, BF16 = torch.float32, torch.float16, torch.bfloat16
+
+
+def make(qm, dev, N, K, M, seed, Ms=None):
+    Ms = P.up(M, 16) if Ms is None else Ms
+    Kp = P.up(K, 128)
+    rng = np.random.default_rng(seed)
+    w8 = P.random_e4m3((N, K), seed)
+    wsc = torch.from_numpy(rng.uniform(0.5e-3, 2e-3, (P.up(N, 128) // 128, Kp // 128)).astype(np.float32))
+    a8 = P.random_e4m3((Ms, Kp), seed + 1)
+    a8[M:] = 0
+    a8[:, K:] = 0
+    asc = torch.from_numpy(rng.uniform(0.5e-2, 2e-2, (Kp // 128, Ms)).astype(np.float32))
+    w = qm.Fp8Weight(w8.to(dev), wsc.to(dev))
+    return w, a8.view(torch.float8_e4m3fn).to(dev), asc.to(dev), P.gemm(w8, wsc, a8, asc, M)
+
+
+def near(got, ref, bound):
+    got = got.double().cpu()
+    assert torch.isfinite(got).all()
+    off = (got - ref).abs()
+    assert bool((off <= bound).all()), float((off / bound).max())
+
+
+SHAPES = [(1, 1, 1), (3, 40, 2), (64, 128, 1), (100, 128, 7), (128, 256, 16), (130, 300, 17), (257, 1000, 33), (512, 640, 64),
+          (5184, 512, 65), (1000, 4096, 48), (640, 2048, 127), (384, 1024, 130), (2049, 896, 200), (256, 128, 500),
+          (1153, 1536, 333), (512, 17408, 5), (448, 8200, 40), (2304, 2176, 260), (4096, 4096, 1), (768, 5120, 513)]
+
+
+@pytest.mark.parametrize("out", [F32, BF16, F16])
+@pytest.mark.parametrize("N,K,M", SHAPES)
+def test_product(qm, dev, N, K, M, out):
+    w, a8, asc, (ref, *sums) = make(qm, dev, N, K, M, N + 3 * K + M)
+    ws = qm.gemm_fp8_workspace(w, M)
+    C = qm.gemm_fp8(w, a8, asc, M=M, out=out, ws=ws)
+    kb = P.up(K, 128) // 128
+    near(C, ref, P.gemm_bound(*sums, kb, out) + P.rounding(out, ref))
+    # without the workspace: the same within the bound
+    C = qm.gemm_fp8(w, a8, asc, M=M, out=F32)
+    near(C, ref, P.gemm_bound(*sums, kb) + P.rounding(F32, ref))
+    w.release()
+
+
+@pytest.mark.parametrize("out", [F32, BF16])
+@pytest.mark.parametrize("N,K,M", [(130, 300, 3), (256, 512, 40), (576, 1024, 150), (640, 2048, 300)])
+def test_accumulate_into_a_window(qm, dev, N, K, M, out):
+    """accumulate 1 and 2 into columns of a wider C; what lies beside the window and behind the last token stays."""
+    w, a8, asc, (ref, *sums) = make(qm, dev, N, K, M, N + M)
+    bound = P.gemm_bound(*sums, P.up(K, 128) // 128, out)
+    for ldc, off in ((N + 12, 4), (N + 7, 3)):
+        g = torch.Generator().manual_seed(N)
+        C0 = torch.randn((M + 2, ldc), generator=g).to(out)
+        for acc in (0, 1, 2):
+            C = C0.to(dev)
+            qm.gemm_fp8(w, a8, asc, M=M, C=C, c_off=off, accumulate=acc, ws=qm.gemm_fp8_workspace(w, M))
+            C, old = C.cpu(), C0.double()[:M, off:off + N]
+            want = ref if acc == 0 else old + ref if acc == 1 else old * torch.sigmoid(old) * ref
+            # (silu in f32: exp, a sum, a quotient, a product, each within two steps)
+            extra = 0 if acc == 0 else P.U32 * want.abs() if acc == 1 else 12 * P.U32 * want.abs()
+            b = bound if acc < 2 else bound * (old * torch.sigmoid(old)).abs() * 1.001
+            near(C[:M, off:off + N], want, b + extra + P.rounding(out, want))
+            C[:M, off:off + N] = C0[:M, off:off + N]
+            assert torch.equal(C, C0)
+    w.release()
+
+
+@pytest.mark.parametrize("out", [F32, BF16])
+@pytest.mark.parametrize("M", [1, 5, 40, 150, 300])
+def test_nan_and_zero_rows_stay_their_own(qm, dev, M, out):
+    """A token with a NaN has NaN results and no other token has; a weight row with a NaN likewise; a zero token gives zeros."""
+    N, K = 320, 640
+    w8 = P.random_e4m3((N, K), 5)
+    a8 = P.random_e4m3((M, K), 6)
+    a8[0, 130] = 0x7F
+    w8[77, 300] = 0xFF
+    if M > 2:
+        a8[2] = 0
+    w = qm.Fp8Weight(w8.to(dev), torch.ones((3, 5), device=dev))
+    C = qm.gemm_fp8(w, a8.view(torch.float8_e4m3fn).to(dev), torch.ones((5, M), device=dev), out=out,
+                    ws=qm.gemm_fp8_workspace(w, M)).float().cpu()
+    nan = torch.zeros((M, N), dtype=torch.bool)
+    nan[0], nan[:, 77] = True, True
+    assert torch.equal(torch.isnan(C), nan)
+    if M > 2:
+        assert torch.equal(C[2][~nan[2]], torch.zeros(N - 1))
+    w.release()
+
+
+def test_weight_from_the_host_and_info(qm, dev):
+    N, K, M = 200, 333, 4
+    w8, a8 = P.random_e4m3((N, K), 1), P.random_e4m3((M, P.up(K, 128)), 2)
+    a8[:, K:] = 0
+    wsc = torch.rand((2, 3)) + 0.5
+    a, s = a8.view(torch.float8_e4m3fn).to(dev), torch.ones((3, M), device=dev)
+    here, there = qm.Fp8Weight(w8, wsc), qm.Fp8Weight(w8.view(torch.float8_e4m3fn).to(dev), wsc.to(dev))
+    assert torch.equal(qm.gemm_fp8(here, a, s), qm.gemm_fp8(there, a, s))
+    import ctypes
+    r, k, kp = ctypes.c_int(), ctypes.c_int(), ctypes.c_int()
+    qm._call("qmatmul_fp8_info", here.handle, ctypes.byref(r), ctypes.byref(k), ctypes.byref(kp))
+    assert (r.value, k.value, kp.value) == (N, K, 384) and here.nbytes >= 256 * 384 + 6 * 4
+    # an unaligned source (rows of 333 bytes, base off by one)
+    buf = torch.zeros(N * K + 1, dtype=torch.uint8, device=dev)
+    buf[1:] = w8.to(dev).flatten()
+    odd = qm.Fp8Weight(buf[1:].view(N, K), wsc.to(dev))
+    assert torch.equal(qm.gemm_fp8(odd, a, s), qm.gemm_fp8(there, a, s))
+    for w in (here, there, odd):
+        w.release()
+
+
+def test_rows_past_32_bit_offsets(qm, dev):
+    """C rows further apart than 2^31 elements in all."""
+    N, K, M = 96, 256, 4
+    w, a8, asc, (ref, *sums) = make(qm, dev, N, K, M, 3)
+    ld = 1 << 30
+    C = torch.empty((M - 1) * ld + N, dtype=F16, device=dev).as_strided((M, N), (ld, 1))
+    qm.gemm_fp8(w, a8, asc, M=M, C=C)
+    near(C, ref, P.gemm_bound(*sums, 2, F16) + P.rounding(F16, ref))
+    w.release()
+
+
+@pytest.mark.parametrize("N,K,M", [(256, 1024, 3), (640, 2048, 40), (1024, 2048, 140), (512, 4096, 300)])
+def test_graphs_and_streams(qm, dev, N, K, M):
+    """Captured and replayed with eager work between; two streams at once with a workspace each; always the eager bits."""
+    w, a8, asc, _ = make(qm, dev, N, K, M, M)
+    want = qm.gemm_fp8(w, a8, asc, M=M, ws=qm.gemm_fp8_workspace(w, M))
+    ws, C = qm.gemm_fp8_workspace(w, M), torch.empty((M, N), device=dev)
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        qm.gemm_fp8(w, a8, asc, M=M, C=C, ws=ws)
+    for _ in range(3):
+        C.fill_(-1.0)
+        graph.replay()
+        assert torch.equal(qm.gemm_fp8(w, a8, asc, M=M, ws=qm.gemm_fp8_workspace(w, M)), want)
+        torch.cuda.synchronize()
+        assert torch.equal(C, want)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = []
+    torch.cuda.synchronize()
+    for _ in range(4):
+        for s in streams:
+            with torch.cuda.stream(s):
+                got.append(qm.gemm_fp8(w, a8, asc, M=M, ws=qm.gemm_fp8_workspace(w, M)))
+    torch.cuda.synchronize()
+    assert all(torch.equal(g, want) for g in got)
+    w.release()
+
+
+# ---- producers -------------------------------------------------------------------------------------------------------
+def same(a8, asc, q, sc, M):
+    assert torch.equal(P.value(a8.cpu())[:M], q), "e4m3 rows"
+    assert torch.equal(asc.cpu()[:, :M], sc), "scales"
+    assert not a8.cpu().view(torch.uint8)[M:].any() and not asc.cpu()[:, M:].any(), "padding"
+
+
+ROWS = [(1, 16, 5120), (7, 8, 2048), (3, 3, 17408), (2, 4, 96), (5, 5, 1), (4, 16, 1001), (300, 304, 640), (33, 48, 2050)]
+
+
+@pytest.mark.parametrize("x_type", [F32, F16, BF16])
+@pytest.mark.parametrize("M,Ms,K", ROWS)
+def test_quantize(qm, dev, M, Ms, K, x_type):
+    rng = np.random.default_rng(M + K)
+    x = torch.from_numpy((rng.standard_normal((M, K)) * 10.0 ** rng.uniform(-3, 3, (M, K))).astype(np.float32))
+    x[0, :128] = 0.0
+    x = x.to(x_type)
+    q, sc = P.quantize32(x.float().numpy())
+    same(*qm.quantize_fp8(x.to(dev), M_stride=Ms), q, sc, M)
+    wide = torch.full((M, K + 9), 7.0, dtype=x_type, device=dev)  # rows of another stride and alignment
+    wide[:, 5:5 + K] = x.to(dev)
+    same(*qm.quantize_fp8(wide[:, 5:5 + K], M_stride=Ms), q, sc, M)
+
+
+def test_quantize_extremes(qm, dev):
+    """Blocks of the largest, tiny, zero, infinite and NaN values: no other block or row is touched."""
+    x = torch.ones((6, 384))
+    x[0, :128] = 3.0e38
+    x[1, :128] = 2.0 ** -101
+    x[2, :128] = 2.0 ** -100
+    x[3, 5] = float("inf")
+    x[4, 7] = float("nan")
+    x[5, :128] = -0.0
+    a8, asc = qm.quantize_fp8(x.to(dev))
+    v, s = P.value(a8.cpu()), asc.cpu()
+    ones = torch.full((128,), 448.0, dtype=torch.float64)
+    assert torch.equal(v[0, :128], ones) and s[0, 0] == np.float32(3.0e38) / np.float32(448)
+    assert not v[1, :128].any() and s[0, 1] == 0 and torch.equal(v[2, :128], ones) and s[0, 2] == np.float32(2.0 ** -100 / 448)
+    assert torch.isinf(s[0, 3]) and torch.isnan(v[3, 5]) and not v[3, :5].any()
+    assert torch.isnan(v[4, 7]) and torch.isnan(v[4]).sum() == 1 and s[0, 4] == np.float32(1 / 448)
+    assert not v[5, :128].any() and s[0, 5] == 0
+    assert torch.equal(v[:, 128:], torch.full((6, 256), 448.0, dtype=torch.float64)) and bool((s[1:] == np.float32(1 / 448)).all())
+    w = qm.Fp8Weight(torch.full((16, 384), 0x38, dtype=torch.uint8, device=dev), torch.ones((1, 3), device=dev))  # ones
+    C = qm.gemm_fp8(w, a8, asc).cpu()
+    assert torch.isnan(C[3]).all() and torch.isnan(C[4]).all() and torch.isfinite(C[[1, 2, 5]]).all()
+    w.release()
+
+
+@pytest.mark.parametrize("x_type", [F32, BF16])
+@pytest.mark.parametrize("M,Ms,K", ROWS + [(2, 2, 40000), (260, 260, 20000)])
+def test_rmsnorm(qm, dev, M, Ms, K, x_type):
+    rng = np.random.default_rng(M + K)
+    x = torch.from_numpy((rng.standard_normal((M, K)) * rng.uniform(0.1, 10)).astype(np.float32)).to(x_type)
+    w = torch.from_numpy(rng.uniform(0.2, 2.0, K).astype(np.float32))
+    a8, asc, h = qm.rmsnorm_fp8(x.to(dev), w.to(dev), 1e-6, M_stride=Ms, want_h=True)
+    x64 = x.double()
+    y = x64 / torch.sqrt((x64 * x64).mean(1, keepdim=True) + 1e-6) * w.double()
+    e = P.norm_error(K, 8 * ((K + 2047) // 2048))
+    near(h, y, e * y.abs() + 1e-40)
+    q, sc = P.quantize32(h.cpu().numpy())  # the quantizer's exact result on the kernel's own y
+    same(a8, asc, q, sc, M)
+    b8, bsc, none = qm.rmsnorm_fp8(x.to(dev), w.to(dev), 1e-6, M_stride=Ms)
+    assert none is None and torch.equal(b8.view(torch.uint8), a8.view(torch.uint8)) and torch.equal(bsc, asc)
+
+
+@pytest.mark.parametrize("gelu", [False, True])
+@pytest.mark.parametrize("x_type", [F32, F16, BF16])
+@pytest.mark.parametrize("M,Ms,F", [(1, 16, 17408), (5, 8, 512), (2, 2, 97), (260, 260, 1024), (19, 32, 2184)])
+def test_swiglu(qm, dev, gelu, M, Ms, F, x_type):
+    rng = np.random.default_rng(F + M)
+    gu = torch.from_numpy((rng.standard_normal((M, 2 * F)) * 3).astype(np.float32)).to(x_type)
+    a8, asc = qm.swiglu_fp8(gu.to(dev), F, gelu=gelu, M_stride=Ms)
+    g, u = gu.double()[:, :F], gu.double()[:, F:]
+    z = 2 * np.sqrt(2 / np.pi) * (g + 0.044715 * g ** 3) if gelu else g
+    y = g * torch.sigmoid(z) * u
+    # silu: exp (two steps), a sum, a quotient, a product; gelu: tanh's argument (|z| U32 times its slope, below 4 in all), tanh, then
+    # 1 + tanh, which cancels where g < 0: absolute against |g u|
+    err = (32 * P.U32 * (g * u).abs()) if gelu else 8 * P.U32 * y.abs()
+    p = torch.zeros((2, M, P.up(F, 128)), dtype=torch.float64)
+    p[0, :, :F], p[1, :, :F] = y, err
+    top, terr = (v.view(M, -1, 128) for v in p)
+    top, terr = top.abs().amax(2), terr.amax(2)
+    assert bool(((asc.cpu().double()[:, :M].T - top / 448).abs() <= terr / 448 + 2 * P.U32 * top / 448).all())
+    s = (448 / top)[:, :, None].expand(-1, -1, 128).reshape(M, -1)
+    v = p[0] * s
+    e = (p[1] * s) + v.abs() * ((terr / top)[:, :, None].expand(-1, -1, 128).reshape(M, -1) + 4 * P.U32)
+    # (an error near a border is a whole step there: the border itself lies half a step from both)
+    assert P.near_e4m3(P.value(a8.cpu())[:M], v, 1.1 * e)
+    assert not a8.cpu().view(torch.uint8)[M:].any() and not a8.cpu().view(torch.uint8)[:, F:].any()
+
+
+def test_ffn_run(qm, dev):
+    """Norm, gate and up, gating, down, as an FFN layer uses them, with C in bf16 and f32; each product against 64 bits on the
+    activations that it met."""
+    E, Fw = 640, 1152
+    ws = {n: (P.random_e4m3(s, i), torch.rand((P.up(s[0], 128) // 128, P.up(s[1], 128) // 128)) * 1e-3 + 1e-4)
+          for i, (n, s) in enumerate((("gate", (Fw, E)), ("up", (Fw, E)), ("down", (E, Fw))))}
+    h = {n: qm.Fp8Weight(a.to(dev), b.to(dev)) for n, (a, b) in ws.items()}
+    for M in (1, 21, 150):
+        x = torch.randn((M, E), generator=torch.Generator().manual_seed(M)).to(dev)
+        norm = torch.rand(E, device=dev) + 0.5
+        a8, asc, _ = qm.rmsnorm_fp8(x, norm, 1e-6, M_stride=P.up(M, 16))
+        gu = torch.empty((M, 2 * Fw), dtype=BF16, device=dev)
+        for n, off in (("gate", 0), ("up", Fw)):
+            qm.gemm_fp8(h[n], a8, asc, M=M, C=gu, c_off=off, ws=qm.gemm_fp8_workspace(h[n], M))
+            ref, *sums = P.gemm(*ws[n], a8.cpu(), asc.cpu(), M)
+            near(gu[:, off:off + Fw], ref, P.gemm_bound(*sums, E // 128, BF16) + P.rounding(BF16, ref))
+        b8, bsc = qm.swiglu_fp8(gu, Fw, M_stride=P.up(M, 16))
+        y = x.clone()
+        qm.gemm_fp8(h["down"], b8, bsc, M=M, C=y, accumulate=1, ws=qm.gemm_fp8_workspace(h["down"], M))
+        ref, *sums = P.gemm(*ws["down"], b8.cpu(), bsc.cpu(), M)
+        ref = ref + x.double().cpu()
+        near(y, ref, P.gemm_bound(*sums, Fw // 128) + 2 * P.rounding(F32, ref))
+    for w in h.values():
+        w.release()
