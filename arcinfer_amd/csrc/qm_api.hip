@@ -761,8 +761,8 @@ static int padded_128(int K) { return (K + 127) / 128 * 128; }
 
 static size_t fp8_payload_bytes(int rows, int K) { return (size_t)((rows + 63) / 64) * 64 * ((size_t)(K + 127) / 128 * 128); }
 static size_t fp8_scale_count(int rows, int K) { return (size_t)((rows + 127) / 128) * ((K + 127) / 128); }
-// (rows and K rounded up stay ints)
-static bool fp8_shape_ok(int rows, int K) { return rows >= 1 && K >= 1 && rows <= 0x7fffff00 && K <= 0x7fffff00; }
+// (rows rounded up stay an int; offsets within a tile's rows stay within 32 bits)
+static bool fp8_shape_ok(int rows, int K) { return rows >= 1 && K >= 1 && rows <= 0x7fffff00 && K <= 1 << 24; }
 
 size_t qmatmul_fp8_weight_bytes(int rows, int K) {
   if (!fp8_shape_ok(rows, K)) return 0;

@@ -33,8 +33,15 @@ struct Fp8GemmArgs {
   float* part;  // partial results of calls whose K is cut (null: it is not)
 };
 hipError_t launch_fp8_repack(const uint8_t* w8, int rows, int K, uint8_t* q, hipStream_t s);
+// Workspace for the pieces of cut products (0: the call is not cut); the launcher takes a part that holds as much or none
 size_t fp8_workspace_bytes(int M, int rows, int kb);
 hipError_t launch_gemm_fp8(const Fp8GemmArgs& a, hipStream_t s);
+
+// The tile kernel (qm_fp8_tile.hip): tiles of 256 rows x 16 mt tokens (mt 4..8, 4..6 for a C of f32), K in `splits` pieces
+constexpr int kFp8Slots = 512;                    // its work-groups that the chip holds at once (two per CU)
+constexpr size_t kFp8PartBytes = (size_t)64 << 20;  // most partial results of one call
+inline size_t fp8_part_bytes(int M, int rows, int splits) { return (size_t)splits * M * ((rows + 63) / 64 * 64) * sizeof(float); }
+hipError_t launch_fp8_tile(const Fp8GemmArgs& a, int mt, int splits, hipStream_t s);
 
 hipError_t launch_quantize_fp8(const void* x, int xtype, int ldx, int M, int M_stride, int K, uint8_t* a8, float* asc,
                                hipStream_t s);

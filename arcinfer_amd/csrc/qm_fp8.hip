@@ -9,95 +9,9 @@
 // between the eights the sum is f32): 1.3e-5 of the result for normal values, whichever fp8 instruction it is. Under a C of 16 bits
 // (rounded by 2^-9 or 2^-12) that is nothing. A C of f32 gets the f16 pipe: e4m3 values are f16 values, their products exact
 // there and the sums f32 (1e-8), for four v_mfma_f32_16x16x32_f16 a block and the conversions.
-#include "qm_fp8.h"
+#include "qm_fp8_dev.h"
 
 namespace qm {
-
-namespace {
-
-typedef int v4i __attribute__((ext_vector_type(4)));
-typedef int v8i __attribute__((ext_vector_type(8)));
-typedef float v4f __attribute__((ext_vector_type(4)));
-
-constexpr int kFragBytes = 2048;
-
-__device__ __forceinline__ v8i join(v4i lo, v4i hi) { return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7); }
-
-typedef _Float16 v2h __attribute__((ext_vector_type(2)));
-typedef _Float16 v8h __attribute__((ext_vector_type(8)));
-
-// Eight e4m3 values as f16 (exact; NaN stays NaN)
-__device__ __forceinline__ v8h widen(int lo, int hi) {
-  const v2h a = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, 1.0f, false), b = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, 1.0f, true);
-  const v2h c = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, 1.0f, false), d = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, 1.0f, true);
-  return v8h{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
-}
-
-// S of one block: 16 rows by 16 tokens, 32 bytes of each a lane. (The builtin without scales is the unscaled instruction.)
-template <bool EXACT>
-__device__ __forceinline__ v4f dot_block(v8i w, v8i a) {
-  v4f s = {0.0f, 0.0f, 0.0f, 0.0f};
-  if constexpr (EXACT) {
-#pragma unroll
-    for (int i = 0; i < 8; i += 2) s = __builtin_amdgcn_mfma_f32_16x16x32_f16(widen(w[i], w[i + 1]), widen(a[i], a[i + 1]), s, 0, 0, 0);
-    return s;
-  } else {
-    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w, a, s, 0, 0, 0, 0, 0, 0);
-  }
-}
-
-// C[i] (op)= v for elements of type T, computed in f32 and rounded once
-template <typename T>
-__device__ __forceinline__ void put(T* C, float v, int accumulate) {
-  if (accumulate == 1) {
-    v += (float)*C;
-  } else if (accumulate == 2) {
-    const float g = (float)*C;
-    v = g / (1.0f + expf(-g)) * v;
-  }
-  *C = (T)v;
-}
-
-// Four neighbouring results n .. n + 3 of token m (n % 4 == 0; rows: the weight's)
-template <typename T>
-__device__ __forceinline__ void put4(T* C, size_t at, v4f v, int left, int accumulate, bool vec) {
-  typedef T v4t __attribute__((ext_vector_type(4)));
-  if (vec && left >= 4) {
-    if (accumulate) {
-      const v4t o = *(const v4t*)(C + at);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float c = (float)o[i];
-        v[i] = accumulate == 1 ? v[i] + c : c / (1.0f + expf(-c)) * v[i];
-      }
-    }
-    v4t r;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) r[i] = (T)v[i];
-    *(v4t*)(C + at) = r;
-    return;
-  }
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-    if (i < left) put(C + at + i, v[i], accumulate);
-}
-
-__device__ __forceinline__ void store4(const Fp8GemmArgs& a, int m, int n, v4f v, bool vec) {
-  const size_t at = (size_t)m * a.ldc + a.c_off + n;
-  const int left = a.w.rows - n;
-  if (left <= 0) return;
-  if (a.ctype == DT_F32) put4((float*)a.C, at, v, left, a.accumulate, vec);
-  else if (a.ctype == DT_F16) put4((_Float16*)a.C, at, v, left, a.accumulate, vec);
-  else put4((__bf16*)a.C, at, v, left, a.accumulate, vec);
-}
-
-// whether every group of four results lies on its own alignment
-__device__ __forceinline__ bool vec_stores(const Fp8GemmArgs& a) {
-  const uintptr_t size = a.ctype == DT_F32 ? 4 : 2;
-  return ((((uintptr_t)a.C / size) | (uintptr_t)a.ldc | (uintptr_t)a.c_off) & 3) == 0;
-}
-
-}  // namespace
 
 // e4m3 rows -> the prepared layout, 16 bytes a thread
 __global__ __launch_bounds__(256) void fp8_repack_kernel(const uint8_t* __restrict__ w, int rows, int K, int kb, size_t n,
@@ -131,76 +45,197 @@ hipError_t launch_fp8_repack(const uint8_t* w8, int rows, int K, uint8_t* q, hip
   return hipGetLastError();
 }
 
-// One fragment of 16 rows against 16 MT tokens: four waves take every fourth block of K, and add their sums in wave order.
-template <int MT, bool EXACT>
-__global__ __launch_bounds__(256) void fp8_few_kernel(Fp8GemmArgs a) {
-  __shared__ v4f red[4][MT][64];
+// Few tokens: RT fragments of 16 rows against 16 MT tokens. The W waves of a work-group take the blocks of K in turn, so that
+// it streams its rows from one end to the other, and add their sums in wave order.
+template <int MT, int RT, int W, bool EXACT>
+__global__ __launch_bounds__(64 * W) void fp8_few_kernel(Fp8GemmArgs a) {
+  __shared__ v4f red[W][RT * MT][64];
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
-  const int tile = blockIdx.x, m0 = blockIdx.y * 16 * MT, kb = a.w.kb;
-  const uint8_t* wp = a.w.q + (size_t)tile * kb * kFragBytes + 16 * lane;
+  const unsigned units = (unsigned)((a.w.rows + 63) / 64 * 4 / RT);  // (neighbouring work-groups take neighbouring rows)
+  const int tile = RT * (int)(blockIdx.x % units), m0 = (int)(blockIdx.x / units) * 16 * MT, kb = a.w.kb;
+  const size_t frag_stride = (size_t)kb * kFragBytes;
+  const uint8_t* wp = a.w.q + (size_t)tile * frag_stride + 16 * lane;
   const float* wsc = a.w.sc + (size_t)(tile >> 3) * kb;
   const size_t Kp = (size_t)kb * 128;
-  v4f acc[MT];
+  const uint8_t* ap = a.a8 + (size_t)(m0 + r) * Kp + 16 * g;
+  const float* asc = a.asc + m0 + r;
+  v4f acc[RT][MT];
 #pragma unroll
-  for (int t = 0; t < MT; ++t) acc[t] = {0.0f, 0.0f, 0.0f, 0.0f};
-  for (int b = wave; b < kb; b += 4) {
-    const v4i w0 = *(const v4i*)(wp + (size_t)b * kFragBytes), w1 = *(const v4i*)(wp + (size_t)b * kFragBytes + 1024);
+  for (int f = 0; f < RT; ++f)
+#pragma unroll
+    for (int t = 0; t < MT; ++t) acc[f][t] = {0.0f, 0.0f, 0.0f, 0.0f};
+  const auto block = [&](int b, const v4i (&w)[RT][2]) {
     const float ws = wsc[b];
 #pragma unroll
     for (int t = 0; t < MT; ++t) {
-      const int m = m0 + 16 * t + r;
       v4i a0 = {0, 0, 0, 0}, a1 = {0, 0, 0, 0};
       float s = 0.0f;
-      if (m < a.M) {
-        const uint8_t* ap = a.a8 + m * Kp + 128 * (size_t)b + 16 * g;
-        a0 = *(const v4i*)ap;
-        a1 = *(const v4i*)(ap + 64);
-        s = a.asc[(size_t)b * a.M_stride + m] * ws;
+      if (m0 + 16 * t + r < a.M) {
+        const uint8_t* p = ap + 16 * t * Kp + 128 * (size_t)b;
+        a0 = *(const v4i*)p;
+        a1 = *(const v4i*)(p + 64);
+        s = asc[(size_t)b * a.M_stride + 16 * t] * ws;
       }
-      const v4f p = dot_block<EXACT>(join(w0, w1), join(a0, a1));
 #pragma unroll
-      for (int i = 0; i < 4; ++i) acc[t][i] = fmaf(s, p[i], acc[t][i]);
+      for (int f = 0; f < RT; ++f) {
+        const v4f p = dot_block<EXACT>(join(w[f][0], w[f][1]), join(a0, a1));
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[f][t][i] = fmaf(s, p[i], acc[f][t][i]);
+      }
     }
+  };
+  const auto load = [&](int b, v4i (&w)[RT][2]) {
+#pragma unroll
+    for (int f = 0; f < RT; ++f) {
+      const uint8_t* p = wp + f * frag_stride + (size_t)b * kFragBytes;
+      w[f][0] = __builtin_nontemporal_load((const v4i*)p);
+      w[f][1] = __builtin_nontemporal_load((const v4i*)(p + 1024));
+    }
+  };
+  // U blocks' weights are under way at once
+  constexpr int U = RT == 1 ? 4 : 2;
+  int b = wave;
+  for (; b + (U - 1) * W < kb; b += U * W) {
+    v4i w[U][RT][2];
+#pragma unroll
+    for (int u = 0; u < U; ++u) load(b + u * W, w[u]);
+#pragma unroll
+    for (int u = 0; u < U; ++u) block(b + u * W, w[u]);
+  }
+  for (; b < kb; b += W) {
+    v4i w[RT][2];
+    load(b, w);
+    block(b, w);
   }
 #pragma unroll
-  for (int t = 0; t < MT; ++t) red[wave][t][lane] = acc[t];
+  for (int f = 0; f < RT; ++f)
+#pragma unroll
+    for (int t = 0; t < MT; ++t) red[wave][f * MT + t][lane] = acc[f][t];
   __syncthreads();
   const bool vec = vec_stores(a);
-  for (int t = wave; t < MT; t += 4) {
-    const int m = m0 + 16 * t + r;
-    v4f v = red[0][t][lane];
+  for (int i = wave; i < RT * MT; i += W) {
+    const int f = i / MT, t = i - f * MT, m = m0 + 16 * t + r;
+    v4f v = red[0][i][lane];
 #pragma unroll
-    for (int w = 1; w < 4; ++w) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) v[i] += red[w][t][lane][i];
-    }
-    if (m < a.M) store4(a, m, 64 * (tile >> 2) + 16 * g + 4 * (tile & 3), v, vec);
+    for (int w = 1; w < W; ++w) v += red[w][i][lane];
+    if (m < a.M) store4(a, m, 64 * (tile >> 2) + 16 * g + 4 * ((tile & 3) + f), v, vec);
   }
-}
-
-size_t fp8_workspace_bytes(int M, int rows, int kb) {
-  (void)M;
-  (void)rows;
-  (void)kb;
-  return 0;
 }
 
 namespace {
 
-template <bool EXACT>
+template <int MT, int RT, int W>
 void launch_few(const Fp8GemmArgs& a, hipStream_t s) {
-  const unsigned tiles = (unsigned)((a.w.rows + 63) / 64 * 4);
-  if (a.M <= 16) fp8_few_kernel<1, EXACT><<<tiles, 256, 0, s>>>(a);
-  else if (a.M <= 32) fp8_few_kernel<2, EXACT><<<tiles, 256, 0, s>>>(a);
-  else fp8_few_kernel<4, EXACT><<<dim3(tiles, (a.M + 63) / 64), 256, 0, s>>>(a);
+  const unsigned grid = (unsigned)((a.w.rows + 63) / 64 * 4 / RT) * (unsigned)((a.M + 16 * MT - 1) / (16 * MT));
+  if (a.ctype == DT_F32) fp8_few_kernel<MT, RT, W, true><<<grid, 64 * W, 0, s>>>(a);
+  else fp8_few_kernel<MT, RT, W, false><<<grid, 64 * W, 0, s>>>(a);
+}
+
+// The few-token kernel's shape. Two fragments a work-group once one would put more than a work-group on every CU (the token
+// reads halve: 5 x 17408 -> 5120 20 us against 24), and as many waves as keep a CU busy and have blocks to take (1 x 4096 -> 4096, 256
+// fragments: 16 waves 5.3 us, 8 6.1, 4 7.2; with more than one work-group a CU 8: 16 x 5120 -> 17408 22.2 against 23.8).
+struct FewShape {
+  int rt, waves;
+};
+FewShape few_shape(int M, int rows, int kb) {
+  const int tiles = (rows + 63) / 64 * 4, rt = tiles > 256 ? 2 : 1, wg = tiles / rt;
+  int w = 8;
+  if (kb < 8 || (M > 16 && wg > 512)) w = 4;
+  else if (kb >= 16 && wg <= 256 && (M <= 16 || (M <= 32 && rt == 1))) w = 16;
+  return {rt, w};
+}
+
+hipError_t launch_few_tokens(const Fp8GemmArgs& a, hipStream_t s) {
+  const FewShape f = few_shape(a.M, a.w.rows, a.w.kb);
+#define QM_FEW(MT, RT) (f.waves == 8 ? launch_few<MT, RT, 8>(a, s) : launch_few<MT, RT, 4>(a, s))
+  if (a.M <= 16) {
+    if (f.waves == 16) f.rt == 1 ? launch_few<1, 1, 16>(a, s) : launch_few<1, 2, 16>(a, s);
+    else f.rt == 1 ? QM_FEW(1, 1) : QM_FEW(1, 2);
+  } else if (a.M <= 32) {
+    if (f.waves == 16) launch_few<2, 1, 16>(a, s);
+    else f.rt == 1 ? QM_FEW(2, 1) : QM_FEW(2, 2);
+  } else if (a.M <= 48) {
+    f.rt == 1 ? QM_FEW(3, 1) : QM_FEW(3, 2);
+  } else {
+    f.rt == 1 ? QM_FEW(4, 1) : QM_FEW(4, 2);
+  }
+#undef QM_FEW
+  return hipGetLastError();
+}
+
+// Times in microseconds, fitted to 2900 (C of 16 bits) and 1700 (f32) measured products of 20 to 4096 tokens and ten weights from
+// 512 x 1024 to 17408 x 5120 (rms 9 and 7 %; what the choice by them costs against the best of all variants: 2.9 and 1.5 %).
+// Tile kernel: `call`; a work-group's blocks and `more` (its prologue and store), each block one + one_mt * MT where work-groups have
+// their CU to themselves (`crowd` of it more with every CU taken), two + two_mt * MT where two share it, a last round behind
+// others `tail` of that; never less than the weight's bytes at `stream` a microsecond; cut: `sum`, and the pieces written and read at `part`.
+// Few-token kernel: few_call; bytes of weight and of tokens (read once a work-group) at few_w and few_t; few_mt a block, token tile and fragment.
+struct Rates {
+  float call, more, one, one_mt, crowd, two, two_mt, tail, stream, sum, part;
+  float few_call, few_w, few_t, few_mt;
+};
+constexpr Rates kRates16 = {2.9f, 3.8f, 0.18f, 0.072f, 0.31f, 0.53f, 0.12f, 0.74f, 4.6e6f, 2.45f, 6.9e6f, 3.8f, 11.1e6f, 7.9e6f, 0.071f};
+constexpr Rates kRates32 = {3.1f, 2.4f, 0.0f, 0.248f, 0.19f, 0.03f, 0.41f, 0.75f, 4.5e6f, 2.6f, 8.1e6f, 4.0f, 8.5e6f, 7.4e6f, 0.094f};
+constexpr float kFewBlock16 = 0.19f;  // (few-token kernel, fp8 pipe: a block of a wave; nothing measurable on the f16 pipe)
+
+float tile_us(const Rates& r, int M, int rows, int kb, int mt, int splits) {
+  const int n = (rows + 255) / 256 * ((M + 16 * mt - 1) / (16 * mt)) * splits, full = n / kFp8Slots, rem = n % kFp8Slots;
+  const float two = r.two + r.two_mt * mt;
+  float rounds = full * two;
+  if (rem) rounds += (rem > kFp8Slots / 2 ? two : (r.one + r.one_mt * mt) * (1.0f + r.crowd * rem / (kFp8Slots / 2))) * (full ? r.tail : 1.0f);
+  const float run = rounds * ((kb + splits - 1) / splits + r.more), read = (float)rows * kb * 128.0f / r.stream;
+  const float run2 = run * run, read2 = read * read;
+  float t = r.call + sqrtf(sqrtf(run2 * run2 + read2 * read2));  // (the larger, and both where they are alike)
+  if (splits > 1) t += r.sum + 8.0f * splits * M * ((rows + 63) / 64 * 64.0f) / r.part;
+  return t;
+}
+
+float few_us(const Rates& r, float block, int M, int rows, int kb) {
+  const FewShape f = few_shape(M, rows, kb);
+  const int tiles = (rows + 63) / 64 * 4, mt = M > 48 ? 4 : (M + 15) / 16, turns = (M + 63) / 64;
+  const float bytes = tiles * 2048.0f * kb;
+  return r.few_call + bytes / r.few_w + bytes / f.rt * mt * turns / r.few_t + (block + r.few_mt * mt * f.rt) * kb / f.waves;
+}
+
+// Up to 16 tokens: the few-token kernel. Beyond, what the times above say: that kernel (mt = 0), or tiles of mt token tiles, each
+// in `splits` pieces of at least three blocks (more than one only with a workspace for their sums).
+struct Plan {
+  int mt, splits;
+};
+Plan plan_of(int M, int M_stride, int rows, int kb, bool exact, bool part) {
+  Plan p{0, 1};
+  // (the tile kernel's token scales are a buffer of 32-bit offsets)
+  if (M <= 16 || (size_t)kb * M_stride >= (size_t)1 << 30) return p;
+  const Rates& r = exact ? kRates32 : kRates16;
+  float best = M <= 1024 ? few_us(r, exact ? 0.0f : kFewBlock16, M, rows, kb) : 1e30f;
+  constexpr int kSplits[] = {1, 2, 3, 4, 5, 6, 8, 10, 12, 16};
+  for (int mt = 4; mt <= (exact ? 6 : 8); ++mt) {
+    for (int s : kSplits) {
+      if (s > 1 && (!part || kb / s < 3 || fp8_part_bytes(M, rows, s) > kFp8PartBytes)) break;
+      const float t = tile_us(r, M, rows, kb, mt, s);
+      if (t < best) {
+        best = t;
+        p = {mt, s};
+      }
+    }
+  }
+  return p;
 }
 
 }  // namespace
 
+size_t fp8_workspace_bytes(int M, int rows, int kb) {
+  // (the larger of both output types': the call's is not known yet)
+  size_t most = 0;
+  for (int exact = 0; exact < 2; ++exact) {
+    const Plan p = plan_of(M, M, rows, kb, exact != 0, true);
+    if (p.splits > 1 && fp8_part_bytes(M, rows, p.splits) > most) most = fp8_part_bytes(M, rows, p.splits);
+  }
+  return most;
+}
+
 hipError_t launch_gemm_fp8(const Fp8GemmArgs& a, hipStream_t s) {
-  if (a.ctype == DT_F32) launch_few<true>(a, s);
-  else launch_few<false>(a, s);
-  return hipGetLastError();
+  const Plan p = plan_of(a.M, a.M_stride, a.w.rows, a.w.kb, a.ctype == DT_F32, a.part != nullptr);
+  return p.mt ? launch_fp8_tile(a, p.mt, p.splits, s) : launch_few_tokens(a, s);
 }
 
 }  // namespace qm

@@ -333,34 +333,37 @@ _DTYPES = {}  # torch dtype -> qm_dtype (filled on first use: torch is imported 
 
 
 def _dtype(t):
-    if not _DTYPES:
+    d = _DTYPES.get(t)
+    if d is None:
         import torch
         _DTYPES.update({torch.float32: 0, torch.float16: 1, torch.bfloat16: 30})
-    try:
-        return _DTYPES[t]
-    except KeyError:
-        raise QMatmulError("dtype", 3, f"{t}: float32, float16 or bfloat16 rows") from None
+        if t not in _DTYPES:
+            raise QMatmulError("dtype", 3, f"{t}: float32, float16 or bfloat16 rows")
+        d = _DTYPES[t]
+    return d
 
 
-def _check(fn, ok, what):
-    if not ok:
-        raise QMatmulError(fn, 1, what)
+def _refuse(fn, what):
+    raise QMatmulError(fn, 1, what)
 
 
-def _check_rows(fn, dim, **tensors):
-    """Every tensor (None passes) is on the current GPU, of `dim` dimensions where dim is given, its last one contiguous."""
+def _current_gpu():
     import torch
-    dev = torch.cuda.current_device()
-    for name, t in tensors.items():
-        if t is None:
-            continue
-        _check(fn, t.is_cuda and t.device.index == dev, f"{name} is not on the current GPU")
-        _check(fn, dim is None or t.dim() == dim, f"{name} has {t.dim()} dimensions, not {dim}")
-        _check(fn, t.numel() == 0 or t.shape[-1] == 1 or t.stride(-1) == 1, f"the last dimension of {name} is not contiguous")
+    return torch.cuda.current_device()
+
+
+def _check_rows(fn, name, t, dim, dev):
+    """t is on GPU `dev`, of `dim` dimensions where dim is given, its last one contiguous."""
+    if not t.is_cuda or t.get_device() != dev:
+        _refuse(fn, f"{name} is on {t.device}, not on the current GPU")
+    if dim and t.dim() != dim:
+        _refuse(fn, f"{name} has {t.dim()} dimensions, not {dim}")
+    if t.stride(-1) != 1 and t.numel() and t.shape[-1] != 1:
+        _refuse(fn, f"the last dimension of {name} is not contiguous")
 
 
 def _row_stride(t):
-    """The row stride of a matrix in elements (of a single row, whose stride says nothing: its length)."""
+    """The row stride of a matrix in elements (of a single row, whose stride says nothing: at least its length)."""
     return t.stride(0) if t.shape[0] > 1 else max(t.shape[1], t.stride(0))
 
 
@@ -372,16 +375,17 @@ class Fp8Weight:
         import torch
         fn = "qmatmul_prepare_fp8"
         self.handle = None
-        _check(fn, w8.dtype in (torch.float8_e4m3fn, torch.uint8), f"w8 is {w8.dtype}: float8_e4m3fn (or its bytes)")
-        _check(fn, w8.dim() == 2 and w8.is_contiguous(), "w8 must be a contiguous matrix")
+        if w8.dtype not in (torch.float8_e4m3fn, torch.uint8) or w8.dim() != 2 or not w8.is_contiguous():
+            _refuse(fn, f"w8 {tuple(w8.shape)} {w8.dtype}: a contiguous matrix of float8_e4m3fn (or its bytes)")
         self.rows, self.K = w8.shape
         self.Kp = (self.K + 127) // 128 * 128
-        _check(fn, scales.dtype == torch.float32 and scales.is_contiguous()
-               and tuple(scales.shape) == ((self.rows + 127) // 128, self.Kp // 128),
-               f"scales {tuple(scales.shape)} {scales.dtype}: contiguous float32, one for each 128 x 128 block")
-        _check(fn, w8.device == scales.device, "w8 and scales are on different devices")
+        if (scales.dtype != torch.float32 or not scales.is_contiguous()
+                or tuple(scales.shape) != ((self.rows + 127) // 128, self.Kp // 128)):
+            _refuse(fn, f"scales {tuple(scales.shape)} {scales.dtype}: contiguous float32, one for each 128 x 128 block")
+        if w8.device != scales.device:
+            _refuse(fn, "w8 and scales are on different devices")
         if w8.is_cuda:
-            _check_rows(fn, 2, w8=w8)
+            _check_rows(fn, "w8", w8, 2, _current_gpu())
         h = ctypes.c_void_p()
         _call(fn, _ptr(w8), _ptr(scales), 1 if w8.is_cuda else 0, self.rows, self.K, _stream(stream), ctypes.byref(h))
         self.handle = h
@@ -404,9 +408,8 @@ class Fp8Weight:
             pass
 
 
-def _out_fp8(fn, x, K, M_stride):
+def _out_fp8(x, M, K, M_stride):
     import torch
-    M = x.shape[0]
     Ms = M if M_stride is None else M_stride
     Kp = (K + 127) // 128 * 128
     return (Ms, torch.empty((Ms, Kp), dtype=torch.float8_e4m3fn, device=x.device),
@@ -417,10 +420,10 @@ def quantize_fp8(x, M_stride=None, stream=None):
     """x [M, K] (float32, float16 or bfloat16, rows of any stride) -> (a8 float8_e4m3fn [M_stride, Kp], asc float32
     [Kp / 128, M_stride]), Kp = K rounded up to 128."""
     fn = "qmatmul_quantize_fp8"
-    _check_rows(fn, 2, x=x)
-    Ms, a8, asc = _out_fp8(fn, x, x.shape[1], M_stride)
-    _call(fn, x.data_ptr(), _dtype(x.dtype), _row_stride(x), x.shape[0], Ms, x.shape[1], a8.data_ptr(), asc.data_ptr(),
-          _stream(stream))
+    _check_rows(fn, "x", x, 2, _current_gpu())
+    M, K = x.shape
+    Ms, a8, asc = _out_fp8(x, M, K, M_stride)
+    _call(fn, x.data_ptr(), _dtype(x.dtype), _row_stride(x), M, Ms, K, a8.data_ptr(), asc.data_ptr(), _stream(stream))
     return a8, asc
 
 
@@ -428,11 +431,13 @@ def rmsnorm_fp8(x, w, eps, M_stride=None, want_h=False, stream=None):
     """x [M, K], w float32 [K] -> (a8, asc, h float32 [M, K] or None)."""
     import torch
     fn = "qmatmul_rmsnorm_fp8"
-    _check_rows(fn, 2, x=x)
-    _check_rows(fn, 1, w=w)
+    dev = _current_gpu()
+    _check_rows(fn, "x", x, 2, dev)
+    _check_rows(fn, "w", w, 1, dev)
     M, K = x.shape
-    _check(fn, w.dtype == torch.float32 and w.numel() == K, "w: float32, one for each column")
-    Ms, a8, asc = _out_fp8(fn, x, K, M_stride)
+    if w.dtype != torch.float32 or w.numel() != K:
+        _refuse(fn, f"w {tuple(w.shape)} {w.dtype}: float32, one for each of {K} columns")
+    Ms, a8, asc = _out_fp8(x, M, K, M_stride)
     h = torch.empty((M, K), dtype=torch.float32, device=x.device) if want_h else None
     _call(fn, x.data_ptr(), _dtype(x.dtype), _row_stride(x), w.data_ptr(), K, M, Ms, eps, a8.data_ptr(), asc.data_ptr(),
           h.data_ptr() if want_h and M else None, K, _stream(stream))
@@ -442,10 +447,12 @@ def rmsnorm_fp8(x, w, eps, M_stride=None, want_h=False, stream=None):
 def swiglu_fp8(gu, F, gelu=False, M_stride=None, stream=None):
     """gu [M, 2 F] (gate then up) -> (a8, asc) of silu(gate) * up, or gelu_tanh(gate) * up."""
     fn = "qmatmul_swiglu_fp8"
-    _check_rows(fn, 2, gu=gu)
-    _check(fn, gu.shape[1] >= 2 * F, f"rows of {gu.shape[1]} elements hold no gate and up of {F}")
-    Ms, a8, asc = _out_fp8(fn, gu, F, M_stride)
-    _call(fn, gu.data_ptr(), _dtype(gu.dtype), _row_stride(gu), F, gu.shape[0], Ms, 1 if gelu else 0, a8.data_ptr(),
+    _check_rows(fn, "gu", gu, 2, _current_gpu())
+    M = gu.shape[0]
+    if gu.shape[1] < 2 * F:
+        _refuse(fn, f"rows of {gu.shape[1]} elements hold no gate and up of {F}")
+    Ms, a8, asc = _out_fp8(gu, M, F, M_stride)
+    _call(fn, gu.data_ptr(), _dtype(gu.dtype), _row_stride(gu), F, M, Ms, 1 if gelu else 0, a8.data_ptr(),
           asc.data_ptr(), _stream(stream))
     return a8, asc
 
@@ -459,26 +466,41 @@ def gemm_fp8_workspace(w, M):
 
 def gemm_fp8(w, a8, asc, M=None, C=None, ldc=None, c_off=0, accumulate=0, out=None, ws=None, stream=None):
     """C [M, rows] (op)= the product of activations (a8, asc) with an Fp8Weight. out: the type of a new C (float32 unless
-    given). C: a matrix of that stride unless ldc is given."""
+    given). C: a matrix of its own row stride unless ldc is given."""
     import torch
     fn = "qmatmul_gemm_fp8"
-    _check_rows(fn, 2, a8=a8, asc=asc, C=C)
+    dev = _current_gpu()
+    _check_rows(fn, "a8", a8, 2, dev)
+    _check_rows(fn, "asc", asc, 2, dev)
     Ms, Kp = a8.shape
-    M = Ms if M is None else M
-    _check(fn, w.handle is not None, "the weight was released")
-    _check(fn, a8.is_contiguous() and a8.element_size() == 1 and Kp == w.Kp, f"a8 {tuple(a8.shape)}: contiguous e4m3 rows of {w.Kp}")
-    _check(fn, asc.is_contiguous() and asc.dtype == torch.float32 and tuple(asc.shape) == (Kp // 128, Ms),
-           f"asc {tuple(asc.shape)}: contiguous float32 [{Kp // 128}, {Ms}]")
+    if M is None:
+        M = Ms
+    if w.handle is None:
+        _refuse(fn, "the weight was released")
+    if Kp != w.Kp or a8.element_size() != 1 or not a8.is_contiguous():
+        _refuse(fn, f"a8 {tuple(a8.shape)} {a8.dtype}: contiguous e4m3 rows of {w.Kp}")
+    if asc.dtype != torch.float32 or asc.shape[0] != Kp // 128 or asc.shape[1] != Ms or not asc.is_contiguous():
+        _refuse(fn, f"asc {tuple(asc.shape)} {asc.dtype}: contiguous float32 [{Kp // 128}, {Ms}]")
     if C is None:
-        _check(fn, accumulate == 0 and c_off == 0 and ldc is None, "accumulate, c_off and ldc need a C")
+        if accumulate or c_off or ldc is not None:
+            _refuse(fn, "accumulate, c_off and ldc need a C")
         C = torch.empty((M, w.rows), dtype=torch.float32 if out is None else out, device=a8.device)
-        ld = w.rows
+        ldc = w.rows
     else:
-        _check(fn, out is None or out == C.dtype, "out is not C's type")
-        ld = _row_stride(C) if ldc is None else ldc
-        _check(fn, M == 0 or (M - 1) * ld + c_off + w.rows <= (C.shape[0] - 1) * C.stride(0) + C.shape[1], "C is too small")
-    _call(fn, w.handle, a8.data_ptr(), asc.data_ptr(), M, Ms, C.data_ptr(), _dtype(C.dtype), ld, c_off, accumulate,
-          None if ws is None else ws.data_ptr(), 0 if ws is None else ws.numel(), _stream(stream))
+        _check_rows(fn, "C", C, 2, dev)
+        if out is not None and out != C.dtype:
+            _refuse(fn, f"out {out} is not C's type")
+        if ldc is None:
+            ldc = _row_stride(C)
+        if M > 0 and (M - 1) * ldc + c_off + w.rows > (C.shape[0] - 1) * C.stride(0) + C.shape[1]:
+            _refuse(fn, f"C {tuple(C.shape)} does not hold {M} rows of {w.rows} from column {c_off} on")
+    if ws is None:
+        ws_ptr, ws_bytes = None, 0
+    else:
+        _check_rows(fn, "ws", ws, 1, dev)
+        ws_ptr, ws_bytes = ws.data_ptr(), ws.numel() * ws.element_size()
+    _call(fn, w.handle, a8.data_ptr(), asc.data_ptr(), M, Ms, C.data_ptr(), _dtype(C.dtype), ldc, c_off, accumulate,
+          ws_ptr, ws_bytes, _stream(stream))
     return C
 
 
@@ -495,45 +517,62 @@ def qk_norm_rope(x, HQ, HK, D, pos, inv_freq, wq=None, wk=None, eps=1e-6, adjace
     unless given), or writes the q and k given (matrices [T, HQ * D] or [T, HQ, D] of any row stride; views of x for in place)."""
     import torch
     fn = "qmatmul_qk_norm_rope"
-    _check_rows(fn, 2, x=x)
-    _check_rows(fn, 1, inv_freq=inv_freq, wq=wq, wk=wk)
-    T = x.shape[0]
-    p = pos if pos.dim() == 2 else pos[None]
-    _check_rows(fn, 2, pos=p)
-    _check(fn, pos.dtype == torch.int32 and p.shape[1] == T, f"pos {tuple(pos.shape)} {pos.dtype}: int32, one column for each of {T} tokens")
-    _check(fn, inv_freq.dtype == torch.float32, "inv_freq: float32")
+    dev = _current_gpu()
+    _check_rows(fn, "x", x, 2, dev)
+    _check_rows(fn, "inv_freq", inv_freq, 1, dev)
+    T, width = x.shape
+    axes, half = 1, inv_freq.numel()
+    _check_rows(fn, "pos", pos, None, dev)
+    if pos.dim() == 2:
+        axes = pos.shape[0]
+    if pos.dtype != torch.int32 or pos.dim() not in (1, 2) or pos.shape[-1] != T:
+        _refuse(fn, f"pos {tuple(pos.shape)} {pos.dtype}: int32, one column for each of {T} tokens")
+    if inv_freq.dtype != torch.float32:
+        _refuse(fn, f"inv_freq {inv_freq.dtype}: float32")
     for w in (wq, wk):
-        _check(fn, w is None or (w.dtype == torch.float32 and w.numel() == D), "wq and wk: float32 [D]")
-    axes, half = p.shape[0], inv_freq.numel()
-    sec = [half] if sections is None else [int(n) for n in sections]
-    _check(fn, len(sec) == axes and axes <= 4 and sum(sec) == half, f"sections {sec}: one for each of {axes} axes, their sum {half}")
-    q_hs = D if q_hs is None else q_hs
-    k_hs = D if k_hs is None else k_hs
-    k_off = q_off + HQ * q_hs if k_off is None else k_off
-    ldx = _row_stride(x)
-    _check(fn, T == 0 or x.shape[1] >= max(q_off + (HQ - 1) * q_hs + D if HQ else 0, k_off + (HK - 1) * k_hs + D if HK else 0),
-           f"rows of {x.shape[1]} elements do not hold the heads")
-    otype = out if out is not None else q.dtype if q is not None else k.dtype if k is not None else x.dtype
-    res, ptrs, lds = [], [], []
-    for t, H in ((q, HQ), (k, HK)):
-        if t is None:
-            t = torch.empty((T, H, D), dtype=otype, device=x.device)
-            ld = H * D
-        else:
-            _check_rows(fn, None, output=t)
-            _check(fn, t.dtype == otype and t.dim() in (2, 3) and t.shape[0] == T
-                   and (t.shape[1] == H * D if t.dim() == 2 else tuple(t.shape[1:]) == (H, D) and (H < 2 or t.stride(1) == D)),
-                   f"output {tuple(t.shape)} {t.dtype}: [T, {H} * {D}] of {otype}")
-            ld = t.stride(0) if T > 1 else max(H * D, t.stride(0))
-        res.append(t)
-        ptrs.append(t.data_ptr() if t.numel() else None)
-        lds.append(ld)
-    rope = QmRope(2 * half, 1 if adjacent else 0, axes, 1 if turns else 0, (_I * 4)(*sec), scale)
-    _call(fn, x.data_ptr(), _dtype(x.dtype), ldx, T, D, q_off, q_hs, HQ, k_off, k_hs, HK,
+        if w is not None:
+            _check_rows(fn, "wq or wk", w, 1, dev)
+            if w.dtype != torch.float32 or w.numel() != D:
+                _refuse(fn, f"wq or wk {tuple(w.shape)} {w.dtype}: float32 [{D}]")
+    rope = QmRope(2 * half, adjacent, axes, turns, scale=scale)
+    if sections is None:
+        sections = (half,)
+    if len(sections) != axes or axes > 4 or sum(sections) != half:
+        _refuse(fn, f"sections {sections}: one for each of {axes} axes (at most 4), their sum {half}")
+    for i, n in enumerate(sections):
+        rope.sections[i] = n
+    if q_hs is None:
+        q_hs = D
+    if k_hs is None:
+        k_hs = D
+    if k_off is None:
+        k_off = q_off + HQ * q_hs
+    if (HQ and q_off + (HQ - 1) * q_hs + D > width) or (HK and k_off + (HK - 1) * k_hs + D > width):
+        _refuse(fn, f"rows of {width} elements do not hold the heads")
+    if out is None:
+        out = q.dtype if q is not None else k.dtype if k is not None else x.dtype
+    if q is None:
+        q, ldq = torch.empty((T, HQ, D), dtype=out, device=x.device), HQ * D
+    else:
+        ldq = _head_rows(fn, "q", q, T, HQ, D, out, dev)
+    if k is None:
+        k, ldk = torch.empty((T, HK, D), dtype=out, device=x.device), HK * D
+    else:
+        ldk = _head_rows(fn, "k", k, T, HK, D, out, dev)
+    _call(fn, x.data_ptr(), _dtype(x.dtype), _row_stride(x), T, D, q_off, q_hs, HQ, k_off, k_hs, HK,
           None if wq is None else wq.data_ptr(), None if wk is None else wk.data_ptr(), eps, ctypes.byref(rope),
-          p.data_ptr(), p.stride(0) if axes > 1 else T, inv_freq.data_ptr(), ptrs[0], ptrs[1], _dtype(otype), lds[0], lds[1],
-          _stream(stream))
-    return res[0], res[1]
+          pos.data_ptr(), pos.stride(0) if axes > 1 else T, inv_freq.data_ptr(), q.data_ptr(), k.data_ptr(), _dtype(out),
+          ldq, ldk, _stream(stream))
+    return q, k
+
+
+def _head_rows(fn, name, t, T, H, D, dtype, dev):
+    """The row stride of an output given by the caller: [T, H * D] or [T, H, D], heads next to each other."""
+    _check_rows(fn, name, t, None, dev)
+    if (t.dtype != dtype or t.dim() not in (2, 3) or t.shape[0] != T
+            or (t.shape[1] != H * D if t.dim() == 2 else tuple(t.shape[1:]) != (H, D) or (H > 1 and t.stride(1) != D))):
+        _refuse(fn, f"{name} {tuple(t.shape)} {t.dtype}: [{T}, {H} * {D}] of {dtype}")
+    return t.stride(0) if T > 1 else max(H * D, t.stride(0))
 
 
 class GgufTensor:
