@@ -88,8 +88,10 @@ __global__ __launch_bounds__(64 * W) void fp8_few_kernel(Fp8GemmArgs a) {
 #pragma unroll
     for (int f = 0; f < RT; ++f) {
       const uint8_t* p = wp + f * frag_stride + (size_t)b * kFragBytes;
-      w[f][0] = __builtin_nontemporal_load((const v4i*)p);
-      w[f][1] = __builtin_nontemporal_load((const v4i*)(p + 1024));
+      // (streaming loads are 5 % faster where nothing is cached, 8 weights of 17408 x 5120 in turn 20.1 us against 21.4, and 10 to 20 %
+      //  slower where the last-level cache holds part of them, 2 in turn 21.5 against 19.4)
+      w[f][0] = *(const v4i*)p;
+      w[f][1] = *(const v4i*)(p + 1024);
     }
   };
   // U blocks' weights are under way at once

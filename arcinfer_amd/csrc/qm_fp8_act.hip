@@ -9,10 +9,16 @@ namespace {
 constexpr float kTop = 448.0f;        // the largest e4m3 value
 constexpr float kTiny = 0x1p-100f;    // blocks below it are zeros: 448 / amax stays finite and amax / 448 normal
 
-__device__ __forceinline__ float wave16_max(float v) {
-#pragma unroll
-  for (int o = 8; o; o >>= 1) v = fmaxf(v, __shfl_xor(v, o, 16));
-  return v;
+// The largest of 16 neighbouring lanes, in each of them (rotations within a row of 16 lanes: no LDS)
+template <int N>
+__device__ __forceinline__ float rotated16(float v) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), 0x120 + N, 0xF, 0xF, false));
+}
+__device__ __forceinline__ float max16(float v) {
+  v = fmaxf(v, rotated16<8>(v));
+  v = fmaxf(v, rotated16<4>(v));
+  v = fmaxf(v, rotated16<2>(v));
+  return fmaxf(v, rotated16<1>(v));
 }
 
 // Eight elements of a row from element i on; those past K are zero. VEC: K % 8 == 0 and 16-byte aligned rows.
@@ -45,7 +51,7 @@ __device__ __forceinline__ void quant16(const float v[8], bool store, int m, int
   float amax = 0.0f;
 #pragma unroll
   for (int j = 0; j < 8; ++j) amax = fmaxf(amax, fabsf(v[j]));
-  amax = wave16_max(amax);
+  amax = max16(amax);
   const float inv = amax >= kTiny ? kTop / amax : 0.0f;
   if (!store) return;
   int lo = __builtin_amdgcn_cvt_pk_fp8_f32(v[0] * inv, v[1] * inv, 0, false);
@@ -56,20 +62,35 @@ __device__ __forceinline__ void quant16(const float v[8], bool store, int m, int
   if ((threadIdx.x & 15) == 0) asc[(size_t)(at >> 7) * M_stride + m] = amax >= kTiny ? amax / kTop : 0.0f;
 }
 
-__device__ __forceinline__ float silu(float x) { return x / (1.0f + expf(-x)); }
-__device__ __forceinline__ float gelu_tanh(float x) {
-  return 0.5f * x * (1.0f + tanhf(0.7978845608f * (x + 0.044715f * x * x * x)));
+// e^x = 2^(x log2 e), the product in two parts: the exponent's rounding would cost |x| / 2 steps of the result. Within 2 steps.
+__device__ __forceinline__ float exp_fast(float x) {
+  constexpr float kHi = 1.44269502f, kLo = 1.92596303e-8f;  // log2 e
+  const float h = x * kHi, l = fmaf(x, kLo, fmaf(x, kHi, -h));
+  const float e = __builtin_amdgcn_exp2f(h);
+  return fmaf(e, l * 0.693147181f, e);
 }
+// x / (1 + e^-z): silu for z = x. The quotient by a reciprocal and one correction, within 2 steps (the correctly rounded division and expf
+// took more of the vector pipe than the rows take of HBM: 2048 rows of 17408 in bf16 45.9 us against 40.7). The exponent is kept where
+// e and the sum are finite: e^83 is over 2^119, what lies beyond is held as zero. A NaN of x stays one.
+__device__ __forceinline__ float gated(float x, float z) {
+  const float d = 1.0f + exp_fast(fminf(fmaxf(-z, -104.0f), 83.0f));
+  const float r = __builtin_amdgcn_rcpf(d), q = x * r;
+  return fmaf(fmaf(-d, q, x), r, q);
+}
+__device__ __forceinline__ float silu(float x) { return gated(x, x); }
+// 0.5 x (1 + tanh z), z = sqrt(2 / pi) (x + 0.044715 x^3): 1 + tanh z is 2 / (1 + e^-2z)
+__device__ __forceinline__ float gelu_tanh(float x) { return gated(x, 1.59576912f * fmaf(0.044715f * x * x, x, x)); }
 
 enum : int { ROWS = 0, SILU = 1, GELU = 2 };
 
 }  // namespace
 
-// One work-group per row and 2048 values.
+// One work-group per row and 2048 values, a row's work-groups next to each other.
 template <typename T, bool VEC, int OP>
 __global__ __launch_bounds__(256) void fp8_rows_kernel(const T* __restrict__ x, int ldx, int K, int M, int M_stride,
                                                        uint8_t* __restrict__ a8, float* __restrict__ asc) {
-  const int m = blockIdx.x, kp = (K + 127) / 128 * 128, at = 2048 * blockIdx.y + 8 * threadIdx.x;
+  const unsigned chunks = (unsigned)(K + 2047) / 2048;
+  const int m = (int)(blockIdx.x / chunks), kp = (K + 127) / 128 * 128, at = 2048 * (int)(blockIdx.x % chunks) + 8 * threadIdx.x;
   const T* r = x + (size_t)m * ldx;
   float v[8] = {};
   if (m < M) {
@@ -156,7 +177,7 @@ bool rows_aligned(const void* p, int ld, int K, int size) {
 
 template <typename T>
 hipError_t rows_of(const T* x, int ldx, int K, int M, int M_stride, int op, uint8_t* a8, float* asc, hipStream_t s) {
-  const dim3 grid(M_stride, (K + 2047) / 2048);
+  const unsigned grid = (unsigned)M_stride * ((K + 2047) / 2048);
   const bool vec = rows_aligned(x, ldx, K, sizeof(T)) && (op == ROWS || (size_t)K * sizeof(T) % 16 == 0);
 #define QM_F8R(OP) \
   if (vec) fp8_rows_kernel<T, true, OP><<<grid, 256, 0, s>>>(x, ldx, K, M, M_stride, a8, asc); \

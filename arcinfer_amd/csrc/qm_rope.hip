@@ -42,11 +42,117 @@ __device__ __forceinline__ void storev(T* p, const float* v) {
 
 }  // namespace
 
-// U: chunks of a lane (1 but for V = 1). tokens: of a work-group. lanes: of a head.
+// One head of one token, as the lanes of a group hold it: U chunks of 2 V elements a lane
 template <typename TI, typename TO, int V, int U>
+struct Head {
+  typedef TI vt __attribute__((ext_vector_type(V)));
+  vt x0[U], x1[U];  // (as loaded: a head on its way costs half the registers that its f32 values would)
+  const float* w;
+  TO* y;
+  int t;  // the token, from the work-group's first on
+  bool live;
+
+  __device__ __forceinline__ static int lo_at(const RopeArgs& a, int k, int turned) { return k < turned && !a.adjacent ? V * k : 2 * V * k; }
+  __device__ __forceinline__ static int hi_at(const RopeArgs& a, int k, int turned) {
+    return k < turned && !a.adjacent ? (a.rot >> 1) + V * k : 2 * V * k + V;
+  }
+
+  __device__ __forceinline__ void load(const RopeArgs& a, int u, int units, int t0, int sub, int lanes, int chunks, int turned) {
+    const int H = a.HQ + a.HK;
+    live = u < units;
+    t = live ? u / H : 0;
+    const int hh = live ? u - t * H : 0, h = hh < a.HQ ? hh : hh - a.HQ;
+    const bool is_q = hh < a.HQ;
+    const size_t row = (size_t)(t0 + t);
+    w = is_q ? a.wq : a.wk;
+    const TI* x = (const TI*)a.x + row * a.ldx + (is_q ? a.q_off + (size_t)h * a.q_hs : a.k_off + (size_t)h * a.k_hs);
+    y = (is_q ? (TO*)a.q + row * a.ldq : (TO*)a.k + row * a.ldk) + (size_t)h * a.D;
+#pragma unroll
+    for (int c = 0; c < U; ++c) {
+      const int k = sub + c * lanes;
+      x0[c] = x1[c] = vt(0);
+      if (live && k < chunks) {
+        x0[c] = *(const vt*)(x + lo_at(a, k, turned));
+        x1[c] = *(const vt*)(x + hi_at(a, k, turned));
+      }
+    }
+  }
+
+  __device__ __forceinline__ void finish(const RopeArgs& a, const float2* table, int sub, int lanes, int chunks, int turned) {
+    float v[U][2 * V];
+#pragma unroll
+    for (int c = 0; c < U; ++c)
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        v[c][i] = (float)x0[c][i];
+        v[c][V + i] = (float)x1[c][i];
+      }
+    float n = 1.0f;
+    if (w) {  // (one head's lanes take the same way; the reduction stays within them)
+      float ss = 0.0f;
+#pragma unroll
+      for (int c = 0; c < U; ++c)
+#pragma unroll
+        for (int i = 0; i < 2 * V; ++i) ss = fmaf(v[c][i], v[c][i], ss);
+      for (int o = lanes >> 1; o; o >>= 1) ss += __shfl_xor(ss, o);
+      n = 1.0f / sqrtf(ss / (float)a.D + a.eps);
+    }
+#pragma unroll
+    for (int c = 0; c < U; ++c) {
+      const int k = sub + c * lanes;
+      if (!live || k >= chunks) continue;
+      const int lo = lo_at(a, k, turned), hi = hi_at(a, k, turned);
+      if (w) {
+        float wv[2 * V];
+        loadv<float, V>(w + lo, wv);
+        loadv<float, V>(w + hi, wv + V);
+#pragma unroll
+        for (int i = 0; i < 2 * V; ++i) v[c][i] = v[c][i] * n * wv[i];
+      }
+      float r[2 * V];
+      if (k < turned) {
+        const float2* cs = table + t * (a.rot >> 1) + V * k;
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          // (both ways are written out: the pairing is the launch's, an index of it would put v into memory)
+          const float e = a.adjacent ? v[c][2 * i] : v[c][i], f = a.adjacent ? v[c][2 * i + 1] : v[c][V + i];
+          const float y0 = e * cs[i].x - f * cs[i].y, y1 = f * cs[i].x + e * cs[i].y;
+          r[i] = y0;
+          r[V + i] = y1;
+        }
+        if (a.adjacent) {
+          float z[2 * V];
+#pragma unroll
+          for (int i = 0; i < V; ++i) {
+            z[2 * i] = r[i];
+            z[2 * i + 1] = r[V + i];
+          }
+#pragma unroll
+          for (int i = 0; i < 2 * V; ++i) r[i] = z[i];
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < 2 * V; ++i) r[i] = v[c][i];
+      }
+      storev<TO, V>(y + lo, r);
+      storev<TO, V>(y + hi, r + V);
+    }
+  }
+};
+
+// tokens: of a work-group. lanes: of a head. A group of lanes holds two batches of B heads: one is on its way while the other is
+// finished, and the first while the table is computed.
+template <typename TI, typename TO, int V, int U, int B>
 __global__ __launch_bounds__(256) void qk_norm_rope_kernel(RopeArgs a, int tokens, int lanes) {
   __shared__ float2 table[kTable];
   const int half = a.rot >> 1, t0 = blockIdx.x * tokens, nt = min(tokens, a.T - t0);
+  const int group = threadIdx.x / lanes, sub = threadIdx.x & (lanes - 1), groups = 256 / lanes;
+  const int chunks = a.D / (2 * V), turned = half / V;
+  const int units = nt * (a.HQ + a.HK), step = groups * (int)gridDim.y;
+  Head<TI, TO, V, U> now[B], next[B];
+  int u = (int)blockIdx.y * groups;
+#pragma unroll
+  for (int i = 0; i < B; ++i) now[i].load(a, u + i * step + group, units, t0, sub, lanes, chunks, turned);
   for (int e = threadIdx.x; e < nt * half; e += 256) {
     const int t = e / half, i = e - t * half;
     // the product of a 31-bit position and a 24-bit frequency is (nearly) exact in f64, and so is what is left of whole turns
@@ -56,92 +162,52 @@ __global__ __launch_bounds__(256) void qk_norm_rope_kernel(RopeArgs a, int token
     table[e] = make_float2(cs * a.scale, sn * a.scale);
   }
   __syncthreads();
-  const int H = a.HQ + a.HK, group = threadIdx.x / lanes, sub = threadIdx.x & (lanes - 1), groups = 256 / lanes;
-  const int chunks = a.D / (2 * V), turned = half / V;
-  const int units = nt * H, step = groups * gridDim.y;
-  for (int u0 = blockIdx.y * groups; u0 < units; u0 += step) {
-    const int u = u0 + group;
-    const bool live = u < units;
-    const int t = live ? u / H : 0, hh = live ? u - t * H : 0;
-    const bool is_q = hh < a.HQ;
-    const int h = is_q ? hh : hh - a.HQ;
-    const float* w = is_q ? a.wq : a.wk;
-    const TI* x = (const TI*)a.x + (size_t)(t0 + t) * a.ldx + (is_q ? a.q_off + (size_t)h * a.q_hs : a.k_off + (size_t)h * a.k_hs);
-    TO* y = is_q ? (TO*)a.q + (size_t)(t0 + t) * a.ldq + (size_t)h * a.D : (TO*)a.k + (size_t)(t0 + t) * a.ldk + (size_t)h * a.D;
-    float v[U][2 * V];
-    int lo[U], hi[U];
-    float ss = 0.0f;
+  while (u < units) {
+    u += B * step;
+    if (u < units) {
 #pragma unroll
-    for (int c = 0; c < U; ++c) {
-      const int k = sub + c * lanes;
-      const bool on = live && k < chunks;
-      lo[c] = k < turned && !a.adjacent ? V * k : 2 * V * k;
-      hi[c] = k < turned && !a.adjacent ? half + V * k : 2 * V * k + V;
-#pragma unroll
-      for (int i = 0; i < 2 * V; ++i) v[c][i] = 0.0f;
-      if (on) {
-        loadv<TI, V>(x + lo[c], v[c]);
-        loadv<TI, V>(x + hi[c], v[c] + V);
-      }
-#pragma unroll
-      for (int i = 0; i < 2 * V; ++i) ss = fmaf(v[c][i], v[c][i], ss);
-    }
-    float n = 1.0f;
-    if (w) {  // (one head's lanes take the same way; the reduction stays within them)
-      for (int o = lanes >> 1; o; o >>= 1) ss += __shfl_xor(ss, o);
-      n = 1.0f / sqrtf(ss / (float)a.D + a.eps);
+      for (int i = 0; i < B; ++i) next[i].load(a, u + i * step + group, units, t0, sub, lanes, chunks, turned);
     }
 #pragma unroll
-    for (int c = 0; c < U; ++c) {
-      const int k = sub + c * lanes;
-      if (!live || k >= chunks) continue;
-      if (w) {
-        float wv[2 * V];
-        loadv<float, V>(w + lo[c], wv);
-        loadv<float, V>(w + hi[c], wv + V);
+    for (int i = 0; i < B; ++i) now[i].finish(a, table, sub, lanes, chunks, turned);
+    if (u < units) {
 #pragma unroll
-        for (int i = 0; i < 2 * V; ++i) v[c][i] = v[c][i] * n * wv[i];
-      }
-      float r[2 * V];
-      if (k < turned) {
-        const float2* cs = table + t * half + V * k;
-#pragma unroll
-        for (int i = 0; i < V; ++i) {
-          const int p = a.adjacent ? 2 * i : i, q = a.adjacent ? 2 * i + 1 : V + i;
-          r[p] = v[c][p] * cs[i].x - v[c][q] * cs[i].y;
-          r[q] = v[c][q] * cs[i].x + v[c][p] * cs[i].y;
-        }
-      } else {
-#pragma unroll
-        for (int i = 0; i < 2 * V; ++i) r[i] = v[c][i];
-      }
-      storev<TO, V>(y + lo[c], r);
-      storev<TO, V>(y + hi[c], r + V);
+      for (int i = 0; i < B; ++i) now[i] = next[i];
     }
   }
 }
 
 namespace {
 
+// eight at a time where both sides are of 16 bits (16 bytes a load and store)
+template <typename TI, typename TO>
+constexpr bool kRopeV8 = sizeof(TI) == 2 && sizeof(TO) == 2;
+
 template <typename TI, typename TO>
 hipError_t rope_of(const RopeArgs& a, hipStream_t s) {
-  // four elements at a time where the pairs' vectors and every row, offset and stride allow it
-  const uintptr_t vi = 4 * sizeof(TI), vo = 4 * sizeof(TO);
-  bool vec = a.D % 8 == 0 && a.rot % 8 == 0 && (uintptr_t)a.x % vi == 0 && a.ldx % 4 == 0;
-  if (a.HQ) vec = vec && a.q_off % 4 == 0 && a.q_hs % 4 == 0 && a.ldq % 4 == 0 && (uintptr_t)a.q % vo == 0 && (uintptr_t)a.wq % 16 == 0;
-  if (a.HK) vec = vec && a.k_off % 4 == 0 && a.k_hs % 4 == 0 && a.ldk % 4 == 0 && (uintptr_t)a.k % vo == 0 && (uintptr_t)a.wk % 16 == 0;
-  const int chunks = a.D / (vec ? 8 : 2), half = a.rot / 2 > 0 ? a.rot / 2 : 1;
+  // V elements at a time where the pairs' vectors and every row, offset and stride allow it
+  const auto fits = [&](int v) {
+    const uintptr_t vi = v * sizeof(TI) < 16 ? v * sizeof(TI) : 16, vo = v * sizeof(TO) < 16 ? v * sizeof(TO) : 16;
+    bool ok = a.D % (2 * v) == 0 && a.rot % (2 * v) == 0 && (uintptr_t)a.x % vi == 0 && a.ldx % v == 0;
+    if (a.HQ) ok = ok && a.q_off % v == 0 && a.q_hs % v == 0 && a.ldq % v == 0 && (uintptr_t)a.q % vo == 0 && (uintptr_t)a.wq % 16 == 0;
+    if (a.HK) ok = ok && a.k_off % v == 0 && a.k_hs % v == 0 && a.ldk % v == 0 && (uintptr_t)a.k % vo == 0 && (uintptr_t)a.wk % 16 == 0;
+    return ok;
+  };
+  const int v = kRopeV8<TI, TO> && fits(8) ? 8 : fits(4) ? 4 : 1;
+  const int chunks = a.D / (2 * v), half = a.rot / 2 > 0 ? a.rot / 2 : 1;
   int lanes = 1;
   while (lanes < chunks && lanes < 64) lanes *= 2;
   int tokens = kTable / half < 4 ? kTable / half : 4;
   if (a.T < 1024) tokens = 1;
   const unsigned gx = (unsigned)((a.T + tokens - 1) / tokens);
   const unsigned iters = (unsigned)((tokens * (a.HQ + a.HK) * lanes + 255) / 256);
-  unsigned gy = gx >= 512 ? 1 : (512 + gx - 1) / gx;  // few tokens: their heads over several work-groups
+  unsigned gy = gx >= 1024 ? 1 : (1024 + gx - 1) / gx;  // few tokens: their heads over several work-groups
   if (gy > iters) gy = iters;
-  if (vec) qk_norm_rope_kernel<TI, TO, 4, 1><<<dim3(gx, gy), 256, 0, s>>>(a, tokens, lanes);
-  else if (chunks <= 64) qk_norm_rope_kernel<TI, TO, 1, 1><<<dim3(gx, gy), 256, 0, s>>>(a, tokens, lanes);
-  else qk_norm_rope_kernel<TI, TO, 1, 4><<<dim3(gx, gy), 256, 0, s>>>(a, tokens, lanes);
+  const dim3 grid(gx, gy);
+  if (v == 8) qk_norm_rope_kernel<TI, TO, 8, 1, 2><<<grid, 256, 0, s>>>(a, tokens, lanes);
+  else if (v == 4) qk_norm_rope_kernel<TI, TO, 4, 1, 2><<<grid, 256, 0, s>>>(a, tokens, lanes);
+  else if (chunks <= 64) qk_norm_rope_kernel<TI, TO, 1, 1, 1><<<grid, 256, 0, s>>>(a, tokens, lanes);
+  else qk_norm_rope_kernel<TI, TO, 1, 4, 1><<<grid, 256, 0, s>>>(a, tokens, lanes);
   return hipGetLastError();
 }
 

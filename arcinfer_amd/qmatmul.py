@@ -121,11 +121,20 @@ def _ptr(t):
     return None if t is None else ctypes.c_void_p(t.data_ptr())
 
 
+_raw_stream = None  # torch's current stream of a device as a number, without the Stream object (2.5 us a call)
+
+
 def _stream(stream):
+    global _raw_stream
     if stream is not None:
         return ctypes.c_void_p(stream)
-    import torch
-    return ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
+    if _raw_stream is None:
+        import torch
+        torch.cuda.current_stream()  # (starts torch's GPU side)
+        raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+        _raw_stream = ((lambda: raw(torch.cuda.current_device())) if raw is not None
+                       else (lambda: torch.cuda.current_stream().cuda_stream))
+    return ctypes.c_void_p(_raw_stream())
 
 
 class QWeight:
@@ -534,13 +543,11 @@ def qk_norm_rope(x, HQ, HK, D, pos, inv_freq, wq=None, wk=None, eps=1e-6, adjace
             _check_rows(fn, "wq or wk", w, 1, dev)
             if w.dtype != torch.float32 or w.numel() != D:
                 _refuse(fn, f"wq or wk {tuple(w.shape)} {w.dtype}: float32 [{D}]")
-    rope = QmRope(2 * half, adjacent, axes, turns, scale=scale)
     if sections is None:
         sections = (half,)
     if len(sections) != axes or axes > 4 or sum(sections) != half:
         _refuse(fn, f"sections {sections}: one for each of {axes} axes (at most 4), their sum {half}")
-    for i, n in enumerate(sections):
-        rope.sections[i] = n
+    rope = QmRope(2 * half, adjacent, axes, turns, tuple(sections), scale)
     if q_hs is None:
         q_hs = D
     if k_hs is None:

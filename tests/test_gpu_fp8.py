@@ -248,6 +248,27 @@ def test_swiglu(qm, dev, gelu, M, Ms, F, x_type):
     assert not a8.cpu().view(torch.uint8)[M:].any() and not a8.cpu().view(torch.uint8)[:, F:].any()
 
 
+@pytest.mark.parametrize("gelu", [False, True])
+def test_swiglu_extremes(qm, dev, gelu):
+    """Gates far out of the exponential's range: the gate itself, or nothing; an infinity or a NaN stays in its row."""
+    gu = torch.ones((5, 512))
+    gu[0, :4] = torch.tensor([1e30, -1e30, 90.0, -90.0])
+    gu[1, 0], gu[2, 0], gu[3, 0], gu[4, 256] = float("inf"), float("-inf"), float("nan"), float("nan")
+    a8, asc = qm.swiglu_fp8(gu.to(dev), 256, gelu=gelu)
+    v, s = P.value(a8.cpu()), asc.cpu().double()
+    assert v[0, 0] == 448 and abs(s[0, 0] * 448 / 1e30 - 1) < 1e-6 and not v[0, 1:128].any()
+    assert torch.isfinite(v[:, 128:]).all() and torch.isfinite(s[1]).all()
+    ones = qm.Fp8Weight(torch.full((16, 256), 0x38, dtype=torch.uint8, device=dev), torch.ones((1, 2), device=dev))
+    C = qm.gemm_fp8(ones, a8, asc).cpu()
+    assert torch.isfinite(C[0]).all() and not torch.isfinite(C[1]).any() and torch.isnan(C[3]).all() and torch.isnan(C[4]).all()
+    gu = torch.full((1, 256), 90.0)  # (a block of far gates alone: what is left of -90 is below 2^-100)
+    gu[0, 64:128] = -90.0
+    a8, asc = qm.swiglu_fp8(gu.to(dev), 128, gelu=gelu)
+    v = P.value(a8.cpu())
+    assert bool((v[0, :64] == 448).all()) and not v[0, 64:].any()
+    ones.release()
+
+
 def test_ffn_run(qm, dev):
     """Norm, gate and up, gating, down, as an FFN layer uses them, with C in bf16 and f32; each product against 64 bits on the
     activations that it met."""
