@@ -842,7 +842,7 @@ static int check_fp8_rows(const char* fn, const void* x, int xtype, int ldx, lon
                           const uint8_t* a8, const float* asc) {
   if (!x || !a8 || !asc) return fail(QM_ERR_ARG, "%s: null pointer", fn);
   if (!dtype_ok(xtype)) return fail(QM_ERR_TYPE, "%s: input type %d (QM_F32, QM_F16 or QM_BF16)", fn, xtype);
-  if (K < 1 || K > 0x3fffff00 || M < 0 || M_stride < 1 || M > M_stride || ldx < width)
+  if (K < 1 || K > 1 << 24 || M < 0 || M_stride < 1 || M > M_stride || ldx < width)
     return fail(QM_ERR_SHAPE, "%s: M %d, M_stride %d, K %d, row stride %d", fn, M, M_stride, K, ldx);
   if (!aligned(x, dtype_size(xtype)) || !aligned(a8, 16) || !aligned(asc, 4))
     return fail(QM_ERR_ARG, "%s: the input must be aligned to its type, a8 to 16 bytes, asc to 4", fn);

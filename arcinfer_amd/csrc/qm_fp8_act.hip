@@ -140,6 +140,7 @@ __global__ __launch_bounds__(256) void fp8_rmsnorm_kernel(const T* __restrict__ 
   __syncthreads();
   ss = ((red[0] + red[1]) + red[2]) + red[3];
   const float n = 1.0f / sqrtf(ss / (float)K + eps);
+  const bool h_vec = VEC && h && (((uintptr_t)h >> 2 | (uintptr_t)ldh) & 3) == 0;
   const auto finish = [&](const float xr[8], int p) {
     const int at = 2048 * p + 8 * threadIdx.x;
     float v[8] = {};
@@ -148,10 +149,16 @@ __global__ __launch_bounds__(256) void fp8_rmsnorm_kernel(const T* __restrict__ 
       load8<float, VEC>(w, at, K, wv);
 #pragma unroll
       for (int j = 0; j < 8; ++j) v[j] = xr[j] * n * wv[j];
-      if (h) {
+      float* hr = h + (size_t)m * ldh + at;
+      if (h_vec) {
+        if (at < K) {
+          *(float4*)hr = make_float4(v[0], v[1], v[2], v[3]);
+          *(float4*)(hr + 4) = make_float4(v[4], v[5], v[6], v[7]);
+        }
+      } else if (h) {
 #pragma unroll
         for (int j = 0; j < 8; ++j)
-          if (at + j < K) h[(size_t)m * ldh + at + j] = v[j];
+          if (at + j < K) hr[j] = v[j];
       }
     }
     quant16(v, at < kp, m, at, M_stride, kp, a8, asc);

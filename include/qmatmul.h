@@ -275,7 +275,7 @@ int qmatmul_release_fp8(qm_fp8_weight* w);
 /* Rows and K of a prepared weight as given, and the activation rows' length Kp (any output pointer may be NULL). */
 int qmatmul_fp8_info(const qm_fp8_weight* w, int* rows, int* K, int* Kp);
 
-/* Producers of e4m3 activations (layout above) from rows of xtype (qm_dtype), row stride ldx in elements, any K >= 1:
+/* Producers of e4m3 activations (layout above) from rows of xtype (qm_dtype), row stride ldx in elements, K from 1 to 2^24:
  * per 128 values y: amax = max |y|; asc = amax / 448; q = y * (448 / amax) rounded to the nearest e4m3, ties to even. A
  * block whose amax is below 2^-100 is zeros with scale 0. A NaN becomes e4m3's NaN (amax is that of the others); a block with
  * an infinity has the scale infinity: both make every product of their token NaN.

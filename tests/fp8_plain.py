@@ -28,7 +28,7 @@ def gemm(w8, wsc, a8, asc, M):
     neighbouring k could have."""
     N, K = w8.shape
     Kp = up(K, 128)
-    w = torch.zeros((N, Kp), dtype=torch.float64)
+    w = torch.zeros((N, Kp), dtype=torch.float64, device=w8.device)
     w[:, :K] = value(w8) * wsc.double().repeat_interleave(128, 0)[:N].repeat_interleave(128, 1)[:, :K]
     a = (value(a8)[:M].view(M, Kp // 128, 128) * asc.double()[:, :M].T[:, :, None]).reshape(M, Kp)
     top = lambda v: v.abs().view(len(v), Kp // 8, 8).amax(2)  # noqa: E731

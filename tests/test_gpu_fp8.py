@@ -23,7 +23,8 @@ def make(qm, dev, N, K, M, seed, Ms=None):
     a8[:, K:] = 0
     asc = torch.from_numpy(rng.uniform(0.5e-2, 2e-2, (Kp // 128, Ms)).astype(np.float32))
     w = qm.Fp8Weight(w8.to(dev), wsc.to(dev))
-    return w, a8.view(torch.float8_e4m3fn).to(dev), asc.to(dev), P.gemm(w8, wsc, a8, asc, M)
+    sums = P.gemm(*(t.to(dev) for t in (w8, wsc, a8, asc)), M)  # (in 64 bits there as well)
+    return w, a8.view(torch.float8_e4m3fn).to(dev), asc.to(dev), [t.cpu() for t in sums]
 
 
 def near(got, ref, bound):
@@ -38,8 +39,18 @@ SHAPES = [(1, 1, 1), (3, 40, 2), (64, 128, 1), (100, 128, 7), (128, 256, 16), (1
           (1153, 1536, 333), (512, 17408, 5), (448, 8200, 40), (2304, 2176, 260), (4096, 4096, 1), (768, 5120, 513)]
 
 
+# every variant that the choice can make: few tokens by one or two fragments and 4, 8 or 16 waves; tiles of 4 to 8 token tiles, whole
+# and in pieces, with one, two, three and no blocks left over of four, and more than 64 blocks
+VARIANTS = [(256, 915, 18), (261, 2123, 17), (4184, 133, 17), (4157, 937, 17), (260, 129, 38), (260, 912, 35), (4202, 132, 33),
+            (4207, 914, 33), (262, 934, 50), (4550, 940, 52), (8200, 2048, 16), (5000, 2100, 9), (258, 138, 1053), (266, 1679, 1143),
+            (1845, 2456, 65), (901, 3983, 69), (272, 9425, 49), (461, 10184, 69), (3530, 1808, 68), (36725, 131, 65),
+            (292, 2583, 2737), (8320, 2332, 68), (4200, 4041, 66), (35526, 130, 91), (33200, 141, 81), (262, 5405, 2699),
+            (35154, 135, 97), (36787, 130, 113), (5000, 520, 4100), (16638, 8536, 342),
+            (6440, 8581, 389), (4063, 9225, 324), (13391, 8435, 321), (14351, 8358, 524), (8420, 8327, 449), (1056, 8549, 2038)]
+
+
 @pytest.mark.parametrize("out", [F32, BF16, F16])
-@pytest.mark.parametrize("N,K,M", SHAPES)
+@pytest.mark.parametrize("N,K,M", SHAPES + VARIANTS)
 def test_product(qm, dev, N, K, M, out):
     w, a8, asc, (ref, *sums) = make(qm, dev, N, K, M, N + 3 * K + M)
     ws = qm.gemm_fp8_workspace(w, M)
