@@ -356,24 +356,33 @@ def _refuse(fn, what):
     raise QMatmulError(fn, 1, what)
 
 
+_torch = None  # (an import statement in a function is 0.3 us a call, and these calls take about ten)
+
+
 def _current_gpu():
-    import torch
-    return torch.cuda.current_device()
+    global _torch
+    if _torch is None:
+        import torch
+        _torch = torch
+    return _torch.cuda.current_device()
 
 
 def _check_rows(fn, name, t, dim, dev):
     """t is on GPU `dev`, of `dim` dimensions where dim is given, its last one contiguous."""
-    if not t.is_cuda or t.get_device() != dev:
+    if t.get_device() == dev and (not dim or t.dim() == dim) and t.stride(-1) == 1:
+        return
+    if t.get_device() != dev:
         _refuse(fn, f"{name} is on {t.device}, not on the current GPU")
     if dim and t.dim() != dim:
         _refuse(fn, f"{name} has {t.dim()} dimensions, not {dim}")
-    if t.stride(-1) != 1 and t.numel() and t.shape[-1] != 1:
+    if t.numel() and t.shape[-1] != 1:
         _refuse(fn, f"the last dimension of {name} is not contiguous")
 
 
 def _row_stride(t):
     """The row stride of a matrix in elements (of a single row, whose stride says nothing: at least its length)."""
-    return t.stride(0) if t.shape[0] > 1 else max(t.shape[1], t.stride(0))
+    ld = t.stride(0)
+    return ld if t.size(0) > 1 else max(t.size(1), ld)
 
 
 class Fp8Weight:
@@ -418,11 +427,9 @@ class Fp8Weight:
 
 
 def _out_fp8(x, M, K, M_stride):
-    import torch
     Ms = M if M_stride is None else M_stride
     Kp = (K + 127) // 128 * 128
-    return (Ms, torch.empty((Ms, Kp), dtype=torch.float8_e4m3fn, device=x.device),
-            torch.empty((Kp // 128, Ms), dtype=torch.float32, device=x.device))
+    return (Ms, x.new_empty((Ms, Kp), dtype=_torch.float8_e4m3fn), x.new_empty((Kp // 128, Ms), dtype=_torch.float32))
 
 
 def quantize_fp8(x, M_stride=None, stream=None):
@@ -438,16 +445,16 @@ def quantize_fp8(x, M_stride=None, stream=None):
 
 def rmsnorm_fp8(x, w, eps, M_stride=None, want_h=False, stream=None):
     """x [M, K], w float32 [K] -> (a8, asc, h float32 [M, K] or None)."""
-    import torch
     fn = "qmatmul_rmsnorm_fp8"
     dev = _current_gpu()
+    torch = _torch
     _check_rows(fn, "x", x, 2, dev)
     _check_rows(fn, "w", w, 1, dev)
     M, K = x.shape
     if w.dtype != torch.float32 or w.numel() != K:
         _refuse(fn, f"w {tuple(w.shape)} {w.dtype}: float32, one for each of {K} columns")
     Ms, a8, asc = _out_fp8(x, M, K, M_stride)
-    h = torch.empty((M, K), dtype=torch.float32, device=x.device) if want_h else None
+    h = x.new_empty((M, K), dtype=torch.float32) if want_h else None
     _call(fn, x.data_ptr(), _dtype(x.dtype), _row_stride(x), w.data_ptr(), K, M, Ms, eps, a8.data_ptr(), asc.data_ptr(),
           h.data_ptr() if want_h and M else None, K, _stream(stream))
     return a8, asc, h
@@ -476,9 +483,9 @@ def gemm_fp8_workspace(w, M):
 def gemm_fp8(w, a8, asc, M=None, C=None, ldc=None, c_off=0, accumulate=0, out=None, ws=None, stream=None):
     """C [M, rows] (op)= the product of activations (a8, asc) with an Fp8Weight. out: the type of a new C (float32 unless
     given). C: a matrix of its own row stride unless ldc is given."""
-    import torch
     fn = "qmatmul_gemm_fp8"
     dev = _current_gpu()
+    torch = _torch
     _check_rows(fn, "a8", a8, 2, dev)
     _check_rows(fn, "asc", asc, 2, dev)
     Ms, Kp = a8.shape
@@ -493,7 +500,7 @@ def gemm_fp8(w, a8, asc, M=None, C=None, ldc=None, c_off=0, accumulate=0, out=No
     if C is None:
         if accumulate or c_off or ldc is not None:
             _refuse(fn, "accumulate, c_off and ldc need a C")
-        C = torch.empty((M, w.rows), dtype=torch.float32 if out is None else out, device=a8.device)
+        C = asc.new_empty((M, w.rows), dtype=out)
         ldc = w.rows
     else:
         _check_rows(fn, "C", C, 2, dev)
@@ -524,9 +531,9 @@ def qk_norm_rope(x, HQ, HK, D, pos, inv_freq, wq=None, wk=None, eps=1e-6, adjace
     pos int32 [T], or [axes, T] with sections (pairs of each axis, behind one another or in turns); inv_freq float32
     [rot / 2]: its length says how many elements of a head turn. Returns (q [T, HQ, D], k [T, HK, D]) of type out (x's
     unless given), or writes the q and k given (matrices [T, HQ * D] or [T, HQ, D] of any row stride; views of x for in place)."""
-    import torch
     fn = "qmatmul_qk_norm_rope"
     dev = _current_gpu()
+    torch = _torch
     _check_rows(fn, "x", x, 2, dev)
     _check_rows(fn, "inv_freq", inv_freq, 1, dev)
     T, width = x.shape
@@ -559,11 +566,11 @@ def qk_norm_rope(x, HQ, HK, D, pos, inv_freq, wq=None, wk=None, eps=1e-6, adjace
     if out is None:
         out = q.dtype if q is not None else k.dtype if k is not None else x.dtype
     if q is None:
-        q, ldq = torch.empty((T, HQ, D), dtype=out, device=x.device), HQ * D
+        q, ldq = x.new_empty((T, HQ, D), dtype=out), HQ * D
     else:
         ldq = _head_rows(fn, "q", q, T, HQ, D, out, dev)
     if k is None:
-        k, ldk = torch.empty((T, HK, D), dtype=out, device=x.device), HK * D
+        k, ldk = x.new_empty((T, HK, D), dtype=out), HK * D
     else:
         ldk = _head_rows(fn, "k", k, T, HK, D, out, dev)
     _call(fn, x.data_ptr(), _dtype(x.dtype), _row_stride(x), T, D, q_off, q_hs, HQ, k_off, k_hs, HK,
