@@ -301,28 +301,27 @@ __global__ __launch_bounds__(256) void fp8_sum_kernel(Fp8GemmArgs a, int splits,
 namespace {
 
 template <int MT>
-void tile_of(const Fp8GemmArgs& a, int splits, hipStream_t s) {
+hipError_t tile_of(const Fp8GemmArgs& a, int splits, hipStream_t s) {
   const int tn = (a.w.rows + 255) / 256, tm = (a.M + 16 * MT - 1) / (16 * MT);
   const unsigned grid = (unsigned)((tn * tm * splits + 7) / 8 * 8);
-  if (a.ctype == DT_F32) {
-    if constexpr (MT <= 6) fp8_tile_kernel<MT, true><<<grid, 256, 0, s>>>(a, tn, tm, splits);
-  } else {
+  if (a.ctype != DT_F32) {
     fp8_tile_kernel<MT, false><<<grid, 256, 0, s>>>(a, tn, tm, splits);
+  } else if constexpr (MT <= 6) {
+    fp8_tile_kernel<MT, true><<<grid, 256, 0, s>>>(a, tn, tm, splits);
+  } else {
+    return hipErrorInvalidValue;
   }
+  return hipGetLastError();
 }
 
 }  // namespace
 
 hipError_t launch_fp8_tile(const Fp8GemmArgs& a, int mt, int splits, hipStream_t s) {
-  if (mt == 4) tile_of<4>(a, splits, s);
-  else if (mt == 5) tile_of<5>(a, splits, s);
-  else if (mt == 6) tile_of<6>(a, splits, s);
-  else if (mt == 7) tile_of<7>(a, splits, s);
-  else tile_of<8>(a, splits, s);
-  if (splits > 1) {
-    const int width = (a.w.rows + 63) / 64 * 64;
-    fp8_sum_kernel<<<dim3(a.M, (width + 2047) / 2048), 256, 0, s>>>(a, splits, width);
-  }
+  const hipError_t e = mt == 4 ? tile_of<4>(a, splits, s) : mt == 5 ? tile_of<5>(a, splits, s) : mt == 6 ? tile_of<6>(a, splits, s)
+                     : mt == 7 ? tile_of<7>(a, splits, s) : mt == 8 ? tile_of<8>(a, splits, s) : hipErrorInvalidValue;
+  if (e != hipSuccess || splits == 1) return e;
+  const int width = (a.w.rows + 63) / 64 * 64;
+  fp8_sum_kernel<<<dim3(a.M, (width + 2047) / 2048), 256, 0, s>>>(a, splits, width);
   return hipGetLastError();
 }
 

@@ -529,8 +529,9 @@ def qk_norm_rope(x, HQ, HK, D, pos, inv_freq, wq=None, wk=None, eps=1e-6, adjace
     """RMS norm (wq, wk float32 [D]; None: no norm) and rotation of the query and key heads in rows x [T, ldx]: query head h at
     column q_off + h * q_hs (D unless given), key head h at k_off + h * k_hs (k_off: behind the query heads unless given).
     pos int32 [T], or [axes, T] with sections (pairs of each axis, behind one another or in turns); inv_freq float32
-    [rot / 2]: its length says how many elements of a head turn. Returns (q [T, HQ, D], k [T, HK, D]) of type out (x's
-    unless given), or writes the q and k given (matrices [T, HQ * D] or [T, HQ, D] of any row stride; views of x for in place)."""
+    [rot / 2]: its length says how many elements of a head turn. Returns (q [T, HQ, D], k [T, HK, D]) of type out (that of
+    a given q or k, else x's), or writes the q and k given (matrices [T, HQ * D] or [T, HQ, D] of any row stride; views of x for
+    in place)."""
     fn = "qmatmul_qk_norm_rope"
     dev = _current_gpu()
     torch = _torch

@@ -168,6 +168,65 @@ def test_graphs_and_streams(qm, dev, N, K, M):
     w.release()
 
 
+def test_refusals(qm, dev):
+    """What a product refuses once there is a weight: nothing is written, and the next call is unharmed."""
+    N, K, M = 200, 300, 5
+    w, a8, asc, (ref, *sums) = make(qm, dev, N, K, M, 1)
+    C = torch.full((M, N), 7.0, device=dev)
+    lib, st = qm.load_library(), qm._stream(None)
+    call = lambda **k: lib.qmatmul_gemm_fp8(*{**dict(w=w.handle, a=a8.data_ptr(), s=asc.data_ptr(), M=M, Ms=16, C=C.data_ptr(), t=0,  # noqa: E731
+                                                     ldc=N, off=0, acc=0, ws=None, wsb=0, st=st), **k}.values())
+    assert call(M=0) == 0 and call(M=0, a=None, C=None) == 0
+    for bad in (dict(a=None), dict(s=None), dict(C=None), dict(acc=3), dict(acc=-1), dict(a=a8.data_ptr() + 8), dict(s=asc.data_ptr() + 2),
+                dict(C=C.data_ptr() + 2), dict(ws=C.data_ptr() + 16, wsb=1 << 20), dict(C=C.data_ptr() + 1, t=30)):
+        assert call(**bad) == 1, bad
+    for bad in (dict(M=-1), dict(M=17), dict(ldc=N - 1), dict(off=1), dict(off=-1), dict(off=2 ** 31 - 1, ldc=2 ** 31 - 1)):
+        assert call(**bad) == 2, bad
+    assert call(t=2) == 3 and call(t=14) == 3
+    for bad in (lambda: qm.gemm_fp8(w, a8[:, :256].contiguous(), asc), lambda: qm.gemm_fp8(w, a8, asc[:, :8].contiguous()),
+                lambda: qm.gemm_fp8(w, a8, asc.double()), lambda: qm.gemm_fp8(w, a8.float(), asc), lambda: qm.gemm_fp8(w, a8.cpu(), asc),
+                lambda: qm.gemm_fp8(w, a8[::2], asc[:, ::2]), lambda: qm.gemm_fp8(w, a8, asc, out=torch.int32),
+                lambda: qm.gemm_fp8(w, a8, asc, M=6, C=C), lambda: qm.gemm_fp8(w, a8, asc, M=M, C=C, out=BF16),
+                lambda: qm.gemm_fp8(w, a8, asc, M=M, accumulate=1), lambda: qm.gemm_fp8(w, a8, asc, M=M, C=C, c_off=1),
+                lambda: qm.gemm_fp8(w, a8, asc, M=M, C=C.t()), lambda: qm.gemm_fp8(w, a8, asc, M=17),
+                lambda: qm.Fp8Weight(torch.zeros((4, 4), device=dev), torch.ones((1, 1), device=dev)),
+                lambda: qm.Fp8Weight(torch.zeros((4, 200), dtype=torch.uint8, device=dev), torch.ones((1, 1), device=dev)),
+                lambda: qm.Fp8Weight(torch.zeros((4, 4), dtype=torch.uint8, device=dev), torch.ones((1, 1))),
+                lambda: qm.Fp8Weight(torch.zeros((4, 8), dtype=torch.uint8, device=dev)[:, ::2], torch.ones((1, 1), device=dev)),
+                lambda: qm.quantize_fp8(torch.zeros((4, 4), dtype=torch.float64, device=dev)), lambda: qm.quantize_fp8(torch.zeros((4, 4))),
+                lambda: qm.quantize_fp8(torch.zeros((4, 4), device=dev), M_stride=3), lambda: qm.quantize_fp8(torch.zeros((8, 4), device=dev).t()),
+                lambda: qm.rmsnorm_fp8(torch.zeros((4, 4), device=dev), torch.ones(5, device=dev), 1e-6),
+                lambda: qm.swiglu_fp8(torch.zeros((4, 7), device=dev), 4)):
+        with pytest.raises(qm.QMatmulError):
+            bad()
+    assert bool((C == 7.0).all())
+    near(qm.gemm_fp8(w, a8, asc, M=M, C=C), ref, P.gemm_bound(*sums, 3) + P.rounding(F32, ref))
+    w.release()
+    with pytest.raises(qm.QMatmulError):
+        qm.gemm_fp8(w, a8, asc, M=M, C=C)
+
+
+@pytest.mark.parametrize("N,K", [(512, 17408), (5184, 5120), (17408, 5120)])
+def test_workspaces_are_bounded_and_optional(qm, dev, N, K):
+    """Never more than 64 MiB; a larger or smaller one than asked for gives the bound's result too."""
+    wsc = torch.rand((P.up(N, 128) // 128, K // 128), device=dev) * 1e-3
+    w = qm.Fp8Weight(P.random_e4m3((N, K), 3).to(dev), wsc)
+    sizes = [qm.load_library().qmatmul_gemm_fp8_workspace_size(w.handle, M) for M in list(range(1, 200, 7)) + [333, 777, 4096, 100000]]
+    assert max(sizes) <= 64 << 20 and sizes[0] == 0 and any(sizes)
+    M = 70
+    a8 = P.random_e4m3((M, K), 4).to(dev).view(torch.float8_e4m3fn)
+    asc = torch.rand((K // 128, M), device=dev) * 1e-2
+    w8 = P.random_e4m3((N, K), 3).to(dev)
+    A = P.gemm(w8, wsc, a8, asc, M)[1]
+    need = qm.load_library().qmatmul_gemm_fp8_workspace_size(w.handle, M)
+    whole = qm.gemm_fp8(w, a8, asc)
+    for n in (need, 64 << 20, max(256, need - 256)):
+        C = qm.gemm_fp8(w, a8, asc, ws=torch.empty(n, dtype=torch.uint8, device=dev))
+        off = (C.double() - whole.double()).abs()  # (both are within the worst case of f32 sums of the absolute values)
+        assert bool((off <= 2 * P.gemm_bound(A, 0, K // 128)).all())
+    w.release()
+
+
 # ---- producers -------------------------------------------------------------------------------------------------------
 def same(a8, asc, q, sc, M):
     assert torch.equal(P.value(a8.cpu())[:M], q), "e4m3 rows"

@@ -180,6 +180,22 @@ def test_graph_and_streams(qm, dev):
     assert torch.equal(got[0], q) and torch.equal(got[1], k)
 
 
+def test_refusals(qm, dev):
+    T, D = 4, 64
+    x, f = torch.zeros((T, 6 * D), device=dev), inv_freq(D).to(dev)
+    p = torch.arange(T, dtype=torch.int32, device=dev)
+    ok = lambda **k: qm.qk_norm_rope(*{**dict(x=x, HQ=4, HK=2, D=D, pos=p, f=f), **{n: k.pop(n) for n in ("x", "pos", "f", "D", "HQ") if n in k}}.values(), **k)  # noqa: E731
+    ok()
+    for bad in (dict(pos=p.long()), dict(pos=p[:3]), dict(pos=p.cpu()), dict(f=f.double()), dict(f=inv_freq(2 * D + 2).to(dev)), dict(D=63),
+                dict(HQ=5), dict(x=x.double()), dict(x=x.cpu()), dict(x=x.t()), dict(wq=torch.ones(D - 1, device=dev)),
+                dict(wk=torch.ones(D, device=dev).half()), dict(sections=(16, 15)), dict(sections=(32, 0)), dict(pos=p.expand(3, T), sections=(12, 10, 10)),
+                dict(pos=p.expand(5, T).contiguous(), sections=(8, 8, 8, 4, 4)), dict(q=torch.zeros((T, 3 * D), device=dev)),
+                dict(q=x[:, D:5 * D]), dict(k=x[:, 4 * D:].to(torch.bfloat16), out=F32), dict(out=torch.int8), dict(q_off=3 * D), dict(k_hs=D - 2),
+                dict(q=torch.zeros((T, D, 4), device=dev).transpose(1, 2))):
+        with pytest.raises(qm.QMatmulError):
+            ok(**bad)
+
+
 @pytest.mark.parametrize("M", [1, 5, 70, 200])
 def test_attention_input_run(qm, dev, M):
     """The input side of an attention layer: norm -> e4m3 rows -> QKV product -> head norms and rotation, in place on the
