@@ -121,20 +121,23 @@ def _ptr(t):
     return None if t is None else ctypes.c_void_p(t.data_ptr())
 
 
-_raw_stream = None  # torch's current stream of a device as a number, without the Stream object (2.5 us a call)
+_raw_stream = None  # device -> torch's current stream there as a number, without the Stream object (2.5 us a call)
 
 
-def _stream(stream):
+def _current_stream(dev):
     global _raw_stream
-    if stream is not None:
-        return ctypes.c_void_p(stream)
     if _raw_stream is None:
         import torch
         torch.cuda.current_stream()  # (starts torch's GPU side)
-        raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
-        _raw_stream = ((lambda: raw(torch.cuda.current_device())) if raw is not None
-                       else (lambda: torch.cuda.current_stream().cuda_stream))
-    return ctypes.c_void_p(_raw_stream())
+        _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda d: torch.cuda.current_stream(d).cuda_stream)
+    return _raw_stream(dev)
+
+
+def _stream(stream):
+    if stream is not None:
+        return ctypes.c_void_p(stream)
+    import torch
+    return ctypes.c_void_p(_current_stream(torch.cuda.current_device()))
 
 
 class QWeight:
@@ -356,6 +359,22 @@ def _refuse(fn, what):
     raise QMatmulError(fn, 1, what)
 
 
+_functions = {}
+
+
+def _function(name):
+    """The library's function, bound once: these calls are short, and what Python does for them is most of their time."""
+    f = _functions.get(name)
+    if f is None:
+        f = _functions[name] = getattr(load_library(), name)
+    return f
+
+
+def _done(fn, status):
+    if status != QM_OK:
+        raise QMatmulError(fn, status, load_library().qmatmul_last_error().decode())
+
+
 _torch = None  # (an import statement in a function is 0.3 us a call, and these calls take about ten)
 
 
@@ -436,10 +455,13 @@ def quantize_fp8(x, M_stride=None, stream=None):
     """x [M, K] (float32, float16 or bfloat16, rows of any stride) -> (a8 float8_e4m3fn [M_stride, Kp], asc float32
     [Kp / 128, M_stride]), Kp = K rounded up to 128."""
     fn = "qmatmul_quantize_fp8"
-    _check_rows(fn, "x", x, 2, _current_gpu())
+    dev = _current_gpu()
+    _check_rows(fn, "x", x, 2, dev)
     M, K = x.shape
     Ms, a8, asc = _out_fp8(x, M, K, M_stride)
-    _call(fn, x.data_ptr(), _dtype(x.dtype), _row_stride(x), M, Ms, K, a8.data_ptr(), asc.data_ptr(), _stream(stream))
+    st = _function(fn)(x.data_ptr(), _dtype(x.dtype), _row_stride(x), M, Ms, K, a8.data_ptr(), asc.data_ptr(),
+                       _current_stream(dev) if stream is None else stream)
+    _done(fn, st)
     return a8, asc
 
 
@@ -455,21 +477,25 @@ def rmsnorm_fp8(x, w, eps, M_stride=None, want_h=False, stream=None):
         _refuse(fn, f"w {tuple(w.shape)} {w.dtype}: float32, one for each of {K} columns")
     Ms, a8, asc = _out_fp8(x, M, K, M_stride)
     h = x.new_empty((M, K), dtype=torch.float32) if want_h else None
-    _call(fn, x.data_ptr(), _dtype(x.dtype), _row_stride(x), w.data_ptr(), K, M, Ms, eps, a8.data_ptr(), asc.data_ptr(),
-          h.data_ptr() if want_h and M else None, K, _stream(stream))
+    st = _function(fn)(x.data_ptr(), _dtype(x.dtype), _row_stride(x), w.data_ptr(), K, M, Ms, eps, a8.data_ptr(),
+                       asc.data_ptr(), h.data_ptr() if want_h and M else None, K,
+                       _current_stream(dev) if stream is None else stream)
+    _done(fn, st)
     return a8, asc, h
 
 
 def swiglu_fp8(gu, F, gelu=False, M_stride=None, stream=None):
     """gu [M, 2 F] (gate then up) -> (a8, asc) of silu(gate) * up, or gelu_tanh(gate) * up."""
     fn = "qmatmul_swiglu_fp8"
-    _check_rows(fn, "gu", gu, 2, _current_gpu())
-    M = gu.shape[0]
-    if gu.shape[1] < 2 * F:
+    dev = _current_gpu()
+    _check_rows(fn, "gu", gu, 2, dev)
+    M = gu.size(0)
+    if gu.size(1) < 2 * F:
         _refuse(fn, f"rows of {gu.shape[1]} elements hold no gate and up of {F}")
     Ms, a8, asc = _out_fp8(gu, M, F, M_stride)
-    _call(fn, gu.data_ptr(), _dtype(gu.dtype), _row_stride(gu), F, M, Ms, 1 if gelu else 0, a8.data_ptr(),
-          asc.data_ptr(), _stream(stream))
+    st = _function(fn)(gu.data_ptr(), _dtype(gu.dtype), _row_stride(gu), F, M, Ms, 1 if gelu else 0, a8.data_ptr(),
+                       asc.data_ptr(), _current_stream(dev) if stream is None else stream)
+    _done(fn, st)
     return a8, asc
 
 
@@ -515,8 +541,9 @@ def gemm_fp8(w, a8, asc, M=None, C=None, ldc=None, c_off=0, accumulate=0, out=No
     else:
         _check_rows(fn, "ws", ws, 1, dev)
         ws_ptr, ws_bytes = ws.data_ptr(), ws.numel() * ws.element_size()
-    _call(fn, w.handle, a8.data_ptr(), asc.data_ptr(), M, Ms, C.data_ptr(), _dtype(C.dtype), ldc, c_off, accumulate,
-          ws_ptr, ws_bytes, _stream(stream))
+    st = _function(fn)(w.handle, a8.data_ptr(), asc.data_ptr(), M, Ms, C.data_ptr(), _dtype(C.dtype), ldc, c_off, accumulate,
+                       ws_ptr, ws_bytes, _current_stream(dev) if stream is None else stream)
+    _done(fn, st)
     return C
 
 
@@ -535,22 +562,28 @@ def qk_norm_rope(x, HQ, HK, D, pos, inv_freq, wq=None, wk=None, eps=1e-6, adjace
     fn = "qmatmul_qk_norm_rope"
     dev = _current_gpu()
     torch = _torch
-    _check_rows(fn, "x", x, 2, dev)
-    _check_rows(fn, "inv_freq", inv_freq, 1, dev)
-    T, width = x.shape
-    axes, half = 1, inv_freq.numel()
-    _check_rows(fn, "pos", pos, None, dev)
-    if pos.dim() == 2:
-        axes = pos.shape[0]
-    if pos.dtype != torch.int32 or pos.dim() not in (1, 2) or pos.shape[-1] != T:
-        _refuse(fn, f"pos {tuple(pos.shape)} {pos.dtype}: int32, one column for each of {T} tokens")
-    if inv_freq.dtype != torch.float32:
-        _refuse(fn, f"inv_freq {inv_freq.dtype}: float32")
-    for w in (wq, wk):
-        if w is not None:
-            _check_rows(fn, "wq or wk", w, 1, dev)
-            if w.dtype != torch.float32 or w.numel() != D:
-                _refuse(fn, f"wq or wk {tuple(w.shape)} {w.dtype}: float32 [{D}]")
+    f32 = torch.float32
+    axes, half = 1 if pos.dim() == 1 else pos.size(0), inv_freq.numel()
+    T = x.size(0)
+    # (one test for what is nearly always so; what fails it is named, or allowed, below)
+    if not (x.get_device() == dev and x.dim() == 2 and x.stride(1) == 1
+            and pos.get_device() == dev and pos.dtype is torch.int32 and pos.size(-1) == T and pos.stride(-1) == 1 and pos.dim() < 3
+            and inv_freq.get_device() == dev and inv_freq.dtype is f32 and inv_freq.dim() == 1 and inv_freq.stride(0) == 1
+            and (wq is None or (wq.get_device() == dev and wq.dtype is f32 and wq.dim() == 1 and wq.size(0) == D and wq.stride(0) == 1))
+            and (wk is None or (wk.get_device() == dev and wk.dtype is f32 and wk.dim() == 1 and wk.size(0) == D and wk.stride(0) == 1))):
+        _check_rows(fn, "x", x, 2, dev)
+        _check_rows(fn, "inv_freq", inv_freq, 1, dev)
+        _check_rows(fn, "pos", pos, None, dev)
+        if pos.dtype != torch.int32 or pos.dim() not in (1, 2) or pos.shape[-1] != T:
+            _refuse(fn, f"pos {tuple(pos.shape)} {pos.dtype}: int32, one column for each of {T} tokens")
+        if inv_freq.dtype != f32:
+            _refuse(fn, f"inv_freq {inv_freq.dtype}: float32")
+        for w in (wq, wk):
+            if w is not None:
+                _check_rows(fn, "wq or wk", w, 1, dev)
+                if w.dtype != f32 or w.numel() != D:
+                    _refuse(fn, f"wq or wk {tuple(w.shape)} {w.dtype}: float32 [{D}]")
+    width = x.size(1)
     if sections is None:
         sections = (half,)
     if len(sections) != axes or axes > 4 or sum(sections) != half:
@@ -574,10 +607,11 @@ def qk_norm_rope(x, HQ, HK, D, pos, inv_freq, wq=None, wk=None, eps=1e-6, adjace
         k, ldk = x.new_empty((T, HK, D), dtype=out), HK * D
     else:
         ldk = _head_rows(fn, "k", k, T, HK, D, out, dev)
-    _call(fn, x.data_ptr(), _dtype(x.dtype), _row_stride(x), T, D, q_off, q_hs, HQ, k_off, k_hs, HK,
-          None if wq is None else wq.data_ptr(), None if wk is None else wk.data_ptr(), eps, ctypes.byref(rope),
-          pos.data_ptr(), pos.stride(0) if axes > 1 else T, inv_freq.data_ptr(), q.data_ptr(), k.data_ptr(), _dtype(out),
-          ldq, ldk, _stream(stream))
+    st = _function(fn)(x.data_ptr(), _dtype(x.dtype), _row_stride(x), T, D, q_off, q_hs, HQ, k_off, k_hs, HK,
+                       None if wq is None else wq.data_ptr(), None if wk is None else wk.data_ptr(), eps, ctypes.byref(rope),
+                       pos.data_ptr(), pos.stride(0) if axes > 1 else T, inv_freq.data_ptr(), q.data_ptr(), k.data_ptr(),
+                       _dtype(out), ldq, ldk, _current_stream(dev) if stream is None else stream)
+    _done(fn, st)
     return q, k
 
 
