@@ -128,7 +128,7 @@ namespace {
 
 template <int MT, int RT, int W>
 void launch_few(const Fp8GemmArgs& a, hipStream_t s) {
-  const unsigned grid = (unsigned)((a.w.rows + 63) / 64 * 4 / RT) * (unsigned)((a.M + 16 * MT - 1) / (16 * MT));
+  const unsigned grid = (unsigned)((a.w.rows + 63) / 64 * 4 / RT) * (((unsigned)a.M + 16 * MT - 1) / (16 * MT));
   if (a.ctype == DT_F32) fp8_few_kernel<MT, RT, W, true><<<grid, 64 * W, 0, s>>>(a);
   else fp8_few_kernel<MT, RT, W, false><<<grid, 64 * W, 0, s>>>(a);
 }
