@@ -971,8 +971,8 @@ int qmatmul_qk_norm_rope(const void* x, int xtype, int ldx, int T, int D, int q_
   const HeadRows xq{(const char*)x + (size_t)q_off * si, T, D, HQ, q_hs, ldx, (long long)si};
   const HeadRows xk{(const char*)x + (size_t)k_off * si, T, D, HK, k_hs, ldx, (long long)si};
   const HeadRows oq{q, T, D, HQ, D, ldq, (long long)so}, ok{k, T, D, HK, D, ldk, (long long)so};
-  const bool q_in = HQ && q == xq.p && si == so && xtype == otype && ldq == ldx && (q_hs == D || HQ == 1);
-  const bool k_in = HK && k == xk.p && si == so && xtype == otype && ldk == ldx && (k_hs == D || HK == 1);
+  const bool q_in = HQ && q == xq.p && si == so && xtype == otype && (ldq == ldx || T == 1) && (q_hs == D || HQ == 1);
+  const bool k_in = HK && k == xk.p && si == so && xtype == otype && (ldk == ldx || T == 1) && (k_hs == D || HK == 1);
   if (rows_overlap(oq, ok) || (!q_in && rows_overlap(oq, xq)) || rows_overlap(oq, xk) || (!k_in && rows_overlap(ok, xk)) ||
       rows_overlap(ok, xq))
     return fail(QM_ERR_ARG, "%s: an output overlaps the input or the other output", fn);

@@ -327,7 +327,8 @@ typedef struct {
  * t*ldx + q_off + h*q_hs, key head h at t*ldx + k_off + h*k_hs (HQ, HK >= 0: none of a kind is allowed). wq, wk [D] (f32):
  * y = x * w / sqrt(mean over D of x^2 + eps); NULL: no norm for that kind. pos int32 [axes][pos_stride], inv_freq f32
  * [rot/2]. Results of otype: q at t*ldq + h*D, k at t*ldk + h*D. Computed in f32, rounded once. q (k) may be the input
- * itself (same address, type and strides); any other overlap of an output with the input or the other output is refused.
+ * itself (same address, type and strides; the row stride of a single row says nothing); any other overlap of an output with
+ * the input or the other output is refused.
  * Rows, offsets and strides of 4 elements' alignment are read and written 4 elements at a time, others by the element. */
 int qmatmul_qk_norm_rope(const void* x, int xtype, int ldx, int T, int D, int q_off, int q_hs, int HQ, int k_off, int k_hs,
                          int HK, const float* wq, const float* wk, float eps, const qm_rope* rope, const int32_t* pos,

@@ -92,3 +92,17 @@ def test_rotation_refuses_overlaps(qm, buf):
                 dict(q=p + row - 64, ldq=512), dict(q=p, ldq=512, q_hs=128, HQ=2), dict(k=p + 256 * 4, ldk=256)):
         assert rope(qm, p, **bad) == ARG, bad
         assert b"overlap" in qm.load_library().qmatmul_last_error()
+
+
+def test_rotation_of_one_token_in_place(qm, buf):
+    """A single row has no stride: the input's place with another ld is in place all the same, parts of it are overlaps. (Not
+    refused as an overlap; without a GPU the call then ends at the device.)"""
+    import torch
+    if torch.cuda.is_available():
+        pytest.skip("would run on the host buffer")
+    p, _ = buf
+    for ok in (dict(q=p), dict(k=p + 256 * 4), dict(q=p, k=p + 256 * 4), dict(q=p, ldq=4096)):
+        assert rope(qm, p, T=1, **ok) not in (0, ARG, SHAPE, TYPE), ok
+    for bad in (dict(q=p + 4), dict(q=p + 256 * 4), dict(q=p, ot=1), dict(q=p, q_hs=128, HQ=2), dict(k=p, ldk=128)):
+        assert rope(qm, p, T=1, **bad) == ARG, bad
+        assert b"overlap" in qm.load_library().qmatmul_last_error()

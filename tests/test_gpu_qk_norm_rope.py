@@ -120,6 +120,20 @@ def test_strides_and_in_place(qm, dev, xt):
     assert torch.equal(z[:, :HQ * D].reshape(T, HQ, D), want[0]) and torch.equal(z[:, HQ * D:].reshape(T, HK, D), want[1])
 
 
+def test_one_token_in_place(qm, dev):
+    """A single row, its heads rotated where they lie, whatever row stride the views of it carry."""
+    HQ, HK, D = 4, 2, 64
+    x = torch.randn((1, (HQ + HK) * D), generator=torch.Generator().manual_seed(3)).to(dev)
+    f, p, w = inv_freq(D).to(dev), torch.tensor([11], dtype=torch.int32, device=dev), torch.ones(D, device=dev)
+    want = qm.qk_norm_rope(x, HQ, HK, D, p, f, wq=w)
+    n = HQ * D
+    for q_of, k_of in ((lambda z: z[:, :n], lambda z: z[:, n:]), (lambda z: z[0, :n].view(1, HQ, D), lambda z: z[0, n:].view(1, HK, D)),
+                       (lambda z: z[0, :n].view(1, n), lambda z: z[0, n:].view(1, HK * D))):
+        z = x.clone()
+        qm.qk_norm_rope(z, HQ, HK, D, p, f, wq=w, q=q_of(z), k=k_of(z))
+        assert torch.equal(z[:, :n].view(1, HQ, D), want[0]) and torch.equal(z[:, n:].view(1, HK, D), want[1])
+
+
 def test_infinities_and_nan_stay_in_their_head(qm, dev):
     T, D = 3, 64
     x = torch.randn((T, 4 * D), generator=torch.Generator().manual_seed(0))
