@@ -532,9 +532,11 @@ def gemm_fp8(w, a8, asc, M=None, C=None, ldc=None, c_off=0, accumulate=0, out=No
         _check_rows(fn, "C", C, 2, dev)
         if out is not None and out != C.dtype:
             _refuse(fn, f"out {out} is not C's type")
-        if ldc is None:
+        own = ldc is None
+        if own:
             ldc = _row_stride(C)
-        if M > 0 and (M - 1) * ldc + c_off + w.rows > (C.shape[0] - 1) * C.stride(0) + C.shape[1]:
+        if M > 0 and (M > C.size(0) or c_off + w.rows > C.size(1) if own else
+                      (M - 1) * ldc + c_off + w.rows > (C.size(0) - 1) * C.stride(0) + C.size(1)):
             _refuse(fn, f"C {tuple(C.shape)} does not hold {M} rows of {w.rows} from column {c_off} on")
     if ws is None:
         ws_ptr, ws_bytes = None, 0

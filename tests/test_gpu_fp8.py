@@ -206,6 +206,20 @@ def test_refusals(qm, dev):
         qm.gemm_fp8(w, a8, asc, M=M, C=C)
 
 
+def test_columns_beside_a_view_are_no_room(qm, dev):
+    """C as a view of some columns: rows that end past its last column are refused, also where the matrix behind has the room."""
+    N, K, M = 200, 300, 5
+    w, a8, asc, (ref, *sums) = make(qm, dev, N, K, M, 1)
+    buf = torch.full((M + 3, 2 * N), 7.0, device=dev)
+    for C, k in ((buf[:, :N], dict(c_off=1)), (buf[:, :N - 1], {}), (buf[:, N // 2:N + N // 2], dict(c_off=N // 2)), (buf[:M - 1, :N], {})):
+        with pytest.raises(qm.QMatmulError):
+            qm.gemm_fp8(w, a8, asc, M=M, C=C, **k)
+    assert bool((buf == 7.0).all())
+    qm.gemm_fp8(w, a8, asc, M=M, C=buf[:, 50:50 + N])
+    near(buf[:M, 50:50 + N], ref, P.gemm_bound(*sums, 3) + P.rounding(F32, ref))
+    assert bool((buf[M:] == 7.0).all()) and bool((buf[:, :50] == 7.0).all()) and bool((buf[:, 50 + N:] == 7.0).all())
+
+
 @pytest.mark.parametrize("N,K", [(512, 17408), (5184, 5120), (17408, 5120)])
 def test_workspaces_are_bounded_and_optional(qm, dev, N, K):
     """Never more than 64 MiB; a larger or smaller one than asked for gives the bound's result too."""
