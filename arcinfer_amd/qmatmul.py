@@ -519,8 +519,8 @@ def gemm_fp8(w, a8, asc, M=None, C=None, ldc=None, c_off=0, accumulate=0, out=No
         M = Ms
     if w.handle is None:
         _refuse(fn, "the weight was released")
-    if Kp != w.Kp or a8.element_size() != 1 or not a8.is_contiguous():
-        _refuse(fn, f"a8 {tuple(a8.shape)} {a8.dtype}: contiguous e4m3 rows of {w.Kp}")
+    if Kp != w.Kp or a8.dtype not in (torch.float8_e4m3fn, torch.uint8) or not a8.is_contiguous():
+        _refuse(fn, f"a8 {tuple(a8.shape)} {a8.dtype}: contiguous rows of {w.Kp} float8_e4m3fn (or their bytes)")
     if asc.dtype != torch.float32 or asc.shape[0] != Kp // 128 or asc.shape[1] != Ms or not asc.is_contiguous():
         _refuse(fn, f"asc {tuple(asc.shape)} {asc.dtype}: contiguous float32 [{Kp // 128}, {Ms}]")
     if C is None:

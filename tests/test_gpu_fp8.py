@@ -206,6 +206,16 @@ def test_refusals(qm, dev):
         qm.gemm_fp8(w, a8, asc, M=M, C=C)
 
 
+def test_activations_of_other_bytes(qm, dev):
+    """Bytes of e4m3 are taken as such; other types of one byte are not read as e4m3."""
+    w, a8, asc, _ = make(qm, dev, 96, 256, 3, 1)
+    want = qm.gemm_fp8(w, a8, asc)
+    assert torch.equal(qm.gemm_fp8(w, a8.view(torch.uint8), asc), want)
+    for t in (torch.int8, torch.float8_e5m2, torch.float8_e4m3fnuz, torch.bool):
+        with pytest.raises(qm.QMatmulError):
+            qm.gemm_fp8(w, a8.view(t), asc)
+
+
 def test_columns_beside_a_view_are_no_room(qm, dev):
     """C as a view of some columns: rows that end past its last column are refused, also where the matrix behind has the room."""
     N, K, M = 200, 300, 5
