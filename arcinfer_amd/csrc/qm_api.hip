@@ -837,6 +837,25 @@ int qmatmul_fp8_info(const qm_fp8_weight* w, int* rows, int* K, int* Kp) {
   return QM_OK;
 }
 
+// Rows in memory: T of them, each `heads` runs of D elements `hs` apart, rows `ld` apart (elements of `size` bytes)
+struct HeadRows {
+  const void* p;
+  long long T, D, heads, hs, ld, size;
+  uintptr_t first() const { return (uintptr_t)p; }
+  uintptr_t width() const { return (uintptr_t)(((heads - 1) * hs + D) * size); }
+  uintptr_t last() const { return first() + (uintptr_t)((T - 1) * ld * size) + width(); }
+};
+
+// Whether two such sets share a byte, or may: rows of one stride are compared within it (the heads' runs taken whole)
+static bool rows_overlap(const HeadRows& a, const HeadRows& b) {
+  if (!a.heads || !b.heads || !a.T) return false;
+  if (a.last() <= b.first() || b.last() <= a.first()) return false;
+  const uintptr_t ld = (uintptr_t)(a.ld * a.size);
+  if (ld != (uintptr_t)(b.ld * b.size)) return true;
+  const uintptr_t d = b.first() >= a.first() ? (b.first() - a.first()) % ld : (ld - (a.first() - b.first()) % ld) % ld;
+  return d < a.width() || d + b.width() > ld;
+}
+
 // what the three producers share: input rows of `width` elements, outputs of K values
 static int check_fp8_rows(const char* fn, const void* x, int xtype, int ldx, long long width, int M, int M_stride, int K,
                           const uint8_t* a8, const float* asc) {
@@ -863,6 +882,9 @@ int qmatmul_rmsnorm_fp8(const void* x, int xtype, int ldx, const float* w, int K
   if (!w) return fail(QM_ERR_ARG, "qmatmul_rmsnorm_fp8: null weight");
   if (!aligned(w, 4) || (h && !aligned(h, 4))) return fail(QM_ERR_ARG, "qmatmul_rmsnorm_fp8: w and h must be 4-byte aligned");
   if (h && ldh < K) return fail(QM_ERR_SHAPE, "qmatmul_rmsnorm_fp8: ldh %d < K %d", ldh, K);
+  const long long size = (long long)dtype_size(xtype);
+  if (h && rows_overlap({x, M, K, 1, K, ldx, size}, {h, M, K, 1, K, ldh, 4}))
+    return fail(QM_ERR_ARG, "qmatmul_rmsnorm_fp8: h overlaps the input");
   QM_CHECK_INIT();
   const hipError_t e = qm::launch_rmsnorm_fp8(x, xtype, ldx, w, K, M, M_stride, eps, a8, asc, h, ldh, (hipStream_t)stream);
   return e == hipSuccess ? QM_OK : hip_fail(e, "qmatmul_rmsnorm_fp8");
@@ -916,25 +938,6 @@ int qmatmul_gemm_fp8(const qm_fp8_weight* w, const uint8_t* a8, const float* asc
 }
 
 // ---- query and key heads
-
-// Rows in memory: T of them, each `heads` runs of D elements `hs` apart, rows `ld` apart (elements of `size` bytes)
-struct HeadRows {
-  const void* p;
-  long long T, D, heads, hs, ld, size;
-  uintptr_t first() const { return (uintptr_t)p; }
-  uintptr_t width() const { return (uintptr_t)(((heads - 1) * hs + D) * size); }
-  uintptr_t last() const { return first() + (uintptr_t)((T - 1) * ld * size) + width(); }
-};
-
-// Whether two such sets share a byte, or may: rows of one stride are compared within it (the heads' runs taken whole)
-static bool rows_overlap(const HeadRows& a, const HeadRows& b) {
-  if (!a.heads || !b.heads || !a.T) return false;
-  if (a.last() <= b.first() || b.last() <= a.first()) return false;
-  const uintptr_t ld = (uintptr_t)(a.ld * a.size);
-  if (ld != (uintptr_t)(b.ld * b.size)) return true;
-  const uintptr_t d = b.first() >= a.first() ? (b.first() - a.first()) % ld : (ld - (a.first() - b.first()) % ld) % ld;
-  return d < a.width() || d + b.width() > ld;
-}
 
 int qmatmul_qk_norm_rope(const void* x, int xtype, int ldx, int T, int D, int q_off, int q_hs, int HQ, int k_off, int k_hs,
                          int HK, const float* wq, const float* wk, float eps, const qm_rope* rope, const int32_t* pos,

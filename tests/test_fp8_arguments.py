@@ -106,3 +106,18 @@ def test_rotation_of_one_token_in_place(qm, buf):
     for bad in (dict(q=p + 4), dict(q=p + 256 * 4), dict(q=p, ot=1), dict(q=p, q_hs=128, HQ=2), dict(k=p, ldk=128)):
         assert rope(qm, p, T=1, **bad) == ARG, bad
         assert b"overlap" in qm.load_library().qmatmul_last_error()
+
+
+def test_normed_copy_beside_its_input(qm, buf):
+    """h over x: several work-groups may read a row while one writes its h, so no overlap is taken; rows in turns are none."""
+    lib, (p, _) = qm.load_library(), buf
+    n = lambda **k: lib.qmatmul_rmsnorm_fp8(*{**dict(x=p, t=0, ld=256, w=p, K=256, M=2, Ms=4, eps=1e-6, a=p, s=p, h=None, ldh=256,  # noqa: E731
+                                                     st=None), **k}.values())
+    for bad in (dict(h=p), dict(h=p + 4), dict(h=p + 255 * 4), dict(h=p + 256 * 4), dict(h=p + 511 * 4), dict(h=p, ldh=512), dict(h=p, t=1),
+                dict(x=p + 2048, h=p + 1024), dict(ld=512, ldh=512, h=p + 255 * 4)):
+        assert n(**bad) == ARG, bad
+        assert b"overlap" in lib.qmatmul_last_error()
+    import torch
+    if not torch.cuda.is_available():  # (not refused: the call ends at the device, which is not there)
+        for ok in (dict(h=p + 512 * 4), dict(ld=512, ldh=512, h=p + 256 * 4), dict(h=p, x=p + 2048), dict(h=p, M=0)):
+            assert n(**ok) not in (0, ARG, SHAPE), ok
