@@ -398,10 +398,24 @@ def _check_rows(fn, name, t, dim, dev):
         _refuse(fn, f"the last dimension of {name} is not contiguous")
 
 
+_INT_MAX = 0x7fffffff
+
+
+def _sizes(fn, *v):
+    """The library's sizes are 32-bit ints, and ctypes takes a larger number modulo 2^32. (Calls test (a | b | ...) >> 31 first:
+    0 where none is negative or too large, in a fifth of the time.)"""
+    if max(v) > _INT_MAX or min(v) < -_INT_MAX:
+        _refuse(fn, f"sizes, offsets and strides are of 32 bits: {[i for i in v if abs(i) > _INT_MAX]}")
+
+
+def _stride_of(ld, length, rows):
+    """A row stride in elements; of a single row, whose stride says nothing, one that holds the row."""
+    return ld if rows > 1 or length <= ld <= _INT_MAX else length
+
+
 def _row_stride(t):
-    """The row stride of a matrix in elements (of a single row, whose stride says nothing: at least its length)."""
     ld = t.stride(0)
-    return ld if t.size(0) > 1 else max(t.size(1), ld)
+    return ld if t.size(0) > 1 else _stride_of(ld, t.size(1), 1)
 
 
 class Fp8Weight:
@@ -416,6 +430,7 @@ class Fp8Weight:
             _refuse(fn, f"w8 {tuple(w8.shape)} {w8.dtype}: a contiguous matrix of float8_e4m3fn (or its bytes)")
         self.rows, self.K = w8.shape
         self.Kp = (self.K + 127) // 128 * 128
+        _sizes(fn, self.rows, self.K)
         if (scales.dtype != torch.float32 or not scales.is_contiguous()
                 or tuple(scales.shape) != ((self.rows + 127) // 128, self.Kp // 128)):
             _refuse(fn, f"scales {tuple(scales.shape)} {scales.dtype}: contiguous float32, one for each 128 x 128 block")
@@ -445,10 +460,13 @@ class Fp8Weight:
             pass
 
 
-def _out_fp8(x, M, K, M_stride):
-    Ms = M if M_stride is None else M_stride
+def _out_fp8(fn, x, M, K, M_stride):
+    """(M_stride, ldx, a8, asc) of a producer's rows x."""
+    Ms, ldx = M if M_stride is None else M_stride, _row_stride(x)
+    if (M | Ms | K | ldx) >> 31:
+        _sizes(fn, M, Ms, K, ldx)
     Kp = (K + 127) // 128 * 128
-    return (Ms, x.new_empty((Ms, Kp), dtype=_torch.float8_e4m3fn), x.new_empty((Kp // 128, Ms), dtype=_torch.float32))
+    return (Ms, ldx, x.new_empty((Ms, Kp), dtype=_torch.float8_e4m3fn), x.new_empty((Kp // 128, Ms), dtype=_torch.float32))
 
 
 def quantize_fp8(x, M_stride=None, stream=None):
@@ -458,8 +476,8 @@ def quantize_fp8(x, M_stride=None, stream=None):
     dev = _current_gpu()
     _check_rows(fn, "x", x, 2, dev)
     M, K = x.shape
-    Ms, a8, asc = _out_fp8(x, M, K, M_stride)
-    st = _function(fn)(x.data_ptr(), _dtype(x.dtype), _row_stride(x), M, Ms, K, a8.data_ptr(), asc.data_ptr(),
+    Ms, ldx, a8, asc = _out_fp8(fn, x, M, K, M_stride)
+    st = _function(fn)(x.data_ptr(), _dtype(x.dtype), ldx, M, Ms, K, a8.data_ptr(), asc.data_ptr(),
                        _current_stream(dev) if stream is None else stream)
     _done(fn, st)
     return a8, asc
@@ -475,9 +493,9 @@ def rmsnorm_fp8(x, w, eps, M_stride=None, want_h=False, stream=None):
     M, K = x.shape
     if w.dtype != torch.float32 or w.numel() != K:
         _refuse(fn, f"w {tuple(w.shape)} {w.dtype}: float32, one for each of {K} columns")
-    Ms, a8, asc = _out_fp8(x, M, K, M_stride)
+    Ms, ldx, a8, asc = _out_fp8(fn, x, M, K, M_stride)
     h = x.new_empty((M, K), dtype=torch.float32) if want_h else None
-    st = _function(fn)(x.data_ptr(), _dtype(x.dtype), _row_stride(x), w.data_ptr(), K, M, Ms, eps, a8.data_ptr(),
+    st = _function(fn)(x.data_ptr(), _dtype(x.dtype), ldx, w.data_ptr(), K, M, Ms, eps, a8.data_ptr(),
                        asc.data_ptr(), h.data_ptr() if want_h and M else None, K,
                        _current_stream(dev) if stream is None else stream)
     _done(fn, st)
@@ -492,8 +510,8 @@ def swiglu_fp8(gu, F, gelu=False, M_stride=None, stream=None):
     M = gu.size(0)
     if gu.size(1) < 2 * F:
         _refuse(fn, f"rows of {gu.shape[1]} elements hold no gate and up of {F}")
-    Ms, a8, asc = _out_fp8(gu, M, F, M_stride)
-    st = _function(fn)(gu.data_ptr(), _dtype(gu.dtype), _row_stride(gu), F, M, Ms, 1 if gelu else 0, a8.data_ptr(),
+    Ms, ldg, a8, asc = _out_fp8(fn, gu, M, F, M_stride)
+    st = _function(fn)(gu.data_ptr(), _dtype(gu.dtype), ldg, F, M, Ms, 1 if gelu else 0, a8.data_ptr(),
                        asc.data_ptr(), _current_stream(dev) if stream is None else stream)
     _done(fn, st)
     return a8, asc
@@ -502,6 +520,7 @@ def swiglu_fp8(gu, F, gelu=False, M_stride=None, stream=None):
 def gemm_fp8_workspace(w, M):
     """A workspace for products of M tokens with w (None where they need none)."""
     import torch
+    _sizes("qmatmul_gemm_fp8_workspace_size", M)
     n = load_library().qmatmul_gemm_fp8_workspace_size(w.handle, M)
     return torch.empty((n,), dtype=torch.uint8, device="cuda") if n else None
 
@@ -523,6 +542,8 @@ def gemm_fp8(w, a8, asc, M=None, C=None, ldc=None, c_off=0, accumulate=0, out=No
         _refuse(fn, f"a8 {tuple(a8.shape)} {a8.dtype}: contiguous rows of {w.Kp} float8_e4m3fn (or their bytes)")
     if asc.dtype != torch.float32 or asc.shape[0] != Kp // 128 or asc.shape[1] != Ms or not asc.is_contiguous():
         _refuse(fn, f"asc {tuple(asc.shape)} {asc.dtype}: contiguous float32 [{Kp // 128}, {Ms}]")
+    if (M | Ms | c_off | accumulate) >> 31:
+        _sizes(fn, M, Ms, c_off, accumulate)
     if C is None:
         if accumulate or c_off or ldc is not None:
             _refuse(fn, "accumulate, c_off and ldc need a C")
@@ -538,6 +559,8 @@ def gemm_fp8(w, a8, asc, M=None, C=None, ldc=None, c_off=0, accumulate=0, out=No
         if M > 0 and (M > C.size(0) or c_off + w.rows > C.size(1) if own else
                       (M - 1) * ldc + c_off + w.rows > (C.size(0) - 1) * C.stride(0) + C.size(1)):
             _refuse(fn, f"C {tuple(C.shape)} does not hold {M} rows of {w.rows} from column {c_off} on")
+        if ldc >> 31:
+            _sizes(fn, ldc)
     if ws is None:
         ws_ptr, ws_bytes = None, 0
     else:
@@ -597,6 +620,9 @@ def qk_norm_rope(x, HQ, HK, D, pos, inv_freq, wq=None, wk=None, eps=1e-6, adjace
         k_hs = D
     if k_off is None:
         k_off = q_off + HQ * q_hs
+    ldx, ps = _row_stride(x), pos.stride(0) if axes > 1 else T
+    if (T | D | HQ | HK | ldx | ps | q_off | q_hs | k_off | k_hs | 2 * half) >> 31 or axes > 1:
+        _sizes(fn, T, D, HQ, HK, ldx, ps, q_off, q_hs, k_off, k_hs, 2 * half, *sections)
     if (HQ and q_off + (HQ - 1) * q_hs + D > width) or (HK and k_off + (HK - 1) * k_hs + D > width):
         _refuse(fn, f"rows of {width} elements do not hold the heads")
     if out is None:
@@ -609,9 +635,9 @@ def qk_norm_rope(x, HQ, HK, D, pos, inv_freq, wq=None, wk=None, eps=1e-6, adjace
         k, ldk = x.new_empty((T, HK, D), dtype=out), HK * D
     else:
         ldk = _head_rows(fn, "k", k, T, HK, D, out, dev)
-    st = _function(fn)(x.data_ptr(), _dtype(x.dtype), _row_stride(x), T, D, q_off, q_hs, HQ, k_off, k_hs, HK,
+    st = _function(fn)(x.data_ptr(), _dtype(x.dtype), ldx, T, D, q_off, q_hs, HQ, k_off, k_hs, HK,
                        None if wq is None else wq.data_ptr(), None if wk is None else wk.data_ptr(), eps, ctypes.byref(rope),
-                       pos.data_ptr(), pos.stride(0) if axes > 1 else T, inv_freq.data_ptr(), q.data_ptr(), k.data_ptr(),
+                       pos.data_ptr(), ps, inv_freq.data_ptr(), q.data_ptr(), k.data_ptr(),
                        _dtype(out), ldq, ldk, _current_stream(dev) if stream is None else stream)
     _done(fn, st)
     return q, k
@@ -623,7 +649,10 @@ def _head_rows(fn, name, t, T, H, D, dtype, dev):
     if (t.dtype != dtype or t.dim() not in (2, 3) or t.shape[0] != T
             or (t.shape[1] != H * D if t.dim() == 2 else tuple(t.shape[1:]) != (H, D) or (H > 1 and t.stride(1) != D))):
         _refuse(fn, f"{name} {tuple(t.shape)} {t.dtype}: [{T}, {H} * {D}] of {dtype}")
-    return t.stride(0) if T > 1 else max(H * D, t.stride(0))
+    ld = _stride_of(t.stride(0), H * D, T)
+    if ld >> 31:
+        _sizes(fn, ld)
+    return ld
 
 
 class GgufTensor:
