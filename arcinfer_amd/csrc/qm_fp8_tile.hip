@@ -36,6 +36,10 @@ __device__ __forceinline__ void meet() {
   asm volatile("" ::: "memory");
 }
 
+// What this wave's lanes wrote to LDS before it, its lanes read behind it. (The hardware keeps a wave's LDS accesses in order; this
+// tells the compiler to.)
+__device__ __forceinline__ void exchange() { __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront", "local"); }
+
 struct Frags {
   v4i lo[4], hi[4];
 };
@@ -249,12 +253,14 @@ __global__ __launch_bounds__(256, 2) void fp8_tile_kernel(Fp8GemmArgs a, int tn,
       float* pj = lds + (kTwo ? (j & 1) * 16 * kRow : 0);
 #pragma unroll
       for (int t = 0; t < 4; ++t) *(v4f*)(pj + w.r * kRow + 16 * g + 4 * t) = w.acc[t][j];
+      exchange();
       v4f lo[2], hi[2];
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         lo[h] = *(const v4f*)(pj + (8 * h + mr) * kRow + 8 * (lane & 7));
         hi[h] = *(const v4f*)(pj + (8 * h + mr) * kRow + 8 * (lane & 7) + 4);
       }
+      exchange();
 #pragma unroll
       for (int h = 0; h < 2; ++h) put(m0 + 16 * j + 8 * h + mr, lo[h], hi[h]);
     }
