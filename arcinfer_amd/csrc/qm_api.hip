@@ -856,6 +856,24 @@ static bool rows_overlap(const HeadRows& a, const HeadRows& b) {
   return d < a.width() || d + b.width() > ld;
 }
 
+// Whether rows share a byte with `bytes` in one piece
+static bool span_overlaps(const HeadRows& rows, const void* p, size_t bytes) {
+  return p && bytes && rows_overlap(rows, {p, 1, (long long)bytes, 1, (long long)bytes, rows.ld * rows.size, 1});
+}
+
+static size_t fp8_rows_bytes(int M_stride, int K) { return (size_t)M_stride * padded_128(K); }
+static size_t fp8_scales_bytes(int M_stride, int K) { return (size_t)M_stride * (padded_128(K) / 128) * sizeof(float); }
+
+// A producer's outputs in its input or in each other: several work-groups may read a row while one writes. (rows: the input, or
+// the normed copy)
+static int check_fp8_apart(const char* fn, const HeadRows& rows, int M_stride, int K, const uint8_t* a8, const float* asc) {
+  const size_t na = fp8_rows_bytes(M_stride, K), ns = fp8_scales_bytes(M_stride, K);
+  if (span_overlaps(rows, a8, na) || span_overlaps(rows, asc, ns) ||
+      ((uintptr_t)a8 < (uintptr_t)asc + ns && (uintptr_t)asc < (uintptr_t)a8 + na))
+    return fail(QM_ERR_ARG, "%s: an output overlaps the input or another output", fn);
+  return QM_OK;
+}
+
 // what the three producers share: input rows of `width` elements, outputs of K values
 static int check_fp8_rows(const char* fn, const void* x, int xtype, int ldx, long long width, int M, int M_stride, int K,
                           const uint8_t* a8, const float* asc) {
@@ -871,6 +889,7 @@ static int check_fp8_rows(const char* fn, const void* x, int xtype, int ldx, lon
 int qmatmul_quantize_fp8(const void* x, int xtype, int ldx, int M, int M_stride, int K, uint8_t* a8, float* asc,
                          void* stream) {
   if (int st = check_fp8_rows("qmatmul_quantize_fp8", x, xtype, ldx, K, M, M_stride, K, a8, asc)) return st;
+  if (int st = check_fp8_apart("qmatmul_quantize_fp8", {x, M, K, 1, K, ldx, (long long)dtype_size(xtype)}, M_stride, K, a8, asc)) return st;
   QM_CHECK_INIT();
   const hipError_t e = qm::launch_quantize_fp8(x, xtype, ldx, M, M_stride, K, a8, asc, (hipStream_t)stream);
   return e == hipSuccess ? QM_OK : hip_fail(e, "qmatmul_quantize_fp8");
@@ -886,6 +905,9 @@ int qmatmul_rmsnorm_fp8(const void* x, int xtype, int ldx, const float* w, int K
   if (h && rows_overlap({x, M, K, 1, K, ldx, size}, {h, M, K, 1, K, ldh, 4}))
     return fail(QM_ERR_ARG, "qmatmul_rmsnorm_fp8: h overlaps the input");
   QM_CHECK_INIT();
+  if (int st = check_fp8_apart("qmatmul_rmsnorm_fp8", {x, M, K, 1, K, ldx, size}, M_stride, K, a8, asc)) return st;
+  if (h)
+    if (int st = check_fp8_apart("qmatmul_rmsnorm_fp8", {h, M, K, 1, K, ldh, 4}, M_stride, K, a8, asc)) return st;
   const hipError_t e = qm::launch_rmsnorm_fp8(x, xtype, ldx, w, K, M, M_stride, eps, a8, asc, h, ldh, (hipStream_t)stream);
   return e == hipSuccess ? QM_OK : hip_fail(e, "qmatmul_rmsnorm_fp8");
 }
@@ -893,6 +915,8 @@ int qmatmul_rmsnorm_fp8(const void* x, int xtype, int ldx, const float* w, int K
 int qmatmul_swiglu_fp8(const void* gu, int xtype, int ldg, int F, int M, int M_stride, int gelu, uint8_t* a8, float* asc,
                        void* stream) {
   if (int st = check_fp8_rows("qmatmul_swiglu_fp8", gu, xtype, ldg, 2LL * F, M, M_stride, F, a8, asc)) return st;
+  if (int st = check_fp8_apart("qmatmul_swiglu_fp8", {gu, M, 2LL * F, 1, 2LL * F, ldg, (long long)dtype_size(xtype)}, M_stride, F, a8, asc))
+    return st;
   QM_CHECK_INIT();
   const hipError_t e = qm::launch_swiglu_fp8(gu, xtype, ldg, F, M, M_stride, gelu ? 1 : 0, a8, asc, (hipStream_t)stream);
   return e == hipSuccess ? QM_OK : hip_fail(e, "qmatmul_swiglu_fp8");
@@ -920,6 +944,13 @@ int qmatmul_gemm_fp8(const qm_fp8_weight* w, const uint8_t* a8, const float* asc
   const hipError_t ed = hipGetDevice(&dev);
   if (ed != hipSuccess) return hip_fail(ed, fn);
   if (dev != w->device) return fail(QM_ERR_ARG, "%s: the weight is on device %d, the current device is %d", fn, w->device, dev);
+  const int Kp = 128 * w->view.kb;
+  const size_t size = dtype_size(ctype), na = fp8_rows_bytes(M_stride, Kp), ns = fp8_scales_bytes(M_stride, Kp);
+  const HeadRows c{(const char*)C + (size_t)c_off * size, M, w->rows, 1, w->rows, ldc, (long long)size};
+  const uintptr_t wsp = (uintptr_t)ws;
+  if (span_overlaps(c, a8, na) || span_overlaps(c, asc, ns) || span_overlaps(c, ws, ws ? ws_bytes : 0) ||
+      (ws && ((wsp < (uintptr_t)a8 + na && (uintptr_t)a8 < wsp + ws_bytes) || (wsp < (uintptr_t)asc + ns && (uintptr_t)asc < wsp + ws_bytes))))
+    return fail(QM_ERR_ARG, "%s: C or the workspace overlaps the activations or the other", fn);
   qm::Fp8GemmArgs a{};
   a.w = w->view;
   a.a8 = a8;

@@ -1,0 +1,66 @@
+"""Outputs of the e4m3 producers and products over their inputs or over each other: several work-groups share a row, and one would
+read what another has written. Refused before any launch; what only lies between the input's rows is not."""
+import ctypes
+
+import pytest
+import torch
+
+ARG = 1
+
+
+@pytest.fixture()
+def at():
+    b = (ctypes.c_uint8 * (1 << 17))()
+    yield (ctypes.addressof(b) + 255) // 256 * 256
+
+
+def is_overlap(qm, st):
+    return st == ARG and b"overlap" in qm.load_library().qmatmul_last_error()
+
+
+def test_rows_and_gates(qm, at):
+    """x: two rows of 256 floats; a8: four rows of 256 bytes; asc: 2 x 4 floats."""
+    lib, p = qm.load_library(), at
+    q = lambda **k: lib.qmatmul_quantize_fp8(*{**dict(x=p, t=0, ld=256, M=2, Ms=4, K=256, a=p + 8192, s=p + 16384, st=None), **k}.values())  # noqa: E731
+    g = lambda **k: lib.qmatmul_swiglu_fp8(*{**dict(x=p, t=1, ld=512, F=256, M=2, Ms=4, gelu=0, a=p + 8192, s=p + 16384, st=None), **k}.values())  # noqa: E731
+    for f in (q, g):
+        for bad in (dict(a=p), dict(s=p), dict(a=p + 2032), dict(s=p + 2044), dict(x=p + 1024, a=p + 16), dict(x=p + 1024, s=p + 996),
+                    dict(a=p + 16384, s=p + 16384), dict(a=p + 16384 - 1008), dict(s=p + 8192 + 1020)):
+            assert is_overlap(qm, f(**bad)), bad
+        row = 4096 * (4 if f is q else 2)  # rows apart: the edges of one, and the gap
+        for bad in (dict(ld=4096, a=p + 1024 - 16, s=p + 40000), dict(ld=4096, a=p + 1024, s=p + row - 28)):
+            assert is_overlap(qm, f(**bad)), bad
+        if not torch.cuda.is_available():  # (not refused: the call ends at the device, which is not there)
+            for ok in ({}, dict(a=p + 2048), dict(s=p + 2048), dict(x=p + 1024, a=p), dict(x=p + 32, s=p), dict(M=0, a=p),
+                       dict(ld=4096, a=p + 1024, s=p + 40000), dict(ld=4096, a=p + 1024, s=p + row - 32)):
+                assert f(**ok) not in (0, ARG, 2, 3), ok
+
+
+@pytest.mark.gpu
+def test_normed_rows(qm, dev):
+    lib, buf = qm.load_library(), torch.zeros(1 << 16, dtype=torch.uint8, device=dev)
+    p, w = (buf.data_ptr() + 255) // 256 * 256, torch.ones(256, device=dev)
+    n = lambda **k: lib.qmatmul_rmsnorm_fp8(*{**dict(x=p, t=0, ld=256, w=w.data_ptr(), K=256, M=2, Ms=4, eps=1e-6, a=p + 8192, s=p + 16384,  # noqa: E731
+                                                     h=p + 20480, ldh=256, st=qm._stream(None)), **k}.values())
+    for bad in (dict(a=p), dict(s=p), dict(a=p + 2032), dict(s=p + 2044), dict(a=p + 16384), dict(h=p + 8192), dict(h=p + 16384),
+                dict(h=p + 8192 - 2044), dict(a=p + 20480), dict(s=p + 20480, h=p + 20480 + 28), dict(h=p)):
+        assert is_overlap(qm, n(**bad)), bad
+    assert not buf.any()
+    assert n() == 0 and n(h=None) == 0 and n(ldh=512, a=p + 20480 + 1024, Ms=2) == 0
+
+
+@pytest.mark.gpu
+def test_products(qm, dev):
+    N, K, M = 256, 256, 5
+    w = qm.Fp8Weight(torch.zeros((N, K), dtype=torch.uint8, device=dev), torch.ones((2, 2), device=dev))
+    lib, buf = qm.load_library(), torch.zeros(1 << 20, dtype=torch.uint8, device=dev)
+    p = (buf.data_ptr() + 255) // 256 * 256
+    f = lambda **k: lib.qmatmul_gemm_fp8(*{**dict(w=w.handle, a=p, s=p + 8192, M=M, Ms=8, C=p + 16384, t=0, ldc=N, off=0, acc=0,  # noqa: E731
+                                                  ws=p + 65536, wsb=65536, st=qm._stream(None)), **k}.values())
+    row = 4 * N
+    for bad in (dict(C=p), dict(C=p + 2044), dict(C=p + 8192 - 5 * row + 4), dict(C=p + 8192), dict(C=p + 65536), dict(ws=p), dict(ws=p + 8192),
+                dict(ws=p + 16384 + 4 * row), dict(ldc=1024, C=p + 65536 - 4096), dict(ldc=2048, off=1024, C=p - 4096 + 2044)):
+        assert is_overlap(qm, f(**bad)), bad
+    assert not buf.any()
+    assert f() == 0 and f(ws=None, wsb=0) == 0 and f(ws=p, wsb=0) == 0 and f(ldc=1024, C=p + 8192 + 256) == 0
+    w.release()
