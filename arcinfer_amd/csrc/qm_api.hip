@@ -962,9 +962,8 @@ int qmatmul_gemm_fp8(const qm_fp8_weight* w, const uint8_t* a8, const float* asc
   a.ldc = ldc;
   a.c_off = c_off;
   a.accumulate = accumulate;
-  const size_t need = qm::fp8_workspace_bytes(M, w->rows, w->view.kb);
-  a.part = need && ws && ws_bytes >= need ? (float*)ws : nullptr;
-  const hipError_t e = qm::launch_gemm_fp8(a, (hipStream_t)stream);
+  a.part = (float*)ws;
+  const hipError_t e = qm::launch_gemm_fp8(a, ws_bytes, (hipStream_t)stream);
   return e == hipSuccess ? QM_OK : hip_fail(e, fn);
 }
 

@@ -147,8 +147,7 @@ FewShape few_shape(int M, int rows, int kb) {
   return {rt, w};
 }
 
-hipError_t launch_few_tokens(const Fp8GemmArgs& a, hipStream_t s) {
-  const FewShape f = few_shape(a.M, a.w.rows, a.w.kb);
+hipError_t launch_few_tokens(const Fp8GemmArgs& a, const Fp8Plan& f, hipStream_t s) {
 #define QM_FEW(MT, RT) (f.waves == 8 ? launch_few<MT, RT, 8>(a, s) : launch_few<MT, RT, 4>(a, s))
   if (a.M <= 16) {
     if (f.waves == 16) f.rt == 1 ? launch_few<1, 1, 16>(a, s) : launch_few<1, 2, 16>(a, s);
@@ -198,13 +197,14 @@ float few_us(const Rates& r, float block, int M, int rows, int kb) {
   return r.few_call + bytes / r.few_w + bytes / f.rt * mt * turns / r.few_t + (block + r.few_mt * mt * f.rt) * kb / f.waves;
 }
 
+}  // namespace
+
 // Up to 16 tokens: the few-token kernel. Beyond, what the times above say: that kernel (mt = 0), or tiles of mt token tiles, each
-// in `splits` pieces of at least three blocks (more than one only with a workspace for their sums).
-struct Plan {
-  int mt, splits;
-};
-Plan plan_of(int M, int M_stride, int rows, int kb, bool exact, bool part) {
-  Plan p{0, 1};
+// in `splits` pieces of at least three blocks, as many as part_bytes of workspace hold the sums of.
+Fp8Plan fp8_plan(int M, int M_stride, int rows, int kb, bool exact, size_t part_bytes) {
+  const FewShape f = few_shape(M, rows, kb);
+  Fp8Plan p{0, 1, f.rt, f.waves};
+  if (part_bytes > kFp8PartBytes) part_bytes = kFp8PartBytes;
   // (the tile kernel's token scales are a buffer of 32-bit offsets)
   if (M <= 16 || (size_t)kb * M_stride >= (size_t)1 << 30) return p;
   const Rates& r = exact ? kRates32 : kRates16;
@@ -212,34 +212,32 @@ Plan plan_of(int M, int M_stride, int rows, int kb, bool exact, bool part) {
   constexpr int kSplits[] = {1, 2, 3, 4, 5, 6, 8, 10, 12, 16};
   for (int mt = exact ? 6 : 8; mt >= 4; --mt) {
     for (int s : kSplits) {
-      if (s > 1 && (!part || kb / s < 3 || fp8_part_bytes(M, rows, s) > kFp8PartBytes)) break;
+      if (s > 1 && (kb / s < 3 || fp8_part_bytes(M, rows, s) > part_bytes)) break;
       const float t = tile_us(r, M, rows, kb, mt, s);
       // (a smaller tile only for 2 %: what the times cannot tell apart is faster with the larger one, 4096 x 5120 -> 17408 329 us against
       //  342; it reads less)
       if (t < best * (p.mt > mt ? 0.98f : 1.0f)) {
         best = t;
-        p = {mt, s};
+        p = {mt, s, 0, 0};
       }
     }
   }
   return p;
 }
 
-}  // namespace
-
 size_t fp8_workspace_bytes(int M, int rows, int kb) {
   // (the larger of both output types': the call's is not known yet)
   size_t most = 0;
   for (int exact = 0; exact < 2; ++exact) {
-    const Plan p = plan_of(M, M, rows, kb, exact != 0, true);
+    const Fp8Plan p = fp8_plan(M, M, rows, kb, exact != 0, kFp8PartBytes);
     if (p.splits > 1 && fp8_part_bytes(M, rows, p.splits) > most) most = fp8_part_bytes(M, rows, p.splits);
   }
   return most;
 }
 
-hipError_t launch_gemm_fp8(const Fp8GemmArgs& a, hipStream_t s) {
-  const Plan p = plan_of(a.M, a.M_stride, a.w.rows, a.w.kb, a.ctype == DT_F32, a.part != nullptr);
-  return p.mt ? launch_fp8_tile(a, p.mt, p.splits, s) : launch_few_tokens(a, s);
+hipError_t launch_gemm_fp8(const Fp8GemmArgs& a, size_t part_bytes, hipStream_t s) {
+  const Fp8Plan p = fp8_plan(a.M, a.M_stride, a.w.rows, a.w.kb, a.ctype == DT_F32, a.part ? part_bytes : 0);
+  return p.mt ? launch_fp8_tile(a, p.mt, p.splits, s) : launch_few_tokens(a, p, s);
 }
 
 }  // namespace qm

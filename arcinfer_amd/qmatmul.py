@@ -518,7 +518,8 @@ def swiglu_fp8(gu, F, gelu=False, M_stride=None, stream=None):
 
 
 def gemm_fp8_workspace(w, M):
-    """A workspace for products of M tokens with w (None where they need none)."""
+    """A workspace for products of M tokens with w (None where they need none). Its size does not grow with M: for calls of several
+    M take the largest, or 64 MiB, which serves every call."""
     import torch
     _sizes("qmatmul_gemm_fp8_workspace_size", M)
     n = load_library().qmatmul_gemm_fp8_workspace_size(w.handle, M)

@@ -297,8 +297,9 @@ int qmatmul_swiglu_fp8(const void* gu, int xtype, int ldg, int F, int M, int M_s
  * C of f32 the products are exact and every sum is f32. With a C of 16 bits the products run on the fp8 matrix pipe, twice as
  * fast, which drops from the sum of each eight neighbouring products what lies 2^-13 below the largest of them (1.3e-5 of the
  * result for normal values, far below C's rounding); the sums of eights and of blocks are f32. a8 is 16-byte aligned.
- * ws: device workspace, 256-byte aligned, of qmatmul_gemm_fp8_workspace_size(w, M) bytes (0 for many calls, never more than
- * 64 MiB; NULL or too small: the call runs without, slower); calls that may overlap need different workspaces. C and ws may not
+ * ws: device workspace, 256-byte aligned, of qmatmul_gemm_fp8_workspace_size(w, M) bytes; NULL or a smaller one: K is cut into
+ * fewer pieces or none, slower. The size is 0 for many M and does not grow with M (often 0 again for the largest): for calls of
+ * several M, the largest of their sizes, or 64 MiB, which is never exceeded. Calls that may overlap need different workspaces. C and ws may not
  * overlap a8, asc or each other. No allocation, no host synchronisation; the call can be captured into a graph. The weight's
  * device must be the current one. */
 size_t qmatmul_gemm_fp8_workspace_size(const qm_fp8_weight* w, int M);

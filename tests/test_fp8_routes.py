@@ -1,0 +1,77 @@
+"""The choice among the variants of the e4m3 product (host code of the built library, no GPU): at shapes where each side was measured the
+call takes the fastest, and a workspace that is too small for all pieces gets fewer. Times in microseconds, one MI355X."""
+import ctypes
+
+import pytest
+
+MOST = 64 << 20  # bytes of workspace that a call uses at most
+
+
+class Plan(ctypes.Structure):
+    _fields_ = [("mt", ctypes.c_int), ("splits", ctypes.c_int), ("rt", ctypes.c_int), ("waves", ctypes.c_int)]
+
+
+@pytest.fixture(scope="module")
+def plan():
+    from arcinfer_amd import qmatmul
+    f = qmatmul.load_library()._ZN2qm8fp8_planEiiiibm
+    f.restype, f.argtypes = Plan, [ctypes.c_int] * 4 + [ctypes.c_bool, ctypes.c_size_t]
+
+    def of(M, N, K, f32, ws=MOST):
+        p = f(M, (M + 15) // 16 * 16, N, (K + 127) // 128, f32, ws)
+        return (p.mt, p.splits) if p.mt else (0, p.rt, p.waves)
+    return of
+
+
+@pytest.mark.parametrize("M,N,K,f32,want", [
+    # few-token kernel
+    (32, 9000, 2048, False, (0, 2, 8)),     # 9.8 against 11.0 of the best tiles
+    (64, 2560, 2560, False, (0, 1, 8)),     # 8.9, 10.8
+    (130, 512, 1024, False, (0, 1, 8)),     # 5.0, 8.0
+    (64, 9000, 2048, True, (0, 2, 8)),      # 16.5, 16.7
+    (1024, 512, 1024, True, (0, 1, 8)),     # 9.3, 13.2
+    # tiles, whole
+    (260, 17408, 1024, False, (6, 1)),      # 12.5; the few-token kernel 36.2
+    (512, 4096, 4096, False, (4, 1)),       # 20.6; in two pieces 22.5
+    (1024, 2560, 2560, False, (4, 1)),      # 15.0; five token tiles 18.9
+    (2900, 9000, 2048, False, (7, 1)),      # 63.7; eight token tiles 65.7
+    (4096, 5120, 17408, False, (7, 1)),     # 328; eight token tiles 334
+    (512, 17408, 1024, True, (5, 1)),       # 26.9; six token tiles 31.6
+    (2048, 5120, 5120, True, (6, 1)),       # 110; four token tiles 113
+    # tiles, K in pieces
+    (64, 5120, 5120, False, (4, 5)),        # 14.2; whole 23.7, few tokens 16.5
+    (96, 2048, 12800, False, (4, 10)),      # 16.5; whole 53.0
+    (200, 5120, 17408, False, (7, 6)),      # 36.9; four token tiles, whole, 89
+    (80, 5120, 17408, True, (5, 12)),       # 31.1; whole 152
+    (333, 2048, 12800, True, (4, 10)),      # 32.6; in five 33.9
+    (420, 5120, 17408, True, (5, 4)),       # 90.7; whole 155
+])
+def test_the_fastest_is_taken(plan, M, N, K, f32, want):
+    assert plan(M, N, K, f32) == want
+
+
+@pytest.mark.parametrize("f32", [True, False])
+@pytest.mark.parametrize("M,N,K", [(66, 1021, 5791), (48, 5120, 17408), (777, 5120, 17408), (333, 5184, 5120), (130, 4096, 4096)])
+def test_a_smaller_workspace_has_fewer_pieces(plan, M, N, K, f32):
+    piece = 4 * M * ((N + 63) // 64 * 64)
+    mt, most = plan(M, N, K, f32)
+    assert mt and most > 1 and most * piece <= MOST
+    assert plan(M, N, K, f32, most * piece) == (mt, most)
+    less = plan(M, N, K, f32, most * piece - 1)  # (fewer pieces, or the few-token kernel where that is faster then)
+    assert not less[0] or less[1] < most and (less[1] > 1 or most == 2)
+    for ws in range(0, most * piece, piece // 2):
+        p = plan(M, N, K, f32, ws)
+        assert not p[0] or p[1] == 1 or p[1] * piece <= ws
+    assert len(plan(M, N, K, f32, 0)) == 3 or plan(M, N, K, f32, 0)[1] == 1
+    assert plan(M, N, K, f32, 1 << 40) == plan(M, N, K, f32)
+
+
+@pytest.mark.parametrize("M,N,K", [(40, 4096, 4096), (66, 1021, 5791), (48, 5120, 17408), (777, 5120, 17408), (1024, 5120, 17408), (2048, 5120, 17408)])
+def test_the_size_that_is_asked_for_holds_all_pieces(plan, M, N, K):
+    from arcinfer_amd import qmatmul
+    size = qmatmul.load_library()._ZN2qm19fp8_workspace_bytesEiii
+    size.restype, size.argtypes = ctypes.c_size_t, [ctypes.c_int] * 3
+    n = size(M, N, K // 128 + (K % 128 > 0))
+    assert n <= MOST
+    for f32 in (True, False):
+        assert plan(M, N, K, f32, n) == plan(M, N, K, f32)
