@@ -1,8 +1,13 @@
 """The choice among the variants of the e4m3 product (host code of the built library, no GPU): at shapes where each side was measured the
-call takes the fastest, and a workspace that is too small for all pieces gets fewer. Times in microseconds, one MI355X."""
+call takes the fastest, the products of tests/test_gpu_fp8.py and tests/test_gpu_fp8_variants.py run every variant that it can take, and a
+workspace that is too small for all pieces gets fewer. Times in microseconds, one MI355X."""
 import ctypes
+import math
+import random
 
 import pytest
+
+from tests import test_gpu_fp8, test_gpu_fp8_variants
 
 MOST = 64 << 20  # bytes of workspace that a call uses at most
 
@@ -48,6 +53,25 @@ def plan():
 ])
 def test_the_fastest_is_taken(plan, M, N, K, f32, want):
     assert plan(M, N, K, f32) == want
+
+
+def variants(plan, N, K, M):
+    for f32 in (True, False):
+        p = plan(M, N, K, f32)
+        if p[0]:
+            yield from ((f32, "tiles", p[0], p[1] > 1), (f32, "pieces", p[1]))
+        else:
+            yield f32, "few", min(4, (M + 15) // 16), *p[1:]
+
+
+def test_every_variant_is_tested(plan):
+    tested = {v for s in test_gpu_fp8.SHAPES + test_gpu_fp8.VARIANTS + test_gpu_fp8_variants.SHAPES for v in variants(plan, *s)}
+    rng = random.Random(0)
+    some = lambda a, b: int(math.exp(rng.uniform(math.log(a), math.log(b))))  # noqa: E731
+    for i in range(30000):
+        shape = some(1, 60000), some(1, 40000), some(1, 300 if i % 2 else 20000)
+        missing = set(variants(plan, *shape)) - tested
+        assert not missing, (shape, missing)
 
 
 @pytest.mark.parametrize("f32", [True, False])
