@@ -204,10 +204,15 @@ hipError_t rope_of(const RopeArgs& a, hipStream_t s) {
   unsigned gy = gx >= 1024 ? 1 : (1024 + gx - 1) / gx;  // few tokens: their heads over several work-groups
   if (gy > iters) gy = iters;
   const dim3 grid(gx, gy);
-  if (v == 8) qk_norm_rope_kernel<TI, TO, 8, 1, 2><<<grid, 256, 0, s>>>(a, tokens, lanes);
-  else if (v == 4) qk_norm_rope_kernel<TI, TO, 4, 1, 2><<<grid, 256, 0, s>>>(a, tokens, lanes);
-  else if (chunks <= 64) qk_norm_rope_kernel<TI, TO, 1, 1, 1><<<grid, 256, 0, s>>>(a, tokens, lanes);
-  else qk_norm_rope_kernel<TI, TO, 1, 4, 1><<<grid, 256, 0, s>>>(a, tokens, lanes);
+  if (v == 8) {
+    if constexpr (kRopeV8<TI, TO>) qk_norm_rope_kernel<TI, TO, 8, 1, 2><<<grid, 256, 0, s>>>(a, tokens, lanes);
+  } else if (v == 4) {
+    qk_norm_rope_kernel<TI, TO, 4, 1, 2><<<grid, 256, 0, s>>>(a, tokens, lanes);
+  } else if (chunks <= 64) {
+    qk_norm_rope_kernel<TI, TO, 1, 1, 1><<<grid, 256, 0, s>>>(a, tokens, lanes);
+  } else {
+    qk_norm_rope_kernel<TI, TO, 1, 4, 1><<<grid, 256, 0, s>>>(a, tokens, lanes);
+  }
   return hipGetLastError();
 }
 
