@@ -773,7 +773,9 @@ int qmatmul_prepare_fp8(const void* w8, const float* wsc, int on_device, int row
                         qm_fp8_weight** out) {
   if (!out || !w8 || !wsc) return fail(QM_ERR_ARG, "qmatmul_prepare_fp8: null pointer");
   *out = nullptr;
-  if (!fp8_shape_ok(rows, K)) return fail(QM_ERR_SHAPE, "qmatmul_prepare_fp8: rows %d, K %d", rows, K);
+  // (64 GiB: a launch that lays a weight out has a thread for each 16 bytes)
+  if (!fp8_shape_ok(rows, K) || fp8_payload_bytes(rows, K) > 16 * ((size_t)qm::kMostThreads - 255))
+    return fail(QM_ERR_SHAPE, "qmatmul_prepare_fp8: rows %d, K %d", rows, K);
   if (!aligned(wsc, 4)) return fail(QM_ERR_ARG, "qmatmul_prepare_fp8: the scales must be 4-byte aligned");
   QM_CHECK_INIT();
   hipStream_t s = (hipStream_t)stream;

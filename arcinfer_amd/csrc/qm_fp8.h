@@ -15,6 +15,8 @@
 
 namespace qm {
 
+constexpr long long kMostThreads = (1LL << 32) - 1;  // of one dimension of a grid
+
 enum : int { DT_F32 = 0, DT_F16 = 1, DT_BF16 = 30 };
 
 struct Fp8View {

@@ -148,6 +148,9 @@ FewShape few_shape(int M, int rows, int kb) {
 }
 
 hipError_t launch_few_tokens(const Fp8GemmArgs& a, const Fp8Plan& f, hipStream_t s) {
+  // (only products that the tile kernel cannot take, of activations beyond 128 GiB, come to that many)
+  const long long mt = a.M > 48 ? 4 : (a.M + 15) / 16, turns = (a.M + 16 * mt - 1) / (16 * mt), units = (a.w.rows + 63) / 64 * 4 / f.rt;
+  if (units * turns * 64 * f.waves > kMostThreads) return hipErrorInvalidConfiguration;
 #define QM_FEW(MT, RT) (f.waves == 8 ? launch_few<MT, RT, 8>(a, s) : launch_few<MT, RT, 4>(a, s))
   if (a.M <= 16) {
     if (f.waves == 16) f.rt == 1 ? launch_few<1, 1, 16>(a, s) : launch_few<1, 2, 16>(a, s);

@@ -184,8 +184,8 @@ bool rows_aligned(const void* p, int ld, int K, int size) {
 }
 
 template <typename T>
-hipError_t rows_of(const T* x, int ldx, int K, int M, int M_stride, int op, uint8_t* a8, float* asc, hipStream_t s) {
-  const unsigned grid = (unsigned)M_stride * ((K + 2047) / 2048);
+hipError_t rows_of(const T* x, int ldx, int K, int M, int rows, int M_stride, int op, uint8_t* a8, float* asc, hipStream_t s) {
+  const unsigned grid = (unsigned)rows * ((K + 2047) / 2048);
   const bool vec = rows_aligned(x, ldx, K, sizeof(T)) && (op == ROWS || (size_t)K * sizeof(T) % 16 == 0);
 #define QM_F8R(OP) \
   if (vec) fp8_rows_kernel<T, true, OP><<<grid, 256, 0, s>>>(x, ldx, K, M, M_stride, a8, asc); \
@@ -198,10 +198,10 @@ hipError_t rows_of(const T* x, int ldx, int K, int M, int M_stride, int op, uint
 }
 
 template <typename T, bool VEC>
-hipError_t norm_of(const T* x, int ldx, const float* w, int K, int M, int M_stride, float eps, uint8_t* a8, float* asc,
+hipError_t norm_of(const T* x, int ldx, const float* w, int K, int M, int rows, int M_stride, float eps, uint8_t* a8, float* asc,
                    float* h, int ldh, hipStream_t s) {
   const int passes = (K + 2047) / 2048;
-  const dim3 grid(M_stride, M_stride < 256 ? passes : 1);  // (few rows: the GPU would be nearly idle)
+  const dim3 grid(rows, M_stride < 256 ? passes : 1);  // (few rows: the GPU would be nearly idle)
 #define QM_F8N(P) fp8_rmsnorm_kernel<T, VEC, P><<<grid, 256, 0, s>>>(x, ldx, w, K, M, M_stride, eps, a8, asc, h, ldh)
   if (passes <= 1) QM_F8N(1);
   else if (passes <= 2) QM_F8N(2);
@@ -212,19 +212,41 @@ hipError_t norm_of(const T* x, int ldx, const float* w, int K, int M, int M_stri
   return hipGetLastError();
 }
 
+// A launch for as many rows as a grid holds, of `groups` work-groups each: f(first row, rows)
+template <typename F>
+hipError_t by_grids(int M_stride, int groups, F f) {
+  const int most = (int)(kMostThreads / 256 / groups);
+  for (int m0 = 0;; m0 += most) {
+    const int rows = M_stride - m0 < most ? M_stride - m0 : most;
+    const hipError_t e = f(m0, rows);
+    if (e != hipSuccess || m0 + rows == M_stride) return e;
+  }
+}
+
 template <typename T>
 hipError_t norm_any(const T* x, int ldx, const float* w, int K, int M, int M_stride, float eps, uint8_t* a8, float* asc,
                     float* h, int ldh, hipStream_t s) {
-  if (rows_aligned(x, ldx, K, sizeof(T)) && (uintptr_t)w % 16 == 0)
-    return norm_of<T, true>(x, ldx, w, K, M, M_stride, eps, a8, asc, h, ldh, s);
-  return norm_of<T, false>(x, ldx, w, K, M, M_stride, eps, a8, asc, h, ldh, s);
+  const size_t kp = ((size_t)K + 127) / 128 * 128;
+  const bool vec = rows_aligned(x, ldx, K, sizeof(T)) && (uintptr_t)w % 16 == 0;
+  return by_grids(M_stride, 1, [&](int m0, int rows) {
+    const T* xr = x + (size_t)m0 * ldx;
+    float* hr = h ? h + (size_t)m0 * ldh : nullptr;
+    return vec ? norm_of<T, true>(xr, ldx, w, K, M - m0, rows, M_stride, eps, a8 + m0 * kp, asc + m0, hr, ldh, s)
+               : norm_of<T, false>(xr, ldx, w, K, M - m0, rows, M_stride, eps, a8 + m0 * kp, asc + m0, hr, ldh, s);
+  });
 }
 
 hipError_t rows_any(const void* x, int xtype, int ldx, int K, int M, int M_stride, int op, uint8_t* a8, float* asc,
                     hipStream_t s) {
-  if (xtype == DT_F32) return rows_of((const float*)x, ldx, K, M, M_stride, op, a8, asc, s);
-  if (xtype == DT_F16) return rows_of((const _Float16*)x, ldx, K, M, M_stride, op, a8, asc, s);
-  return rows_of((const __bf16*)x, ldx, K, M, M_stride, op, a8, asc, s);
+  const size_t kp = ((size_t)K + 127) / 128 * 128;
+  return by_grids(M_stride, (K + 2047) / 2048, [&](int m0, int rows) {
+    const size_t at = (size_t)m0 * ldx;
+    uint8_t* qr = a8 + m0 * kp;
+    float* sr = asc + m0;
+    if (xtype == DT_F32) return rows_of((const float*)x + at, ldx, K, M - m0, rows, M_stride, op, qr, sr, s);
+    if (xtype == DT_F16) return rows_of((const _Float16*)x + at, ldx, K, M - m0, rows, M_stride, op, qr, sr, s);
+    return rows_of((const __bf16*)x + at, ldx, K, M - m0, rows, M_stride, op, qr, sr, s);
+  });
 }
 
 }  // namespace

@@ -226,9 +226,19 @@ hipError_t rope_to(const RopeArgs& a, hipStream_t s) {
 }  // namespace
 
 hipError_t launch_qk_norm_rope(const RopeArgs& a, hipStream_t s) {
-  if (a.xtype == DT_F32) return rope_to<float>(a, s);
-  if (a.xtype == DT_F16) return rope_to<_Float16>(a, s);
-  return rope_to<__bf16>(a, s);
+  // a launch for as many tokens as a grid holds for certain
+  constexpr int kMost = (int)(kMostThreads / 256);
+  const size_t si = a.xtype == DT_F32 ? 4 : 2, so = a.otype == DT_F32 ? 4 : 2;
+  RopeArgs b = a;
+  for (int t0 = 0;; t0 += kMost) {
+    b.T = a.T - t0 < kMost ? a.T - t0 : kMost;
+    const hipError_t e = a.xtype == DT_F32 ? rope_to<float>(b, s) : a.xtype == DT_F16 ? rope_to<_Float16>(b, s) : rope_to<__bf16>(b, s);
+    if (e != hipSuccess || t0 + b.T == a.T) return e;
+    b.x = (const char*)b.x + kMost * si * (size_t)a.ldx;
+    if (b.q) b.q = (char*)b.q + kMost * so * (size_t)a.ldq;
+    if (b.k) b.k = (char*)b.k + kMost * so * (size_t)a.ldk;
+    if (b.pos) b.pos += kMost;
+  }
 }
 
 }  // namespace qm

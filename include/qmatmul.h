@@ -265,9 +265,9 @@ typedef struct qm_fp8_weight qm_fp8_weight; /* opaque: a prepared e4m3 weight ma
 size_t qmatmul_fp8_weight_bytes(int rows, int K);
 
 /* Prepares a weight: w8 e4m3 [rows][K] row-major and wsc float [ceil(rows/128)][ceil(K/128)], the scale each block is
- * multiplied by (the last blocks of a row or column may be cut: any rows >= 1, K from 1 to 2^24). Both are device pointers if
- * on_device, else host pointers (the call then waits for the copy). The layout is this library's own; the sources may be
- * freed once the stream has passed the call. The weight belongs to the current device. */
+ * multiplied by (the last blocks of a row or column may be cut: any rows >= 1, K from 1 to 2^24, below 64 GiB in all). Both are
+ * device pointers if on_device, else host pointers (the call then waits for the copy). The layout is this library's own; the
+ * sources may be freed once the stream has passed the call. The weight belongs to the current device. */
 int qmatmul_prepare_fp8(const void* w8, const float* wsc, int on_device, int rows, int K, void* stream,
                         qm_fp8_weight** out);
 /* Frees a prepared weight (waits for the device). */
