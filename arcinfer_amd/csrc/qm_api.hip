@@ -879,7 +879,7 @@ static int check_fp8_apart(const char* fn, const HeadRows& rows, int M_stride, i
 // what the three producers share: input rows of `width` elements, outputs of K values
 static int check_fp8_rows(const char* fn, const void* x, int xtype, int ldx, long long width, int M, int M_stride, int K,
                           const uint8_t* a8, const float* asc) {
-  if (!x || !a8 || !asc) return fail(QM_ERR_ARG, "%s: null pointer", fn);
+  if ((!x && M) || !a8 || !asc) return fail(QM_ERR_ARG, "%s: null pointer", fn);
   if (!dtype_ok(xtype)) return fail(QM_ERR_TYPE, "%s: input type %d (QM_F32, QM_F16 or QM_BF16)", fn, xtype);
   if (K < 1 || K > 1 << 24 || M < 0 || M_stride < 1 || M > M_stride || ldx < width)
     return fail(QM_ERR_SHAPE, "%s: M %d, M_stride %d, K %d, row stride %d", fn, M, M_stride, K, ldx);

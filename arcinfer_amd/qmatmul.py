@@ -461,10 +461,13 @@ class Fp8Weight:
 
 
 def _out_fp8(fn, x, M, K, M_stride):
-    """(M_stride, ldx, a8, asc) of a producer's rows x."""
+    """(M_stride, ldx, a8, asc) of a producer's rows x; where M_stride is 0 there is nothing to call for."""
     Ms, ldx = M if M_stride is None else M_stride, _row_stride(x)
-    if (M | Ms | K | ldx) >> 31:
+    if (M | Ms | K | ldx) >> 31 or Ms == 0:
         _sizes(fn, M, Ms, K, ldx)
+        _dtype(x.dtype)
+        if Ms < M or K < 1:
+            _refuse(fn, f"M {M}, M_stride {Ms}, K {K}")
     Kp = (K + 127) // 128 * 128
     return (Ms, ldx, x.new_empty((Ms, Kp), dtype=_torch.float8_e4m3fn), x.new_empty((Kp // 128, Ms), dtype=_torch.float32))
 
@@ -477,6 +480,8 @@ def quantize_fp8(x, M_stride=None, stream=None):
     _check_rows(fn, "x", x, 2, dev)
     M, K = x.shape
     Ms, ldx, a8, asc = _out_fp8(fn, x, M, K, M_stride)
+    if Ms == 0:
+        return a8, asc
     st = _function(fn)(x.data_ptr(), _dtype(x.dtype), ldx, M, Ms, K, a8.data_ptr(), asc.data_ptr(),
                        _current_stream(dev) if stream is None else stream)
     _done(fn, st)
@@ -495,6 +500,8 @@ def rmsnorm_fp8(x, w, eps, M_stride=None, want_h=False, stream=None):
         _refuse(fn, f"w {tuple(w.shape)} {w.dtype}: float32, one for each of {K} columns")
     Ms, ldx, a8, asc = _out_fp8(fn, x, M, K, M_stride)
     h = x.new_empty((M, K), dtype=torch.float32) if want_h else None
+    if Ms == 0:
+        return a8, asc, h
     st = _function(fn)(x.data_ptr(), _dtype(x.dtype), ldx, w.data_ptr(), K, M, Ms, eps, a8.data_ptr(),
                        asc.data_ptr(), h.data_ptr() if want_h and M else None, K,
                        _current_stream(dev) if stream is None else stream)
@@ -511,6 +518,8 @@ def swiglu_fp8(gu, F, gelu=False, M_stride=None, stream=None):
     if gu.size(1) < 2 * F:
         _refuse(fn, f"rows of {gu.shape[1]} elements hold no gate and up of {F}")
     Ms, ldg, a8, asc = _out_fp8(fn, gu, M, F, M_stride)
+    if Ms == 0:
+        return a8, asc
     st = _function(fn)(gu.data_ptr(), _dtype(gu.dtype), ldg, F, M, Ms, 1 if gelu else 0, a8.data_ptr(),
                        asc.data_ptr(), _current_stream(dev) if stream is None else stream)
     _done(fn, st)
@@ -545,6 +554,8 @@ def gemm_fp8(w, a8, asc, M=None, C=None, ldc=None, c_off=0, accumulate=0, out=No
         _refuse(fn, f"asc {tuple(asc.shape)} {asc.dtype}: contiguous float32 [{Kp // 128}, {Ms}]")
     if (M | Ms | c_off | accumulate) >> 31:
         _sizes(fn, M, Ms, c_off, accumulate)
+        if M < 0:
+            _refuse(fn, f"M {M}")
     if C is None:
         if accumulate or c_off or ldc is not None:
             _refuse(fn, "accumulate, c_off and ldc need a C")
@@ -624,6 +635,8 @@ def qk_norm_rope(x, HQ, HK, D, pos, inv_freq, wq=None, wk=None, eps=1e-6, adjace
     ldx, ps = _row_stride(x), pos.stride(0) if axes > 1 else T
     if (T | D | HQ | HK | ldx | ps | q_off | q_hs | k_off | k_hs | 2 * half) >> 31 or axes > 1:
         _sizes(fn, T, D, HQ, HK, ldx, ps, q_off, q_hs, k_off, k_hs, 2 * half, *sections)
+        if min(D, HQ, HK) < 0:
+            _refuse(fn, f"D {D}, HQ {HQ}, HK {HK}")
     if (HQ and q_off + (HQ - 1) * q_hs + D > width) or (HK and k_off + (HK - 1) * k_hs + D > width):
         _refuse(fn, f"rows of {width} elements do not hold the heads")
     if out is None:

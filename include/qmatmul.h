@@ -283,7 +283,8 @@ int qmatmul_fp8_info(const qm_fp8_weight* w, int* rows, int* K, int* Kp);
  * ldh, rows < M) receives y; an h that overlaps x is refused.   qmatmul_swiglu_fp8: y = silu(gate) * up (gelu_tanh(gate) *
  * up with gelu) from rows [gate(F) | up(F)], an infinite gate giving NaN. y is computed in f32 (of the gate's exponential, what is
  * below 2^-126 may count as zero). Rows that are 16-byte aligned (base and stride) and of a
- * K % 8 == 0 are read 16 bytes at a time, others by the element. Outputs that overlap the input or each other are refused. */
+ * K % 8 == 0 are read 16 bytes at a time, others by the element. Outputs that overlap the input or each other are refused. M may be 0
+ * (x NULL): M_stride rows of zeros, at least one. */
 int qmatmul_quantize_fp8(const void* x, int xtype, int ldx, int M, int M_stride, int K, uint8_t* a8, float* asc,
                          void* stream);
 int qmatmul_rmsnorm_fp8(const void* x, int xtype, int ldx, const float* w, int K, int M, int M_stride, float eps,

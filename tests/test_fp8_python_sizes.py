@@ -95,3 +95,21 @@ def test_far_sizes_are_refused(qm, calls):
         with pytest.raises(qm.QMatmulError):
             bad()
     assert not calls
+
+
+def test_no_rows_and_negative_counts(qm, calls):
+    """A batch of no rows has empty results, without a call; counts below zero are the library's own errors."""
+    for x in (meta(0, 300), meta(0, 300, dtype=torch.bfloat16)):
+        for a8, asc, *_ in (qm.quantize_fp8(x), qm.rmsnorm_fp8(x, meta(300), 1e-6, want_h=True), qm.swiglu_fp8(meta(0, 600), 300)):
+            assert a8.shape == (0, 384) and asc.shape == (3, 0)
+    assert not calls
+    qm.quantize_fp8(meta(0, 300), M_stride=4)
+    assert calls.pop()[1][3:6] == (0, 4, 300)
+    for bad in (lambda: qm.quantize_fp8(meta(3, 300), M_stride=-1), lambda: qm.quantize_fp8(meta(0, 300), M_stride=-1),
+                lambda: qm.quantize_fp8(meta(3, 300), M_stride=0), lambda: qm.quantize_fp8(meta(0, 300, dtype=torch.int32)),
+                lambda: qm.quantize_fp8(meta(0, 0)), lambda: qm.swiglu_fp8(meta(0, 600), 0), lambda: qm.swiglu_fp8(meta(3, 600), -200),
+                lambda: product(qm, M=-1), lambda: product(qm, M=-1, C=meta(3, 200)),
+                *(lambda H=H: qm.qk_norm_rope(meta(3, 384), *H, meta(3, dtype=torch.int32), meta(32)) for H in ((-1, 2, 64), (4, -2, 64), (4, 2, -64)))):
+        with pytest.raises(qm.QMatmulError):
+            bad()
+    assert not calls
