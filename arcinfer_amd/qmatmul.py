@@ -462,7 +462,7 @@ class Fp8Weight:
 
 def _out_fp8(fn, x, M, K, M_stride):
     """(M_stride, ldx, a8, asc) of a producer's rows x; where M_stride is 0 there is nothing to call for."""
-    Ms, ldx = M if M_stride is None else M_stride, _row_stride(x)
+    Ms, ldx = M if M_stride is None else M_stride, x.stride(0) if M > 1 else _row_stride(x)
     if (M | Ms | K | ldx) >> 31 or Ms == 0:
         _sizes(fn, M, Ms, K, ldx)
         _dtype(x.dtype)
@@ -632,8 +632,9 @@ def qk_norm_rope(x, HQ, HK, D, pos, inv_freq, wq=None, wk=None, eps=1e-6, adjace
         k_hs = D
     if k_off is None:
         k_off = q_off + HQ * q_hs
-    ldx, ps = _row_stride(x), pos.stride(0) if axes > 1 else T
-    if (T | D | HQ | HK | ldx | ps | q_off | q_hs | k_off | k_hs | 2 * half) >> 31 or axes > 1:
+    ldx, ps = x.stride(0) if T > 1 else _row_stride(x), pos.stride(0) if axes > 1 else T
+    # (sections of none below zero are within their sum)
+    if (T | D | HQ | HK | ldx | ps | q_off | q_hs | k_off | k_hs | 2 * half) >> 31 or (axes > 1 and min(sections) < 0):
         _sizes(fn, T, D, HQ, HK, ldx, ps, q_off, q_hs, k_off, k_hs, 2 * half, *sections)
         if min(D, HQ, HK) < 0:
             _refuse(fn, f"D {D}, HQ {HQ}, HK {HK}")
