@@ -946,8 +946,9 @@ int qmatmul_gemm_fp8(const qm_fp8_weight* w, const uint8_t* a8, const float* asc
   const hipError_t ed = hipGetDevice(&dev);
   if (ed != hipSuccess) return hip_fail(ed, fn);
   if (dev != w->device) return fail(QM_ERR_ARG, "%s: the weight is on device %d, the current device is %d", fn, w->device, dev);
-  const int Kp = 128 * w->view.kb;
-  const size_t size = dtype_size(ctype), na = fp8_rows_bytes(M_stride, Kp), ns = fp8_scales_bytes(M_stride, Kp);
+  // (M rows of a8 and of each scale row: the call may be for a part of a longer batch)
+  const size_t size = dtype_size(ctype), na = (size_t)M * 128 * w->view.kb;
+  const size_t ns = ((size_t)(w->view.kb - 1) * M_stride + M) * sizeof(float);
   const HeadRows c{(const char*)C + (size_t)c_off * size, M, w->rows, 1, w->rows, ldc, (long long)size};
   const uintptr_t wsp = (uintptr_t)ws;
   if (span_overlaps(c, a8, na) || span_overlaps(c, asc, ns) || span_overlaps(c, ws, ws ? ws_bytes : 0) ||

@@ -58,9 +58,10 @@ def test_products(qm, dev):
     f = lambda **k: lib.qmatmul_gemm_fp8(*{**dict(w=w.handle, a=p, s=p + 8192, M=M, Ms=8, C=p + 16384, t=0, ldc=N, off=0, acc=0,  # noqa: E731
                                                   ws=p + 65536, wsb=65536, st=qm._stream(None)), **k}.values())
     row = 4 * N
-    for bad in (dict(C=p), dict(C=p + 2044), dict(C=p + 8192 - 5 * row + 4), dict(C=p + 8192), dict(C=p + 65536), dict(ws=p), dict(ws=p + 8192),
-                dict(ws=p + 16384 + 4 * row), dict(ldc=1024, C=p + 65536 - 4096), dict(ldc=2048, off=1024, C=p - 4096 + 2044)):
+    for bad in (dict(C=p), dict(C=p + 1276), dict(C=p + 8192 - 5 * row + 4), dict(C=p + 8192), dict(C=p + 65536), dict(ws=p), dict(ws=p + 8192),
+                dict(ws=p + 16384 + 4 * row), dict(ldc=1024, C=p + 65536 - 4096), dict(ldc=2048, off=1024, C=p - 4096 + 1276)):
         assert is_overlap(qm, f(**bad)), bad
     assert not buf.any()
+    assert f(C=p + 1280) == 0 and f(Ms=4096, C=p + 1280) == 0  # (behind the call's own rows: it may be a part of a longer batch)
     assert f() == 0 and f(ws=None, wsb=0) == 0 and f(ws=p, wsb=0) == 0 and f(ldc=1024, C=p + 8192 + 256) == 0
     w.release()
