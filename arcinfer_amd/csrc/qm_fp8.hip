@@ -147,10 +147,15 @@ FewShape few_shape(int M, int rows, int kb) {
   return {rt, w};
 }
 
+// Whether its work-groups fit a grid (those of up to 16 tokens do: a weight is below 64 GiB)
+bool few_fits(int M, int rows, FewShape f) {
+  const long long mt = M > 48 ? 4 : (M + 15) / 16, turns = (M + 16 * mt - 1) / (16 * mt), units = (rows + 63) / 64 * 4 / f.rt;
+  return units * turns * 64 * f.waves <= kMostThreads;
+}
+
 hipError_t launch_few_tokens(const Fp8GemmArgs& a, const Fp8Plan& f, hipStream_t s) {
   // (only products that the tile kernel cannot take, of activations beyond 128 GiB, come to that many)
-  const long long mt = a.M > 48 ? 4 : (a.M + 15) / 16, turns = (a.M + 16 * mt - 1) / (16 * mt), units = (a.w.rows + 63) / 64 * 4 / f.rt;
-  if (units * turns * 64 * f.waves > kMostThreads) return hipErrorInvalidConfiguration;
+  if (!few_fits(a.M, a.w.rows, {f.rt, f.waves})) return hipErrorInvalidConfiguration;
 #define QM_FEW(MT, RT) (f.waves == 8 ? launch_few<MT, RT, 8>(a, s) : launch_few<MT, RT, 4>(a, s))
   if (a.M <= 16) {
     if (f.waves == 16) f.rt == 1 ? launch_few<1, 1, 16>(a, s) : launch_few<1, 2, 16>(a, s);
@@ -211,7 +216,7 @@ Fp8Plan fp8_plan(int M, int M_stride, int rows, int kb, bool exact, size_t part_
   // (the tile kernel's token scales are a buffer of 32-bit offsets)
   if (M <= 16 || (size_t)kb * M_stride >= (size_t)1 << 30) return p;
   const Rates& r = exact ? kRates32 : kRates16;
-  float best = M <= 1024 ? few_us(r, exact ? 0.0f : kFewBlock16, M, rows, kb) : 1e30f;
+  float best = M <= 1024 && few_fits(M, rows, f) ? few_us(r, exact ? 0.0f : kFewBlock16, M, rows, kb) : 1e30f;
   constexpr int kSplits[] = {1, 2, 3, 4, 5, 6, 8, 10, 12, 16};
   for (int mt = exact ? 6 : 8; mt >= 4; --mt) {
     for (int s : kSplits) {

@@ -75,6 +75,23 @@ def test_every_variant_is_tested(plan):
 
 
 @pytest.mark.parametrize("f32", [True, False])
+def test_work_groups_fit_a_grid(plan, f32):
+    """The most rows of a weight, and tokens whose C is within the card's memory: 2^32 threads are not reached."""
+    for K in (1, 128, 256, 900, 1100, 2048, 1 << 14, 1 << 24):
+        for N in (((1 << 36) - 4096) // ((K + 127) // 128 * 128) // 64 * 64, (1 << 32) // ((K + 127) // 128 * 128)):
+            for M in (1, 16, 17, 33, 64, 100, 300, 512, 1000, 1024, 5000, 1 << 20):
+                if M * N * (4 if f32 else 2) > 288 << 30:
+                    continue
+                p = plan(M, N, K, f32)
+                if p[0]:
+                    groups, waves = (N + 255) // 256 * ((M + 16 * p[0] - 1) // (16 * p[0])) * p[1], 4
+                else:
+                    mt = min(4, (M + 15) // 16)
+                    groups, waves = (N + 63) // 64 * 4 // p[1] * ((M + 16 * mt - 1) // (16 * mt)), p[2]
+                assert 0 < groups * 64 * waves < 1 << 32, (M, N, K, p)
+
+
+@pytest.mark.parametrize("f32", [True, False])
 @pytest.mark.parametrize("M,N,K", [(66, 1021, 5791), (48, 5120, 17408), (777, 5120, 17408), (333, 5184, 5120), (130, 4096, 4096)])
 def test_a_smaller_workspace_has_fewer_pieces(plan, M, N, K, f32):
     piece = 4 * M * ((N + 63) // 64 * 64)
