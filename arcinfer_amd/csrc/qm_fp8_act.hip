@@ -69,18 +69,19 @@ __device__ __forceinline__ float exp_fast(float x) {
   const float e = __builtin_amdgcn_exp2f(h);
   return fmaf(e, l * 0.693147181f, e);
 }
-// x / (1 + e^-z): silu for z = x. By t = e^-|z|, which is one at most: x / (1 + t), and x t / (1 + t) where z is negative, so that a far
-// gate is as exact as a near one and what is left of it goes to zero whatever x is (t below 2^-126 may be zero). The quotient by a reciprocal
-// and one correction, within 2 steps (the correctly rounded division and expf took more of the vector pipe than the rows take of HBM:
-// 2048 rows of 17408 in bf16 45.9 us against 40.7). A NaN of x stays one, an infinite x becomes one.
+// x / (1 + e^-z): silu for z = x. The quotient by a reciprocal and one correction, within 2 steps (the correctly rounded division and expf
+// took more of the vector pipe than the rows take of HBM: 2048 rows of 17408 in bf16 45.9 us against 40.2). The exponent is kept where
+// e and the sum are finite; what lies beyond is far_gated's. A NaN of x stays one, an infinite x becomes one.
+constexpr float kFar = -83.0f;  // (e^83 is over 2^119)
 __device__ __forceinline__ float gated(float x, float z) {
-  const float t = exp_fast(fmaxf(-fabsf(z), -104.0f)), d = 1.0f + t, n = z < 0.0f ? x * t : x;
-  const float r = __builtin_amdgcn_rcpf(d), q = n * r;
-  return fmaf(fmaf(-d, q, n), r, q);
+  const float d = 1.0f + exp_fast(fminf(fmaxf(-z, -104.0f), -kFar));
+  const float r = __builtin_amdgcn_rcpf(d), q = x * r;
+  return fmaf(fmaf(-d, q, x), r, q);
 }
-__device__ __forceinline__ float silu(float x) { return gated(x, x); }
-// 0.5 x (1 + tanh z), z = sqrt(2 / pi) (x + 0.044715 x^3): 1 + tanh z is 2 / (1 + e^-2z)
-__device__ __forceinline__ float gelu_tanh(float x) { return gated(x, 1.59576912f * fmaf(0.044715f * x * x, x, x)); }
+// The same for z below kFar, where the sum is its exponential: x e^z, of which what is below 2^-126 may be zero
+__device__ __forceinline__ float far_gated(float x, float z) { return x * exp_fast(fmaxf(z, -104.0f)); }
+// gelu: 0.5 x (1 + tanh y), y = sqrt(2 / pi) (x + 0.044715 x^3): 1 + tanh y is 2 / (1 + e^-2y)
+__device__ __forceinline__ float gelu_z(float x) { return 1.59576912f * fmaf(0.044715f * x * x, x, x); }
 
 enum : int { ROWS = 0, SILU = 1, GELU = 2 };
 
@@ -99,8 +100,19 @@ __global__ __launch_bounds__(256) void fp8_rows_kernel(const T* __restrict__ x, 
     if constexpr (OP != ROWS) {
       float u[8];
       load8<T, VEC>(r + K, at, K, u);
+      float z[8], low = 0.0f, g[8];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] = (OP == SILU ? silu(v[j]) : gelu_tanh(v[j])) * u[j];
+      for (int j = 0; j < 8; ++j) {
+        z[j] = OP == SILU ? v[j] : gelu_z(v[j]);
+        g[j] = v[j];
+        low = fminf(low, z[j]);
+        v[j] = gated(g[j], z[j]) * u[j];
+      }
+      if (low < kFar) {  // (hardly ever: a branch for eight values)
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          if (z[j] < kFar) v[j] = far_gated(g[j], z[j]) * u[j];
+      }
     }
   }
   quant16(v, at < kp, m, at, M_stride, kp, a8, asc);
