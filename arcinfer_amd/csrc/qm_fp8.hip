@@ -172,8 +172,9 @@ hipError_t launch_few_tokens(const Fp8GemmArgs& a, const Fp8Plan& f, hipStream_t
   return hipGetLastError();
 }
 
-// Times in microseconds, fitted to 2900 (C of 16 bits) and 1700 (f32) measured products of 20 to 4096 tokens and ten weights from
-// 512 x 1024 to 17408 x 5120 (rms 9 and 7 %; what the choice by them costs against the best of all variants: 2.9 and 1.5 %).
+// Times in microseconds, fitted to those of profiles/fp8_variants.txt: 7300 (C of 16 bits) and 4460 (f32) of 200 products of 20 to 4096
+// tokens and ten weights from 512 x 1024 to 17408 x 5120 (rms 9 and 7 %). The choice by them loses 3.0 and 1.6 % on average against the
+// fastest variant, 37 and 28 % at most (64 x 5120 -> 17408, 64 x 4096 -> 4096).
 // Tile kernel: `call`; a work-group's blocks and `more` (its prologue and store), each block one + one_mt * MT where work-groups have
 // their CU to themselves (`crowd` of it more with every CU taken), two + two_mt * MT where two share it, a last round behind
 // others `tail` of that; never less than the weight's bytes at `stream` a microsecond; cut: `sum`, and the pieces written and read at `part`.
