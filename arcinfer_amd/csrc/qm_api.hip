@@ -950,9 +950,12 @@ int qmatmul_gemm_fp8(const qm_fp8_weight* w, const uint8_t* a8, const float* asc
   const size_t size = dtype_size(ctype), na = (size_t)M * 128 * w->view.kb;
   const size_t ns = ((size_t)(w->view.kb - 1) * M_stride + M) * sizeof(float);
   const HeadRows c{(const char*)C + (size_t)c_off * size, M, w->rows, 1, w->rows, ldc, (long long)size};
+  // (and of the workspace what this call's pieces take)
+  const qm::Fp8Plan plan = qm::fp8_plan(M, M_stride, w->rows, w->view.kb, ctype == QM_F32, ws ? ws_bytes : 0);
+  const size_t nw = plan.splits > 1 ? qm::fp8_part_bytes(M, w->rows, plan.splits) : 0;
   const uintptr_t wsp = (uintptr_t)ws;
-  if (span_overlaps(c, a8, na) || span_overlaps(c, asc, ns) || span_overlaps(c, ws, ws ? ws_bytes : 0) ||
-      (ws && ((wsp < (uintptr_t)a8 + na && (uintptr_t)a8 < wsp + ws_bytes) || (wsp < (uintptr_t)asc + ns && (uintptr_t)asc < wsp + ws_bytes))))
+  if (span_overlaps(c, a8, na) || span_overlaps(c, asc, ns) || span_overlaps(c, ws, nw) ||
+      (nw && ((wsp < (uintptr_t)a8 + na && (uintptr_t)a8 < wsp + nw) || (wsp < (uintptr_t)asc + ns && (uintptr_t)asc < wsp + nw))))
     return fail(QM_ERR_ARG, "%s: C or the workspace overlaps the activations or the other", fn);
   qm::Fp8GemmArgs a{};
   a.w = w->view;
@@ -966,7 +969,7 @@ int qmatmul_gemm_fp8(const qm_fp8_weight* w, const uint8_t* a8, const float* asc
   a.c_off = c_off;
   a.accumulate = accumulate;
   a.part = (float*)ws;
-  const hipError_t e = qm::launch_gemm_fp8(a, ws_bytes, (hipStream_t)stream);
+  const hipError_t e = qm::launch_gemm_fp8(a, plan, (hipStream_t)stream);
   return e == hipSuccess ? QM_OK : hip_fail(e, fn);
 }
 

@@ -32,7 +32,7 @@ struct Fp8GemmArgs {
   int M, M_stride;
   void* C;
   int ctype, ldc, c_off, accumulate;
-  float* part;  // partial results of calls whose K is cut (null: none is)
+  float* part;  // partial results of calls whose K is cut
 };
 hipError_t launch_fp8_repack(const uint8_t* w8, int rows, int K, uint8_t* q, hipStream_t s);
 // Workspace for the pieces of cut products (0: the call is not cut)
@@ -42,9 +42,9 @@ size_t fp8_workspace_bytes(int M, int rows, int kb);
 struct Fp8Plan {
   int mt, splits, rt, waves;
 };
+// part_bytes: the workspace at hand (less than the call would use: fewer pieces)
 Fp8Plan fp8_plan(int M, int M_stride, int rows, int kb, bool exact, size_t part_bytes);
-// part_bytes: what a.part holds (less than the call would use: fewer pieces)
-hipError_t launch_gemm_fp8(const Fp8GemmArgs& a, size_t part_bytes, hipStream_t s);
+hipError_t launch_gemm_fp8(const Fp8GemmArgs& a, const Fp8Plan& plan, hipStream_t s);
 
 // The tile kernel (qm_fp8_tile.hip): tiles of 256 rows x 16 mt tokens (mt 4..8, 4..6 for a C of f32), K in `splits` pieces
 constexpr int kFp8Slots = 512;                    // its work-groups that the chip holds at once (two per CU)

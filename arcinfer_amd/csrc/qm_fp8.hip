@@ -244,8 +244,7 @@ size_t fp8_workspace_bytes(int M, int rows, int kb) {
   return most;
 }
 
-hipError_t launch_gemm_fp8(const Fp8GemmArgs& a, size_t part_bytes, hipStream_t s) {
-  const Fp8Plan p = fp8_plan(a.M, a.M_stride, a.w.rows, a.w.kb, a.ctype == DT_F32, a.part ? part_bytes : 0);
+hipError_t launch_gemm_fp8(const Fp8GemmArgs& a, const Fp8Plan& p, hipStream_t s) {
   return p.mt ? launch_fp8_tile(a, p.mt, p.splits, s) : launch_few_tokens(a, p, s);
 }
 

@@ -414,6 +414,7 @@ def _stride_of(ld, length, rows):
 
 
 def _row_stride(t):
+    """The row stride of a matrix in elements."""
     ld = t.stride(0)
     return ld if t.size(0) > 1 else _stride_of(ld, t.size(1), 1)
 

@@ -282,9 +282,9 @@ int qmatmul_fp8_info(const qm_fp8_weight* w, int* rows, int* K, int* Kp);
  * qmatmul_quantize_fp8: y = x.   qmatmul_rmsnorm_fp8: y = x * w / sqrt(mean(x^2) + eps); h (optional, f32, row stride
  * ldh, rows < M) receives y; an h that overlaps x is refused.   qmatmul_swiglu_fp8: y = silu(gate) * up (gelu_tanh(gate) *
  * up with gelu) from rows [gate(F) | up(F)], an infinite gate giving NaN. y is computed in f32 (of the gate's exponential, what is
- * below 2^-126 may count as zero). Rows that are 16-byte aligned (base and stride) and of a
- * K % 8 == 0 are read 16 bytes at a time, others by the element. Outputs that overlap the input or each other are refused. M may be 0
- * (x NULL): M_stride rows of zeros, at least one. */
+ * below 2^-126 may count as zero). Rows that are 16-byte aligned (base and stride) and of a K % 8 == 0 are read 16 bytes at a
+ * time, others by the element. Outputs that overlap the input or each other are refused. M may be 0 (x NULL): M_stride rows of
+ * zeros, at least one. */
 int qmatmul_quantize_fp8(const void* x, int xtype, int ldx, int M, int M_stride, int K, uint8_t* a8, float* asc,
                          void* stream);
 int qmatmul_rmsnorm_fp8(const void* x, int xtype, int ldx, const float* w, int K, int M, int M_stride, float eps,
@@ -300,9 +300,9 @@ int qmatmul_swiglu_fp8(const void* gu, int xtype, int ldg, int F, int M, int M_s
  * result for normal values, far below C's rounding); the sums of eights and of blocks are f32. a8 is 16-byte aligned.
  * ws: device workspace, 256-byte aligned, of qmatmul_gemm_fp8_workspace_size(w, M) bytes; NULL or a smaller one: K is cut into
  * fewer pieces or none, slower. The size is 0 for many M and does not grow with M (often 0 again for the largest): for calls of
- * several M, the largest of their sizes, or 64 MiB, which is never exceeded. Calls that may overlap need different workspaces. C and ws may not
- * overlap a8, asc or each other. No allocation, no host synchronisation; the call can be captured into a graph. The weight's
- * device must be the current one. */
+ * several M, the largest of their sizes, or 64 MiB, which is never exceeded. Calls that may overlap need different workspaces.
+ * C and ws may not overlap a8, asc or each other. No allocation, no host synchronisation; the call can be captured into a
+ * graph. The weight's device must be the current one. */
 size_t qmatmul_gemm_fp8_workspace_size(const qm_fp8_weight* w, int M);
 int qmatmul_gemm_fp8(const qm_fp8_weight* w, const uint8_t* a8, const float* asc, int M, int M_stride, void* C, int ctype,
                      int ldc, int c_off, int accumulate, void* ws, size_t ws_bytes, void* stream);

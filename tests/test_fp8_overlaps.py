@@ -58,10 +58,34 @@ def test_products(qm, dev):
     f = lambda **k: lib.qmatmul_gemm_fp8(*{**dict(w=w.handle, a=p, s=p + 8192, M=M, Ms=8, C=p + 16384, t=0, ldc=N, off=0, acc=0,  # noqa: E731
                                                   ws=p + 65536, wsb=65536, st=qm._stream(None)), **k}.values())
     row = 4 * N
-    for bad in (dict(C=p), dict(C=p + 1276), dict(C=p + 8192 - 5 * row + 4), dict(C=p + 8192), dict(C=p + 65536), dict(ws=p), dict(ws=p + 8192),
-                dict(ws=p + 16384 + 4 * row), dict(ldc=1024, C=p + 65536 - 4096), dict(ldc=2048, off=1024, C=p - 4096 + 1276)):
+    for bad in (dict(C=p), dict(C=p + 1276), dict(C=p + 8192 - 5 * row + 4), dict(C=p + 8192), dict(ldc=2048, off=1024, C=p - 4096 + 1276)):
         assert is_overlap(qm, f(**bad)), bad
     assert not buf.any()
     assert f(C=p + 1280) == 0 and f(Ms=4096, C=p + 1280) == 0  # (behind the call's own rows: it may be a part of a longer batch)
     assert f() == 0 and f(ws=None, wsb=0) == 0 and f(ws=p, wsb=0) == 0 and f(ldc=1024, C=p + 8192 + 256) == 0
+    assert f(ws=p) == 0 and f(C=p + 65536) == 0  # (so few tokens use no workspace)
+    w.release()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("t", [0, 30])
+def test_workspaces(qm, dev, t):
+    """What the pieces take of the workspace, and no more of it than that."""
+    N, K, M = 2048, 9600, 200
+    w = qm.Fp8Weight(torch.zeros((N, K), dtype=torch.uint8, device=dev), torch.ones((16, 75), device=dev))
+    piece, lib = 4 * M * N, qm.load_library()
+    need = lib.qmatmul_gemm_fp8_workspace_size(w.handle, M)
+    assert need >= 2 * piece
+    buf = torch.zeros(64 << 20, dtype=torch.uint8, device=dev)
+    p, size = (buf.data_ptr() + 255) // 256 * 256, 2 if t else 4
+    a, s, C, ws = p, p + (2 << 20), p + (3 << 20), p + (8 << 20)
+    row = size * N
+    f = lambda **k: lib.qmatmul_gemm_fp8(*{**dict(w=w.handle, a=a, s=s, M=M, Ms=M, C=C, t=t, ldc=N, off=0, acc=0, ws=ws, wsb=2 * piece,  # noqa: E731
+                                                  st=qm._stream(None)), **k}.values())
+    for bad in (dict(ws=a), dict(ws=s), dict(ws=C), dict(ws=C + 199 * row), dict(C=ws), dict(C=ws + 2 * piece - 16), dict(C=ws - 199 * row),
+                dict(a=ws + 4096), dict(s=ws + 2 * piece - 4), dict(ldc=4 * N, C=ws - 4 * row)):
+        assert is_overlap(qm, f(**bad)), bad
+    assert not buf.any()
+    assert f() == 0 and f(C=ws + 2 * piece) == 0 and f(C=ws - 200 * row) == 0 and f(ws=C, wsb=piece - 1) == 0
+    assert f(wsb=(64 << 20) - (8 << 20) - 256, a=ws + need) == 0
     w.release()
