@@ -11,6 +11,7 @@
 #include "../../include/qmatmul.h"
 #include "qm_fp8.h"
 #include "qm_gguf.h"
+#include "qm_kv.h"
 #include "qm_launch.h"
 
 struct qm_weight {
@@ -975,6 +976,31 @@ int qmatmul_gemm_fp8(const qm_fp8_weight* w, const uint8_t* a8, const float* asc
 
 // ---- query and key heads
 
+// The rotation of heads of D elements, T tokens' positions of row stride pos_stride
+static int check_rotation(const char* fn, const qm_rope* rope, int D, int T, int pos_stride) {
+  if (!rope) return fail(QM_ERR_ARG, "%s: null rotation", fn);
+  if (rope->rot < 0 || rope->rot > D || rope->rot % 2 || rope->axes < 1 || rope->axes > 4)
+    return fail(QM_ERR_SHAPE, "%s: rot %d (even, 0..D %d), axes %d (1..4)", fn, rope->rot, D, rope->axes);
+  if (rope->axes > 1) {
+    long long sum = 0;
+    for (int i = 0; i < rope->axes; ++i) {
+      if (rope->sections[i] < 0) return fail(QM_ERR_SHAPE, "%s: sections[%d] = %d", fn, i, rope->sections[i]);
+      sum += rope->sections[i];
+    }
+    if (sum != rope->rot / 2) return fail(QM_ERR_SHAPE, "%s: sections sum to %lld, rot / 2 is %d", fn, sum, rope->rot / 2);
+    if (pos_stride < T) return fail(QM_ERR_SHAPE, "%s: pos_stride %d < T %d", fn, pos_stride, T);
+  }
+  return QM_OK;
+}
+static void set_rotation(qm::RopeArgs* a, const qm_rope* rope) {
+  a->rot = rope->rot;
+  a->adjacent = rope->adjacent ? 1 : 0;
+  a->axes = rope->axes;
+  a->turns = rope->turns ? 1 : 0;
+  for (int i = 0; i < 4; ++i) a->sections[i] = rope->sections[i];
+  a->scale = rope->scale;
+}
+
 int qmatmul_qk_norm_rope(const void* x, int xtype, int ldx, int T, int D, int q_off, int q_hs, int HQ, int k_off, int k_hs,
                          int HK, const float* wq, const float* wk, float eps, const qm_rope* rope, const int32_t* pos,
                          int pos_stride, const float* inv_freq, void* q, void* k, int otype, int ldq, int ldk,
@@ -985,22 +1011,12 @@ int qmatmul_qk_norm_rope(const void* x, int xtype, int ldx, int T, int D, int q_
     return fail(QM_ERR_TYPE, "%s: types %d -> %d (QM_F32, QM_F16 or QM_BF16)", fn, xtype, otype);
   if (T < 0 || D < 2 || D > 512 || D % 2 || HQ < 0 || HK < 0 || HQ > 65536 || HK > 65536)
     return fail(QM_ERR_SHAPE, "%s: T %d, D %d (even, 2..512), HQ %d, HK %d", fn, T, D, HQ, HK);
-  if (rope->rot < 0 || rope->rot > D || rope->rot % 2 || rope->axes < 1 || rope->axes > 4)
-    return fail(QM_ERR_SHAPE, "%s: rot %d (even, 0..D %d), axes %d (1..4)", fn, rope->rot, D, rope->axes);
-  if (rope->axes > 1) {
-    long long sum = 0;
-    for (int i = 0; i < rope->axes; ++i) {
-      if (rope->sections[i] < 0) return fail(QM_ERR_SHAPE, "%s: sections[%d] = %d", fn, i, rope->sections[i]);
-      sum += rope->sections[i];
-    }
-    if (sum != rope->rot / 2) return fail(QM_ERR_SHAPE, "%s: sections sum to %lld, rot / 2 is %d", fn, sum, rope->rot / 2);
-  }
+  if (const int st = check_rotation(fn, rope, D, T, pos_stride)) return st;
   const long long qw = (long long)(HQ - 1) * q_hs + D, kw = (long long)(HK - 1) * k_hs + D;
   if ((HQ && (q_off < 0 || q_hs < (HQ > 1 ? D : 0) || q_off + qw > ldx || ldq < (long long)HQ * D)) ||
       (HK && (k_off < 0 || k_hs < (HK > 1 ? D : 0) || k_off + kw > ldx || ldk < (long long)HK * D)))
     return fail(QM_ERR_SHAPE, "%s: D %d; q: offset %d, %d heads of stride %d, ldq %d; k: offset %d, %d heads of stride %d, "
                 "ldk %d; ldx %d", fn, D, q_off, HQ, q_hs, ldq, k_off, HK, k_hs, ldk, ldx);
-  if (rope->axes > 1 && pos_stride < T) return fail(QM_ERR_SHAPE, "%s: pos_stride %d < T %d", fn, pos_stride, T);
   if (T == 0 || HQ + HK == 0) return QM_OK;
   if (!x || (HQ && !q) || (HK && !k) || (rope->rot && (!pos || !inv_freq))) return fail(QM_ERR_ARG, "%s: null pointer", fn);
   const size_t si = dtype_size(xtype), so = dtype_size(otype);
@@ -1031,12 +1047,7 @@ int qmatmul_qk_norm_rope(const void* x, int xtype, int ldx, int T, int D, int q_
   a.wq = wq;
   a.wk = wk;
   a.eps = eps;
-  a.rot = rope->rot;
-  a.adjacent = rope->adjacent ? 1 : 0;
-  a.axes = rope->axes;
-  a.turns = rope->turns ? 1 : 0;
-  for (int i = 0; i < 4; ++i) a.sections[i] = rope->sections[i];
-  a.scale = rope->scale;
+  set_rotation(&a, rope);
   a.pos = pos;
   a.pos_stride = pos_stride;
   a.inv_freq = inv_freq;
@@ -1046,6 +1057,315 @@ int qmatmul_qk_norm_rope(const void* x, int xtype, int ldx, int T, int D, int q_
   a.ldq = ldq;
   a.ldk = ldk;
   const hipError_t e = qm::launch_qk_norm_rope(a, (hipStream_t)stream);
+  return e == hipSuccess ? QM_OK : hip_fail(e, fn);
+}
+
+// ---- keys and values in pages, and attention over them
+
+// Bytes in one piece
+struct Span {
+  const void* p;
+  size_t bytes;
+};
+static bool spans_meet(const Span& a, const Span& b) {
+  const uintptr_t x = (uintptr_t)a.p, y = (uintptr_t)b.p;
+  return a.p && b.p && a.bytes && b.bytes && x < y + b.bytes && y < x + a.bytes;
+}
+
+// The dimensions of a cache but the last, from the smallest stride on, those of one entry left out
+struct KvDims {
+  int n;
+  long long count[3], stride[3];
+};
+static KvDims kv_dims(const qm_kv* kv) {
+  KvDims d{};
+  const long long count[3] = {kv->pages, kv->heads, kv->page}, stride[3] = {kv->page_stride, kv->head_stride, kv->token_stride};
+  for (int i = 0; i < 3; ++i) {
+    if (count[i] == 1) continue;
+    int at = d.n++;
+    for (; at > 0 && d.stride[at - 1] > stride[i]; --at) {
+      d.count[at] = d.count[at - 1];
+      d.stride[at] = d.stride[at - 1];
+    }
+    d.count[at] = count[i];
+    d.stride[at] = stride[i];
+  }
+  return d;
+}
+// Whether rows of D elements `delta` apart share one for some pair of places (dimensions 0 .. n - 1, each within the next one's stride)
+static bool rows_meet(const KvDims& d, int n, long long delta, int D) {
+  if (n == 0) return delta < D && delta > -D;
+  const long long s = d.stride[n - 1], q = delta / s;
+  for (long long a = q - 1; a <= q + 1; ++a)
+    if (a < d.count[n - 1] && a > -d.count[n - 1] && rows_meet(d, n - 1, delta - a * s, D)) return true;
+  return false;
+}
+
+static size_t kv_size(int type) { return type == QM_E4M3 ? 1 : 2; }
+static long long kv_extent(const qm_kv* kv) {  // elements from the first to the last
+  return (kv->pages - 1) * kv->page_stride + (kv->heads - 1) * kv->head_stride + (kv->page - 1) * kv->token_stride + kv->D;
+}
+
+// Sizes and types alone
+static int check_kv_sizes(const char* fn, const qm_kv* kv) {
+  if (!kv) return fail(QM_ERR_ARG, "%s: null cache", fn);
+  if (kv->type != QM_F16 && kv->type != QM_BF16 && kv->type != QM_E4M3)
+    return fail(QM_ERR_TYPE, "%s: cache type %d (QM_F16, QM_BF16 or QM_E4M3)", fn, kv->type);
+  if (kv->D < 16 || kv->D > 256 || kv->D % 16 || kv->heads < 1 || kv->heads > 65536 || kv->page < 16 || kv->page > 256 ||
+      (kv->page & (kv->page - 1)) || kv->pages < 1 || (long long)kv->pages * kv->page > 0x7fffffff)
+    return fail(QM_ERR_SHAPE, "%s: D %d (a multiple of 16, 16..256), %d heads, %d pages of %d tokens (16, 32, 64, 128 or 256)", fn, kv->D,
+                kv->heads, kv->pages, kv->page);
+  return QM_OK;
+}
+
+static int check_kv(const char* fn, const qm_kv* kv, bool data, qm::KvView* out) {
+  if (const int st = check_kv_sizes(fn, kv)) return st;
+  const size_t size = kv_size(kv->type);
+  if (data) {
+    if (!kv->k || !kv->v || (kv->type == QM_E4M3 && (!kv->k_scale || !kv->v_scale))) return fail(QM_ERR_ARG, "%s: null pointer in the cache", fn);
+    const long long most = 1LL << 46, unit = (long long)(16 / size);
+    if (kv->page_stride < 0 || kv->head_stride < 0 || kv->token_stride < 0 || kv->page_stride > most / kv->pages ||
+        kv->head_stride > most / kv->heads || kv->token_stride > most / kv->page)
+      return fail(QM_ERR_SHAPE, "%s: cache strides %lld, %lld, %lld", fn, kv->page_stride, kv->head_stride, kv->token_stride);
+    if ((kv->pages > 1 && kv->page_stride % unit) || (kv->heads > 1 && kv->head_stride % unit) || kv->token_stride % unit || !aligned(kv->k, 16) ||
+        !aligned(kv->v, 16) || (kv->type == QM_E4M3 && (!aligned(kv->k_scale, 16) || !aligned(kv->v_scale, 16))))
+      return fail(QM_ERR_ARG, "%s: the cache's rows and scales must be 16-byte aligned", fn);
+    const KvDims d = kv_dims(kv);
+    long long extent = kv->D;
+    for (int i = 0; i < d.n; ++i) {
+      if (d.stride[i] < extent)
+        return fail(QM_ERR_SHAPE, "%s: cache strides %lld, %lld, %lld put two elements at one place", fn, kv->page_stride, kv->head_stride,
+                    kv->token_stride);
+      extent += (d.count[i] - 1) * d.stride[i];
+    }
+  }
+  if (!aligned(kv->mean, 16)) return fail(QM_ERR_ARG, "%s: the cache's means must be 16-byte aligned", fn);
+  int lg = 4;
+  while (1 << lg < kv->page) ++lg;
+  *out = {kv->type, kv->D, kv->heads, kv->page, lg, kv->pages, kv->page_stride, kv->head_stride, kv->token_stride, kv->k, kv->v,
+          kv->k_scale, kv->v_scale, kv->mean};
+  return QM_OK;
+}
+
+// The cache's buffers: keys, values, scales, means
+static int kv_spans(const qm_kv* kv, Span* out) {
+  const size_t rows = (size_t)kv->pages * kv->heads * kv->page, bytes = (size_t)kv_extent(kv) * kv_size(kv->type);
+  const bool e8 = kv->type == QM_E4M3;
+  out[0] = {kv->k, bytes};
+  out[1] = {kv->v, bytes};
+  out[2] = {e8 ? kv->k_scale : nullptr, rows * 4};
+  out[3] = {e8 ? kv->v_scale : nullptr, rows * 4};
+  out[4] = {kv->mean, (size_t)kv->pages * kv->heads * kv->D * 2};
+  return 5;
+}
+
+int qmatmul_kv_append(const void* x, int xtype, int ldx, int T, int q_off, int q_hs, int HQ, int k_off, int k_hs, int v_off,
+                      int v_hs, const float* wq, const float* wk, float eps, const qm_rope* rope, const int32_t* pos,
+                      int pos_stride, const float* inv_freq, const int32_t* slots, const qm_kv* kv, void* q, int qtype, int ldq,
+                      void* stream) {
+  const char* fn = "qmatmul_kv_append";
+  qm::AppendArgs a{};
+  if (const int st = check_kv(fn, kv, true, &a.kv)) return st;
+  const int D = kv->D, HK = kv->heads;
+  if (const int st = check_rotation(fn, rope, D, T, pos_stride)) return st;
+  if (!dtype_ok(xtype) || !dtype_ok(qtype))
+    return fail(QM_ERR_TYPE, "%s: types %d -> %d (QM_F32, QM_F16 or QM_BF16)", fn, xtype, qtype);
+  if (T < 0 || T >= 1 << 24 || HQ < 0 || HQ > 65536) return fail(QM_ERR_SHAPE, "%s: T %d (below 2^24), HQ %d", fn, T, HQ);
+  const long long qw = (long long)(HQ - 1) * q_hs + D, kw = (long long)(HK - 1) * k_hs + D, vw = (long long)(HK - 1) * v_hs + D;
+  if ((HQ && (q_off < 0 || q_hs < (HQ > 1 ? D : 0) || q_off + qw > ldx || ldq < (long long)HQ * D)) || k_off < 0 ||
+      k_hs < (HK > 1 ? D : 0) || k_off + kw > ldx || v_off < 0 || v_hs < (HK > 1 ? D : 0) || v_off + vw > ldx)
+    return fail(QM_ERR_SHAPE, "%s: D %d; q: offset %d, %d heads of stride %d, ldq %d; k: offset %d, %d heads of stride %d; v: offset %d, "
+                "stride %d; ldx %d", fn, D, q_off, HQ, q_hs, ldq, k_off, HK, k_hs, v_off, v_hs, ldx);
+  if (T == 0) return QM_OK;
+  if (!x || !slots || (HQ && !q) || (rope->rot && (!pos || !inv_freq))) return fail(QM_ERR_ARG, "%s: null pointer", fn);
+  const size_t si = dtype_size(xtype), so = dtype_size(qtype);
+  if (!aligned(x, si) || (HQ && !aligned(q, so)) || !aligned(pos, 4) || !aligned(inv_freq, 4) || !aligned(wq, 4) || !aligned(wk, 4) ||
+      !aligned(slots, 4))
+    return fail(QM_ERR_ARG, "%s: every pointer must be aligned to its type", fn);
+  const HeadRows xq{(const char*)x + (size_t)q_off * si, T, D, HQ, q_hs, ldx, (long long)si};
+  const HeadRows xk{(const char*)x + (size_t)k_off * si, T, D, HK, k_hs, ldx, (long long)si};
+  const HeadRows xv{(const char*)x + (size_t)v_off * si, T, D, HK, v_hs, ldx, (long long)si};
+  const HeadRows oq{q, T, D, HQ, D, ldq, (long long)so};
+  const bool q_in = HQ && q == xq.p && xtype == qtype && (ldq == ldx || T == 1) && (q_hs == D || HQ == 1);
+  bool over = (!q_in && rows_overlap(oq, xq)) || rows_overlap(oq, xk) || rows_overlap(oq, xv);
+  const int half = rope->rot / 2, n_axes = rope->axes;
+  const Span in[] = {{slots, (size_t)T * 4}, {half ? pos : nullptr, ((size_t)(n_axes - 1) * (n_axes > 1 ? pos_stride : 0) + T) * 4},
+                     {half ? inv_freq : nullptr, (size_t)half * 4}, {HQ ? wq : nullptr, (size_t)D * 4}, {wk, (size_t)D * 4}};
+  Span held[5];
+  const int n = kv_spans(kv, held);
+  for (const Span& s : in) {
+    over = over || span_overlaps(oq, s.p, s.bytes);
+    for (int i = 0; i < n; ++i) over = over || spans_meet(s, held[i]);
+  }
+  for (int i = 0; i < n; ++i) {
+    for (const HeadRows* r : {&xq, &xk, &xv, &oq}) over = over || span_overlaps(*r, held[i].p, held[i].bytes);
+    for (int j = i + 1; j < n; ++j) {
+      const bool both = i == 0 && j == 1;  // (keys and values may lie in turns)
+      over = over || (both ? rows_meet(kv_dims(kv), kv_dims(kv).n, ((const char*)kv->v - (const char*)kv->k) / (long long)kv_size(kv->type), D)
+                           : spans_meet(held[i], held[j]));
+    }
+  }
+  if (over) return fail(QM_ERR_ARG, "%s: an output overlaps an input or another output", fn);
+  QM_CHECK_INIT();
+  qm::RopeArgs& r = a.r;
+  r.x = x;
+  r.xtype = xtype;
+  r.ldx = ldx;
+  r.T = T;
+  r.D = D;
+  r.q_off = HQ ? q_off : 0;
+  r.q_hs = q_hs;
+  r.HQ = HQ;
+  r.k_off = k_off;
+  r.k_hs = k_hs;
+  r.HK = HK;
+  r.wq = wq;
+  r.wk = wk;
+  r.eps = eps;
+  set_rotation(&r, rope);
+  r.pos = pos;
+  r.pos_stride = pos_stride;
+  r.inv_freq = inv_freq;
+  r.q = q;
+  r.otype = qtype;
+  r.ldq = ldq;
+  a.v_off = v_off;
+  a.v_hs = v_hs;
+  a.slots = slots;
+  const hipError_t e = qm::launch_kv_append(a, (hipStream_t)stream);
+  return e == hipSuccess ? QM_OK : hip_fail(e, fn);
+}
+
+// What the calls that read a cache share: q's rows and the batch. Nothing to do: *none.
+static int check_seqs(const char* fn, const void* q, int qtype, int ldq, int HQ, const qm_seqs* s, const qm_kv* kv, qm::Seqs* out, bool* none) {
+  if (!s) return fail(QM_ERR_ARG, "%s: null batch", fn);
+  if (qtype != QM_F16 && qtype != QM_BF16) return fail(QM_ERR_TYPE, "%s: q of type %d (QM_F16 or QM_BF16)", fn, qtype);
+  if (HQ < 1 || HQ > 65536 || HQ % kv->heads || ldq < (long long)HQ * kv->D)
+    return fail(QM_ERR_SHAPE, "%s: %d query heads of %d for %d key heads, ldq %d", fn, HQ, kv->D, kv->heads, ldq);
+  if (s->T < 0 || s->B < 0 || (!s->start && s->T != s->B)) return fail(QM_ERR_SHAPE, "%s: %d rows of %d sequences%s", fn, s->T, s->B, s->start ? "" : " of one each");
+  *none = s->T == 0 || s->B == 0;
+  if (*none) return QM_OK;
+  if (s->table_stride < 1 || (long long)s->table_stride * kv->page > 1 << 30)
+    return fail(QM_ERR_SHAPE, "%s: %d pages of %d tokens a sequence", fn, s->table_stride, kv->page);
+  if (!q || !s->len || !s->table) return fail(QM_ERR_ARG, "%s: null pointer", fn);
+  if (!aligned(q, 2) || !aligned(s->start, 4) || !aligned(s->len, 4) || !aligned(s->table, 4))
+    return fail(QM_ERR_ARG, "%s: every pointer must be aligned to its type", fn);
+  *out = {s->B, s->T, s->start, s->len, s->table, s->table_stride};
+  return QM_OK;
+}
+
+size_t qmatmul_attn_workspace_size(const qm_kv* kv, int T, int B, int HQ, int prefix_len) {
+  if (check_kv_sizes("qmatmul_attn_workspace_size", kv) || T < 1 || B < 1 || HQ < 1 || HQ > 65536 || HQ % kv->heads || prefix_len < 0 || prefix_len > 1 << 30)
+    return 0;
+  return qm::attn_workspace_bytes(T, B, HQ, kv->heads, kv->D, prefix_len);
+}
+
+// Attention: over everything (sel null), or chosen pages
+static int attention(const char* fn, const void* q, int qtype, int ldq, int HQ, const qm_seqs* seqs, const qm_kv* kv, const int32_t* prefix,
+                     int prefix_len, const int32_t* sel, int k, float scale, void* o, int otype, int ldo, void* ws, size_t ws_bytes, void* stream) {
+  qm::AttnArgs a{};
+  bool none = false;
+  if (const int st = check_kv(fn, kv, true, &a.kv)) return st;
+  if (const int st = check_seqs(fn, q, qtype, ldq, HQ, seqs, kv, &a.s, &none)) return st;
+  if (kv->type != QM_E4M3 && kv->type != qtype) return fail(QM_ERR_TYPE, "%s: q of type %d, the cache of %d", fn, qtype, kv->type);
+  if (otype != qtype && otype != QM_F32) return fail(QM_ERR_TYPE, "%s: output type %d (q's or QM_F32)", fn, otype);
+  if (ldo < (long long)HQ * kv->D || prefix_len < 0 || prefix_len > 1 << 30) return fail(QM_ERR_SHAPE, "%s: ldo %d, prefix_len %d", fn, ldo, prefix_len);
+  if (none) return QM_OK;
+  if (!o || (prefix_len && !prefix)) return fail(QM_ERR_ARG, "%s: null pointer", fn);
+  const size_t so = dtype_size(otype);
+  if (!aligned(o, so) || !aligned(prefix, 4) || !aligned(sel, 4)) return fail(QM_ERR_ARG, "%s: every pointer must be aligned to its type", fn);
+  if (ws && !aligned(ws, 256)) return fail(QM_ERR_ARG, "%s: the workspace must be 256-byte aligned", fn);
+  const int T = seqs->T, B = sel ? T : seqs->B;
+  const bool start = !sel && seqs->start;
+  const qm::AttnPlan p = qm::attn_plan(T, B, start, HQ, kv->heads, kv->D, prefix_len, ws ? ws_bytes : 0);
+  if (!qm::attn_grid(p, T, B, start, HQ, kv->heads)) return fail(QM_ERR_SHAPE, "%s: %d rows of %d heads are more than a grid holds", fn, T, HQ);
+  size_t used = (size_t)p.slots * qm::attn_slot_bytes(p.mt, kv->D);
+  if (p.shared) used += (size_t)kv->heads * p.shared_tiles * p.shared * qm::attn_slot_bytes(p.shared_mt, kv->D);
+  const HeadRows rq{q, T, kv->D, HQ, kv->D, ldq, 2}, ro{o, T, kv->D, HQ, kv->D, ldo, (long long)so};
+  const Span work{ws, used};
+  const Span in[] = {{seqs->start, ((size_t)seqs->B + 1) * 4}, {seqs->len, (size_t)seqs->B * 4}, {seqs->table, (size_t)seqs->B * seqs->table_stride * 4},
+                     {prefix_len ? prefix : nullptr, (size_t)((prefix_len + kv->page - 1) / kv->page) * 4},
+                     {sel, (size_t)T * kv->heads * k * 4}};
+  Span held[5];
+  const int n = kv_spans(kv, held);
+  bool over = rows_overlap(ro, rq) || span_overlaps(ro, ws, used) || span_overlaps(rq, ws, used);
+  for (const Span& s : in) over = over || span_overlaps(ro, s.p, s.bytes) || spans_meet(work, s);
+  for (int i = 0; i < n; ++i) over = over || span_overlaps(ro, held[i].p, held[i].bytes) || spans_meet(work, held[i]);
+  if (over) return fail(QM_ERR_ARG, "%s: the output or the workspace overlaps an input or the other", fn);
+  QM_CHECK_INIT();
+  a.q = q;
+  a.qtype = qtype;
+  a.ldq = ldq;
+  a.HQ = HQ;
+  a.G = HQ / kv->heads;
+  a.prefix = prefix;
+  a.prefix_len = prefix_len;
+  a.sel = sel;
+  a.k = k;
+  a.c = scale * 1.44269504088896341f;
+  a.o = o;
+  a.otype = otype;
+  a.ldo = ldo;
+  a.part = (float*)ws;
+  const hipError_t e = qm::launch_attn(a, p, (hipStream_t)stream);
+  return e == hipSuccess ? QM_OK : hip_fail(e, fn);
+}
+
+int qmatmul_attn_prefix(const void* q, int qtype, int ldq, int HQ, const qm_seqs* seqs, const qm_kv* kv, const int32_t* prefix,
+                        int prefix_len, float scale, void* o, int otype, int ldo, void* ws, size_t ws_bytes, void* stream) {
+  return attention("qmatmul_attn_prefix", q, qtype, ldq, HQ, seqs, kv, prefix, prefix_len, nullptr, 0, scale, o, otype, ldo, ws, ws_bytes, stream);
+}
+
+int qmatmul_attn_pages(const void* q, int qtype, int ldq, int HQ, const qm_seqs* seqs, const qm_kv* kv, const int32_t* sel, int k,
+                       float scale, void* o, int otype, int ldo, void* ws, size_t ws_bytes, void* stream) {
+  const char* fn = "qmatmul_attn_pages";
+  if (check_kv_sizes(fn, kv)) return check_kv_sizes(fn, kv);
+  if (k < 1 || (long long)k * kv->page > 1 << 30) return fail(QM_ERR_SHAPE, "%s: %d pages of %d tokens", fn, k, kv->page);
+  if (!sel) return fail(QM_ERR_ARG, "%s: null pointer", fn);
+  return attention(fn, q, qtype, ldq, HQ, seqs, kv, nullptr, 0, sel, k, scale, o, otype, ldo, ws, ws_bytes, stream);
+}
+
+size_t qmatmul_select_workspace_size(const qm_kv* kv, int T, int table_stride) {
+  if (check_kv_sizes("qmatmul_select_workspace_size", kv) || T < 1 || table_stride < 1) return 0;
+  return ((size_t)T * kv->heads * table_stride * sizeof(double) + 255) / 256 * 256;
+}
+
+int qmatmul_select_pages(const void* q, int qtype, int ldq, int HQ, const qm_seqs* seqs, const qm_kv* kv, int k, int first, int last,
+                         int32_t* sel, void* ws, size_t ws_bytes, void* stream) {
+  const char* fn = "qmatmul_select_pages";
+  qm::SelectArgs a{};
+  bool none = false;
+  if (const int st = check_kv(fn, kv, false, &a.kv)) return st;
+  if (!kv->mean) return fail(QM_ERR_ARG, "%s: a cache without means", fn);
+  if (const int st = check_seqs(fn, q, qtype, ldq, HQ, seqs, kv, &a.s, &none)) return st;
+  if (k < 1 || first < 0 || last < 1 || (long long)first + last > k) return fail(QM_ERR_SHAPE, "%s: %d pages, the first %d and the last %d (1 at least) among them", fn, k, first, last);
+  if (none) return QM_OK;
+  if (!sel) return fail(QM_ERR_ARG, "%s: null pointer", fn);
+  if (!aligned(sel, 4)) return fail(QM_ERR_ARG, "%s: every pointer must be aligned to its type", fn);
+  const size_t need = seqs->table_stride > k ? (size_t)seqs->T * kv->heads * seqs->table_stride * sizeof(double) : 0;
+  const long long groups = (long long)seqs->T * kv->heads * ((seqs->table_stride + 255) / 256);
+  if (groups * 256 > qm::kMostThreads) return fail(QM_ERR_SHAPE, "%s: %d rows of %d heads and %d pages are more than a grid holds", fn, seqs->T, kv->heads, seqs->table_stride);
+  if (need && (!ws || ws_bytes < need)) return fail(QM_ERR_WORKSPACE, "%s: a workspace of %zu bytes, %zu needed", fn, ws ? ws_bytes : 0, need);
+  if (need && !aligned(ws, 256)) return fail(QM_ERR_ARG, "%s: the workspace must be 256-byte aligned", fn);
+  const HeadRows rq{q, seqs->T, kv->D, HQ, kv->D, ldq, 2};
+  const Span out{sel, (size_t)seqs->T * kv->heads * k * 4}, work{need ? ws : nullptr, need};
+  const Span in[] = {{seqs->start, ((size_t)seqs->B + 1) * 4}, {seqs->len, (size_t)seqs->B * 4}, {seqs->table, (size_t)seqs->B * seqs->table_stride * 4},
+                     {kv->mean, (size_t)kv->pages * kv->heads * kv->D * 2}};
+  bool over = span_overlaps(rq, out.p, out.bytes) || span_overlaps(rq, work.p, work.bytes) || spans_meet(out, work);
+  for (const Span& s : in) over = over || spans_meet(out, s) || spans_meet(work, s);
+  if (over) return fail(QM_ERR_ARG, "%s: the pages or the workspace overlap an input or the other", fn);
+  QM_CHECK_INIT();
+  a.q = q;
+  a.qtype = qtype;
+  a.ldq = ldq;
+  a.HQ = HQ;
+  a.G = HQ / kv->heads;
+  a.k = k;
+  a.first = first;
+  a.last = last;
+  a.scores = (double*)ws;
+  a.sel = sel;
+  const hipError_t e = qm::launch_select(a, (hipStream_t)stream);
   return e == hipSuccess ? QM_OK : hip_fail(e, fn);
 }
 

@@ -1,0 +1,29 @@
+// Launches of attn_kernel for one pair of types (each pair is compiled in a file of its own)
+#pragma once
+#include "qm_attn_impl.h"
+
+namespace qm {
+
+template <typename TQ, typename TC, int DC, int MT, int PARTS>
+hipError_t attn_mode(const AttnArgs& a, int mode, unsigned grid, hipStream_t s) {
+  if (mode == SHARED) attn_kernel<TQ, TC, DC, MT, PARTS, SHARED><<<grid, 256, 0, s>>>(a);
+  else if (mode == CHOSEN) attn_kernel<TQ, TC, DC, MT, PARTS, CHOSEN><<<grid, 256, 0, s>>>(a);
+  else attn_kernel<TQ, TC, DC, MT, PARTS, OWN><<<grid, 256, 0, s>>>(a);
+  return hipGetLastError();
+}
+
+template <typename TQ, typename TC, int PARTS>
+hipError_t attn_parts(const AttnArgs& a, int mt, int mode, unsigned grid, hipStream_t s) {
+  if (a.kv.D <= 64) return mt == 1 ? attn_mode<TQ, TC, 64, 1, PARTS>(a, mode, grid, s) : mt == 2 ? attn_mode<TQ, TC, 64, 2, PARTS>(a, mode, grid, s) : attn_mode<TQ, TC, 64, 4, PARTS>(a, mode, grid, s);
+  if (a.kv.D <= 128) return mt == 1 ? attn_mode<TQ, TC, 128, 1, PARTS>(a, mode, grid, s) : mt == 2 ? attn_mode<TQ, TC, 128, 2, PARTS>(a, mode, grid, s) : attn_mode<TQ, TC, 128, 4, PARTS>(a, mode, grid, s);
+  return mt == 1 ? attn_mode<TQ, TC, 256, 1, PARTS>(a, mode, grid, s) : attn_mode<TQ, TC, 256, 2, PARTS>(a, mode, grid, s);
+}
+
+// Two parts of P where the result keeps more bits than one: f32, or f16 behind an 8-bit cache (P is bf16 there)
+template <typename TQ, typename TC>
+hipError_t attn_types(const AttnArgs& a, int mt, int mode, unsigned grid, hipStream_t s) {
+  if constexpr (sizeof(TC) == 1 && __is_same(TQ, _Float16)) return attn_parts<TQ, TC, 2>(a, mt, mode, grid, s);
+  else return a.otype == DT_F32 ? attn_parts<TQ, TC, 2>(a, mt, mode, grid, s) : attn_parts<TQ, TC, 1>(a, mt, mode, grid, s);
+}
+
+}  // namespace qm

@@ -1,0 +1,79 @@
+// Host-side launchers of the paged cache of keys and values: appending, attention over it, and the choice of pages. Shapes are
+// checked by the C-ABI layer (qm_api.hip) beforehand.
+#pragma once
+#include "qm_fp8.h"
+
+namespace qm {
+
+enum : int { DT_E4M3 = 256 };
+
+// The cache. Element d of the head h of token i of page p: p * ps + h * hs + i * ts + d, in keys and in values.
+struct KvView {
+  int type, D, HK, page, lg, pages;  // page = 1 << lg tokens
+  long long ps, hs, ts;
+  void *k, *v;
+  float *ksc, *vsc;  // e4m3: [pages][HK][page]
+  uint16_t* mean;    // bf16 [pages][HK][D], or null
+};
+
+struct AppendArgs {
+  RopeArgs r;  // (q, otype, ldq: the queries' result; k, ldk are not used)
+  int v_off, v_hs;
+  const int32_t* slots;
+  KvView kv;
+};
+hipError_t launch_kv_append(const AppendArgs& a, hipStream_t s);
+
+// The sequences of a batch: rows start[b] .. start[b + 1] of q (start null: row b), the last of its len[b] tokens
+struct Seqs {
+  int B, T;
+  const int32_t *start, *len, *table;
+  int W;  // the table's row stride: pages of a sequence at most
+};
+
+struct AttnArgs {
+  const void* q;
+  int qtype, ldq, HQ, G;
+  KvView kv;
+  Seqs s;
+  const int32_t* prefix;
+  int prefix_len;       // keys in front of each sequence's own that this launch reads
+  const int32_t* sel;   // pages of each row and key head [T][HK][k] (null: all)
+  int k;
+  float c;              // scale * log2 e
+  void* o;
+  int otype, ldo;
+  // The split. A piece is a run of blocks of 128 keys of one row tile and head; its partial result goes to the slot of its number.
+  float* part;          // null: nothing is split, each row tile writes its result
+  int target, slots;    // pieces that are aimed at, partial results that `part` holds
+  int pieces, blocks;   // chosen pages: pieces of a row tile, and blocks of 128 keys of one
+  // The pieces of the shared prefix for the rows of the whole batch (shared > 0): pieces a row tile, tiles of shared_rt rows of a key
+  // head, blocks of 128 keys of a piece; slot ((head * shared_tiles) + tile) * shared + piece
+  float* shared_part;
+  int shared, shared_rt, shared_tiles, shared_blocks;
+};
+
+// How a call runs: mt row tiles of 16 a work-group; pieces and blocks as in AttnArgs
+struct AttnPlan {
+  int mt, target, slots;                               // target 0: nothing is split
+  int shared, shared_mt, shared_tiles, shared_blocks;  // shared 0: the prefix is read with each sequence's own keys
+};
+size_t attn_slot_bytes(int mt, int D);
+AttnPlan attn_plan(int T, int B, bool start, int HQ, int HK, int D, int prefix_len, size_t ws_bytes);
+size_t attn_workspace_bytes(int T, int B, int HQ, int HK, int D, int prefix_len);
+// Work-groups of the calls's launches at most (0: more than a grid holds)
+long long attn_grid(const AttnPlan& p, int T, int B, bool start, int HQ, int HK);
+hipError_t launch_attn(const AttnArgs& a, const AttnPlan& p, hipStream_t s);
+
+struct SelectArgs {
+  const void* q;
+  int qtype, ldq, HQ, G;
+  KvView kv;
+  Seqs s;
+  int k, first, last;
+  double* scores;  // [T][HK][W]
+  int32_t* sel;    // [T][HK][k]
+};
+hipError_t launch_select(const SelectArgs& a, hipStream_t s);
+
+}  // namespace qm

@@ -5,42 +5,9 @@
 // and rot/2 + V c, or, with adjacent pairs, 2 V c and 2 V c + V), the rest pass (two neighbouring vectors). A pair never
 // crosses a lane: a group of L lanes holds one head, the mean square is a reduction over them.
 // The cosines and sines of a token are computed once for all its heads, into LDS.
-#include "qm_fp8.h"
+#include "qm_rope_dev.h"
 
 namespace qm {
-
-namespace {
-
-constexpr int kTable = 1024;  // cosine / sine pairs of a work-group
-
-__device__ __forceinline__ int axis_of(const RopeArgs& a, int i) {
-  if (a.axes == 1) return 0;
-  if (a.turns) {
-    const int x = i % a.axes;
-    return i < a.axes * a.sections[x] ? x : 0;
-  }
-  int x = 0, end = a.sections[0];
-  while (i >= end && x < a.axes - 1) end += a.sections[++x];
-  return x;
-}
-
-template <typename T, int V>
-__device__ __forceinline__ void loadv(const T* p, float* v) {
-  typedef T vt __attribute__((ext_vector_type(V)));
-  const vt t = *(const vt*)p;
-#pragma unroll
-  for (int i = 0; i < V; ++i) v[i] = (float)t[i];
-}
-template <typename T, int V>
-__device__ __forceinline__ void storev(T* p, const float* v) {
-  typedef T vt __attribute__((ext_vector_type(V)));
-  vt t;
-#pragma unroll
-  for (int i = 0; i < V; ++i) t[i] = (T)v[i];
-  *(vt*)p = t;
-}
-
-}  // namespace
 
 // One head of one token, as the lanes of a group hold it: U chunks of 2 V elements a lane
 template <typename TI, typename TO, int V, int U>

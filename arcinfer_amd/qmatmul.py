@@ -58,6 +58,12 @@ SIGNATURES = [
     ("qmatmul_gemm_fp8", _I, [_P, _P, _P, _I, _I, _P, _I, _I, _I, _I, _P, _Z, _P]),
     ("qmatmul_qk_norm_rope", _I, [_P, _I, _I, _I, _I, _I, _I, _I, _I, _I, _I, _P, _P, _c.c_float, _P, _P, _I, _P, _P, _P,
                                   _I, _I, _I, _P]),
+    ("qmatmul_kv_append", _I, [_P, _I, _I, _I, _I, _I, _I, _I, _I, _I, _I, _P, _P, _c.c_float, _P, _P, _I, _P, _P, _P, _P, _I, _I, _P]),
+    ("qmatmul_attn_workspace_size", _Z, [_P, _I, _I, _I, _I]),
+    ("qmatmul_attn_prefix", _I, [_P, _I, _I, _I, _P, _P, _P, _I, _c.c_float, _P, _I, _I, _P, _Z, _P]),
+    ("qmatmul_select_workspace_size", _Z, [_P, _I, _I]),
+    ("qmatmul_select_pages", _I, [_P, _I, _I, _I, _P, _P, _I, _I, _I, _P, _P, _Z, _P]),
+    ("qmatmul_attn_pages", _I, [_P, _I, _I, _I, _P, _P, _P, _I, _c.c_float, _P, _I, _I, _P, _Z, _P]),
     ("qmatmul_gguf_open", _I, [_c.c_char_p, _c.POINTER(_P)]),
     ("qmatmul_gguf_close", _I, [_P]),
     ("qmatmul_gguf_tensor_count", _I, [_P, _c.POINTER(_I)]),
@@ -669,6 +675,255 @@ def _head_rows(fn, name, t, T, H, D, dtype, dev):
     if ld >> 31:
         _sizes(fn, ld)
     return ld
+
+
+# ---- keys and values in pages, and attention over them ----------------------------------------------------------------
+class QmKv(ctypes.Structure):
+    _fields_ = [("type", _I), ("D", _I), ("heads", _I), ("page", _I), ("pages", _I), ("page_stride", _c.c_longlong),
+                ("head_stride", _c.c_longlong), ("token_stride", _c.c_longlong), ("k", _P), ("v", _P), ("k_scale", _P),
+                ("v_scale", _P), ("mean", _P)]
+
+
+class QmSeqs(ctypes.Structure):
+    _fields_ = [("T", _I), ("B", _I), ("start", _P), ("len", _P), ("table", _P), ("table_stride", _I)]
+
+
+class KvCache:
+    """One layer's keys and values in pages: k, v [pages, heads, page, D] of float16, bfloat16 or float8_e4m3fn (views of any order
+    in memory, both of one; the last dimension contiguous), with k_scale, v_scale float32 [pages, heads, page] for 8 bits, and
+    mean bfloat16 [pages, heads, D] where pages are to be selected. The tensors stay the caller's."""
+
+    def __init__(self, k, v, k_scale=None, v_scale=None, mean=None):
+        import torch
+        fn = "KvCache"
+        dev = _current_gpu()
+        kinds = {torch.float16: 1, torch.bfloat16: 30, torch.float8_e4m3fn: 256}
+        for name, t in (("k", k), ("v", v)):
+            _check_rows(fn, name, t, 4, dev)
+            if t.dtype not in kinds:
+                raise QMatmulError(fn, 3, f"{name} of {t.dtype}: float16, bfloat16 or float8_e4m3fn")
+        if k.shape != v.shape or k.dtype != v.dtype or any(a != b for a, b, n in zip(k.stride(), v.stride(), k.shape) if n > 1):
+            _refuse(fn, f"k {tuple(k.shape)} {k.dtype} {k.stride()} and v {tuple(v.shape)} {v.dtype} {v.stride()} are laid out differently")
+        pages, heads, page, D = k.shape
+        _sizes(fn, pages, heads, page, D)
+        if (k_scale is None) != (k.dtype != torch.float8_e4m3fn) or (k_scale is None) != (v_scale is None):
+            _refuse(fn, "k_scale and v_scale belong to float8_e4m3fn, and to nothing else")
+        for name, t, shape, dtype in (("k_scale", k_scale, (pages, heads, page), torch.float32), ("v_scale", v_scale, (pages, heads, page), torch.float32),
+                                      ("mean", mean, (pages, heads, D), torch.bfloat16)):
+            if t is not None:
+                _check_rows(fn, name, t, 3, dev)
+                if tuple(t.shape) != shape or t.dtype != dtype or not t.is_contiguous():
+                    _refuse(fn, f"{name} {tuple(t.shape)} {t.dtype}: contiguous {dtype} {shape}")
+        self.k, self.v, self.k_scale, self.v_scale, self.mean = k, v, k_scale, v_scale, mean
+        self.pages, self.heads, self.page, self.D, self.dtype, self.device_index = pages, heads, page, D, k.dtype, dev
+        at = lambda t: None if t is None else t.data_ptr()  # noqa: E731
+        self.view = QmKv(kinds[k.dtype], D, heads, page, pages, k.stride(0), k.stride(1), k.stride(2), k.data_ptr(), v.data_ptr(),
+                         at(k_scale), at(v_scale), at(mean))
+        self.ref = ctypes.byref(self.view)
+
+    @classmethod
+    def new(cls, pages, heads, page, D, dtype, mean=False):
+        """An empty cache on the current GPU."""
+        import torch
+        made = lambda *shape, dtype: torch.zeros(shape, dtype=dtype, device="cuda")  # noqa: E731
+        k, v = (made(pages, heads, page, D, dtype=torch.uint8 if dtype == torch.float8_e4m3fn else dtype) for _ in range(2))
+        scales = [made(pages, heads, page, dtype=torch.float32) for _ in range(2)] if dtype == torch.float8_e4m3fn else [None, None]
+        return cls(k.view(dtype), v.view(dtype), *scales, made(pages, heads, D, dtype=torch.bfloat16) if mean else None)
+
+
+def _check_int32(fn, name, t, dim, dev):
+    _check_rows(fn, name, t, dim, dev)
+    if t.dtype != _torch.int32 or not t.is_contiguous():
+        _refuse(fn, f"{name} {tuple(t.shape)} {t.dtype}: contiguous int32")
+
+
+def _check_cache(fn, kv, dev):
+    if kv.device_index != dev:
+        _refuse(fn, "the cache is not on the current GPU")
+
+
+def kv_append(x, HQ, kv, slots, pos, inv_freq, wq=None, wk=None, eps=1e-6, adjacent=False, sections=None, turns=False, scale=1.0,
+              q_off=0, q_hs=None, k_off=None, k_hs=None, v_off=None, v_hs=None, q=None, out=None, stream=None):
+    """qk_norm_rope of rows x [T, ldx] with the keys and the value heads (neither normed nor turned) to a KvCache: token t to its place
+    slots[t] (int32 [T]: page * tokens of a page + place in it; one outside the cache, as a negative one, is not stored; no two the same).
+    Value head h is at column v_off + h * v_hs (behind the key heads unless given). With kv.mean: the mean key of each page whose last
+    token is among these. Returns q [T, HQ, D] of type out (that of a given q, else the cache's, bfloat16 for an 8-bit one), or the q given."""
+    fn = "qmatmul_kv_append"
+    dev = _current_gpu()
+    torch = _torch
+    f32 = torch.float32
+    D, HK = kv.D, kv.heads
+    _check_cache(fn, kv, dev)
+    _check_rows(fn, "x", x, 2, dev)
+    T, width = x.shape
+    _check_int32(fn, "slots", slots, 1, dev)
+    axes, half = 1 if pos.dim() == 1 else pos.size(0), inv_freq.numel()
+    _check_rows(fn, "pos", pos, None, dev)
+    _check_rows(fn, "inv_freq", inv_freq, 1, dev)
+    if pos.dtype != torch.int32 or pos.dim() not in (1, 2) or pos.shape[-1] != T or slots.numel() != T:
+        _refuse(fn, f"pos {tuple(pos.shape)} {pos.dtype}, slots {tuple(slots.shape)}: int32, one column for each of {T} tokens")
+    if inv_freq.dtype != f32:
+        _refuse(fn, f"inv_freq {inv_freq.dtype}: float32")
+    for w in (wq, wk):
+        if w is not None:
+            _check_rows(fn, "wq or wk", w, 1, dev)
+            if w.dtype != f32 or w.numel() != D:
+                _refuse(fn, f"wq or wk {tuple(w.shape)} {w.dtype}: float32 [{D}]")
+    if sections is None:
+        sections = (half,)
+    if len(sections) != axes or axes > 4 or sum(sections) != half:
+        _refuse(fn, f"sections {sections}: one for each of {axes} axes (at most 4), their sum {half}")
+    q_hs, k_hs, v_hs = (D if hs is None else hs for hs in (q_hs, k_hs, v_hs))
+    if k_off is None:
+        k_off = q_off + HQ * q_hs
+    if v_off is None:
+        v_off = k_off + HK * k_hs
+    ldx, ps = x.stride(0) if T > 1 else _row_stride(x), pos.stride(0) if axes > 1 else T
+    if (T | HQ | ldx | ps | q_off | q_hs | k_off | k_hs | v_off | v_hs | 2 * half) >> 31 or (axes > 1 and min(sections) < 0):
+        _sizes(fn, T, HQ, ldx, ps, q_off, q_hs, k_off, k_hs, v_off, v_hs, 2 * half, *sections)
+        if HQ < 0:
+            _refuse(fn, f"HQ {HQ}")
+    rope = QmRope(2 * half, adjacent, axes, turns, tuple(sections), scale)
+    if max(q_off + (HQ - 1) * q_hs if HQ else 0, k_off + (HK - 1) * k_hs, v_off + (HK - 1) * v_hs) + D > width:
+        _refuse(fn, f"rows of {width} elements do not hold the heads")
+    if out is None:
+        out = q.dtype if q is not None else kv.dtype if kv.dtype != torch.float8_e4m3fn else torch.bfloat16
+    if q is None:
+        q, ldq = x.new_empty((T, HQ, D), dtype=out), HQ * D
+    else:
+        ldq = _head_rows(fn, "q", q, T, HQ, D, out, dev)
+    st = _function(fn)(x.data_ptr(), _dtype(x.dtype), ldx, T, q_off, q_hs, HQ, k_off, k_hs, v_off, v_hs,
+                       None if wq is None else wq.data_ptr(), None if wk is None else wk.data_ptr(), eps, ctypes.byref(rope),
+                       pos.data_ptr(), ps, inv_freq.data_ptr(), slots.data_ptr(), kv.ref, q.data_ptr(), _dtype(out), ldq,
+                       _current_stream(dev) if stream is None else stream)
+    _done(fn, st)
+    return q
+
+
+def _query(fn, q, kv, dev):
+    """(T, HQ, ldq) of queries [T, HQ, D] (heads next to each other)."""
+    _check_cache(fn, kv, dev)
+    _check_rows(fn, "q", q, 3, dev)
+    T, HQ, D = q.shape
+    if D != kv.D or (HQ > 1 and q.stride(1) != D):
+        _refuse(fn, f"q {tuple(q.shape)}, strides {q.stride()}: heads of {kv.D} next to each other")
+    ldq = _stride_of(q.stride(0), HQ * D, T)
+    if (T | HQ | ldq) >> 31:
+        _sizes(fn, T, HQ, ldq)
+    return T, HQ, ldq
+
+
+def _batch(fn, T, lens, table, start, dev):
+    _check_int32(fn, "lens", lens, 1, dev)
+    _check_int32(fn, "table", table, 2, dev)
+    B = lens.numel()
+    if start is not None:
+        _check_int32(fn, "start", start, 1, dev)
+    if table.size(0) != B or (T != B if start is None else start.numel() != B + 1):
+        _refuse(fn, f"{T} rows, lens {tuple(lens.shape)}, table {tuple(table.shape)}, start {None if start is None else tuple(start.shape)}: "
+                    "a length and a row of pages for each sequence, start one more (or a row of q for each)")
+    _sizes(fn, B, table.size(1))
+    return QmSeqs(T, B, None if start is None else start.data_ptr(), lens.data_ptr(), table.data_ptr(), table.size(1))
+
+
+def _workspace(fn, ws, dev):
+    if ws is None:
+        return None, 0
+    _check_rows(fn, "ws", ws, 1, dev)
+    return ws.data_ptr(), ws.numel() * ws.element_size()
+
+
+def attn_workspace(kv, T, B, HQ, prefix_len=0):
+    """A workspace for attn_prefix of T rows of B sequences (None where it needs none), or with B = T for attn_pages. Its size grows
+    with neither the lengths nor the cache."""
+    import torch
+    fn = "qmatmul_attn_workspace_size"
+    _sizes(fn, T, B, HQ, prefix_len)
+    n = _function(fn)(kv.ref, T, B, HQ, prefix_len)
+    return torch.empty((n,), dtype=torch.uint8, device="cuda") if n else None
+
+
+def _attention(fn, q, kv, lens, table, start, scale, o, out, ws, stream, *more):
+    dev = _current_gpu()
+    T, HQ, ldq = _query(fn, q, kv, dev)
+    seqs = _batch(fn, T, lens, table, start, dev)
+    if out is None:
+        out = q.dtype if o is None else o.dtype
+    if o is None:
+        # (rows of no sequence are not written: without a list of rows there are none)
+        o, ldo = (q.new_empty if start is None else q.new_zeros)((T, HQ, kv.D), dtype=out), HQ * kv.D
+    else:
+        ldo = _head_rows(fn, "o", o, T, HQ, kv.D, out, dev)
+    ws_ptr, ws_bytes = _workspace(fn, ws, dev)
+    st = _function(fn)(q.data_ptr(), _dtype(q.dtype), ldq, HQ, ctypes.byref(seqs), kv.ref, *more, kv.D ** -0.5 if scale is None else scale,
+                       o.data_ptr(), _dtype(out), ldo, ws_ptr, ws_bytes, _current_stream(dev) if stream is None else stream)
+    _done(fn, st)
+    return o
+
+
+def attn_prefix(q, kv, lens, table, start=None, prefix=None, prefix_len=0, scale=None, o=None, out=None, ws=None, stream=None):
+    """Attention of q [T, HQ, D] (float16 or bfloat16, the cache's type unless that is of 8 bits) over a KvCache: over prefix_len tokens that
+    all sequences share, in pages prefix (int32), and over each sequence's own up to the row itself. Sequence b has lens[b] tokens (int32
+    [B]), these rows among them, in pages table[b] (int32 [B, pages]), and rows start[b] .. start[b + 1] - 1 of q (int32 [B + 1]; None: row b).
+    scale: D ** -0.5 unless given. Returns o [T, HQ, D] of type out (q's, or float32; rows of no sequence zeros), or writes the o given (rows of no
+    sequence stay). ws: of attn_workspace, for one call at a time; without one the prefix is not shared and long sequences not cut."""
+    fn = "qmatmul_attn_prefix"
+    prefix_ptr = None
+    if prefix_len:
+        _sizes(fn, prefix_len)
+        if prefix is None:
+            _refuse(fn, "prefix_len without a prefix")
+        _check_int32(fn, "prefix", prefix, 1, _current_gpu())
+        if prefix_len < 0 or prefix.numel() * kv.page < prefix_len:
+            _refuse(fn, f"{prefix.numel()} pages of {kv.page} tokens do not hold a prefix of {prefix_len}")
+        prefix_ptr = prefix.data_ptr()
+    return _attention(fn, q, kv, lens, table, start, scale, o, out, ws, stream, prefix_ptr, prefix_len)
+
+
+def attn_pages(q, kv, lens, table, sel, start=None, scale=None, o=None, out=None, ws=None, stream=None):
+    """attn_prefix (without a prefix) over chosen pages only: sel int32 [T, heads, k], numbers of pages in the row's sequence for each key
+    head, others than those of the table none (-1). ws: of attn_workspace(kv, T, T, HQ)."""
+    fn = "qmatmul_attn_pages"
+    _check_int32(fn, "sel", sel, 3, _current_gpu())
+    if tuple(sel.shape[:2]) != (q.size(0), kv.heads):
+        _refuse(fn, f"sel {tuple(sel.shape)}: pages for each of {q.size(0)} rows and {kv.heads} key heads")
+    _sizes(fn, sel.size(2))
+    return _attention(fn, q, kv, lens, table, start, scale, o, out, ws, stream, sel.data_ptr(), sel.size(2))
+
+
+def select_workspace(kv, T, pages):
+    """A workspace for select_pages of T rows with tables of `pages` pages."""
+    import torch
+    fn = "qmatmul_select_workspace_size"
+    _sizes(fn, T, pages)
+    n = _function(fn)(kv.ref, T, pages)
+    return torch.empty((n,), dtype=torch.uint8, device="cuda") if n else None
+
+
+def select_pages(q, kv, lens, table, k, start=None, first=1, last=1, sel=None, ws=None, stream=None):
+    """The k pages of its sequence that each row's query heads score highest, by the pages' mean keys (kv.mean), the `first` first and `last`
+    last ones always among them: int32 [T, heads, k], ascending, -1 behind them, for attn_pages (rows of no sequence: -1; in a sel
+    given they stay). ws: of select_workspace; made for the call where it is not given and needed."""
+    fn = "qmatmul_select_pages"
+    dev = _current_gpu()
+    T, HQ, ldq = _query(fn, q, kv, dev)
+    seqs = _batch(fn, T, lens, table, start, dev)
+    if kv.mean is None:
+        _refuse(fn, "the cache has no means")
+    _sizes(fn, k, first, last)
+    if sel is None:
+        sel = lens.new_empty((T, kv.heads, k)) if start is None else lens.new_full((T, kv.heads, k), -1)
+    else:
+        _check_int32(fn, "sel", sel, 3, dev)
+        if tuple(sel.shape) != (T, kv.heads, k):
+            _refuse(fn, f"sel {tuple(sel.shape)}: [{T}, {kv.heads}, {k}]")
+    if ws is None and table.size(1) > k:
+        ws = select_workspace(kv, T, table.size(1))
+    ws_ptr, ws_bytes = _workspace(fn, ws, dev)
+    st = _function(fn)(q.data_ptr(), _dtype(q.dtype), ldq, HQ, ctypes.byref(seqs), kv.ref, k, first, last, sel.data_ptr(), ws_ptr, ws_bytes,
+                       _current_stream(dev) if stream is None else stream)
+    _done(fn, st)
+    return sel
 
 
 class GgufTensor:

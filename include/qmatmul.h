@@ -309,7 +309,7 @@ int qmatmul_gemm_fp8(const qm_fp8_weight* w, const uint8_t* a8, const float* asc
 
 /* ---- Query and key heads ------------------------------------------------------------------------------------------
  * The step after the QKV product: RMS norm of each query and key head and the rotation by the token's position, in one
- * pass (attention itself is not part of this library).
+ * pass. (With a cache of keys and values: qmatmul_kv_append below.)
  *
  * Rotation: the first rot elements of a head (rot even, <= D) are rot/2 pairs, the rest pass. Pair i is elements
  * (i, i + rot/2), or (2i, 2i + 1) with adjacent, and turns by pos[axis(i)][t] * inv_freq[i]:
@@ -338,6 +338,82 @@ int qmatmul_qk_norm_rope(const void* x, int xtype, int ldx, int T, int D, int q_
                          int HK, const float* wq, const float* wk, float eps, const qm_rope* rope, const int32_t* pos,
                          int pos_stride, const float* inv_freq, void* q, void* k, int otype, int ldq, int ldk,
                          void* stream);
+
+/* ---- Keys and values in pages, and attention over them ----------------------------------------------------------------
+ * The cache of one layer: pages of `page` tokens (16, 32, 64, 128 or 256), each with every key head's keys and values of D
+ * elements (a multiple of 16, 16..256). Element d of head h of token i of page p is at p * page_stride + h * head_stride +
+ * i * token_stride + d, in k and in v alike (strides in elements; every row of D 16-byte aligned; no two elements at one
+ * place). Any order of the dimensions serves; heads outside tokens, as in [pages][heads][page][D], is read fastest.
+ * Types: QM_F16, QM_BF16, or QM_E4M3 with an f32 scale for each token and head, k_scale and v_scale [pages][heads][page]
+ * (16-byte aligned; the value is scale * e4m3). mean (or NULL): bf16 [pages][heads][D], the mean key of each page that was
+ * filled, which qmatmul_select_pages scores pages by. pages * page < 2^31. The buffers are the caller's.
+ *
+ * A list of pages is trusted with values, not with memory: a page number outside 0..pages-1 is a page whose keys are masked (and a
+ * token that has no place there is not stored); lengths and rows are clamped to the call's sizes. */
+enum { QM_E4M3 = 256 }; /* a cache's element type only */
+typedef struct {
+  int type, D, heads, page, pages;
+  long long page_stride, head_stride, token_stride;
+  void *k, *v;
+  float *k_scale, *v_scale; /* QM_E4M3 */
+  uint16_t* mean;           /* or NULL */
+} qm_kv;
+
+/* The sequences of a batch. q has T rows (tokens): rows start[b] .. start[b+1] - 1 are sequence b's, the last tokens of its
+ * len[b]; its token i is in page table[b * table_stride + i / page]. start NULL: T = B, row b is the last token of sequence b.
+ * start (not descending), len and table are device pointers, read when the call runs: a captured graph's sequences may grow.
+ * Rows of no sequence (before start[0], from start[B] on) are left as they are. table_stride * page <= 2^30. */
+typedef struct {
+  int T, B;
+  const int32_t* start; /* [B + 1], or NULL */
+  const int32_t* len;   /* [B] */
+  const int32_t* table; /* [B][table_stride] */
+  int table_stride;
+} qm_seqs;
+
+/* qmatmul_qk_norm_rope with the keys and values to a cache: the arguments are its own but for v_off and v_hs (the value heads in x,
+ * HK = kv->heads of them, neither normed nor turned), slots int32 [T] (token t goes to token slots[t] % page of page slots[t] / page;
+ * outside the cache, as a negative one is: not stored) and kv, instead of k, otype being q's. The slots of a call are
+ * distinct (of two tokens with one, either's elements may stay). Keys and values are computed in f32 and rounded once; to e4m3 by the scale
+ * amax / 448 of their head (a head whose amax is below 2^-100: zeros and scale 0; NaN and infinities as in qmatmul_quantize_fp8).
+ * With kv->mean: the mean of each page whose last token the call stored, of its keys as they are held. q may be NULL with HQ = 0. T < 2^24.
+ * Outputs that overlap an input or each other are refused, but for q in place. */
+int qmatmul_kv_append(const void* x, int xtype, int ldx, int T, int q_off, int q_hs, int HQ, int k_off, int k_hs, int v_off,
+                      int v_hs, const float* wq, const float* wk, float eps, const qm_rope* rope, const int32_t* pos,
+                      int pos_stride, const float* inv_freq, const int32_t* slots, const qm_kv* kv, void* q, int qtype, int ldq,
+                      void* stream);
+
+/* Attention of each sequence's rows over prefix_len tokens that all sequences share and over their own up to the row itself:
+ *   o[t][h] = sum_j w_j v_j / sum_j w_j,  w_j = e^(scale q[t][h] . k_j),  k_j, v_j of key head h / (HQ / heads)
+ * j over the prefix (token i in page prefix[i / page]; prefix_len <= 2^30, 0 and NULL: none) and over the sequence's own tokens, of
+ * which row i of n sees the first len - n + i + 1. A row that sees no key is zeros. What lies in masked places (behind a sequence, in
+ * pages that are none, in later tokens) has no effect, whatever it holds.
+ * q: qtype QM_F16 or QM_BF16, that of the cache unless it is QM_E4M3; head h of row t at t * ldq + h * D; HQ a multiple of
+ * kv->heads. o: otype qtype or QM_F32, row stride ldo. Products are exact, sums f32; weights are rounded to 16 bits for the second product
+ * where o is of a type with no more of them (bf16; f16 behind an f16 cache), and held in two parts of 16 bits elsewhere.
+ * ws: device workspace, 256-byte aligned, of qmatmul_attn_workspace_size bytes (which grows with neither lengths nor the cache); NULL or a
+ * smaller one: the prefix is read by each sequence for itself, and sequences are cut into fewer pieces or none, slower. Calls that may
+ * overlap need different workspaces. o and ws may not overlap each other, q or the cache. No allocation, no host synchronisation; the
+ * call can be captured into a graph. */
+size_t qmatmul_attn_workspace_size(const qm_kv* kv, int T, int B, int HQ, int prefix_len);
+int qmatmul_attn_prefix(const void* q, int qtype, int ldq, int HQ, const qm_seqs* seqs, const qm_kv* kv, const int32_t* prefix,
+                        int prefix_len, float scale, void* o, int otype, int ldo, void* ws, size_t ws_bytes, void* stream);
+
+/* The pages that attention is worth for: of the pages of its sequence that row t sees, sel[t][h] lists k for each key head h (all where
+ * there are no more), ascending, -1 behind them: the `first` first and the `last` last ones (last >= 1: the page that is being
+ * filled has no mean yet; first + last <= k), and of the others those with the largest scores,
+ *   score = max over the query heads g of h of q[t][g] . mean[page][h]  (in f64; a NaN is passed over; ties to the lower page)
+ * sel int32 [T][kv->heads][k]. kv->mean is required (k and v are not read); a page that is none scores minus infinity. q as above, of either type. ws: required
+ * where table_stride > k, qmatmul_select_workspace_size bytes (8 for each row, key head and page of the table), 256-byte aligned. */
+size_t qmatmul_select_workspace_size(const qm_kv* kv, int T, int table_stride);
+int qmatmul_select_pages(const void* q, int qtype, int ldq, int HQ, const qm_seqs* seqs, const qm_kv* kv, int k, int first, int last,
+                         int32_t* sel, void* ws, size_t ws_bytes, void* stream);
+
+/* qmatmul_attn_prefix over chosen pages only: row t sees, for key head h, the tokens up to its own of the pages sel[t][h][0..k-1] (their
+ * numbers in the sequence, in any order; others than 0..table_stride-1 are none, one that is listed twice counts twice). k * page <= 2^30. ws:
+ * qmatmul_attn_workspace_size(kv, T, T, HQ, 0) bytes, or NULL or less as above. */
+int qmatmul_attn_pages(const void* q, int qtype, int ldq, int HQ, const qm_seqs* seqs, const qm_kv* kv, const int32_t* sel, int k,
+                       float scale, void* o, int otype, int ldo, void* ws, size_t ws_bytes, void* stream);
 
 /* GGUF files (host side). Maps a GGUF v2/v3 file read-only and indexes its metadata and tensors, so a weight can
  * go to qmatmul_prepare_weight straight from the mapping (raw_on_device = 0; rows = dims[1] * dims[2] * ..., K =
