@@ -8,98 +8,79 @@ hipError_t attn_f16(const AttnArgs& a, int mt, int mode, unsigned grid, hipStrea
 hipError_t attn_bf16_e4m3(const AttnArgs& a, int mt, int mode, unsigned grid, hipStream_t s);
 hipError_t attn_f16_e4m3(const AttnArgs& a, int mt, int mode, unsigned grid, hipStream_t s);
 
-// Joins the pieces of one row: o = sum_p 2^(m_p - m) o_p / sum_p 2^(m_p - m) l_p, in the order of the pieces, the prefix's first. A
-// work-group a row (a query head of a token): D / 4 lanes of four elements, the pieces dealt to 1024 / D groups of lanes. Every
-// partial result is read once; rows of a single piece are left as attn_kernel wrote them.
+// Joins the pieces of one row: o = sum_p 2^(m_p - m) o_p / sum_p 2^(m_p - m) l_p, in one pass over them with the running maximum. A
+// work-group a row (a query head of a token): D / 4 lanes of four elements, the pieces dealt to 1024 / D groups of lanes, the groups joined
+// in their order. Every partial result is read once; rows of a single piece are left as attn_kernel wrote them. What a row needs to
+// know of the split stands in its tile's first slot. Latency-bound: a launch, that slot's words, the partial results.
 __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a, int RT, int chosen) {
-  __shared__ long long red[4];
-  __shared__ float wave_max[4], lsum[256];
+  __shared__ float gmax[256], gsum[256];
   __shared__ float4 osum[256];
-  const int hq = blockIdx.x % a.HQ, t = blockIdx.x / a.HQ, h = hq / a.G, D = a.kv.D;
+  const int hq = blockIdx.x % a.HQ, t = blockIdx.x / a.HQ, h = hq / a.G, g = hq % a.G, D = a.kv.D;
   const int b = sequence_of(a.s, t);
   if (b < 0) return;
-  const int row0 = row_from(a.s, b), rows = rows_of(a.s, b);
-  long long unit, step;  // the slot of this row tile's first piece, and from one piece to the next
-  int own, at;           // own pieces, and the row's place in its tile
-  if (chosen) {
-    const int rts = (a.G + RT - 1) / RT, rt = hq % a.G / RT;
-    own = a.pieces;
-    at = hq % a.G % RT;
-    unit = (long long)t * rts * a.pieces + rt;
-    step = rts;
-  } else {
-    const int blocks = piece_blocks(a, RT, red);
-    const int r = (t - row0) * a.G + hq % a.G, rt = r / RT, rts = (rows * a.G + RT - 1) / RT;
-    at = r % RT;
-    long long before = 0;
-    for (int i = threadIdx.x; i < b; i += 256) {
-      const int n = (rows_of(a.s, i) * a.G + RT - 1) / RT;
-      before += n ? (long long)n * pieces_of(a, i, blocks) : 0;
-    }
-    unit = sum256(before, red) + rt;
-    step = rts;
-    // (the keys that the tile's last row sees, as attn_kernel counts them)
-    const int last = min(rt * RT + RT, rows * a.G) - 1;
-    const long long most = (long long)a.s.W << a.kv.lg;
-    const int lim = (int)min((long long)max(a.s.len[b] - rows + last / a.G + 1, 0), min(most, 0x7fffffffLL));
-    const int n = (a.prefix_len + kBlock - 1) / kBlock + (int)(((long long)lim + kBlock - 1) / kBlock);
-    own = (int)(((n + kWaves - 1) / kWaves + (long long)blocks - 1) / blocks);
-    if (own < 1) own = 1;
-    if (!a.shared && own == 1) return;
-  }
-  const int all = a.shared + own;
-  const long long srow = (long long)t * a.G + hq % a.G;
-  const auto slot = [&](int p, int& rt, int& r) -> const float* {
-    if (p < a.shared) {
-      rt = a.shared_rt;
-      r = (int)(srow % rt);
-      return a.shared_part + ((size_t)(h * a.shared_tiles + srow / rt) * a.shared + p) * ((size_t)rt * (D + 2));
-    }
-    rt = RT;
-    r = at;
-    const long long i = (unit + (p - a.shared) * step) * a.kv.HK + h;
-    return i < a.slots ? a.part + (size_t)i * ((size_t)rt * (D + 2)) : nullptr;
-  };
-  float top = -__builtin_inff();
-  for (int p = threadIdx.x; p < all; p += 256) {
-    int rt, r;
-    const float* s = slot(p, rt, r);
-    // (a piece whose rows saw nothing has the sum 0, whatever its maximum says)
-    if (s && s[rt + r] != 0.0f) top = fmaxf(top, s[r]);
-  }
-  for (int o = 32; o; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
-  if ((threadIdx.x & 63) == 0) wave_max[threadIdx.x >> 6] = top;
-  __syncthreads();
-  top = fmaxf(fmaxf(wave_max[0], wave_max[1]), fmaxf(wave_max[2], wave_max[3]));
+  const int row0 = chosen ? t : row_from(a.s, b), r0 = (t - row0) * a.G + g, rt = r0 / RT;
+  const long long n0 = (long long)(chosen ? t * ((a.G + RT - 1) / RT) + rt : first_slot(a, RT, b, row0, rt)) * a.kv.HK + h;
+  if (n0 >= a.slots) return;
+  const size_t size = slot_floats(RT, D);
+  const float* first = a.part + (size_t)n0 * size;
+  const int4 head = *(const int4*)first;
+  if (!a.shared && head.x == 1) return;
+  const int all = a.shared + head.x;
+  const long long srow = (long long)t * a.G + g;
+  const size_t ssize = slot_floats(a.shared_rt, D);
   const int lanes = D / 4, groups = 256 / lanes, group = (int)threadIdx.x / lanes, d = 4 * ((int)threadIdx.x % lanes);
-  float l = 0.0f;
+  float top = -__builtin_inff(), l = 0.0f;
   float4 o = {0.0f, 0.0f, 0.0f, 0.0f};
-  if (group < groups)
+  if (group < groups) {
+#pragma unroll 4
     for (int p = group; p < all; p += groups) {
-      int rt, r;
-      const float* s = slot(p, rt, r);
-      if (!s || s[rt + r] == 0.0f) continue;
-      const float f = __builtin_amdgcn_exp2f(s[r] - top);
-      const float4 v = *(const float4*)(s + 2 * rt + (size_t)r * D + d);
-      l = fmaf(f, s[rt + r], l);
-      o.x = fmaf(f, v.x, o.x);
-      o.y = fmaf(f, v.y, o.y);
-      o.z = fmaf(f, v.z, o.z);
-      o.w = fmaf(f, v.w, o.w);
+      const float* s;
+      int rows = RT, r = r0 % RT;
+      if (p < a.shared) {
+        rows = a.shared_rt;
+        r = (int)(srow % rows);
+        s = a.shared_part + ((size_t)(h * a.shared_tiles + srow / rows) * a.shared + p) * ssize;
+      } else if (p == a.shared) {
+        s = first;
+      } else {
+        const long long n = ((long long)head.y + (long long)(p - a.shared - 1) * head.z) * a.kv.HK + h;
+        if (n >= a.slots) continue;
+        s = a.part + (size_t)n * size;
+      }
+      s += 4;
+      const float m = s[r], w = s[rows + r];
+      const float4 v = *(const float4*)(s + 2 * rows + (size_t)r * D + d);
+      if (w == 0.0f) continue;  // (a piece that the row sees nothing of)
+      const float now = fmaxf(top, m), f0 = top == now ? 1.0f : __builtin_amdgcn_exp2f(top - now), f = __builtin_amdgcn_exp2f(m - now);
+      top = now;
+      l = fmaf(f, w, l * f0);
+      o.x = fmaf(f, v.x, o.x * f0);
+      o.y = fmaf(f, v.y, o.y * f0);
+      o.z = fmaf(f, v.z, o.z * f0);
+      o.w = fmaf(f, v.w, o.w * f0);
     }
-  lsum[threadIdx.x] = l;
+  }
+  gmax[threadIdx.x] = top;
+  gsum[threadIdx.x] = l;
   osum[threadIdx.x] = o;
   __syncthreads();
   if (group) return;
-  for (int i = 1; i < groups; ++i) {
-    const float4 v = osum[i * lanes + threadIdx.x];
-    l += lsum[i * lanes + threadIdx.x];
-    o.x += v.x;
-    o.y += v.y;
-    o.z += v.z;
-    o.w += v.w;
+  float most = top;
+  for (int i = 1; i < groups; ++i) most = fmaxf(most, gmax[i * lanes + threadIdx.x]);
+  l = 0.0f;
+  o = {0.0f, 0.0f, 0.0f, 0.0f};
+  for (int i = 0; i < groups; ++i) {
+    const int at = i * lanes + threadIdx.x;
+    if (gsum[at] == 0.0f) continue;
+    const float f = __builtin_amdgcn_exp2f(gmax[at] - most);
+    const float4 v = osum[at];
+    l = fmaf(f, gsum[at], l);
+    o.x = fmaf(f, v.x, o.x);
+    o.y = fmaf(f, v.y, o.y);
+    o.z = fmaf(f, v.z, o.z);
+    o.w = fmaf(f, v.w, o.w);
   }
-  const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
+  const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;  // (a row that sees no key is zeros)
   const float y[4] = {o.x * inv, o.y * inv, o.z * inv, o.w * inv};
   const size_t to = (size_t)t * a.ldo + (size_t)hq * D + d;
 #pragma unroll
@@ -116,16 +97,21 @@ constexpr int kTarget = 1024;        // pieces that a call is cut into
 constexpr int kSharedTarget = 512;   // pieces of the shared prefix
 constexpr int kSharedFrom = 256;     // a shorter prefix is read with each sequence's own keys
 
-int tiles_for(long long rows, int D) { return rows <= 16 ? 1 : rows <= 32 || D > 128 ? 2 : 4; }
+// Row tiles of 16 a work-group: what its registers hold
+int tiles_for(long long rows, int D) {
+  const int most = D <= 64 ? 4 : D <= 128 ? 2 : 1;
+  const int want = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
+  return want < most ? want : most;
+}
 long long div_up(long long a, long long b) { return (a + b - 1) / b; }
 // Row tiles of all sequences at most
 long long row_tiles(int T, int B, bool start, int G, int rt) {
-  return start ? (long long)T * G / rt + (B < T ? B : T) : (B < T ? B : T) * div_up(G, rt);
+  return start ? (long long)T * G / rt + B : B * div_up(G, rt);  // (as first_slot counts them)
 }
 
 }  // namespace
 
-size_t attn_slot_bytes(int mt, int D) { return (size_t)16 * mt * (D + 2) * sizeof(float); }
+size_t attn_slot_bytes(int mt, int D) { return (4 + (size_t)16 * mt * (D + 2)) * sizeof(float); }
 
 AttnPlan attn_plan(int T, int B, bool start, int HQ, int HK, int D, int prefix_len, size_t ws_bytes) {
   AttnPlan p{};
@@ -154,6 +140,7 @@ AttnPlan attn_plan(int T, int B, bool start, int HQ, int HK, int D, int prefix_l
     p.target = (int)(n < kTarget ? n : kTarget);
   }
   p.slots = p.target || p.shared ? (int)(items + p.target) : 0;
+  p.firsts = (int)(items / HK);
   return p;
 }
 
@@ -190,10 +177,12 @@ hipError_t launch_attn(const AttnArgs& args, const AttnPlan& p, hipStream_t s) {
   float* ws = a.part;
   a.target = p.target;
   a.slots = p.slots;
+  a.firsts = p.firsts;
   a.shared = 0;
+  a.shared_rt = 16;
   if (a.sel) {  // as many pieces for every token: the target's, within the slots
     const long long items = row_tiles(a.s.T, a.s.T, false, a.G, 16 * p.mt) * a.kv.HK, blocks = div_up((long long)a.k * a.kv.page, 128);
-    long long n = p.slots / items;
+    long long n = p.slots / items;  // (as all first pieces, and as many more)
     if (n > blocks) n = blocks;
     if (n < 1) n = 1;
     a.blocks = (int)div_up(blocks, n);

@@ -78,6 +78,9 @@ __device__ __forceinline__ v4i widen8(int lo, int hi) {
   return v4i{widen2<T, false>(lo), widen2<T, true>(lo), widen2<T, false>(hi), widen2<T, true>(hi)};
 }
 
+// p[i] by the scalar unit (i is the same for the whole wave): a vector load would have to be waited for behind the keys' and values'
+__device__ __forceinline__ int scalar(const int32_t* p, size_t i) { return ((const __attribute__((address_space(4))) int32_t*)p)[i]; }
+
 // N results to a row of any alignment, 16 bytes at a time where it is aligned to them (N values)
 template <typename T, int N>
 __device__ __forceinline__ void store_row(T* p, const float* y) {
@@ -97,19 +100,48 @@ __device__ __forceinline__ void store_row(T* p, const float* y) {
   }
 }
 
-// Whether a 16-bit word holds a value that is not finite in either half
+// Whether a word of the cache's type holds a value that is not finite
 template <typename T>
-__device__ __forceinline__ bool odd_half(int w) {
-  constexpr int e = __is_same(T, _Float16) ? 0x7C00 : 0x7F80;
-  return (w & e) == e || (w >> 16 & e) == e;
+__device__ __forceinline__ bool odd_word(int w) {
+  if constexpr (sizeof(T) == 1) {
+    const unsigned x = (unsigned)w & 0x7f7f7f7fu;  // (0x7f and 0xff are NaN: a byte that 1 carries out of)
+    return ((x + 0x01010101u) & 0x80808080u) != 0;
+  } else {
+    constexpr int e = __is_same(T, _Float16) ? 0x7C00 : 0x7F80;
+    return ((w & e) == e) | ((w >> 16 & e) == e);
+  }
 }
 
-// TQ: q's type. TC: the cache's, TQ or uint8_t (e4m3). DC: D rounded up to 64, 128 or 256. MT: row tiles of 16. PARTS: of P. MODE: the keys of
+// Values that are not finite, in a word of two 16-bit values: as ones where they are of a kind (0 NaN, 1 plus and 2 minus infinity), else zeros
+template <typename T>
+__device__ __forceinline__ constexpr int one16() { return __is_same(T, _Float16) ? 0x3C00 : 0x3F80; }
+template <typename T>
+__device__ __forceinline__ int odd_ones(int w, int kind) {
+  constexpr int e = __is_same(T, _Float16) ? 0x7C00 : 0x7F80;
+  const auto one = [&](int v) {
+    const bool is = kind == 0 ? (v & 0x7FFF) > e : kind == 1 ? v == e : v == (e | 0x8000);
+    return is ? one16<T>() : 0;
+  };
+  return one(w & 0xFFFF) | one(w >> 16 & 0xFFFF) << 16;
+}
+// The word with zeros in their place
+template <typename T>
+__device__ __forceinline__ int without_odd(int w) {
+  if constexpr (sizeof(T) == 1) {
+    const unsigned at = (((unsigned)w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
+    return w & ~(int)((at >> 7) * 255u);
+  } else {
+    constexpr int e = __is_same(T, _Float16) ? 0x7C00 : 0x7F80;
+    return w & ~(((w & e) == e ? 0xFFFF : 0) | ((w >> 16 & e) == e ? (int)0xFFFF0000 : 0));
+  }
+}
+
+// TQ: q's type. TC: the cache's, TQ or uint8_t (e4m3). DC: D rounded up to 64, 128 or 256 (FULL: it is that). MT: row tiles of 16. PARTS: of P. MODE: the keys of
 // each sequence (OWN), of the prefix for the rows of the whole batch (SHARED), or of chosen pages (CHOSEN).
 enum : int { OWN = 0, SHARED = 1, CHOSEN = 2 };
 
-template <typename TQ, typename TC, int DC, int MT, int PARTS, int MODE>
-__global__ __launch_bounds__(256) void attn_kernel(AttnArgs a) {
+template <typename TQ, typename TC, int DC, bool FULL, int MT, int PARTS, int MODE>
+__global__ __launch_bounds__(256, 2) void attn_kernel(AttnArgs a) {
   constexpr bool E8 = sizeof(TC) == 1;
   typedef std::conditional_t<E8, __bf16, TQ> TP;           // of P and V on the matrix pipe
   constexpr float kBias = __is_same(TP, _Float16) ? 6.0f : 0.0f;  // f16 weights are held times 2^6: with kSlack below 2^14, and small ones longer
@@ -118,15 +150,18 @@ __global__ __launch_bounds__(256) void attn_kernel(AttnArgs a) {
   constexpr int KL = E8 ? KS / 2 : KS;                     // loads of a key's 16 bytes
   typedef int kvec __attribute__((ext_vector_type(4)));
   typedef int vvec __attribute__((ext_vector_type(VE * (E8 ? 1 : 2) / 4)));
+  constexpr int VW = VE * (E8 ? 1 : 2) / 4;                // 32-bit words of a V vector
   constexpr int NO = VB * VE * MT;                         // results of four values
-  __shared__ float xo[2 * NO * 4 * 64];
+  constexpr bool QL = MT * DC >= 256;                      // q in LDS
+  constexpr bool LATE = MT * DC >= 256;                    // the next keys are asked for after the softmax: before it their registers are its own
+  constexpr int kJoin = (kWaves - 1) * NO / 4 * 64, kQs = QL ? MT * KS * 64 : 0, kLds = kJoin > kQs ? kJoin : kQs;  // (q's place is free when the waves join)
+  __shared__ v4f lds[kLds];
   __shared__ float stat[kWaves][2][RT];
-  __shared__ long long red[4];
-  __shared__ Item found;
 
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 15, g = lane >> 4;
   const KvView& kv = a.kv;
-  int h, b = 0, rt, c = 0, blocks = 0x7fffffff, row0 = 0, rows, unit = 0, after = 0;  // (after: tokens of the sequence behind these rows)
+  int h, b = 0, rt, c = 0, blocks = 0x7fffffff, row0 = 0, rows, after = 0;  // (after: tokens of the sequence behind these rows)
+  int rts = 1, more = 0;
   if constexpr (MODE == SHARED) {
     // the row tiles of one piece and head lie 8 work-groups apart: on one XCD, whose L2 then reads the piece once
     const unsigned w = blockIdx.x, at = w >> 3, pc = (at / a.shared_tiles) * 8 + (w & 7);
@@ -138,26 +173,27 @@ __global__ __launch_bounds__(256) void attn_kernel(AttnArgs a) {
     rows = a.s.T;
   } else if constexpr (MODE == CHOSEN) {
     // (each token's pages are its own: the tile is of one token, and every token has the same number of pieces)
+    const int unit = blockIdx.x / kv.HK;
     h = blockIdx.x % kv.HK;
-    unit = blockIdx.x / kv.HK;
-    const int rts = (a.G + RT - 1) / RT;
-    const int t = unit / (rts * a.pieces);
+    rts = (a.G + RT - 1) / RT;
+    row0 = unit / (rts * a.pieces);
     rt = unit % rts;
     c = unit / rts % a.pieces;
     blocks = a.blocks;
-    b = sequence_of(a.s, t);
+    b = sequence_of(a.s, row0);
     if (b < 0) return;  // (a row of no sequence)
-    row0 = t;
     rows = 1;
-    after = row_from(a.s, b) + rows_of(a.s, b) - 1 - t;
+    after = row_from(a.s, b) + rows_of(a.s, b) - 1 - row0;
   } else {
-    h = blockIdx.x % kv.HK;
-    unit = blockIdx.x / kv.HK;
-    if (!find_item<RT>(a, unit, &found, red)) return;
-    b = __builtin_amdgcn_readfirstlane(found.b);
-    rt = __builtin_amdgcn_readfirstlane(found.rt);
-    c = __builtin_amdgcn_readfirstlane(found.c);
-    blocks = __builtin_amdgcn_readfirstlane(found.blocks);
+    Item it;
+    if (!find_item(a, RT, blockIdx.x, it)) return;
+    b = __builtin_amdgcn_readfirstlane(it.b);
+    h = __builtin_amdgcn_readfirstlane(it.h);
+    rt = __builtin_amdgcn_readfirstlane(it.rt);
+    c = __builtin_amdgcn_readfirstlane(it.c);
+    rts = __builtin_amdgcn_readfirstlane(it.rts);
+    blocks = __builtin_amdgcn_readfirstlane(it.blocks);
+    more = __builtin_amdgcn_readfirstlane(it.more);
     row0 = __builtin_amdgcn_readfirstlane(row_from(a.s, b));
     rows = __builtin_amdgcn_readfirstlane(rows_of(a.s, b));
   }
@@ -183,30 +219,47 @@ __global__ __launch_bounds__(256) void attn_kernel(AttnArgs a) {
   const int end = (int)min((long long)begin + (long long)blocks * kWaves, (long long)all_blocks);
   if (MODE != SHARED && c > 0 && begin >= all_blocks) return;  // (a piece that this tile's rows do not see)
 
-  // q: k step t of row col holds elements 32 t + 8 g .. + 7 (8-bit keys: 64 (t / 2) + 16 g + 8 (t % 2), as their loads lie)
-  v4i q[MT][KS];
+  // q: k step t of row col holds elements 32 t + 8 g .. + 7 (8-bit keys: 64 (t / 2) + 16 g + 8 (t % 2), as their loads lie). Of larger
+  // tiles it stays in LDS, in operand order: the registers are the result's.
+  v4i* qs = (v4i*)lds;
+  v4i q[QL ? 1 : MT][QL ? 1 : KS];
   const bool qvec = ((uintptr_t)a.q & 15) == 0 && (a.ldq & 7) == 0;
 #pragma unroll
   for (int m = 0; m < MT; ++m) {
-    const int r = first + 16 * m + col;
+    if (QL && m % kWaves != wave) continue;
+    const int r = min(first + 16 * m + col, nrows - 1);
     const TQ* p = (const TQ*)a.q + (size_t)(row0 + r / a.G) * a.ldq + (size_t)(h * a.G + r % a.G) * kv.D;
+    v4i f[KS];
+    if (qvec) {
+#pragma unroll
+      for (int t = 0; t < KS; ++t) {
+        const int d = E8 ? 64 * (t / 2) + 16 * g + 8 * (t & 1) : 32 * t + 8 * g;
+        f[t] = *(const v4i*)(p + (FULL || d < kv.D ? d : 0));
+      }
+    } else {
+#pragma unroll
+      for (int t = 0; t < KS; ++t) {
+        const int d = E8 ? 64 * (t / 2) + 16 * g + 8 * (t & 1) : 32 * t + 8 * g;
+        typedef TQ v8t __attribute__((ext_vector_type(8)));
+        v8t e;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) e[i] = p[(FULL || d < kv.D ? d : 0) + i];
+        f[t] = __builtin_bit_cast(v4i, e);
+      }
+    }
 #pragma unroll
     for (int t = 0; t < KS; ++t) {
       const int d = E8 ? 64 * (t / 2) + 16 * g + 8 * (t & 1) : 32 * t + 8 * g;
-      q[m][t] = v4i(0);
-      if (r < nrows && d < kv.D) {
-        if (qvec) {
-          q[m][t] = *(const v4i*)(p + d);
-        } else {
-          typedef TQ v8t __attribute__((ext_vector_type(8)));
-          v8t e;
-#pragma unroll
-          for (int i = 0; i < 8; ++i) e[i] = p[d + i];
-          q[m][t] = __builtin_bit_cast(v4i, e);
-        }
-      }
+      if (!FULL && d >= kv.D) f[t] = v4i(0);
+      if constexpr (QL) qs[(m * KS + t) * 64 + lane] = f[t];
+      else q[m][t] = f[t];
     }
   }
+  if constexpr (QL) __syncthreads();
+  const auto query = [&](int m, int t) -> v4i {
+    if constexpr (QL) return qs[(m * KS + t) * 64 + lane];
+    else return q[m][t];
+  };
 
   v4f o[VB][VE][MT];
   float mx[MT], sum[MT];
@@ -220,108 +273,136 @@ __global__ __launch_bounds__(256) void attn_kernel(AttnArgs a) {
       for (int j = 0; j < VE; ++j) o[vb][j][m] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
   }
 
-  // Where the 16 keys of half s of block i lie: the page (-1: masked) and the first one's place in it, and in the sequence
-  const auto place = [&](int i, int s, int& page, int& in, int& pos, int& limit) {
-    page = -1;
-    limit = 0;
+  // Where the 16 keys of half s of block i lie
+  struct Place {
+    long long base;  // bytes from the cache's first key (value) to the first of them (a masked page's: of the first page)
+    size_t scale;    // and of their scales, in elements
+    int pos, limit;  // the first one's place among the prefix's keys, of which `limit` are seen, or (limit -1) in the sequence
+    bool dead;       // masked
+    __device__ __forceinline__ int sees(int lim) const { return dead ? 0 : (limit >= 0 ? limit : lim) - pos; }  // how many of them a row of limit lim sees
+  };
+  const auto place = [&](int i, int s) {
+    Place r;
+    int page = -1, pos;
+    r.limit = -1;
     if (MODE != CHOSEN && i < shared_blocks32) {
       pos = i * kBlock + 16 * s;
-      limit = a.prefix_len;
-      if (pos < limit) page = a.prefix[pos >> kv.lg];
+      r.limit = a.prefix_len;
+      if (pos < a.prefix_len) page = scalar(a.prefix, pos >> kv.lg);
     } else {
-      pos = (i - shared_blocks32) * kBlock + 16 * s;
-      limit = -1;  // each row's own
+      pos = i < end ? (i - shared_blocks32) * kBlock + 16 * s : 0x7fffffff;
       if constexpr (MODE == CHOSEN) {
-        const int e = pos >> kv.lg;
-        const int n = e < a.k ? a.sel[((size_t)row0 * kv.HK + h) * a.k + e] : -1;
-        in = pos & (kv.page - 1);
+        const int e = pos >> kv.lg, in = pos & (kv.page - 1);
+        const int n = e < a.k ? scalar(a.sel, ((size_t)row0 * kv.HK + h) * a.k + e) : -1;
         pos = n >= 0 && n < a.s.W ? (int)min(((long long)n << kv.lg) + in, 0x7fffffffLL) : 0x7fffffff;
       }
-      if (MODE != SHARED && pos < hi_lim) page = a.s.table[(size_t)b * a.s.W + (pos >> kv.lg)];
+      if (MODE != SHARED && pos < hi_lim) page = scalar(a.s.table, (size_t)b * a.s.W + (pos >> kv.lg));
     }
-    in = pos & (kv.page - 1);
-    if ((unsigned)page >= (unsigned)kv.pages) page = -1;
     page = __builtin_amdgcn_readfirstlane(page);
-    pos = __builtin_amdgcn_readfirstlane(pos);
-    in = __builtin_amdgcn_readfirstlane(in);
+    r.pos = __builtin_amdgcn_readfirstlane(pos);
+    r.dead = (unsigned)page >= (unsigned)kv.pages;
+    const int pg = r.dead ? 0 : page, in = r.dead ? 0 : r.pos & (kv.page - 1);
+    r.base = (pg * kv.ps + h * kv.hs + in * kv.ts) * (long long)sizeof(TC);
+    r.scale = ((size_t)pg * kv.HK + h) * kv.page + in;
+    return r;
   };
 
-  const bool ragged = kv.D < DC;
-  for (int i = begin + wave; i < end; i += kWaves) {
-    kvec kr[2][KL];
-    vvec vr[2][4][VB];
-    v4f ks[2], vs[2];
-    int page[2], in[2], pos[2], limit[2];
+  // a lane's places in 16 keys (token_stride is below 2^26 elements)
+  const unsigned k_row = (unsigned)col * (unsigned)kv.ts * (unsigned)sizeof(TC), v_row = 4u * (unsigned)g * (unsigned)kv.ts * (unsigned)sizeof(TC);
+  kvec kr[2][KL];
+  vvec vr[VB][2][4];
+  v4f ks[2], vs[2];
+  const auto load_k = [&](int s, const Place& at) {
 #pragma unroll
-    for (int s = 0; s < 2; ++s) {
-      place(i, s, page[s], in[s], pos[s], limit[s]);
-      const int pg = page[s] < 0 ? 0 : page[s], at = page[s] < 0 ? 0 : in[s];  // (a masked page's place is read from the first one)
-      const long long base = pg * kv.ps + h * kv.hs + at * kv.ts;
-      const TC* kp = (const TC*)kv.k + base + col * kv.ts;
-      const TC* vp = (const TC*)kv.v + base + 4 * g * kv.ts;
-#pragma unroll
-      for (int t = 0; t < KL; ++t) {
-        const int d = (E8 ? 64 * t + 16 * g : 32 * t + 8 * g);
-        kr[s][t] = *(const kvec*)(kp + (d < kv.D ? d : 0));
-      }
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-#pragma unroll
-        for (int vb = 0; vb < VB; ++vb) {
-          const int d = vb * 128 + VE * col;
-          vr[s][e][vb] = *(const vvec*)(vp + e * kv.ts + (d < kv.D ? d : 0));
-        }
-      if constexpr (E8) {
-        const size_t at4 = ((size_t)pg * kv.HK + h) * kv.page + at + 4 * g;
-        ks[s] = *(const v4f*)(kv.ksc + at4);
-        vs[s] = *(const v4f*)(kv.vsc + at4);
-      }
+    for (int t = 0; t < KL; ++t) {
+      const int d = (E8 ? 64 * t + 16 * g : 32 * t + 8 * g);
+      kr[s][t] = *(const kvec*)((const char*)kv.k + at.base + (k_row + (FULL || d < kv.D ? d : 0) * (unsigned)sizeof(TC)));
     }
+    if constexpr (E8) ks[s] = *(const v4f*)(kv.ksc + at.scale + 4 * g);
+  };
+  const auto load_v = [&](int vb, int s, const Place& at) {
+    const int d = vb * 128 + VE * col;
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      vr[vb][s][e] = *(const vvec*)((const char*)kv.v + at.base + e * kv.ts * (long long)sizeof(TC) + (v_row + (FULL || d < kv.D ? d : 0) * (unsigned)sizeof(TC)));
+    if (E8 && vb == 0) vs[s] = *(const v4f*)(kv.vsc + at.scale + 4 * g);
+  };
+  // Registers of K and of V are loaded for the next block as soon as this one's products have taken them: what a block waits for was asked
+  // for nearly a block before.
+  Place now[2], next[2];
+#pragma unroll
+  for (int s = 0; s < 2; ++s) now[s] = place(begin + wave, s);
+#pragma unroll
+  for (int s = 0; s < 2; ++s) load_k(s, now[s]);
+#pragma unroll
+  for (int vb = 0; vb < VB; ++vb)
+#pragma unroll
+    for (int s = 0; s < 2; ++s) load_v(vb, s, now[s]);
+  for (int i = begin + wave; i < end; i += kWaves) {
+    asm volatile("" ::: "memory");  // (q is read from LDS for each block: kept in registers it would not leave room for the rest)
+#pragma unroll
+    for (int s = 0; s < 2; ++s) next[s] = place(i + kWaves, s);
 
     // S^T: lane (col, g) has keys 4 g .. + 3 of each half for row col
     v4f x[2][MT];
 #pragma unroll
-    for (int s = 0; s < 2; ++s) {
+    for (int s = 0; s < 2; ++s)
 #pragma unroll
       for (int m = 0; m < MT; ++m) x[s][m] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-      for (int t = 0; t < KS; ++t) {
-        v4i k;
-        if constexpr (E8) k = widen8<TQ>(kr[s][t / 2][2 * (t & 1)], kr[s][t / 2][2 * (t & 1) + 1]);
-        else k = kr[s][t];
-        if (ragged) {  // (what was read in place of elements behind the head must not meet q's zeros: it may be infinite)
-          const int d = E8 ? 64 * (t / 2) + 16 * g + 8 * (t & 1) : 32 * t + 8 * g;
-          if (d >= kv.D) k = v4i(0);
-        }
+    for (int t = 0; t < KS; ++t) {
+      v4i k[2];
 #pragma unroll
-        for (int m = 0; m < MT; ++m) x[s][m] = mfma16<TQ>(k, q[m][t], x[s][m]);
+      for (int s = 0; s < 2; ++s) {
+        if constexpr (E8) k[s] = widen8<TQ>(kr[s][t / 2][2 * (t & 1)], kr[s][t / 2][2 * (t & 1) + 1]);
+        else k[s] = kr[s][t];
+        if constexpr (!FULL) {  // (what was read in place of elements behind the head must not meet q's zeros: it may be infinite)
+          const int d = E8 ? 64 * (t / 2) + 16 * g + 8 * (t & 1) : 32 * t + 8 * g;
+          if (d >= kv.D) k[s] = v4i(0);
+        }
+      }
+#pragma unroll
+      for (int m = 0; m < MT; ++m) {
+        const v4i f = query(m, t);
+#pragma unroll
+        for (int s = 0; s < 2; ++s) x[s][m] = mfma16<TQ>(k[s], f, x[s][m]);
       }
     }
-
-    // scale and mask
-    bool partial = false, dead[2];
-    int edge[2];
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
-      // keys that some row sees, and whether all rows see all 16
-      const int most = limit[s] >= 0 ? limit[s] : hi_lim, least = limit[s] >= 0 ? limit[s] : lo_lim;
-      dead[s] = page[s] < 0;
-      edge[s] = dead[s] ? 0 : most - pos[s];
-      partial = partial || dead[s] || pos[s] > least - 16;
 #pragma unroll
       for (int m = 0; m < MT; ++m)
 #pragma unroll
         for (int e = 0; e < 4; ++e) x[s][m][e] *= E8 ? a.c * ks[s][e] : a.c;
+      if (!LATE) load_k(s, next[s]);
     }
-    if (partial) {
+
+    // mask; values of keys that no row sees become zeros (they may hold anything)
+    bool partial = false, odd = false;
 #pragma unroll
-      for (int s = 0; s < 2; ++s)
+    for (int s = 0; s < 2; ++s) partial |= now[s].dead | (now[s].sees(lo_lim) < 16);
+    if (__builtin_expect(partial, 0)) {
+      bool bad = false;  // a value that is not finite, of a key that some rows see and others may not
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        const int edge = now[s].sees(hi_lim);
 #pragma unroll
         for (int m = 0; m < MT; ++m) {
-          const int l = dead[s] ? 0 : (limit[s] >= 0 ? limit[s] : lim[m]) - pos[s] - 4 * g;
+          const int l = now[s].sees(lim[m]) - 4 * g;
 #pragma unroll
           for (int e = 0; e < 4; ++e) x[s][m][e] = e < l ? x[s][m][e] : kMinusInf;
         }
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+#pragma unroll
+          for (int vb = 0; vb < VB; ++vb)
+#pragma unroll
+            for (int w = 0; w < VW; ++w) {
+              if (4 * g + e >= edge) vr[vb][s][e][w] = 0;
+              if (MODE == OWN) bad |= odd_word<TC>(vr[vb][s][e][w]);
+            }
+      }
+      odd = MODE == OWN && lo_lim != hi_lim && __builtin_amdgcn_ballot_w64(bad) != 0;
     }
 
     // the rows' maxima: renewed when one is passed by more than kSlack (rarely, after the first blocks)
@@ -334,7 +415,7 @@ __global__ __launch_bounds__(256) void attn_kernel(AttnArgs a) {
       top[m] = max_groups(t);
       renew = renew || top[m] > mx[m] + kSlack;
     }
-    if (__builtin_amdgcn_ballot_w64(renew)) {
+    if (__builtin_expect(__builtin_amdgcn_ballot_w64(renew) != 0, 0)) {
 #pragma unroll
       for (int m = 0; m < MT; ++m) {
         const bool up = top[m] > mx[m] + kSlack;
@@ -367,80 +448,85 @@ __global__ __launch_bounds__(256) void attn_kernel(AttnArgs a) {
       }
     }
 
-    // V^T: the operand of result (vb, j), keys masked for every row as zeros (they may hold anything)
-    int vw[2][4][VB][VE / 2];
+    // V^T: the operands of results (vb, 2 w) and (vb, 2 w + 1)
+    const auto operands = [&](int vb, int w, v4i& even, v4i& odd_one) {
+      int x8[8];
 #pragma unroll
-    for (int s = 0; s < 2; ++s)
+      for (int e = 0; e < 8; ++e) {
+        const vvec& r = vr[vb][e >> 2][e & 3];
+        if constexpr (E8) x8[e] = w & 1 ? widen2<TP, true>(r[w / 2]) : widen2<TP, false>(r[w / 2]);
+        else x8[e] = r[w];
+      }
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
-#pragma unroll
-        for (int vb = 0; vb < VB; ++vb) {
-#pragma unroll
-          for (int w = 0; w < VE / 2; ++w) {
-            if constexpr (E8) vw[s][e][vb][w] = w & 1 ? widen2<TP, true>(vr[s][e][vb][w / 2]) : widen2<TP, false>(vr[s][e][vb][w / 2]);
-            else vw[s][e][vb][w] = vr[s][e][vb][w];
-          }
-          if (partial && 4 * g + e >= edge[s]) {
-#pragma unroll
-            for (int w = 0; w < VE / 2; ++w) vw[s][e][vb][w] = 0;
-          }
-        }
-    const auto operand = [&](int vb, int j) {
-      v4i r;
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-        r[e] = __builtin_amdgcn_perm(vw[e >> 1][2 * (e & 1) + 1][vb][j / 2], vw[e >> 1][2 * (e & 1)][vb][j / 2], j & 1 ? 0x07060302 : 0x05040100);
-      return r;
+      for (int e = 0; e < 4; ++e) {
+        even[e] = __builtin_amdgcn_perm(x8[2 * e + 1], x8[2 * e], 0x05040100);
+        odd_one[e] = __builtin_amdgcn_perm(x8[2 * e + 1], x8[2 * e], 0x07060302);
+      }
     };
-    bool odd = false;
-    if (partial && MODE != SHARED) {  // a value that is not finite, of a key that some rows see and others do not
-      bool bad = false;
+    if (LATE) {
 #pragma unroll
-      for (int s = 0; s < 2; ++s)
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-#pragma unroll
-          for (int vb = 0; vb < VB; ++vb)
-#pragma unroll
-            for (int w = 0; w < VE / 2; ++w) bad = bad || odd_half<TP>(vw[s][e][vb][w]);
-      odd = __builtin_amdgcn_ballot_w64(bad) != 0;
+      for (int s = 0; s < 2; ++s) load_k(s, next[s]);
     }
-    if (!odd) {
+    if (__builtin_expect(odd, 0)) {
+      // Zero times infinity would reach the rows that do not see the key. How many NaN and infinities of either sign each row sees is a product
+      // of ones and zeros; then they are zeros in V.
+      v4i seen[MT];
 #pragma unroll
-      for (int vb = 0; vb < VB; ++vb)
+      for (int m = 0; m < MT; ++m)
 #pragma unroll
-        for (int j = 0; j < VE; ++j) {
-          const v4i v = operand(vb, j);
-#pragma unroll
-          for (int m = 0; m < MT; ++m)
-#pragma unroll
-            for (int n = 0; n < PARTS; ++n) o[vb][j][m] = mfma16<TP>(v, p[n][m], o[vb][j][m]);
+        for (int e = 0; e < 4; ++e) {
+          const int l = now[e >> 1].sees(lim[m]) - 4 * g - 2 * (e & 1);
+          seen[m][e] = (l > 0 ? one16<TP>() : 0) | (l > 1 ? one16<TP>() << 16 : 0);
         }
-    } else {
-      // One key at a time, added to the rows that see it (zero times infinity would reach the others)
 #pragma unroll 1
-      for (int key = 0; key < kBlock; ++key) {
-        const int s = key >> 4, mine = (key & 15) - 4 * g, word = 2 * s + ((mine & 3) >> 1);
-        const bool here = mine >= 0 && mine < 4;
-        const unsigned half = mine & 1 ? 0xffff0000u : 0xffffu;
+      for (int kind = 0; kind < (E8 ? 1 : 3); ++kind)
 #pragma unroll
         for (int vb = 0; vb < VB; ++vb)
 #pragma unroll
-          for (int j = 0; j < VE; ++j) {
-            v4i v = operand(vb, j);
+          for (int w = 0; w < VE / 2; ++w) {
+            v4i v[2];
+            operands(vb, w, v[0], v[1]);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) v[e] = here && e == word ? (int)(v[e] & half) : 0;
+            for (int j = 0; j < 2; ++j) {
 #pragma unroll
-            for (int m = 0; m < MT; ++m) {
-              const bool sees = !dead[s] && (key & 15) + pos[s] < (limit[s] >= 0 ? limit[s] : lim[m]);
-              v4f y = {0.0f, 0.0f, 0.0f, 0.0f};
+              for (int e = 0; e < 4; ++e) v[j][e] = odd_ones<TP>(v[j][e], kind);
 #pragma unroll
-              for (int n = 0; n < PARTS; ++n) y = mfma16<TP>(v, p[n][m], y);
-              if (sees) o[vb][j][m] += y;
+              for (int m = 0; m < MT; ++m) {
+                const v4f n = mfma16<TP>(v[j], seen[m], v4f{0.0f, 0.0f, 0.0f, 0.0f});
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                  if (n[e] > 0.0f) o[vb][2 * w + j][m][e] += kind == 0 ? __builtin_nanf("") : kind == 1 ? -kMinusInf : kMinusInf;
+              }
             }
           }
-      }
+#pragma unroll
+      for (int vb = 0; vb < VB; ++vb)
+#pragma unroll
+        for (int s = 0; s < 2; ++s)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+#pragma unroll
+            for (int w = 0; w < VW; ++w) vr[vb][s][e][w] = without_odd<TC>(vr[vb][s][e][w]);
     }
+#pragma unroll
+    for (int vb = 0; vb < VB; ++vb)
+#pragma unroll
+      for (int w = 0; w < VE / 2; ++w) {
+        v4i v[2];
+        operands(vb, w, v[0], v[1]);
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+          for (int m = 0; m < MT; ++m)
+#pragma unroll
+              for (int n = 0; n < PARTS; ++n) o[vb][2 * w + j][m] = mfma16<TP>(v[j], p[n][m], o[vb][2 * w + j][m]);
+      }
+#pragma unroll
+    for (int vb = 0; vb < VB; ++vb)
+#pragma unroll
+      for (int s = 0; s < 2; ++s) load_v(vb, s, next[s]);
+#pragma unroll
+    for (int s = 0; s < 2; ++s) now[s] = next[s];
   }
 
   // Join the waves: each result relative to the largest maximum of its row, then the sums, two waves at a time through LDS
@@ -469,48 +555,67 @@ __global__ __launch_bounds__(256) void attn_kernel(AttnArgs a) {
 #pragma unroll
       for (int j = 0; j < VE; ++j) o[vb][j][m] *= f;
   }
-  v4f* buf = (v4f*)xo;
-  const auto give = [&](int at) {
+  // wave i ends with value i of each four: row col of each tile, elements VE (4 g + i) + j of each 128
+  float y[VB][VE][MT];
 #pragma unroll
-    for (int n = 0; n < NO; ++n) buf[(at * NO + n) * 64 + lane] = o[n / (VE * MT)][n / MT % VE][n % MT];
-  };
-  const auto take = [&](int at) {
+  for (int i = 0; i < kWaves; ++i) {
+    __syncthreads();
+    if (wave != i) {
+      const int at = (wave < i ? wave : wave - 1) * (NO / 4);
 #pragma unroll
-    for (int n = 0; n < NO; ++n) o[n / (VE * MT)][n / MT % VE][n % MT] += buf[(at * NO + n) * 64 + lane];
-  };
-  if (wave >= 2) give(wave - 2);
-  __syncthreads();
-  if (wave < 2) take(wave);
-  __syncthreads();
-  if (wave == 1) give(0);
-  __syncthreads();
-  if (wave > 0) return;
-  take(0);
+      for (int n = 0; n < NO; n += 4) {
+        v4f t;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) t[e] = o[(n + e) / (VE * MT)][(n + e) / MT % VE][(n + e) % MT][i];
+        lds[(at + n / 4) * 64 + lane] = t;
+      }
+    } else {
+#pragma unroll
+      for (int n = 0; n < NO; ++n) y[n / (VE * MT)][n / MT % VE][n % MT] = o[n / (VE * MT)][n / MT % VE][n % MT][i];
+    }
+    __syncthreads();
+    if (wave == i) {
+#pragma unroll
+      for (int w = 0; w < kWaves - 1; ++w)
+#pragma unroll
+        for (int n = 0; n < NO; n += 4) {
+          const v4f t = lds[(w * (NO / 4) + n / 4) * 64 + lane];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) y[(n + e) / (VE * MT)][(n + e) / MT % VE][(n + e) % MT] += t[e];
+        }
+    }
+  }
 
-  // lane (col, g): row col of each tile, elements VE (4 g + i) + j of each 128
-  const bool split = MODE == SHARED || (MODE == OWN && a.shared > 0) || (all_blocks + kWaves - 1) / kWaves > blocks;
+  const int all_pieces = MODE == CHOSEN ? a.pieces : ((all_blocks + kWaves - 1) / kWaves + (long long)blocks - 1) / blocks;
+  const bool split = MODE == SHARED || (MODE == OWN && a.shared > 0) || all_pieces > 1;
+  float* slot = nullptr;
+  if (MODE == SHARED) {
+    slot = a.shared_part + ((size_t)(h * a.shared_tiles + rt) * a.shared + c) * slot_floats(RT, kv.D);
+  } else if (a.slots) {
+    const int at = MODE == CHOSEN ? row0 * rts + rt : first_slot(a, RT, b, row0, rt);
+    const int others = a.firsts + (MODE == CHOSEN ? row0 * rts * (a.pieces - 1) : more) + rt;
+    const long long n = ((long long)(c ? others + (c - 1) * rts : at)) * kv.HK + h;
+    if (n >= a.slots) return;  // (rows of lists that are none)
+    slot = a.part + (size_t)n * slot_floats(RT, kv.D);
+    if (c == 0 && threadIdx.x == 0) *(int4*)slot = int4{all_pieces > 1 ? all_pieces : 1, others, rts, 0};
+  }
   if (split) {
-    float* slot = MODE == SHARED ? a.shared_part + ((size_t)(h * a.shared_tiles + rt) * a.shared + c) * (RT * (kv.D + 2))
-                                 : a.part + ((size_t)unit * kv.HK + h) * (RT * (kv.D + 2));
-    if (MODE != SHARED && (long long)unit * kv.HK + h >= a.slots) return;
+    slot += 4;
 #pragma unroll
     for (int m = 0; m < MT; ++m) {
       const int r = 16 * m + col;
       if (first + r > last) continue;
-      if (g == 0) {
+      if (g == 0 && wave == 0) {
         slot[r] = top[m] - kBias;
         slot[RT + r] = all[m];
       }
 #pragma unroll
-      for (int vb = 0; vb < VB; ++vb)
+      for (int vb = 0; vb < VB; ++vb) {
+        const int d = vb * 128 + VE * (4 * g + wave);
+        if (!FULL && d >= kv.D) continue;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int d = vb * 128 + VE * (4 * g + i);
-          if (d >= kv.D) continue;
-#pragma unroll
-          for (int j = 0; j < VE; j += 4)
-            *(v4f*)(slot + 2 * RT + (size_t)r * kv.D + d + j) = v4f{o[vb][j][m][i], o[vb][j + 1][m][i], o[vb][j + 2][m][i], o[vb][j + 3][m][i]};
-        }
+        for (int j = 0; j < VE; j += 4) *(v4f*)(slot + 2 * RT + (size_t)r * kv.D + d + j) = v4f{y[vb][j][m], y[vb][j + 1][m], y[vb][j + 2][m], y[vb][j + 3][m]};
+      }
     }
     return;
   }
@@ -521,17 +626,15 @@ __global__ __launch_bounds__(256) void attn_kernel(AttnArgs a) {
     const float inv = all[m] > 0.0f || all[m] != all[m] ? 1.0f / all[m] : 0.0f;  // (a row that sees no key is zeros)
     const size_t at = (size_t)(row0 + r / a.G) * a.ldo + (size_t)(h * a.G + r % a.G) * kv.D;
 #pragma unroll
-    for (int vb = 0; vb < VB; ++vb)
+    for (int vb = 0; vb < VB; ++vb) {
+      const int d = vb * 128 + VE * (4 * g + wave);
+      if (!FULL && d >= kv.D) continue;
+      float z[VE];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int d = vb * 128 + VE * (4 * g + i);
-        if (d >= kv.D) continue;
-        float y[VE];
-#pragma unroll
-        for (int j = 0; j < VE; ++j) y[j] = o[vb][j][m][i] * inv;
-        if (a.otype == DT_F32) store_row<float, VE>((float*)a.o + at + d, y);
-        else store_row<TQ, VE>((TQ*)a.o + at + d, y);
-      }
+      for (int j = 0; j < VE; ++j) z[j] = y[vb][j][m] * inv;
+      if (a.otype == DT_F32) store_row<float, VE>((float*)a.o + at + d, z);
+      else store_row<TQ, VE>((TQ*)a.o + at + d, z);
+    }
   }
 }
 

@@ -4,11 +4,17 @@
 
 namespace qm {
 
+template <typename TQ, typename TC, int DC, bool FULL, int MT, int PARTS>
+void attn_full(const AttnArgs& a, int mode, unsigned grid, hipStream_t s) {
+  if (mode == SHARED) attn_kernel<TQ, TC, DC, FULL, MT, PARTS, SHARED><<<grid, 256, 0, s>>>(a);
+  else if (mode == CHOSEN) attn_kernel<TQ, TC, DC, FULL, MT, PARTS, CHOSEN><<<grid, 256, 0, s>>>(a);
+  else attn_kernel<TQ, TC, DC, FULL, MT, PARTS, OWN><<<grid, 256, 0, s>>>(a);
+}
+
 template <typename TQ, typename TC, int DC, int MT, int PARTS>
 hipError_t attn_mode(const AttnArgs& a, int mode, unsigned grid, hipStream_t s) {
-  if (mode == SHARED) attn_kernel<TQ, TC, DC, MT, PARTS, SHARED><<<grid, 256, 0, s>>>(a);
-  else if (mode == CHOSEN) attn_kernel<TQ, TC, DC, MT, PARTS, CHOSEN><<<grid, 256, 0, s>>>(a);
-  else attn_kernel<TQ, TC, DC, MT, PARTS, OWN><<<grid, 256, 0, s>>>(a);
+  if (a.kv.D == DC) attn_full<TQ, TC, DC, true, MT, PARTS>(a, mode, grid, s);
+  else attn_full<TQ, TC, DC, false, MT, PARTS>(a, mode, grid, s);
   return hipGetLastError();
 }
 

@@ -8,6 +8,7 @@ namespace qm {
 
 constexpr int kWaves = 4;   // of a work-group
 constexpr int kBlock = 32;  // keys of a wave's step
+constexpr int kLeast = 1;   // blocks of 128 keys of a piece at least
 
 // Rows of a sequence, clamped to the call's (device lists are not trusted with memory)
 __device__ __forceinline__ int row_from(const Seqs& s, int b) {
@@ -32,12 +33,6 @@ __device__ __forceinline__ int sequence_of(const Seqs& s, int t) {
   return lo < s.B && t - row_from(s, lo) < rows_of(s, lo) && t >= row_from(s, lo) ? lo : -1;
 }
 
-// The item of a work-group: a row tile rt of sequence b, and piece c of its blocks
-struct Item {
-  int b, rt, c, blocks;  // blocks of 128 keys of a piece
-  int unit;              // the first piece's number of the sequence
-};
-
 // Blocks of 128 keys of sequence b, the prefix in front of them
 __device__ __forceinline__ long long blocks_of(const AttnArgs& a, int b) {
   const long long most = (long long)a.s.W << a.kv.lg;
@@ -46,68 +41,87 @@ __device__ __forceinline__ long long blocks_of(const AttnArgs& a, int b) {
   return ((n + 31) / 32 + (a.prefix_len + 31) / 32 + 3) >> 2;
 }
 
-// Sum over a work-group of 256 (every thread gets it)
-__device__ __forceinline__ long long sum256(long long v, long long* red) {
-  for (int o = 32; o; o >>= 1) v += __shfl_xor(v, o);
-  __syncthreads();
-  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
-  __syncthreads();
-  return red[0] + red[1] + red[2] + red[3];
+// The place of the result of row tile rt's first piece among the slots (of a head): row tiles of RT rows, of a sequence whose rows begin at
+// row0. Known without the other sequences' lengths: the tiles of the rows before are at most row0 G / RT and one for each sequence.
+__device__ __forceinline__ int first_slot(const AttnArgs& a, int RT, int b, int row0, int rt) {
+  return a.s.start ? (int)((long long)row0 * a.G / RT) + b + rt : b * ((a.G + RT - 1) / RT) + rt;
 }
 
-// Blocks of a piece: the batch's (row tile, block) pairs of all heads over the pieces aimed at
-__device__ __forceinline__ int piece_blocks(const AttnArgs& a, int RT, long long* red) {
-  if (!a.target) return 0x7fffffff;
-  long long all = 0;
-  for (int b = threadIdx.x; b < a.s.B; b += 256) all += (long long)((rows_of(a.s, b) * a.G + RT - 1) / RT) * blocks_of(a, b);
-  all = sum256(all, red) * a.kv.HK;
-  const long long n = (all + a.target - 1) / a.target;
-  return n > 1 ? (int)n : 1;
-}
+// What a work-group does: row tile rt of key head h of sequence b, piece c of its keys. Pieces behind the first have their results behind all
+// first ones: number `more` and on, `rts` from one to the next.
+struct Item {
+  int b, h, rt, c, rts;
+  int blocks;  // blocks of 128 keys of a piece
+  int more;
+};
 
-// Pieces of one row tile of sequence b
-__device__ __forceinline__ int pieces_of(const AttnArgs& a, int b, int blocks) {
-  const long long n = (blocks_of(a, b) + blocks - 1) / blocks;
-  return n > 1 ? (int)n : 1;
-}
+struct Sums {
+  long long units, tiles;  // work-groups and row tiles
+};
+__device__ __forceinline__ Sums operator+(Sums a, Sums b) { return {a.units + b.units, a.tiles + b.tiles}; }
 
-// The item of piece number `unit` (piece c of row tile rt is number first + c * row tiles + rt of its sequence); false: there is none
-template <int RT>
-__device__ __forceinline__ bool find_item(const AttnArgs& a, int unit, Item* out, long long* red) {
-  const int blocks = piece_blocks(a, RT, red);
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  if (threadIdx.x == 0) out->b = -1;
-  long long base = 0;
-  for (int b0 = 0; b0 < a.s.B && base <= unit; b0 += 256) {
-    const int b = b0 + threadIdx.x;
-    const int rts = b < a.s.B ? (rows_of(a.s, b) * a.G + RT - 1) / RT : 0;
-    const long long units = rts ? (long long)rts * pieces_of(a, b, blocks) : 0;
-    long long end = units;  // inclusive sums: of the wave's lanes, then of the waves before
-    for (int o = 1; o < 64; o <<= 1) {
-      const long long v = __shfl_up(end, o);
-      if (lane >= o) end += v;
+// Sequences are looked at 64 at a time by each wave for itself (no wave waits for another): the sum over all of them, then the scan that says
+// whose unit number this is.
+__device__ __forceinline__ bool find_item(const AttnArgs& a, int RT, int unit, Item& out) {
+  const int lane = threadIdx.x & 63, HK = a.kv.HK;
+  const auto tiles_of = [&](int b) { return b < a.s.B ? (int)(((long long)rows_of(a.s, b) * a.G + RT - 1) / RT) : 0; };
+  // (the first 64 sequences are held: most batches are no larger)
+  const int rts0 = tiles_of(lane);
+  const long long blocks0 = rts0 ? blocks_of(a, lane) : 0;
+  int blocks = 0x7fffffff;
+  if (a.target) {
+    long long all = rts0 * blocks0;
+    for (int b = lane + 64; b < a.s.B; b += 64) {
+      const int n = tiles_of(b);
+      if (n) all += n * blocks_of(a, b);
     }
-    __syncthreads();
-    if (lane == 63) red[wave] = end;
-    __syncthreads();
-    long long all = 0;
-    for (int w = 0; w < 4; ++w) {
-      if (w < wave) end += red[w];
-      all += red[w];
-    }
-    const long long first = base + end - units;
-    if (units && unit >= first && unit < first + units) {
-      const int at = (int)(unit - first);
-      out->b = b;
-      out->rt = at % rts;
-      out->c = at / rts;
-      out->blocks = blocks;
-      out->unit = (int)first;
-    }
-    base += all;
+    for (int o = 32; o; o >>= 1) all += __shfl_xor(all, o);
+    const long long n = (all * HK + a.target - 1) / a.target;
+    blocks = n > kLeast ? (int)(n < 0x7fffffff ? n : 0x7fffffff) : kLeast;
   }
-  __syncthreads();
-  return out->b >= 0;
+  Sums base = {0, 0};
+  for (int b0 = 0; b0 < a.s.B; b0 += 64) {
+    const int rts = b0 ? tiles_of(b0 + lane) : rts0;
+    const long long n = !rts ? 0 : ((b0 ? blocks_of(a, b0 + lane) : blocks0) + blocks - 1) / blocks;
+    const int pieces = n > 1 ? (int)n : 1;
+    const Sums mine = {(long long)rts * pieces * HK, rts};
+    Sums end = mine;
+    for (int o = 1; o < 64; o <<= 1) {
+      const Sums v = {__shfl_up(end.units, o), __shfl_up(end.tiles, o)};
+      if (lane >= o) end = end + v;
+    }
+    const unsigned long long past = __ballot(base.units + end.units > unit);
+    if (past) {
+      const int at = __ffsll(past) - 1;
+      out.b = b0 + at;
+      out.rts = __builtin_amdgcn_readlane(rts, at);
+      out.blocks = blocks;
+      const int np = __builtin_amdgcn_readlane(pieces, at) * HK;
+      const long long units0 = base.units + __shfl(end.units - mine.units, at), tiles0 = base.tiles + __shfl(end.tiles - mine.tiles, at);
+      // The row tiles of one piece and head lie 8 work-groups apart: on one XCD, whose L2 then reads the piece once. The last rows' tiles, which
+      // see the most keys, begin.
+      const int j = (int)(unit - units0), whole = np / 8 * 8, rest = np - whole;
+      int pair, rt;
+      if (j < whole * out.rts) {
+        pair = j / (8 * out.rts) * 8 + j % 8;
+        rt = j % (8 * out.rts) / 8;
+      } else {
+        pair = whole + (j - whole * out.rts) % rest;
+        rt = (j - whole * out.rts) / rest;
+      }
+      out.rt = out.rts - 1 - rt;
+      out.h = pair % HK;
+      out.c = pair / HK;
+      out.more = (int)(units0 / HK - tiles0);
+      return true;
+    }
+    base = base + Sums{__shfl(end.units, 63), __shfl(end.tiles, 63)};
+  }
+  return false;
 }
+
+// The slots: partial results of row tiles. A slot is four words, the RT rows' maxima and sums, and their results; the words of a row tile's
+// first one are how many pieces there are, and the places of the others (the second one's, and from one to the next).
+__device__ __forceinline__ size_t slot_floats(int RT, int D) { return 4 + (size_t)RT * (D + 2); }
 
 }  // namespace qm

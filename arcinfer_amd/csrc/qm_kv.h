@@ -45,7 +45,8 @@ struct AttnArgs {
   int otype, ldo;
   // The split. A piece is a run of blocks of 128 keys of one row tile and head; its partial result goes to the slot of its number.
   float* part;          // null: nothing is split, each row tile writes its result
-  int target, slots;    // pieces that are aimed at, partial results that `part` holds
+  int target, slots;    // pieces that are aimed at (0: whole row tiles), and partial results that `part` holds, those of
+  int firsts;           // first pieces (of a head) in front
   int pieces, blocks;   // chosen pages: pieces of a row tile, and blocks of 128 keys of one
   // The pieces of the shared prefix for the rows of the whole batch (shared > 0): pieces a row tile, tiles of shared_rt rows of a key
   // head, blocks of 128 keys of a piece; slot ((head * shared_tiles) + tile) * shared + piece
@@ -55,7 +56,7 @@ struct AttnArgs {
 
 // How a call runs: mt row tiles of 16 a work-group; pieces and blocks as in AttnArgs
 struct AttnPlan {
-  int mt, target, slots;                               // target 0: nothing is split
+  int mt, target, slots, firsts;                       // target 0: nothing is split
   int shared, shared_mt, shared_tiles, shared_blocks;  // shared 0: the prefix is read with each sequence's own keys
 };
 size_t attn_slot_bytes(int mt, int D);
