@@ -1125,7 +1125,7 @@ static int check_kv(const char* fn, const qm_kv* kv, bool data, qm::KvView* out)
     if (!kv->k || !kv->v || (kv->type == QM_E4M3 && (!kv->k_scale || !kv->v_scale))) return fail(QM_ERR_ARG, "%s: null pointer in the cache", fn);
     const long long most = 1LL << 46, unit = (long long)(16 / size);
     if (kv->page_stride < 0 || kv->head_stride < 0 || kv->token_stride < 0 || kv->page_stride > most / kv->pages ||
-        kv->head_stride > most / kv->heads || kv->token_stride > most / kv->page)
+        kv->head_stride > most / kv->heads || kv->token_stride >= 1LL << 26)
       return fail(QM_ERR_SHAPE, "%s: cache strides %lld, %lld, %lld", fn, kv->page_stride, kv->head_stride, kv->token_stride);
     if ((kv->pages > 1 && kv->page_stride % unit) || (kv->heads > 1 && kv->head_stride % unit) || kv->token_stride % unit || !aligned(kv->k, 16) ||
         !aligned(kv->v, 16) || (kv->type == QM_E4M3 && (!aligned(kv->k_scale, 16) || !aligned(kv->v_scale, 16))))
@@ -1279,8 +1279,7 @@ static int attention(const char* fn, const void* q, int qtype, int ldq, int HQ, 
   const bool start = !sel && seqs->start;
   const qm::AttnPlan p = qm::attn_plan(T, B, start, HQ, kv->heads, kv->D, prefix_len, ws ? ws_bytes : 0);
   if (!qm::attn_grid(p, T, B, start, HQ, kv->heads)) return fail(QM_ERR_SHAPE, "%s: %d rows of %d heads are more than a grid holds", fn, T, HQ);
-  size_t used = (size_t)p.slots * qm::attn_slot_bytes(p.mt, kv->D);
-  if (p.shared) used += (size_t)kv->heads * p.shared_tiles * p.shared * qm::attn_slot_bytes(p.shared_mt, kv->D);
+  const size_t used = qm::attn_used_bytes(p, kv->heads, kv->D);
   const HeadRows rq{q, T, kv->D, HQ, kv->D, ldq, 2}, ro{o, T, kv->D, HQ, kv->D, ldo, (long long)so};
   const Span work{ws, used};
   const Span in[] = {{seqs->start, ((size_t)seqs->B + 1) * 4}, {seqs->len, (size_t)seqs->B * 4}, {seqs->table, (size_t)seqs->B * seqs->table_stride * 4},

@@ -3,19 +3,20 @@
 
 namespace qm {
 
-hipError_t attn_bf16(const AttnArgs& a, int mt, int mode, unsigned grid, hipStream_t s);
-hipError_t attn_f16(const AttnArgs& a, int mt, int mode, unsigned grid, hipStream_t s);
-hipError_t attn_bf16_e4m3(const AttnArgs& a, int mt, int mode, unsigned grid, hipStream_t s);
-hipError_t attn_f16_e4m3(const AttnArgs& a, int mt, int mode, unsigned grid, hipStream_t s);
+hipError_t attn_bf16(const AttnArgs& a, int mt, unsigned grid, hipStream_t s);
+hipError_t attn_f16(const AttnArgs& a, int mt, unsigned grid, hipStream_t s);
+hipError_t attn_bf16_e4m3(const AttnArgs& a, int mt, unsigned grid, hipStream_t s);
+hipError_t attn_f16_e4m3(const AttnArgs& a, int mt, unsigned grid, hipStream_t s);
 
-// Joins the pieces of one row: o = sum_p 2^(m_p - m) o_p / sum_p 2^(m_p - m) l_p, in one pass over them with the running maximum. A
-// work-group a row (a query head of a token): D / 4 lanes of four elements, the pieces dealt to 1024 / D groups of lanes, the groups joined
-// in their order. Every partial result is read once; rows of a single piece are left as attn_kernel wrote them. What a row needs to
-// know of the split stands in its tile's first slot. Latency-bound: a launch, that slot's words, the partial results.
+// Joins the pieces of one row: o = sum_p 2^(m_p - m) o_p / sum_p 2^(m_p - m) l_p. A work-group a row (a query head of a token): D / 4 lanes of four
+// elements, the pieces dealt to 1024 / D groups of lanes, whose sums are joined in their order. Every partial result is read once; rows
+// of a single piece are left as attn_kernel wrote them. What a row needs to know of the split stands in its tile's first slot.
+// Latency-bound: a launch, that slot's words, then the pieces' maxima and sums and kAhead results of each group at once.
+constexpr int kAhead = 8;
 __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a, int RT, int chosen) {
-  __shared__ float gmax[256], gsum[256];
+  __shared__ float wave_max[4], weight[256], gsum[256];
   __shared__ float4 osum[256];
-  const int hq = blockIdx.x % a.HQ, t = blockIdx.x / a.HQ, h = hq / a.G, g = hq % a.G, D = a.kv.D;
+  const int hq = blockIdx.x % a.HQ, t = blockIdx.x / a.HQ, h = hq / a.G, g = hq % a.G, D = a.kv.D, tid = threadIdx.x;
   const int b = sequence_of(a.s, t);
   if (b < 0) return;
   const int row0 = chosen ? t : row_from(a.s, b), r0 = (t - row0) * a.G + g, rt = r0 / RT;
@@ -27,58 +28,87 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a, int RT, int 
   if (!a.shared && head.x == 1) return;
   const int all = a.shared + head.x;
   const long long srow = (long long)t * a.G + g;
-  const size_t ssize = slot_floats(a.shared_rt, D);
-  const int lanes = D / 4, groups = 256 / lanes, group = (int)threadIdx.x / lanes, d = 4 * ((int)threadIdx.x % lanes);
-  float top = -__builtin_inff(), l = 0.0f;
+  // the partial result of piece p: of its row, the maximum; the sum lies RT behind it, the elements from 2 RT on
+  const float* sfirst = a.shared_part + (size_t)(h * a.shared_tiles + srow / RT) * a.shared * size + 4;
+  const auto slot = [&](int p) -> const float* {
+    if (p < a.shared) return sfirst + (size_t)p * size;
+    if (p == a.shared) return first + 4;
+    const long long n = ((long long)head.y + (long long)(p - a.shared - 1) * head.z) * a.kv.HK + h;
+    return (n < a.slots ? a.part + (size_t)n * size : first) + 4;
+  };
+  const auto row_of = [&](int p) { return p < a.shared ? (int)(srow % RT) : r0 % RT; };
+  const int lanes = D / 4, groups = 256 / lanes, group = tid / lanes, d = 4 * (tid % lanes);
+  float l = 0.0f, top = -__builtin_inff();
   float4 o = {0.0f, 0.0f, 0.0f, 0.0f};
-  if (group < groups) {
-#pragma unroll 4
-    for (int p = group; p < all; p += groups) {
-      const float* s;
-      int rows = RT, r = r0 % RT;
-      if (p < a.shared) {
-        rows = a.shared_rt;
-        r = (int)(srow % rows);
-        s = a.shared_part + ((size_t)(h * a.shared_tiles + srow / rows) * a.shared + p) * ssize;
-      } else if (p == a.shared) {
-        s = first;
-      } else {
-        const long long n = ((long long)head.y + (long long)(p - a.shared - 1) * head.z) * a.kv.HK + h;
-        if (n >= a.slots) continue;
-        s = a.part + (size_t)n * size;
+  for (int p0 = 0; p0 < all; p0 += 256) {
+    // 256 pieces at a time: their maxima and sums, and the first results of each group, are asked for together
+    const int n = min(256, all - p0);
+    float4 v[kAhead];
+    const auto ask = [&](int i, int from) {
+      const int p = p0 + min(group + (from + i) * groups, n - 1);
+      v[i] = *(const float4*)(slot(p) + 2 * RT + (size_t)row_of(p) * D + d);
+    };
+    const bool in = tid < n;
+    const float* s = slot(p0 + (in ? tid : 0)) + row_of(p0 + (in ? tid : 0));
+    const float m = s[0], w = in ? s[RT] : 0.0f;
+    if (group < groups) {
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i)
+        if (i * groups < n) ask(i, 0);
+    }
+    // (a piece that the row sees nothing of has the sum 0)
+    float most = w != 0.0f ? m : -__builtin_inff();
+    for (int k = 32; k; k >>= 1) most = fmaxf(most, __shfl_xor(most, k));
+    __syncthreads();
+    if ((tid & 63) == 0) wave_max[tid >> 6] = most;
+    __syncthreads();
+    most = fmaxf(top, fmaxf(fmaxf(wave_max[0], wave_max[1]), fmaxf(wave_max[2], wave_max[3])));
+    if (most != top) {
+      const float f = __builtin_amdgcn_exp2f(top - most);
+      l *= f;
+      o.x *= f;
+      o.y *= f;
+      o.z *= f;
+      o.w *= f;
+      top = most;
+    }
+    const float f = w != 0.0f ? __builtin_amdgcn_exp2f(m - top) : 0.0f;
+    weight[tid] = f;
+    l += f * w;
+    __syncthreads();
+    if (group < groups) {
+      for (int from = 0; group + from * groups < n; from += kAhead) {
+        if (from) {
+#pragma unroll
+          for (int i = 0; i < kAhead; ++i)
+            if ((from + i) * groups < n) ask(i, from);
+        }
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) {
+          const int p = group + (from + i) * groups;
+          if (p >= n) continue;
+          const float k = weight[p];
+          if (k == 0.0f) continue;  // (the slot may hold anything)
+          o.x = fmaf(k, v[i].x, o.x);
+          o.y = fmaf(k, v[i].y, o.y);
+          o.z = fmaf(k, v[i].z, o.z);
+          o.w = fmaf(k, v[i].w, o.w);
+        }
       }
-      s += 4;
-      const float m = s[r], w = s[rows + r];
-      const float4 v = *(const float4*)(s + 2 * rows + (size_t)r * D + d);
-      if (w == 0.0f) continue;  // (a piece that the row sees nothing of)
-      const float now = fmaxf(top, m), f0 = top == now ? 1.0f : __builtin_amdgcn_exp2f(top - now), f = __builtin_amdgcn_exp2f(m - now);
-      top = now;
-      l = fmaf(f, w, l * f0);
-      o.x = fmaf(f, v.x, o.x * f0);
-      o.y = fmaf(f, v.y, o.y * f0);
-      o.z = fmaf(f, v.z, o.z * f0);
-      o.w = fmaf(f, v.w, o.w * f0);
     }
   }
-  gmax[threadIdx.x] = top;
-  gsum[threadIdx.x] = l;
-  osum[threadIdx.x] = o;
+  for (int k = 32; k; k >>= 1) l += __shfl_xor(l, k);
+  osum[tid] = o;
+  if ((tid & 63) == 0) gsum[tid >> 6] = l;
   __syncthreads();
   if (group) return;
-  float most = top;
-  for (int i = 1; i < groups; ++i) most = fmaxf(most, gmax[i * lanes + threadIdx.x]);
-  l = 0.0f;
-  o = {0.0f, 0.0f, 0.0f, 0.0f};
-  for (int i = 0; i < groups; ++i) {
-    const int at = i * lanes + threadIdx.x;
-    if (gsum[at] == 0.0f) continue;
-    const float f = __builtin_amdgcn_exp2f(gmax[at] - most);
-    const float4 v = osum[at];
-    l = fmaf(f, gsum[at], l);
-    o.x = fmaf(f, v.x, o.x);
-    o.y = fmaf(f, v.y, o.y);
-    o.z = fmaf(f, v.z, o.z);
-    o.w = fmaf(f, v.w, o.w);
+  l = gsum[0] + gsum[1] + gsum[2] + gsum[3];
+  for (int i = 1; i < groups; ++i) {
+    const float4 v = osum[i * lanes + tid];
+    o.x += v.x;
+    o.y += v.y;
+    o.z += v.z;
+    o.w += v.w;
   }
   const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;  // (a row that sees no key is zeros)
   const float y[4] = {o.x * inv, o.y * inv, o.z * inv, o.w * inv};
@@ -93,8 +123,8 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a, int RT, int 
 
 namespace {
 
-constexpr int kTarget = 1024;        // pieces that a call is cut into
-constexpr int kSharedTarget = 512;   // pieces of the shared prefix
+constexpr int kTarget = 512;        // pieces that a call is cut into
+constexpr int kSharedTarget = 256;   // pieces of the shared prefix
 constexpr int kSharedFrom = 256;     // a shorter prefix is read with each sequence's own keys
 
 // Row tiles of 16 a work-group: what its registers hold
@@ -113,32 +143,32 @@ long long row_tiles(int T, int B, bool start, int G, int rt) {
 
 size_t attn_slot_bytes(int mt, int D) { return (4 + (size_t)16 * mt * (D + 2)) * sizeof(float); }
 
+static size_t shared_slots(const AttnPlan& p, int HK) { return (size_t)HK * p.shared_tiles * p.shared; }
+static unsigned shared_grid(const AttnPlan& p, int HK) { return (unsigned)(div_up((long long)HK * p.shared, 8) * 8 * p.shared_tiles); }
+
 AttnPlan attn_plan(int T, int B, bool start, int HQ, int HK, int D, int prefix_len, size_t ws_bytes) {
-  AttnPlan p{};
   const int G = HQ / HK;
   const long long rows = start ? div_up(T, B < T ? B : T) * G : G;  // of a sequence, on average
-  p.mt = tiles_for(rows, D);
-  const long long items = row_tiles(T, B, start, G, 16 * p.mt) * HK;
-  const size_t slot = attn_slot_bytes(p.mt, D);
   const size_t have = ws_bytes / 256 * 256;
+  AttnPlan p{};
   if (prefix_len >= kSharedFrom && B > 1 && T > 1 && rows < 64) {
-    p.shared_mt = tiles_for((long long)T * G, D);
-    p.shared_tiles = (int)div_up((long long)T * G, 16 * p.shared_mt);
+    // (one size of row tile for both: the batch's rows fill it, and a sequence's own keys take no longer for it)
+    p.mt = tiles_for((long long)T * G, D);
+    p.shared_tiles = (int)div_up((long long)T * G, 16 * p.mt);
     const int blocks = (int)div_up(prefix_len, 128);
     long long n = kSharedTarget / ((long long)HK * p.shared_tiles);
     if (n > blocks) n = blocks;
     if (n < 1) n = 1;
     p.shared_blocks = (int)div_up(blocks, n);
     p.shared = (int)div_up(blocks, p.shared_blocks);
-    const size_t need = (size_t)HK * p.shared_tiles * p.shared * attn_slot_bytes(p.shared_mt, D) + items * slot;
-    if (need > have) p.shared = 0;
+    const long long items = row_tiles(T, B, start, G, 16 * p.mt) * HK;
+    if ((shared_slots(p, HK) + items) * attn_slot_bytes(p.mt, D) > have) p = AttnPlan{};
   }
-  const size_t left = have - (p.shared ? (size_t)HK * p.shared_tiles * p.shared * attn_slot_bytes(p.shared_mt, D) : 0);
-  // (pieces of all row tiles are at most the target and one more for each of them)
-  if (items < 2 * kTarget && left / slot > (size_t)items) {
-    const long long n = (long long)(left / slot) - items;
-    p.target = (int)(n < kTarget ? n : kTarget);
-  }
+  if (!p.shared) p.mt = tiles_for(rows, D);
+  const long long items = row_tiles(T, B, start, G, 16 * p.mt) * HK;
+  const long long left = (long long)(have / attn_slot_bytes(p.mt, D)) - (long long)shared_slots(p, HK) - items;
+  // (pieces of all row tiles are at most the target and one more for each of them; row tiles that fill the chip are left whole)
+  if (left > 0 && items < (rows < 64 ? 2 * kTarget : kTarget / 2)) p.target = (int)(left < kTarget ? left : kTarget);
   p.slots = p.target || p.shared ? (int)(items + p.target) : 0;
   p.firsts = (int)(items / HK);
   return p;
@@ -148,65 +178,58 @@ size_t attn_workspace_bytes(int T, int B, int HQ, int HK, int D, int prefix_len)
   size_t most = 0;
   for (int start = 0; start < 2; ++start) {
     const AttnPlan p = attn_plan(T, B, start, HQ, HK, D, prefix_len, (size_t)1 << 62);
-    size_t n = (size_t)p.slots * attn_slot_bytes(p.mt, D);
-    if (p.shared) n += (size_t)HK * p.shared_tiles * p.shared * attn_slot_bytes(p.shared_mt, D);
+    const size_t n = attn_used_bytes(p, HK, D);
     if (n > most) most = n;
   }
   return (most + 255) / 256 * 256;
 }
 
+size_t attn_used_bytes(const AttnPlan& p, int HK, int D) { return (p.slots + shared_slots(p, HK)) * attn_slot_bytes(p.mt, D); }
+
 long long attn_grid(const AttnPlan& p, int T, int B, bool start, int HQ, int HK) {
   const long long own = p.slots ? p.slots : row_tiles(T, B, start, HQ / HK, 16 * p.mt) * HK;
-  const long long shared = p.shared ? div_up((long long)HK * p.shared, 8) * 8 * p.shared_tiles : 0;
-  const long long join = p.slots ? (long long)T * HQ : 0;
-  const long long most = own > shared ? own > join ? own : join : shared > join ? shared : join;
+  const long long grid = own + (p.shared ? shared_grid(p, HK) : 0), join = p.slots ? (long long)T * HQ : 0;
+  const long long most = grid > join ? grid : join;
   return most * 256 <= kMostThreads ? most : 0;
 }
 
 namespace {
 
-hipError_t attn_any(const AttnArgs& a, int mt, int mode, unsigned grid, hipStream_t s) {
-  if (a.kv.type == DT_E4M3) return a.qtype == DT_F16 ? attn_f16_e4m3(a, mt, mode, grid, s) : attn_bf16_e4m3(a, mt, mode, grid, s);
-  return a.qtype == DT_F16 ? attn_f16(a, mt, mode, grid, s) : attn_bf16(a, mt, mode, grid, s);
+hipError_t attn_any(const AttnArgs& a, int mt, unsigned grid, hipStream_t s) {
+  if (a.kv.type == DT_E4M3) return a.qtype == DT_F16 ? attn_f16_e4m3(a, mt, grid, s) : attn_bf16_e4m3(a, mt, grid, s);
+  return a.qtype == DT_F16 ? attn_f16(a, mt, grid, s) : attn_bf16(a, mt, grid, s);
 }
 
 }  // namespace
 
 hipError_t launch_attn(const AttnArgs& args, const AttnPlan& p, hipStream_t s) {
   AttnArgs a = args;
-  float* ws = a.part;
   a.target = p.target;
   a.slots = p.slots;
   a.firsts = p.firsts;
-  a.shared = 0;
-  a.shared_rt = 16;
+  a.shared_grid = a.shared = 0;
+  long long grid = p.slots ? p.slots : row_tiles(a.s.T, a.s.B, a.s.start != nullptr, a.G, 16 * p.mt) * a.kv.HK;
   if (a.sel) {  // as many pieces for every token: the target's, within the slots
-    const long long items = row_tiles(a.s.T, a.s.T, false, a.G, 16 * p.mt) * a.kv.HK, blocks = div_up((long long)a.k * a.kv.page, 128);
-    long long n = p.slots / items;  // (as all first pieces, and as many more)
+    const long long items = (long long)a.s.T * div_up(a.G, 16 * p.mt) * a.kv.HK, blocks = div_up((long long)a.k * a.kv.page, 128);
+    long long n = p.slots / items;
     if (n > blocks) n = blocks;
     if (n < 1) n = 1;
     a.blocks = (int)div_up(blocks, n);
     a.pieces = (int)div_up(blocks, a.blocks);
-    hipError_t e = attn_any(a, p.mt, 2, (unsigned)(items * a.pieces), s);
-    if (e != hipSuccess || a.pieces == 1) return e;
-    attn_join_kernel<<<(unsigned)((long long)a.s.T * a.HQ), 256, 0, s>>>(a, 16 * p.mt, 1);
-    return hipGetLastError();
-  }
-  if (p.shared) {
+    grid = items * a.pieces;
+    if (a.pieces == 1) a.slots = 0;
+  } else if (p.shared) {
+    a.shared_grid = (int)shared_grid(p, a.kv.HK);
     a.shared = p.shared;
-    a.shared_rt = 16 * p.shared_mt;
     a.shared_tiles = p.shared_tiles;
     a.shared_blocks = p.shared_blocks;
-    a.shared_part = ws;
-    a.part = ws + (size_t)a.kv.HK * p.shared_tiles * p.shared * (attn_slot_bytes(p.shared_mt, a.kv.D) / sizeof(float));
-    const hipError_t e = attn_any(a, p.shared_mt, 1, (unsigned)(div_up((long long)a.kv.HK * p.shared, 8) * 8 * p.shared_tiles), s);
-    if (e != hipSuccess) return e;
-    a.prefix_len = 0;
+    a.shared_part = a.part;
+    a.part += shared_slots(p, a.kv.HK) * (attn_slot_bytes(p.mt, a.kv.D) / sizeof(float));
+    grid += a.shared_grid;
   }
-  const long long grid = p.slots ? p.slots : row_tiles(a.s.T, a.s.B, a.s.start != nullptr, a.G, 16 * p.mt) * a.kv.HK;
-  const hipError_t e = attn_any(a, p.mt, 0, (unsigned)grid, s);
-  if (e != hipSuccess || !p.slots) return e;
-  attn_join_kernel<<<(unsigned)((long long)a.s.T * a.HQ), 256, 0, s>>>(a, 16 * p.mt, 0);
+  const hipError_t e = attn_any(a, p.mt, (unsigned)grid, s);
+  if (e != hipSuccess || !a.slots) return e;
+  attn_join_kernel<<<(unsigned)((long long)a.s.T * a.HQ), 256, 0, s>>>(a, 16 * p.mt, a.sel ? 1 : 0);
   return hipGetLastError();
 }
 

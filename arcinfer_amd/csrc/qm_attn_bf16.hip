@@ -2,5 +2,5 @@
 #include "qm_attn_launch.h"
 
 namespace qm {
-hipError_t attn_bf16(const AttnArgs& a, int mt, int mode, unsigned grid, hipStream_t s) { return attn_types<__bf16, __bf16>(a, mt, mode, grid, s); }
+hipError_t attn_bf16(const AttnArgs& a, int mt, unsigned grid, hipStream_t s) { return attn_types<__bf16, __bf16>(a, mt, grid, s); }
 }  // namespace qm

@@ -136,11 +136,10 @@ __device__ __forceinline__ int without_odd(int w) {
   }
 }
 
-// TQ: q's type. TC: the cache's, TQ or uint8_t (e4m3). DC: D rounded up to 64, 128 or 256 (FULL: it is that). MT: row tiles of 16. PARTS: of P. MODE: the keys of
-// each sequence (OWN), of the prefix for the rows of the whole batch (SHARED), or of chosen pages (CHOSEN).
-enum : int { OWN = 0, SHARED = 1, CHOSEN = 2 };
+// TQ: q's type. TC: the cache's, TQ or uint8_t (e4m3). DC: D rounded up to 64, 128 or 256 (FULL: it is that). MT: row tiles of 16. PARTS: of P. CHOSEN: chosen pages of
+// each token; else each sequence's own keys, and in the first work-groups those of the prefix for the rows of the whole batch.
 
-template <typename TQ, typename TC, int DC, bool FULL, int MT, int PARTS, int MODE>
+template <typename TQ, typename TC, int DC, bool FULL, int MT, int PARTS, bool CHOSEN>
 __global__ __launch_bounds__(256, 2) void attn_kernel(AttnArgs a) {
   constexpr bool E8 = sizeof(TC) == 1;
   typedef std::conditional_t<E8, __bf16, TQ> TP;           // of P and V on the matrix pipe
@@ -160,18 +159,10 @@ __global__ __launch_bounds__(256, 2) void attn_kernel(AttnArgs a) {
 
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 15, g = lane >> 4;
   const KvView& kv = a.kv;
-  int h, b = 0, rt, c = 0, blocks = 0x7fffffff, row0 = 0, rows, after = 0;  // (after: tokens of the sequence behind these rows)
+  int h, b = 0, rt, c = 0, blocks = 0x7fffff00, row0 = 0, rows, after = 0;  // (after: tokens of the sequence behind these rows)
   int rts = 1, more = 0;
-  if constexpr (MODE == SHARED) {
-    // the row tiles of one piece and head lie 8 work-groups apart: on one XCD, whose L2 then reads the piece once
-    const unsigned w = blockIdx.x, at = w >> 3, pc = (at / a.shared_tiles) * 8 + (w & 7);
-    rt = at % a.shared_tiles;
-    h = pc % kv.HK;
-    c = pc / kv.HK;
-    if (c >= a.shared) return;
-    blocks = a.shared_blocks;
-    rows = a.s.T;
-  } else if constexpr (MODE == CHOSEN) {
+  const bool shared = !CHOSEN && (int)blockIdx.x < a.shared_grid;
+  if constexpr (CHOSEN) {
     // (each token's pages are its own: the tile is of one token, and every token has the same number of pieces)
     const int unit = blockIdx.x / kv.HK;
     h = blockIdx.x % kv.HK;
@@ -184,9 +175,18 @@ __global__ __launch_bounds__(256, 2) void attn_kernel(AttnArgs a) {
     if (b < 0) return;  // (a row of no sequence)
     rows = 1;
     after = row_from(a.s, b) + rows_of(a.s, b) - 1 - row0;
+  } else if (shared) {
+    // the row tiles of one piece and head lie 8 work-groups apart: on one XCD, whose L2 then reads the piece once
+    const unsigned w = blockIdx.x, at = w >> 3, pc = (at / a.shared_tiles) * 8 + (w & 7);
+    rt = at % a.shared_tiles;
+    h = pc % kv.HK;
+    c = pc / kv.HK;
+    if (c >= a.shared) return;
+    blocks = a.shared_blocks;
+    rows = a.s.T;
   } else {
     Item it;
-    if (!find_item(a, RT, blockIdx.x, it)) return;
+    if (!find_item(a, RT, blockIdx.x - a.shared_grid, it)) return;
     b = __builtin_amdgcn_readfirstlane(it.b);
     h = __builtin_amdgcn_readfirstlane(it.h);
     rt = __builtin_amdgcn_readfirstlane(it.rt);
@@ -199,25 +199,25 @@ __global__ __launch_bounds__(256, 2) void attn_kernel(AttnArgs a) {
   }
   // (rows: tokens; a row of the tile is token r / G, query head h G + r % G)
   const int nrows = rows * a.G, first = rt * RT, last = min(first + RT, nrows) - 1;
-  const int capacity = MODE == SHARED ? 0 : (int)min((long long)a.s.W << kv.lg, 0x7fffffffLL);
-  const int len = MODE == SHARED ? 0 : __builtin_amdgcn_readfirstlane(a.s.len[b]) - after;
+  const int capacity = shared ? 0 : (int)min((long long)a.s.W << kv.lg, 0x7fffffffLL);
+  const int len = shared ? 0 : __builtin_amdgcn_readfirstlane(a.s.len[b]) - after;
   // keys that the tile's first and last tokens see of their own
-  const int lo_lim = MODE == SHARED ? 0 : min(max(len - rows + first / a.G + 1, 0), capacity);
-  const int hi_lim = MODE == SHARED ? 0 : min(max(len - rows + last / a.G + 1, 0), capacity);
+  const int lo_lim = min(max(len - rows + first / a.G + 1, 0), capacity);
+  const int hi_lim = min(max(len - rows + last / a.G + 1, 0), capacity);
   int lim[MT];
 #pragma unroll
   for (int m = 0; m < MT; ++m) {
     const int r = first + 16 * m + col;
-    lim[m] = MODE == SHARED ? 0 : min(max(len - rows + r / a.G + 1, 0), capacity);
+    lim[m] = min(max(len - rows + r / a.G + 1, 0), capacity);
   }
 
   // blocks of 32 keys: of the prefix, then of the sequence's own (or of the chosen pages)
-  const int shared_blocks32 = MODE == CHOSEN ? 0 : (a.prefix_len + kBlock - 1) / kBlock;
-    const int own_blocks = MODE == SHARED ? 0 : MODE == CHOSEN ? (int)(((long long)a.k * kv.page + kBlock - 1) / kBlock) : (int)(((long long)hi_lim + kBlock - 1) / kBlock);
+  const int shared_blocks32 = CHOSEN || (a.shared_grid && !shared) ? 0 : (a.prefix_len + kBlock - 1) / kBlock;
+  const int own_blocks = CHOSEN ? (int)(((long long)a.k * kv.page + kBlock - 1) / kBlock) : (int)(((long long)hi_lim + kBlock - 1) / kBlock);
   const int all_blocks = shared_blocks32 + own_blocks;
   const int begin = (int)min((long long)c * blocks * kWaves, (long long)all_blocks);
   const int end = (int)min((long long)begin + (long long)blocks * kWaves, (long long)all_blocks);
-  if (MODE != SHARED && c > 0 && begin >= all_blocks) return;  // (a piece that this tile's rows do not see)
+  if (!shared && c > 0 && begin >= all_blocks) return;  // (a piece that this tile's rows do not see)
 
   // q: k step t of row col holds elements 32 t + 8 g .. + 7 (8-bit keys: 64 (t / 2) + 16 g + 8 (t % 2), as their loads lie). Of larger
   // tiles it stays in LDS, in operand order: the registers are the result's.
@@ -273,7 +273,8 @@ __global__ __launch_bounds__(256, 2) void attn_kernel(AttnArgs a) {
       for (int j = 0; j < VE; ++j) o[vb][j][m] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
   }
 
-  // Where the 16 keys of half s of block i lie
+  // Where the 16 keys of each half of a block lie. The numbers of pages come by scalar loads, asked for one block ahead of the address that
+  // they make, and of chosen pages the places in the list one more: nothing waits for them.
   struct Place {
     long long base;  // bytes from the cache's first key (value) to the first of them (a masked page's: of the first page)
     size_t scale;    // and of their scales, in elements
@@ -281,27 +282,40 @@ __global__ __launch_bounds__(256, 2) void attn_kernel(AttnArgs a) {
     bool dead;       // masked
     __device__ __forceinline__ int sees(int lim) const { return dead ? 0 : (limit >= 0 ? limit : lim) - pos; }  // how many of them a row of limit lim sees
   };
-  const auto place = [&](int i, int s) {
-    Place r;
-    int page = -1, pos;
-    r.limit = -1;
-    if (MODE != CHOSEN && i < shared_blocks32) {
-      pos = i * kBlock + 16 * s;
-      r.limit = a.prefix_len;
-      if (pos < a.prefix_len) page = scalar(a.prefix, pos >> kv.lg);
-    } else {
-      pos = i < end ? (i - shared_blocks32) * kBlock + 16 * s : 0x7fffffff;
-      if constexpr (MODE == CHOSEN) {
-        const int e = pos >> kv.lg, in = pos & (kv.page - 1);
-        const int n = e < a.k ? scalar(a.sel, ((size_t)row0 * kv.HK + h) * a.k + e) : -1;
-        pos = n >= 0 && n < a.s.W ? (int)min(((long long)n << kv.lg) + in, 0x7fffffffLL) : 0x7fffffff;
+  const int32_t* table = a.s.table + (size_t)b * a.s.W;
+  const int32_t* sel = a.sel + ((size_t)row0 * kv.HK + h) * a.k;
+  struct Asked {
+    int page[2], pos[2], limit;
+  };
+  const auto chosen = [&](int i, int s) {  // the entry of the list of chosen pages
+    const int e = (i * kBlock + 16 * s) >> kv.lg;
+    return scalar(sel, e < a.k ? e : 0);
+  };
+  const auto ask = [&](int i, const int* pick) {
+    Asked r;
+    const bool pre = !CHOSEN && i < shared_blocks32;
+    r.limit = pre ? a.prefix_len : -1;
+    const int32_t* list = pre ? a.prefix : table;
+    const int most = pre ? a.prefix_len : hi_lim;
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      int pos = i < end ? (pre ? i : i - shared_blocks32) * kBlock + 16 * s : 0x7fffffff;
+      if constexpr (CHOSEN) {
+        const int in = (i * kBlock + 16 * s) & (kv.page - 1), n = pick[s];
+        pos = i < end && (i * kBlock + 16 * s) >> kv.lg < a.k && n >= 0 && n < a.s.W ? (n << kv.lg) + in : 0x7fffffff;
       }
-      if (MODE != SHARED && pos < hi_lim) page = scalar(a.s.table, (size_t)b * a.s.W + (pos >> kv.lg));
+      r.pos[s] = pos;
+      r.page[s] = scalar(list, pos < most ? pos >> kv.lg : 0);  // (without a branch: one would wait; `placed` looks at the place)
     }
-    page = __builtin_amdgcn_readfirstlane(page);
-    r.pos = __builtin_amdgcn_readfirstlane(pos);
-    r.dead = (unsigned)page >= (unsigned)kv.pages;
-    const int pg = r.dead ? 0 : page, in = r.dead ? 0 : r.pos & (kv.page - 1);
+    return r;
+  };
+  const auto placed = [&](const Asked& q, int s) {
+    Place r;
+    r.pos = q.pos[s];
+    r.limit = q.limit;
+    const int page = q.page[s];
+    r.dead = (unsigned)page >= (unsigned)kv.pages || r.pos >= (q.limit >= 0 ? q.limit : hi_lim);
+    const int pg = r.dead ? 0 : page, in = r.dead ? 0 : r.pos & (kv.page - 1);  // (16 rows from there are the page's: place 0 of page 0 always is)
     r.base = (pg * kv.ps + h * kv.hs + in * kv.ts) * (long long)sizeof(TC);
     r.scale = ((size_t)pg * kv.HK + h) * kv.page + in;
     return r;
@@ -330,8 +344,20 @@ __global__ __launch_bounds__(256, 2) void attn_kernel(AttnArgs a) {
   // Registers of K and of V are loaded for the next block as soon as this one's products have taken them: what a block waits for was asked
   // for nearly a block before.
   Place now[2], next[2];
+  int pick[2] = {0, 0};
+  const auto list = [&](int i) {
+    if constexpr (CHOSEN) {
+      pick[0] = chosen(i, 0);
+      pick[1] = chosen(i, 1);
+    }
+  };
+  list(begin + wave);
+  Asked asked = ask(begin + wave, pick);
+  list(begin + wave + kWaves);
 #pragma unroll
-  for (int s = 0; s < 2; ++s) now[s] = place(begin + wave, s);
+  for (int s = 0; s < 2; ++s) now[s] = placed(asked, s);
+  asked = ask(begin + wave + kWaves, pick);
+  list(begin + wave + 2 * kWaves);
 #pragma unroll
   for (int s = 0; s < 2; ++s) load_k(s, now[s]);
 #pragma unroll
@@ -341,7 +367,7 @@ __global__ __launch_bounds__(256, 2) void attn_kernel(AttnArgs a) {
   for (int i = begin + wave; i < end; i += kWaves) {
     asm volatile("" ::: "memory");  // (q is read from LDS for each block: kept in registers it would not leave room for the rest)
 #pragma unroll
-    for (int s = 0; s < 2; ++s) next[s] = place(i + kWaves, s);
+    for (int s = 0; s < 2; ++s) next[s] = placed(asked, s);
 
     // S^T: lane (col, g) has keys 4 g .. + 3 of each half for row col
     v4f x[2][MT];
@@ -377,6 +403,9 @@ __global__ __launch_bounds__(256, 2) void attn_kernel(AttnArgs a) {
       if (!LATE) load_k(s, next[s]);
     }
 
+    asked = ask(i + 2 * kWaves, pick);  // (here: a wait for q from LDS would be one for these too)
+    list(i + 3 * kWaves);
+
     // mask; values of keys that no row sees become zeros (they may hold anything)
     bool partial = false, odd = false;
 #pragma unroll
@@ -399,10 +428,10 @@ __global__ __launch_bounds__(256, 2) void attn_kernel(AttnArgs a) {
 #pragma unroll
             for (int w = 0; w < VW; ++w) {
               if (4 * g + e >= edge) vr[vb][s][e][w] = 0;
-              if (MODE == OWN) bad |= odd_word<TC>(vr[vb][s][e][w]);
+              if (!CHOSEN) bad |= odd_word<TC>(vr[vb][s][e][w]);
             }
       }
-      odd = MODE == OWN && lo_lim != hi_lim && __builtin_amdgcn_ballot_w64(bad) != 0;
+      odd = !CHOSEN && lo_lim != hi_lim && __builtin_amdgcn_ballot_w64(bad) != 0;
     }
 
     // the rows' maxima: renewed when one is passed by more than kSlack (rarely, after the first blocks)
@@ -586,14 +615,14 @@ __global__ __launch_bounds__(256, 2) void attn_kernel(AttnArgs a) {
     }
   }
 
-  const int all_pieces = MODE == CHOSEN ? a.pieces : ((all_blocks + kWaves - 1) / kWaves + (long long)blocks - 1) / blocks;
-  const bool split = MODE == SHARED || (MODE == OWN && a.shared > 0) || all_pieces > 1;
+  const int all_pieces = CHOSEN ? a.pieces : ((all_blocks + kWaves - 1) / kWaves + blocks - 1) / blocks;
+  const bool split = a.shared_grid > 0 || all_pieces > 1;
   float* slot = nullptr;
-  if (MODE == SHARED) {
+  if (shared) {
     slot = a.shared_part + ((size_t)(h * a.shared_tiles + rt) * a.shared + c) * slot_floats(RT, kv.D);
   } else if (a.slots) {
-    const int at = MODE == CHOSEN ? row0 * rts + rt : first_slot(a, RT, b, row0, rt);
-    const int others = a.firsts + (MODE == CHOSEN ? row0 * rts * (a.pieces - 1) : more) + rt;
+    const int at = CHOSEN ? row0 * rts + rt : first_slot(a, RT, b, row0, rt);
+    const int others = a.firsts + (CHOSEN ? row0 * rts * (a.pieces - 1) : more) + rt;
     const long long n = ((long long)(c ? others + (c - 1) * rts : at)) * kv.HK + h;
     if (n >= a.slots) return;  // (rows of lists that are none)
     slot = a.part + (size_t)n * slot_floats(RT, kv.D);

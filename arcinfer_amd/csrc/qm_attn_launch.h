@@ -5,31 +5,31 @@
 namespace qm {
 
 template <typename TQ, typename TC, int DC, bool FULL, int MT, int PARTS>
-void attn_full(const AttnArgs& a, int mode, unsigned grid, hipStream_t s) {
-  if (mode == SHARED) attn_kernel<TQ, TC, DC, FULL, MT, PARTS, SHARED><<<grid, 256, 0, s>>>(a);
-  else if (mode == CHOSEN) attn_kernel<TQ, TC, DC, FULL, MT, PARTS, CHOSEN><<<grid, 256, 0, s>>>(a);
-  else attn_kernel<TQ, TC, DC, FULL, MT, PARTS, OWN><<<grid, 256, 0, s>>>(a);
+void attn_full(const AttnArgs& a, unsigned grid, hipStream_t s) {
+  if (a.sel) attn_kernel<TQ, TC, DC, FULL, MT, PARTS, true><<<grid, 256, 0, s>>>(a);
+  else attn_kernel<TQ, TC, DC, FULL, MT, PARTS, false><<<grid, 256, 0, s>>>(a);
 }
 
 template <typename TQ, typename TC, int DC, int MT, int PARTS>
-hipError_t attn_mode(const AttnArgs& a, int mode, unsigned grid, hipStream_t s) {
-  if (a.kv.D == DC) attn_full<TQ, TC, DC, true, MT, PARTS>(a, mode, grid, s);
-  else attn_full<TQ, TC, DC, false, MT, PARTS>(a, mode, grid, s);
+hipError_t attn_mode(const AttnArgs& a, unsigned grid, hipStream_t s) {
+  if (a.kv.D == DC) attn_full<TQ, TC, DC, true, MT, PARTS>(a, grid, s);
+  else attn_full<TQ, TC, DC, false, MT, PARTS>(a, grid, s);
   return hipGetLastError();
 }
 
 template <typename TQ, typename TC, int PARTS>
-hipError_t attn_parts(const AttnArgs& a, int mt, int mode, unsigned grid, hipStream_t s) {
-  if (a.kv.D <= 64) return mt == 1 ? attn_mode<TQ, TC, 64, 1, PARTS>(a, mode, grid, s) : mt == 2 ? attn_mode<TQ, TC, 64, 2, PARTS>(a, mode, grid, s) : attn_mode<TQ, TC, 64, 4, PARTS>(a, mode, grid, s);
-  if (a.kv.D <= 128) return mt == 1 ? attn_mode<TQ, TC, 128, 1, PARTS>(a, mode, grid, s) : mt == 2 ? attn_mode<TQ, TC, 128, 2, PARTS>(a, mode, grid, s) : attn_mode<TQ, TC, 128, 4, PARTS>(a, mode, grid, s);
-  return mt == 1 ? attn_mode<TQ, TC, 256, 1, PARTS>(a, mode, grid, s) : attn_mode<TQ, TC, 256, 2, PARTS>(a, mode, grid, s);
+hipError_t attn_parts(const AttnArgs& a, int mt, unsigned grid, hipStream_t s) {
+  // (row tiles: what the registers hold, as tiles_for has it)
+  if (a.kv.D <= 64) return mt == 1 ? attn_mode<TQ, TC, 64, 1, PARTS>(a, grid, s) : mt == 2 ? attn_mode<TQ, TC, 64, 2, PARTS>(a, grid, s) : attn_mode<TQ, TC, 64, 4, PARTS>(a, grid, s);
+  if (a.kv.D <= 128) return mt == 1 ? attn_mode<TQ, TC, 128, 1, PARTS>(a, grid, s) : attn_mode<TQ, TC, 128, 2, PARTS>(a, grid, s);
+  return attn_mode<TQ, TC, 256, 1, PARTS>(a, grid, s);
 }
 
 // Two parts of P where the result keeps more bits than one: f32, or f16 behind an 8-bit cache (P is bf16 there)
 template <typename TQ, typename TC>
-hipError_t attn_types(const AttnArgs& a, int mt, int mode, unsigned grid, hipStream_t s) {
-  if constexpr (sizeof(TC) == 1 && __is_same(TQ, _Float16)) return attn_parts<TQ, TC, 2>(a, mt, mode, grid, s);
-  else return a.otype == DT_F32 ? attn_parts<TQ, TC, 2>(a, mt, mode, grid, s) : attn_parts<TQ, TC, 1>(a, mt, mode, grid, s);
+hipError_t attn_types(const AttnArgs& a, int mt, unsigned grid, hipStream_t s) {
+  if constexpr (sizeof(TC) == 1 && __is_same(TQ, _Float16)) return attn_parts<TQ, TC, 2>(a, mt, grid, s);
+  else return a.otype == DT_F32 ? attn_parts<TQ, TC, 2>(a, mt, grid, s) : attn_parts<TQ, TC, 1>(a, mt, grid, s);
 }
 
 }  // namespace qm

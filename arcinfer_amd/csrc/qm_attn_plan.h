@@ -33,18 +33,16 @@ __device__ __forceinline__ int sequence_of(const Seqs& s, int t) {
   return lo < s.B && t - row_from(s, lo) < rows_of(s, lo) && t >= row_from(s, lo) ? lo : -1;
 }
 
-// Blocks of 128 keys of sequence b, the prefix in front of them
-__device__ __forceinline__ long long blocks_of(const AttnArgs& a, int b) {
-  const long long most = (long long)a.s.W << a.kv.lg;
-  long long n = a.s.len[b];
-  n = n < 0 ? 0 : n < most ? n : most;
-  return ((n + 31) / 32 + (a.prefix_len + 31) / 32 + 3) >> 2;
+// Blocks of 128 keys of sequence b, the prefix in front of them (below 2^25: a prefix and a table hold 2^30 keys each)
+__device__ __forceinline__ int blocks_of(const AttnArgs& a, int b) {
+  const int most = a.s.W << a.kv.lg, n = min(max(a.s.len[b], 0), most);
+  return (int)(((unsigned)(n + 31) / 32 + (a.shared_grid ? 0u : (unsigned)(a.prefix_len + 31) / 32) + 3) / 4);
 }
 
 // The place of the result of row tile rt's first piece among the slots (of a head): row tiles of RT rows, of a sequence whose rows begin at
 // row0. Known without the other sequences' lengths: the tiles of the rows before are at most row0 G / RT and one for each sequence.
 __device__ __forceinline__ int first_slot(const AttnArgs& a, int RT, int b, int row0, int rt) {
-  return a.s.start ? (int)((long long)row0 * a.G / RT) + b + rt : b * ((a.G + RT - 1) / RT) + rt;
+  return a.s.start ? row0 * a.G / RT + b + rt : b * ((a.G + RT - 1) / RT) + rt;
 }
 
 // What a work-group does: row tile rt of key head h of sequence b, piece c of its keys. Pieces behind the first have their results behind all
@@ -55,67 +53,65 @@ struct Item {
   int more;
 };
 
-struct Sums {
-  long long units, tiles;  // work-groups and row tiles
-};
-__device__ __forceinline__ Sums operator+(Sums a, Sums b) { return {a.units + b.units, a.tiles + b.tiles}; }
-
 // Sequences are looked at 64 at a time by each wave for itself (no wave waits for another): the sum over all of them, then the scan that says
-// whose unit number this is.
+// whose unit number this is. (A call's units and row tiles are below 2^24, as its grid is; sums over lists that are none may wrap.)
 __device__ __forceinline__ bool find_item(const AttnArgs& a, int RT, int unit, Item& out) {
   const int lane = threadIdx.x & 63, HK = a.kv.HK;
-  const auto tiles_of = [&](int b) { return b < a.s.B ? (int)(((long long)rows_of(a.s, b) * a.G + RT - 1) / RT) : 0; };
+  const auto tiles_of = [&](int b) { return b < a.s.B ? (rows_of(a.s, b) * a.G + RT - 1) / RT : 0; };
   // (the first 64 sequences are held: most batches are no larger)
-  const int rts0 = tiles_of(lane);
-  const long long blocks0 = rts0 ? blocks_of(a, lane) : 0;
-  int blocks = 0x7fffffff;
+  const int rts0 = tiles_of(lane), blocks0 = rts0 ? blocks_of(a, lane) : 0;
+  int blocks = 0x7fffff00;
   if (a.target) {
-    long long all = rts0 * blocks0;
+    float all = (float)rts0 * (float)blocks0;  // (a few parts in a million more or less do not matter)
     for (int b = lane + 64; b < a.s.B; b += 64) {
       const int n = tiles_of(b);
-      if (n) all += n * blocks_of(a, b);
+      if (n) all += (float)n * (float)blocks_of(a, b);
     }
     for (int o = 32; o; o >>= 1) all += __shfl_xor(all, o);
-    const long long n = (all * HK + a.target - 1) / a.target;
-    blocks = n > kLeast ? (int)(n < 0x7fffffff ? n : 0x7fffffff) : kLeast;
+    blocks = max((int)ceilf(all * (float)HK / (float)a.target * 1.00001f), kLeast);
   }
-  Sums base = {0, 0};
+  int units0 = 0, tiles0 = 0;
   for (int b0 = 0; b0 < a.s.B; b0 += 64) {
-    const int rts = b0 ? tiles_of(b0 + lane) : rts0;
-    const long long n = !rts ? 0 : ((b0 ? blocks_of(a, b0 + lane) : blocks0) + blocks - 1) / blocks;
-    const int pieces = n > 1 ? (int)n : 1;
-    const Sums mine = {(long long)rts * pieces * HK, rts};
-    Sums end = mine;
+    const int rts = b0 ? tiles_of(b0 + lane) : rts0, n = b0 ? (rts ? blocks_of(a, b0 + lane) : 0) : blocks0;
+    const int pieces = max((n + blocks - 1) / blocks, 1), mine = rts * pieces * HK;
+    int units = mine, tiles = rts;
     for (int o = 1; o < 64; o <<= 1) {
-      const Sums v = {__shfl_up(end.units, o), __shfl_up(end.tiles, o)};
-      if (lane >= o) end = end + v;
+      const int u = __shfl_up(units, o), t = __shfl_up(tiles, o);
+      if (lane >= o) {
+        units += u;
+        tiles += t;
+      }
     }
-    const unsigned long long past = __ballot(base.units + end.units > unit);
+    const unsigned long long past = __ballot(units0 + units > unit);
     if (past) {
       const int at = __ffsll(past) - 1;
       out.b = b0 + at;
       out.rts = __builtin_amdgcn_readlane(rts, at);
       out.blocks = blocks;
       const int np = __builtin_amdgcn_readlane(pieces, at) * HK;
-      const long long units0 = base.units + __shfl(end.units - mine.units, at), tiles0 = base.tiles + __shfl(end.tiles - mine.tiles, at);
+      units0 += __builtin_amdgcn_readlane(units - mine, at);
+      tiles0 += __builtin_amdgcn_readlane(tiles - rts, at);
       // The row tiles of one piece and head lie 8 work-groups apart: on one XCD, whose L2 then reads the piece once. The last rows' tiles, which
       // see the most keys, begin.
-      const int j = (int)(unit - units0), whole = np / 8 * 8, rest = np - whole;
-      int pair, rt;
-      if (j < whole * out.rts) {
-        pair = j / (8 * out.rts) * 8 + j % 8;
-        rt = j % (8 * out.rts) / 8;
-      } else {
-        pair = whole + (j - whole * out.rts) % rest;
-        rt = (j - whole * out.rts) / rest;
+      const int j = unit - units0, whole = np / 8 * 8, rest = np - whole;
+      int pair = j, rt = 0;
+      if (out.rts > 1) {
+        if (j < whole * out.rts) {
+          pair = j / (8 * out.rts) * 8 + j % 8;
+          rt = j % (8 * out.rts) / 8;
+        } else {
+          pair = whole + (j - whole * out.rts) % rest;
+          rt = (j - whole * out.rts) / rest;
+        }
       }
       out.rt = out.rts - 1 - rt;
       out.h = pair % HK;
       out.c = pair / HK;
-      out.more = (int)(units0 / HK - tiles0);
+      out.more = units0 / HK - tiles0;
       return true;
     }
-    base = base + Sums{__shfl(end.units, 63), __shfl(end.tiles, 63)};
+    units0 += __builtin_amdgcn_readlane(units, 63);
+    tiles0 += __builtin_amdgcn_readlane(tiles, 63);
   }
   return false;
 }

@@ -37,7 +37,7 @@ struct AttnArgs {
   KvView kv;
   Seqs s;
   const int32_t* prefix;
-  int prefix_len;       // keys in front of each sequence's own that this launch reads
+  int prefix_len;       // keys in front of each sequence's own
   const int32_t* sel;   // pages of each row and key head [T][HK][k] (null: all)
   int k;
   float c;              // scale * log2 e
@@ -48,19 +48,21 @@ struct AttnArgs {
   int target, slots;    // pieces that are aimed at (0: whole row tiles), and partial results that `part` holds, those of
   int firsts;           // first pieces (of a head) in front
   int pieces, blocks;   // chosen pages: pieces of a row tile, and blocks of 128 keys of one
-  // The pieces of the shared prefix for the rows of the whole batch (shared > 0): pieces a row tile, tiles of shared_rt rows of a key
-  // head, blocks of 128 keys of a piece; slot ((head * shared_tiles) + tile) * shared + piece
+  // The prefix for the rows of the whole batch (shared_grid work-groups in front of the others; 0: it is read with each sequence's own keys):
+  // pieces of `shared_blocks` blocks of 128 keys, `shared` of them, for each of shared_tiles row tiles of a key head; slot
+  // (head * shared_tiles + tile) * shared + piece
   float* shared_part;
-  int shared, shared_rt, shared_tiles, shared_blocks;
+  int shared_grid, shared, shared_tiles, shared_blocks;
 };
 
-// How a call runs: mt row tiles of 16 a work-group; pieces and blocks as in AttnArgs
+// How a call runs: row tiles of 16 mt; pieces and blocks as in AttnArgs
 struct AttnPlan {
-  int mt, target, slots, firsts;                       // target 0: nothing is split
-  int shared, shared_mt, shared_tiles, shared_blocks;  // shared 0: the prefix is read with each sequence's own keys
+  int mt, target, slots, firsts;            // target 0: nothing is split
+  int shared, shared_tiles, shared_blocks;  // shared 0: the prefix is read with each sequence's own keys
 };
 size_t attn_slot_bytes(int mt, int D);
 AttnPlan attn_plan(int T, int B, bool start, int HQ, int HK, int D, int prefix_len, size_t ws_bytes);
+size_t attn_used_bytes(const AttnPlan& p, int HK, int D);
 size_t attn_workspace_bytes(int T, int B, int HQ, int HK, int D, int prefix_len);
 // Work-groups of the calls's launches at most (0: more than a grid holds)
 long long attn_grid(const AttnPlan& p, int T, int B, bool start, int HQ, int HK);

@@ -343,7 +343,7 @@ int qmatmul_qk_norm_rope(const void* x, int xtype, int ldx, int T, int D, int q_
  * The cache of one layer: pages of `page` tokens (16, 32, 64, 128 or 256), each with every key head's keys and values of D
  * elements (a multiple of 16, 16..256). Element d of head h of token i of page p is at p * page_stride + h * head_stride +
  * i * token_stride + d, in k and in v alike (strides in elements; every row of D 16-byte aligned; no two elements at one
- * place). Any order of the dimensions serves; heads outside tokens, as in [pages][heads][page][D], is read fastest.
+ * place; token_stride below 2^26). Any order of the dimensions serves; heads outside tokens, as in [pages][heads][page][D], is read fastest.
  * Types: QM_F16, QM_BF16, or QM_E4M3 with an f32 scale for each token and head, k_scale and v_scale [pages][heads][page]
  * (16-byte aligned; the value is scale * e4m3). mean (or NULL): bf16 [pages][heads][D], the mean key of each page that was
  * filled, which qmatmul_select_pages scores pages by. pages * page < 2^31. The buffers are the caller's.
