@@ -1342,8 +1342,7 @@ int qmatmul_select_pages(const void* q, int qtype, int ldq, int HQ, const qm_seq
   if (!sel) return fail(QM_ERR_ARG, "%s: null pointer", fn);
   if (!aligned(sel, 4)) return fail(QM_ERR_ARG, "%s: every pointer must be aligned to its type", fn);
   const size_t need = seqs->table_stride > k ? (size_t)seqs->T * kv->heads * seqs->table_stride * sizeof(double) : 0;
-  const long long groups = (long long)seqs->T * kv->heads * ((seqs->table_stride + 255) / 256);
-  if (groups * 256 > qm::kMostThreads) return fail(QM_ERR_SHAPE, "%s: %d rows of %d heads and %d pages are more than a grid holds", fn, seqs->T, kv->heads, seqs->table_stride);
+  if (qm::select_grid(seqs->T, kv->heads, seqs->table_stride) * 256 > qm::kMostThreads) return fail(QM_ERR_SHAPE, "%s: %d rows of %d heads and %d pages are more than a grid holds", fn, seqs->T, kv->heads, seqs->table_stride);
   if (need && (!ws || ws_bytes < need)) return fail(QM_ERR_WORKSPACE, "%s: a workspace of %zu bytes, %zu needed", fn, ws ? ws_bytes : 0, need);
   if (need && !aligned(ws, 256)) return fail(QM_ERR_ARG, "%s: the workspace must be 256-byte aligned", fn);
   const HeadRows rq{q, seqs->T, kv->D, HQ, kv->D, ldq, 2};

@@ -13,9 +13,11 @@ hipError_t attn_f16_e4m3(const AttnArgs& a, int mt, unsigned grid, hipStream_t s
 // of a single piece are left as attn_kernel wrote them. What a row needs to know of the split stands in its tile's first slot.
 // Latency-bound: a launch, that slot's words, then the pieces' maxima and sums and kAhead results of each group at once.
 constexpr int kAhead = 8;
-__global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a, int RT, int chosen) {
-  __shared__ float wave_max[4], weight[256], gsum[256];
-  __shared__ float4 osum[256];
+template <int THREADS>
+__global__ __launch_bounds__(THREADS) void attn_join_kernel(AttnArgs a, int RT, int chosen) {
+  constexpr int kWavesHere = THREADS / 64;
+  __shared__ float wave_max[kWavesHere], weight[THREADS], wsum[kWavesHere];
+  __shared__ float4 osum[THREADS];
   const int hq = blockIdx.x % a.HQ, t = blockIdx.x / a.HQ, h = hq / a.G, g = hq % a.G, D = a.kv.D, tid = threadIdx.x;
   const int b = sequence_of(a.s, t);
   if (b < 0) return;
@@ -25,10 +27,9 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a, int RT, int 
   const size_t size = slot_floats(RT, D);
   const float* first = a.part + (size_t)n0 * size;
   const int4 head = *(const int4*)first;
-  if (!a.shared && head.x == 1) return;
-  const int all = a.shared + head.x;
   const long long srow = (long long)t * a.G + g;
-  // the partial result of piece p: of its row, the maximum; the sum lies RT behind it, the elements from 2 RT on
+  // the partial result of piece p: of its row, the maximum; the sum lies RT behind it, the elements from 2 RT on. (The prefix's pieces and the
+  // first one are known without the slot's words.)
   const float* sfirst = a.shared_part + (size_t)(h * a.shared_tiles + srow / RT) * a.shared * size + 4;
   const auto slot = [&](int p) -> const float* {
     if (p < a.shared) return sfirst + (size_t)p * size;
@@ -37,12 +38,17 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a, int RT, int 
     return (n < a.slots ? a.part + (size_t)n * size : first) + 4;
   };
   const auto row_of = [&](int p) { return p < a.shared ? (int)(srow % RT) : r0 % RT; };
-  const int lanes = D / 4, groups = 256 / lanes, group = tid / lanes, d = 4 * (tid % lanes);
+  const int lanes = D / 4, groups = THREADS / lanes, group = tid / lanes, d = 4 * (tid % lanes);
   float l = 0.0f, top = -__builtin_inff();
   float4 o = {0.0f, 0.0f, 0.0f, 0.0f};
-  for (int p0 = 0; p0 < all; p0 += 256) {
-    // 256 pieces at a time: their maxima and sums, and the first results of each group, are asked for together
-    const int n = min(256, all - p0);
+  int all = a.shared + 1;
+  if (!a.shared) {
+    if (head.x == 1) return;  // (attn_kernel wrote the result)
+    all = head.x;
+  }
+  for (int p0 = 0; p0 < all;) {
+    // up to THREADS pieces at a time: their maxima and sums, and the first results of each group, are asked for together
+    const int n = min(THREADS, all - p0);
     float4 v[kAhead];
     const auto ask = [&](int i, int from) {
       const int p = p0 + min(group + (from + i) * groups, n - 1);
@@ -56,13 +62,16 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a, int RT, int 
       for (int i = 0; i < kAhead; ++i)
         if (i * groups < n) ask(i, 0);
     }
+    all = a.shared + head.x;
     // (a piece that the row sees nothing of has the sum 0)
     float most = w != 0.0f ? m : -__builtin_inff();
     for (int k = 32; k; k >>= 1) most = fmaxf(most, __shfl_xor(most, k));
     __syncthreads();
     if ((tid & 63) == 0) wave_max[tid >> 6] = most;
     __syncthreads();
-    most = fmaxf(top, fmaxf(fmaxf(wave_max[0], wave_max[1]), fmaxf(wave_max[2], wave_max[3])));
+    most = top;
+#pragma unroll
+    for (int i = 0; i < kWavesHere; ++i) most = fmaxf(most, wave_max[i]);
     if (most != top) {
       const float f = __builtin_amdgcn_exp2f(top - most);
       l *= f;
@@ -74,7 +83,7 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a, int RT, int 
     }
     const float f = w != 0.0f ? __builtin_amdgcn_exp2f(m - top) : 0.0f;
     weight[tid] = f;
-    l += f * w;
+    if (w != 0.0f) l = fmaf(f, w, l);
     __syncthreads();
     if (group < groups) {
       for (int from = 0; group + from * groups < n; from += kAhead) {
@@ -96,13 +105,16 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a, int RT, int 
         }
       }
     }
+    p0 += n;
   }
   for (int k = 32; k; k >>= 1) l += __shfl_xor(l, k);
   osum[tid] = o;
-  if ((tid & 63) == 0) gsum[tid >> 6] = l;
+  if ((tid & 63) == 0) wsum[tid >> 6] = l;
   __syncthreads();
   if (group) return;
-  l = gsum[0] + gsum[1] + gsum[2] + gsum[3];
+  l = 0.0f;
+#pragma unroll
+  for (int i = 0; i < kWavesHere; ++i) l += wsum[i];
   for (int i = 1; i < groups; ++i) {
     const float4 v = osum[i * lanes + tid];
     o.x += v.x;
@@ -229,7 +241,10 @@ hipError_t launch_attn(const AttnArgs& args, const AttnPlan& p, hipStream_t s) {
   }
   const hipError_t e = attn_any(a, p.mt, (unsigned)grid, s);
   if (e != hipSuccess || !a.slots) return e;
-  attn_join_kernel<<<(unsigned)((long long)a.s.T * a.HQ), 256, 0, s>>>(a, 16 * p.mt, a.sel ? 1 : 0);
+  // (a wave a row where there are rows enough: work-groups of four waves, most of which have nothing to do, take longer to start than that)
+  const long long rows = (long long)a.s.T * a.HQ;
+  if (rows >= 1024) attn_join_kernel<64><<<(unsigned)rows, 64, 0, s>>>(a, 16 * p.mt, a.sel ? 1 : 0);
+  else attn_join_kernel<256><<<(unsigned)rows, 256, 0, s>>>(a, 16 * p.mt, a.sel ? 1 : 0);
   return hipGetLastError();
 }
 

@@ -53,6 +53,29 @@ struct Item {
   int more;
 };
 
+// Inclusive sums over the lanes of a wave, by moves within rows of 16 and from one row's end to the next (no LDS)
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int moved(int v) { return __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xF, false); }
+__device__ __forceinline__ int scan64(int v) {
+  v += moved<0x111, 0xF>(v);
+  v += moved<0x112, 0xF>(v);
+  v += moved<0x114, 0xF>(v);
+  v += moved<0x118, 0xF>(v);
+  v += moved<0x142, 0xA>(v);  // (a row's last lane to the row behind it, of the second and fourth rows)
+  return v + moved<0x143, 0xC>(v);  // (the second row's last lane to the third and fourth)
+}
+template <int CTRL, int ROWS>
+__device__ __forceinline__ float moved_f(float v) { return __builtin_bit_cast(float, moved<CTRL, ROWS>(__builtin_bit_cast(int, v))); }
+__device__ __forceinline__ float sum64(float v) {
+  v += moved_f<0x111, 0xF>(v);
+  v += moved_f<0x112, 0xF>(v);
+  v += moved_f<0x114, 0xF>(v);
+  v += moved_f<0x118, 0xF>(v);
+  v += moved_f<0x142, 0xA>(v);
+  v += moved_f<0x143, 0xC>(v);
+  return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), 63));
+}
+
 // Sequences are looked at 64 at a time by each wave for itself (no wave waits for another): the sum over all of them, then the scan that says
 // whose unit number this is. (A call's units and row tiles are below 2^24, as its grid is; sums over lists that are none may wrap.)
 __device__ __forceinline__ bool find_item(const AttnArgs& a, int RT, int unit, Item& out) {
@@ -67,21 +90,14 @@ __device__ __forceinline__ bool find_item(const AttnArgs& a, int RT, int unit, I
       const int n = tiles_of(b);
       if (n) all += (float)n * (float)blocks_of(a, b);
     }
-    for (int o = 32; o; o >>= 1) all += __shfl_xor(all, o);
+    all = sum64(all);
     blocks = max((int)ceilf(all * (float)HK / (float)a.target * 1.00001f), kLeast);
   }
   int units0 = 0, tiles0 = 0;
   for (int b0 = 0; b0 < a.s.B; b0 += 64) {
     const int rts = b0 ? tiles_of(b0 + lane) : rts0, n = b0 ? (rts ? blocks_of(a, b0 + lane) : 0) : blocks0;
     const int pieces = max((n + blocks - 1) / blocks, 1), mine = rts * pieces * HK;
-    int units = mine, tiles = rts;
-    for (int o = 1; o < 64; o <<= 1) {
-      const int u = __shfl_up(units, o), t = __shfl_up(tiles, o);
-      if (lane >= o) {
-        units += u;
-        tiles += t;
-      }
-    }
+    const int units = scan64(mine), tiles = scan64(rts);
     const unsigned long long past = __ballot(units0 + units > unit);
     if (past) {
       const int at = __ffsll(past) - 1;

@@ -77,6 +77,7 @@ struct SelectArgs {
   double* scores;  // [T][HK][W]
   int32_t* sel;    // [T][HK][k]
 };
+long long select_grid(int T, int HK, int W);  // work-groups
 hipError_t launch_select(const SelectArgs& a, hipStream_t s);
 
 }  // namespace qm

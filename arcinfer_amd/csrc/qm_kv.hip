@@ -212,19 +212,19 @@ __global__ __launch_bounds__(256) void kv_append_kernel(AppendArgs a, int tokens
 }
 
 // The mean key of each page that a token of the call completes (its last place), from the keys as the cache holds them: a second
-// launch, since a page's other tokens may be other work-groups'. A work-group looks at kMeanTokens tokens for one head: 256 / (D / 8) rows at
+// launch, since a page's other tokens may be other work-groups'. A work-group looks at 64 tokens for one head: 256 / (D / 8) rows at
 // a time, 8 elements a lane, the rows' sums joined in one order.
-constexpr int kMeanTokens = 16;
+constexpr int kMeanTokens = 64;
 template <typename TC>
 __global__ __launch_bounds__(256) void page_mean_kernel(AppendArgs a) {
   __shared__ float red[256 * 8];
   const KvView& kv = a.kv;
   const int h = blockIdx.y, lanes = kv.D / 8, rows = 256 / lanes, d = (int)threadIdx.x % lanes, row = (int)threadIdx.x / lanes;
-  const long long t0 = (long long)blockIdx.x * kMeanTokens;
-  for (int e = 0; e < kMeanTokens; ++e) {
-    if (t0 + e >= a.r.T) return;
-    const int slot = a.slots[t0 + e], page = slot >> kv.lg;
-    if (slot < 0 || page >= kv.pages || (slot & (kv.page - 1)) != kv.page - 1) continue;  // (the same for the whole work-group)
+  const long long t = (long long)blockIdx.x * kMeanTokens + (threadIdx.x & 63);
+  const int mine = t < a.r.T ? a.slots[t] : -1;  // (each wave sees all of them)
+  unsigned long long full = __ballot(mine >= 0 && mine >> kv.lg < kv.pages && (mine & (kv.page - 1)) == kv.page - 1);
+  for (; full; full &= full - 1) {
+    const int page = __builtin_amdgcn_readlane(mine, __ffsll(full) - 1) >> kv.lg;
     float sum[8] = {};
     if (row < rows)
       for (int i = row; i < kv.page; i += rows) {
