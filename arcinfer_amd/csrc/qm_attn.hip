@@ -7,6 +7,10 @@ hipError_t attn_bf16(const AttnArgs& a, int mt, unsigned grid, hipStream_t s);
 hipError_t attn_f16(const AttnArgs& a, int mt, unsigned grid, hipStream_t s);
 hipError_t attn_bf16_e4m3(const AttnArgs& a, int mt, unsigned grid, hipStream_t s);
 hipError_t attn_f16_e4m3(const AttnArgs& a, int mt, unsigned grid, hipStream_t s);
+hipError_t attn_tile_bf16(const AttnArgs& a, int mt, unsigned grid, hipStream_t s);
+hipError_t attn_tile_f16(const AttnArgs& a, int mt, unsigned grid, hipStream_t s);
+hipError_t attn_tile_bf16_e4m3(const AttnArgs& a, int mt, unsigned grid, hipStream_t s);
+hipError_t attn_tile_f16_e4m3(const AttnArgs& a, int mt, unsigned grid, hipStream_t s);
 
 // Joins the pieces of one row: o = sum_p 2^(m_p - m) o_p / sum_p 2^(m_p - m) l_p. A work-group a row (a query head of a token): D / 4 lanes of four
 // elements, the pieces dealt to 1024 / D groups of lanes, whose sums are joined in their order. Every partial result is read once; rows
@@ -28,16 +32,19 @@ __global__ __launch_bounds__(THREADS) void attn_join_kernel(AttnArgs a, int RT, 
   const float* first = a.part + (size_t)n0 * size;
   const int4 head = *(const int4*)first;
   const long long srow = (long long)t * a.G + g;
-  // the partial result of piece p: of its row, the maximum; the sum lies RT behind it, the elements from 2 RT on. (The prefix's pieces and the
+  // the partial result of piece p: of its row, the maximum; the sum lies a tile's rows behind it, the elements from two on. (The prefix's pieces and the
   // first one are known without the slot's words.)
-  const float* sfirst = a.shared_part + (size_t)(h * a.shared_tiles + srow / RT) * a.shared * size + 4;
+  const int srt = a.shared_rt;
+  const size_t ssize = slot_floats(srt, D);
+  const float* sfirst = a.shared_part + (size_t)(h * a.shared_tiles + srow / srt) * a.shared * ssize + 4;
   const auto slot = [&](int p) -> const float* {
-    if (p < a.shared) return sfirst + (size_t)p * size;
+    if (p < a.shared) return sfirst + (size_t)p * ssize;
     if (p == a.shared) return first + 4;
     const long long n = ((long long)head.y + (long long)(p - a.shared - 1) * head.z) * a.kv.HK + h;
     return (n < a.slots ? a.part + (size_t)n * size : first) + 4;
   };
-  const auto row_of = [&](int p) { return p < a.shared ? (int)(srow % RT) : r0 % RT; };
+  const auto row_of = [&](int p) { return p < a.shared ? (int)(srow % srt) : r0 % RT; };
+  const auto tile_of = [&](int p) { return p < a.shared ? srt : RT; };
   const int lanes = D / 4, groups = THREADS / lanes, group = tid / lanes, d = 4 * (tid % lanes);
   float l = 0.0f, top = -__builtin_inff();
   float4 o = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -52,11 +59,11 @@ __global__ __launch_bounds__(THREADS) void attn_join_kernel(AttnArgs a, int RT, 
     float4 v[kAhead];
     const auto ask = [&](int i, int from) {
       const int p = p0 + min(group + (from + i) * groups, n - 1);
-      v[i] = *(const float4*)(slot(p) + 2 * RT + (size_t)row_of(p) * D + d);
+      v[i] = *(const float4*)(slot(p) + 2 * tile_of(p) + (size_t)row_of(p) * D + d);
     };
     const bool in = tid < n;
     const float* s = slot(p0 + (in ? tid : 0)) + row_of(p0 + (in ? tid : 0));
-    const float m = s[0], w = in ? s[RT] : 0.0f;
+    const float m = s[0], w = in ? s[tile_of(p0 + tid)] : 0.0f;
     if (group < groups) {
 #pragma unroll
       for (int i = 0; i < kAhead; ++i)
@@ -135,17 +142,19 @@ __global__ __launch_bounds__(THREADS) void attn_join_kernel(AttnArgs a, int RT, 
 
 namespace {
 
-constexpr int kTarget = 512;        // pieces that a call is cut into
+constexpr int kTarget = 512;         // pieces that a call is cut into: two work-groups a CU
 constexpr int kSharedTarget = 256;   // pieces of the shared prefix
 constexpr int kSharedFrom = 256;     // a shorter prefix is read with each sequence's own keys
+constexpr int kTileFrom = 64;        // rows of a key head from which attn_tile_kernel takes them
 
-// Row tiles of 16 a work-group: what its registers hold
-int tiles_for(long long rows, int D) {
-  const int most = D <= 64 ? 4 : D <= 128 ? 2 : 1;
-  const int want = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
+long long div_up(long long a, long long b) { return (a + b - 1) / b; }
+// Rows of a tile, for `rows` of a sequence on average (or of the batch): what attn_kernel's registers hold, or 64 and 128 of attn_tile_kernel
+int tile_rows(long long rows, int D, int* tile) {
+  *tile = rows >= kTileFrom;
+  if (*tile) return rows > 64 && D <= 128 ? 128 : 64;
+  const int most = D <= 64 ? 64 : D <= 128 ? 32 : 16, want = rows <= 16 ? 16 : rows <= 32 ? 32 : 64;
   return want < most ? want : most;
 }
-long long div_up(long long a, long long b) { return (a + b - 1) / b; }
 // Row tiles of all sequences at most
 long long row_tiles(int T, int B, bool start, int G, int rt) {
   return start ? (long long)T * G / rt + B : B * div_up(G, rt);  // (as first_slot counts them)
@@ -153,34 +162,35 @@ long long row_tiles(int T, int B, bool start, int G, int rt) {
 
 }  // namespace
 
-size_t attn_slot_bytes(int mt, int D) { return (4 + (size_t)16 * mt * (D + 2)) * sizeof(float); }
-
-static size_t shared_slots(const AttnPlan& p, int HK) { return (size_t)HK * p.shared_tiles * p.shared; }
+static size_t slot_bytes(int rt, int D) { return (4 + (size_t)rt * (D + 2)) * sizeof(float); }
+static size_t shared_bytes(const AttnPlan& p, int HK, int D) { return p.shared ? (size_t)HK * p.shared_tiles * p.shared * slot_bytes(p.shared_rt, D) : 0; }
 static unsigned shared_grid(const AttnPlan& p, int HK) { return (unsigned)(div_up((long long)HK * p.shared, 8) * 8 * p.shared_tiles); }
 
-AttnPlan attn_plan(int T, int B, bool start, int HQ, int HK, int D, int prefix_len, size_t ws_bytes) {
+size_t attn_used_bytes(const AttnPlan& p, int HK, int D) { return shared_bytes(p, HK, D) + p.slots * slot_bytes(p.rt, D); }
+
+AttnPlan attn_plan(int T, int B, bool start, bool chosen, int HQ, int HK, int D, int prefix_len, size_t ws_bytes) {
   const int G = HQ / HK;
   const long long rows = start ? div_up(T, B < T ? B : T) * G : G;  // of a sequence, on average
   const size_t have = ws_bytes / 256 * 256;
   AttnPlan p{};
-  if (prefix_len >= kSharedFrom && B > 1 && T > 1 && rows < 64) {
-    // (one size of row tile for both: the batch's rows fill it, and a sequence's own keys take no longer for it)
-    p.mt = tiles_for((long long)T * G, D);
-    p.shared_tiles = (int)div_up((long long)T * G, 16 * p.mt);
+  p.rt = tile_rows(chosen && rows >= kTileFrom ? kTileFrom - 1 : rows, D, &p.tile);  // (chosen pages are a row's own: never many rows)
+  const AttnPlan alone = p;
+  if (prefix_len >= kSharedFrom && B > 1 && T > 1 && !p.tile) {
+    p.shared_rt = tile_rows((long long)T * G, D, &p.shared_tile);
+    if (!p.shared_tile) p.rt = p.shared_rt;  // (one launch for both: the batch's rows fill the tile, and a sequence's own keys take no longer for it)
+    p.shared_tiles = (int)div_up((long long)T * G, p.shared_rt);
     const int blocks = (int)div_up(prefix_len, 128);
     long long n = kSharedTarget / ((long long)HK * p.shared_tiles);
     if (n > blocks) n = blocks;
     if (n < 1) n = 1;
     p.shared_blocks = (int)div_up(blocks, n);
     p.shared = (int)div_up(blocks, p.shared_blocks);
-    const long long items = row_tiles(T, B, start, G, 16 * p.mt) * HK;
-    if ((shared_slots(p, HK) + items) * attn_slot_bytes(p.mt, D) > have) p = AttnPlan{};
+    if (shared_bytes(p, HK, D) + row_tiles(T, B, start, G, p.rt) * HK * slot_bytes(p.rt, D) > have) p = alone;
   }
-  if (!p.shared) p.mt = tiles_for(rows, D);
-  const long long items = row_tiles(T, B, start, G, 16 * p.mt) * HK;
-  const long long left = (long long)(have / attn_slot_bytes(p.mt, D)) - (long long)shared_slots(p, HK) - items;
+  const long long items = row_tiles(T, B, start, G, p.rt) * HK;
+  const long long left = ((long long)have - (long long)shared_bytes(p, HK, D)) / (long long)slot_bytes(p.rt, D) - items;
   // (pieces of all row tiles are at most the target and one more for each of them; row tiles that fill the chip are left whole)
-  if (left > 0 && items < (rows < 64 ? 2 * kTarget : kTarget / 2)) p.target = (int)(left < kTarget ? left : kTarget);
+  if (left > 0 && items < (p.tile ? kTarget / 2 : 2 * kTarget)) p.target = (int)(left < kTarget ? left : kTarget);
   p.slots = p.target || p.shared ? (int)(items + p.target) : 0;
   p.firsts = (int)(items / HK);
   return p;
@@ -188,18 +198,15 @@ AttnPlan attn_plan(int T, int B, bool start, int HQ, int HK, int D, int prefix_l
 
 size_t attn_workspace_bytes(int T, int B, int HQ, int HK, int D, int prefix_len) {
   size_t most = 0;
-  for (int start = 0; start < 2; ++start) {
-    const AttnPlan p = attn_plan(T, B, start, HQ, HK, D, prefix_len, (size_t)1 << 62);
-    const size_t n = attn_used_bytes(p, HK, D);
+  for (int mode = 0; mode < 3; ++mode) {  // a row a sequence, rows of the caller's, chosen pages
+    const size_t n = attn_used_bytes(attn_plan(T, mode == 2 ? T : B, mode == 1, mode == 2, HQ, HK, D, mode == 2 ? 0 : prefix_len, (size_t)1 << 60), HK, D);
     if (n > most) most = n;
   }
   return (most + 255) / 256 * 256;
 }
 
-size_t attn_used_bytes(const AttnPlan& p, int HK, int D) { return (p.slots + shared_slots(p, HK)) * attn_slot_bytes(p.mt, D); }
-
 long long attn_grid(const AttnPlan& p, int T, int B, bool start, int HQ, int HK) {
-  const long long own = p.slots ? p.slots : row_tiles(T, B, start, HQ / HK, 16 * p.mt) * HK;
+  const long long own = p.slots ? p.slots : row_tiles(T, B, start, HQ / HK, p.rt) * HK;
   const long long grid = own + (p.shared ? shared_grid(p, HK) : 0), join = p.slots ? (long long)T * HQ : 0;
   const long long most = grid > join ? grid : join;
   return most * 256 <= kMostThreads ? most : 0;
@@ -207,7 +214,13 @@ long long attn_grid(const AttnPlan& p, int T, int B, bool start, int HQ, int HK)
 
 namespace {
 
-hipError_t attn_any(const AttnArgs& a, int mt, unsigned grid, hipStream_t s) {
+hipError_t attn_any(const AttnArgs& a, int rt, int tile, unsigned grid, hipStream_t s) {
+  if (tile) {
+    const int mt = rt / 64;
+    if (a.kv.type == DT_E4M3) return a.qtype == DT_F16 ? attn_tile_f16_e4m3(a, mt, grid, s) : attn_tile_bf16_e4m3(a, mt, grid, s);
+    return a.qtype == DT_F16 ? attn_tile_f16(a, mt, grid, s) : attn_tile_bf16(a, mt, grid, s);
+  }
+  const int mt = rt / 16;
   if (a.kv.type == DT_E4M3) return a.qtype == DT_F16 ? attn_f16_e4m3(a, mt, grid, s) : attn_bf16_e4m3(a, mt, grid, s);
   return a.qtype == DT_F16 ? attn_f16(a, mt, grid, s) : attn_bf16(a, mt, grid, s);
 }
@@ -220,9 +233,11 @@ hipError_t launch_attn(const AttnArgs& args, const AttnPlan& p, hipStream_t s) {
   a.slots = p.slots;
   a.firsts = p.firsts;
   a.shared_grid = a.shared = 0;
-  long long grid = p.slots ? p.slots : row_tiles(a.s.T, a.s.B, a.s.start != nullptr, a.G, 16 * p.mt) * a.kv.HK;
+  a.shared_rt = p.rt;
+  int tile = p.tile;
+  long long grid = p.slots ? p.slots : row_tiles(a.s.T, a.s.B, a.s.start != nullptr, a.G, p.rt) * a.kv.HK;
   if (a.sel) {  // as many pieces for every token: the target's, within the slots
-    const long long items = (long long)a.s.T * div_up(a.G, 16 * p.mt) * a.kv.HK, blocks = div_up((long long)a.k * a.kv.page, 128);
+    const long long items = (long long)a.s.T * div_up(a.G, p.rt) * a.kv.HK, blocks = div_up((long long)a.k * a.kv.page, 128);
     long long n = p.slots / items;
     if (n > blocks) n = blocks;
     if (n < 1) n = 1;
@@ -233,18 +248,25 @@ hipError_t launch_attn(const AttnArgs& args, const AttnPlan& p, hipStream_t s) {
   } else if (p.shared) {
     a.shared_grid = (int)shared_grid(p, a.kv.HK);
     a.shared = p.shared;
+    a.shared_rt = p.shared_rt;
     a.shared_tiles = p.shared_tiles;
     a.shared_blocks = p.shared_blocks;
     a.shared_part = a.part;
-    a.part += shared_slots(p, a.kv.HK) * (attn_slot_bytes(p.mt, a.kv.D) / sizeof(float));
-    grid += a.shared_grid;
+    a.part += shared_bytes(p, a.kv.HK, a.kv.D) / sizeof(float);
+    if (p.shared_tile) {
+      const hipError_t e = attn_any(a, p.shared_rt, 1, (unsigned)a.shared_grid, s);
+      if (e != hipSuccess) return e;
+      a.shared_grid = 0;
+    } else {
+      grid += a.shared_grid;
+    }
   }
-  const hipError_t e = attn_any(a, p.mt, (unsigned)grid, s);
+  const hipError_t e = attn_any(a, p.rt, tile, (unsigned)grid, s);
   if (e != hipSuccess || !a.slots) return e;
   // (a wave a row where there are rows enough: work-groups of four waves, most of which have nothing to do, take longer to start than that)
   const long long rows = (long long)a.s.T * a.HQ;
-  if (rows >= 1024) attn_join_kernel<64><<<(unsigned)rows, 64, 0, s>>>(a, 16 * p.mt, a.sel ? 1 : 0);
-  else attn_join_kernel<256><<<(unsigned)rows, 256, 0, s>>>(a, 16 * p.mt, a.sel ? 1 : 0);
+  if (rows >= 1024) attn_join_kernel<64><<<(unsigned)rows, 64, 0, s>>>(a, p.rt, a.sel ? 1 : 0);
+  else attn_join_kernel<256><<<(unsigned)rows, 256, 0, s>>>(a, p.rt, a.sel ? 1 : 0);
   return hipGetLastError();
 }
 

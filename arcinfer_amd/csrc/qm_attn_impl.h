@@ -39,11 +39,13 @@ __device__ __forceinline__ void with_other(float v, float& a, float& b) {
   a = __builtin_bit_cast(float, r0);
   b = __builtin_bit_cast(float, r1);
 }
+// The larger one (NaN if one is: its row's result is)
+__device__ __forceinline__ float larger(float a, float b) { return __builtin_elementwise_maximum(a, b); }
 __device__ __forceinline__ float max_groups(float v) {  // of the four lanes that hold a row
   float a, b;
   with_other<16>(v, a, b);
-  with_other<32>(fmaxf(a, b), a, b);
-  return fmaxf(a, b);
+  with_other<32>(larger(a, b), a, b);
+  return larger(a, b);
 }
 __device__ __forceinline__ float sum_groups(float v) {
   float a, b;
@@ -64,8 +66,19 @@ __device__ __forceinline__ int pack2(float x, float y) {
 }
 template <typename T>
 __device__ __forceinline__ float part_of(int w, int i) {
-  typedef T v2t __attribute__((ext_vector_type(2)));
-  return (float)__builtin_bit_cast(v2t, w)[i];
+  if constexpr (__is_same(T, _Float16)) return (float)__builtin_bit_cast(v2h, w)[i];
+  else return __builtin_bit_cast(float, i ? w & (int)0xFFFF0000 : w << 16);
+}
+// Two weights as PARTS words of two values: rounded, and what each rounding left
+template <typename T, int PARTS, typename F>
+__device__ __forceinline__ void in_parts(float x, float y, F put) {
+#pragma unroll
+  for (int n = 0; n < PARTS; ++n) {
+    const int w = pack2<T>(x, y);
+    put(n, w);
+    x -= part_of<T>(w, 0);
+    y -= part_of<T>(w, 1);
+  }
 }
 // Two e4m3 values (bytes 2 HI, 2 HI + 1 of w) as T, exact
 template <typename T, bool HI>
@@ -212,7 +225,7 @@ __global__ __launch_bounds__(256, 2) void attn_kernel(AttnArgs a) {
   }
 
   // blocks of 32 keys: of the prefix, then of the sequence's own (or of the chosen pages)
-  const int shared_blocks32 = CHOSEN || (a.shared_grid && !shared) ? 0 : (a.prefix_len + kBlock - 1) / kBlock;
+  const int shared_blocks32 = CHOSEN || (a.shared && !shared) ? 0 : (a.prefix_len + kBlock - 1) / kBlock;
   const int own_blocks = CHOSEN ? (int)(((long long)a.k * kv.page + kBlock - 1) / kBlock) : (int)(((long long)hi_lim + kBlock - 1) / kBlock);
   const int all_blocks = shared_blocks32 + own_blocks;
   const int begin = (int)min((long long)c * blocks * kWaves, (long long)all_blocks);
@@ -471,10 +484,7 @@ __global__ __launch_bounds__(256, 2) void attn_kernel(AttnArgs a) {
         if constexpr (E8) w[e] = x[e >> 2][m][e & 3] == kMinusInf ? 0.0f : w[e] * vs[e >> 2][e & 3];  // (a masked key's scale may be anything)
       }
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        p[0][m][e] = pack2<TP>(w[2 * e], w[2 * e + 1]);
-        if constexpr (PARTS == 2) p[1][m][e] = pack2<TP>(w[2 * e] - part_of<TP>(p[0][m][e], 0), w[2 * e + 1] - part_of<TP>(p[0][m][e], 1));
-      }
+      for (int e = 0; e < 4; ++e) in_parts<TP, PARTS>(w[2 * e], w[2 * e + 1], [&](int n, int v) { p[n][m][e] = v; });
     }
 
     // V^T: the operands of results (vb, 2 w) and (vb, 2 w + 1)
@@ -616,7 +626,7 @@ __global__ __launch_bounds__(256, 2) void attn_kernel(AttnArgs a) {
   }
 
   const int all_pieces = CHOSEN ? a.pieces : ((all_blocks + kWaves - 1) / kWaves + blocks - 1) / blocks;
-  const bool split = a.shared_grid > 0 || all_pieces > 1;
+  const bool split = a.shared > 0 || all_pieces > 1;
   float* slot = nullptr;
   if (shared) {
     slot = a.shared_part + ((size_t)(h * a.shared_tiles + rt) * a.shared + c) * slot_floats(RT, kv.D);

@@ -25,11 +25,12 @@ hipError_t attn_parts(const AttnArgs& a, int mt, unsigned grid, hipStream_t s) {
   return attn_mode<TQ, TC, 256, 1, PARTS>(a, grid, s);
 }
 
-// Two parts of P where the result keeps more bits than one: f32, or f16 behind an 8-bit cache (P is bf16 there)
+// Parts of P by the bits that the result keeps: f16 behind an 8-bit cache (P is bf16 there) two; f32 two of f16, three of bf16 (two would
+// leave 2^-18 of a weight: 2.4e-6 of the result, where f32 sums leave 1e-6)
 template <typename TQ, typename TC>
 hipError_t attn_types(const AttnArgs& a, int mt, unsigned grid, hipStream_t s) {
-  if constexpr (sizeof(TC) == 1 && __is_same(TQ, _Float16)) return attn_parts<TQ, TC, 2>(a, mt, grid, s);
-  else return a.otype == DT_F32 ? attn_parts<TQ, TC, 2>(a, mt, grid, s) : attn_parts<TQ, TC, 1>(a, mt, grid, s);
+  if constexpr (sizeof(TC) == 1 && __is_same(TQ, _Float16)) return a.otype == DT_F32 ? attn_parts<TQ, TC, 3>(a, mt, grid, s) : attn_parts<TQ, TC, 2>(a, mt, grid, s);
+  else return a.otype == DT_F32 ? attn_parts<TQ, TC, sizeof(TC) == 2 && __is_same(TQ, _Float16) ? 2 : 3>(a, mt, grid, s) : attn_parts<TQ, TC, 1>(a, mt, grid, s);
 }
 
 }  // namespace qm

@@ -36,7 +36,7 @@ __device__ __forceinline__ int sequence_of(const Seqs& s, int t) {
 // Blocks of 128 keys of sequence b, the prefix in front of them (below 2^25: a prefix and a table hold 2^30 keys each)
 __device__ __forceinline__ int blocks_of(const AttnArgs& a, int b) {
   const int most = a.s.W << a.kv.lg, n = min(max(a.s.len[b], 0), most);
-  return (int)(((unsigned)(n + 31) / 32 + (a.shared_grid ? 0u : (unsigned)(a.prefix_len + 31) / 32) + 3) / 4);
+  return (int)(((unsigned)(n + 31) / 32 + (a.shared ? 0u : (unsigned)(a.prefix_len + 31) / 32) + 3) / 4);
 }
 
 // The place of the result of row tile rt's first piece among the slots (of a head): row tiles of RT rows, of a sequence whose rows begin at

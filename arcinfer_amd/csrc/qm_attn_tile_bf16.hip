@@ -1,0 +1,6 @@
+// Attention of many rows over a paged cache: q of bf16, the cache too (qm_attn_tile.h)
+#include "qm_attn_tile_launch.h"
+
+namespace qm {
+hipError_t attn_tile_bf16(const AttnArgs& a, int mt, unsigned grid, hipStream_t s) { return tile_types<__bf16, __bf16>(a, mt, grid, s); }
+}  // namespace qm

@@ -48,20 +48,19 @@ struct AttnArgs {
   int target, slots;    // pieces that are aimed at (0: whole row tiles), and partial results that `part` holds, those of
   int firsts;           // first pieces (of a head) in front
   int pieces, blocks;   // chosen pages: pieces of a row tile, and blocks of 128 keys of one
-  // The prefix for the rows of the whole batch (shared_grid work-groups in front of the others; 0: it is read with each sequence's own keys):
-  // pieces of `shared_blocks` blocks of 128 keys, `shared` of them, for each of shared_tiles row tiles of a key head; slot
+  // The prefix for the rows of the whole batch (shared pieces; 0: it is read with each sequence's own keys), by shared_grid work-groups in front
+  // of the launch's others: pieces of shared_blocks blocks of 128 keys for each of shared_tiles tiles of shared_rt rows of a key head; slot
   // (head * shared_tiles + tile) * shared + piece
   float* shared_part;
-  int shared_grid, shared, shared_tiles, shared_blocks;
+  int shared_grid, shared, shared_rt, shared_tiles, shared_blocks;
 };
 
-// How a call runs: row tiles of 16 mt; pieces and blocks as in AttnArgs
+// How a call runs: tiles of rt rows (16 to 64: attn_kernel; more, or `tile`: attn_tile_kernel); pieces and blocks as in AttnArgs
 struct AttnPlan {
-  int mt, target, slots, firsts;            // target 0: nothing is split
-  int shared, shared_tiles, shared_blocks;  // shared 0: the prefix is read with each sequence's own keys
+  int rt, tile, target, slots, firsts;                              // target 0: nothing is split
+  int shared, shared_rt, shared_tile, shared_tiles, shared_blocks;  // shared 0: the prefix is read with each sequence's own keys
 };
-size_t attn_slot_bytes(int mt, int D);
-AttnPlan attn_plan(int T, int B, bool start, int HQ, int HK, int D, int prefix_len, size_t ws_bytes);
+AttnPlan attn_plan(int T, int B, bool start, bool chosen, int HQ, int HK, int D, int prefix_len, size_t ws_bytes);
 size_t attn_used_bytes(const AttnPlan& p, int HK, int D);
 size_t attn_workspace_bytes(int T, int B, int HQ, int HK, int D, int prefix_len);
 // Work-groups of the calls's launches at most (0: more than a grid holds)

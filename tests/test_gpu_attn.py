@@ -302,6 +302,131 @@ def test_caches_past_32_bit_offsets(qm, dev):
     K.check(got, *K.attention(q, small, torch.tensor([0, 1]), ln, torch.tensor([[0, 1, 2, 3]], dtype=torch.int32), BF16), BF16)
 
 
+# ---- many rows: prompts, and a prefix for the rows of a large batch
+@pytest.mark.parametrize("out", [None, F32])
+@pytest.mark.parametrize("qt,ct", KINDS)
+@pytest.mark.parametrize("D,page", [(16, 16), (64, 64), (80, 16), (128, 32), (144, 16), (192, 128), (256, 16)])
+def test_many_rows(qm, dev, D, page, qt, ct, out):
+    """Prompts from their first token and behind others, one token among them; tiles that end inside a token's heads; whole and in pieces."""
+    for ws in (True, False):
+        run(qm, dev, [90, 64, 1, 333], [90, 40, 1, 70], 6, 2, D, page, qt, ct, out=out, ws=ws, seed=D)
+
+
+@pytest.mark.parametrize("prefix_len", [1, 33, 100, 300])
+@pytest.mark.parametrize("qt,ct", KINDS)
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_many_rows_behind_a_prefix(qm, dev, D, qt, ct, prefix_len):
+    run(qm, dev, [70, 5], [70, 1], 5, 1, D, 16, qt, ct, prefix_len=prefix_len, seed=prefix_len)
+    run(qm, dev, [66], [65], 2, 2, D, 32, qt, ct, prefix_len=prefix_len, seed=prefix_len, ws=False)
+
+
+@pytest.mark.parametrize("qt,ct", KINDS)
+@pytest.mark.parametrize("D", [64, 80, 128, 256])
+def test_prefix_of_a_large_batch(qm, dev, D, qt, ct):
+    """64 rows of a key head and more: the prefix by their tiles, the sequences' own keys by themselves."""
+    lens = [1 + 7 * i % 90 for i in range(30)]
+    for out, n in ((None, 256), (F32, 700), (None, 1111)):
+        run(qm, dev, lens, [1] * 30, 10, 2, D, 16, qt, ct, out=out, prefix_len=n, seed=n)
+    run(qm, dev, lens[:23], [min(n, 3) for n in lens[:23]], 2, 2, D, 32, qt, ct, prefix_len=300, seed=1)
+
+
+@pytest.mark.parametrize("rows", [63, 64, 65, 127, 128, 129, 257])
+def test_around_tiles(qm, dev, rows):
+    for D in (64, 128, 192):
+        run(qm, dev, [rows + 3], [rows], 1, 1, D, 16, BF16, BF16, seed=rows)
+        run(qm, dev, [5000], [rows], 1, 1, D, 64, F16, F16, seed=rows)
+
+
+@pytest.mark.parametrize("ct", [BF16, E4M3])
+@pytest.mark.parametrize("order,pad", [((0, 2, 1), 0), ((1, 0, 2), 16)])
+def test_many_rows_strides(qm, dev, order, pad, ct):
+    run(qm, dev, [150, 3, 129], [90, 3, 100], 4, 2, 80, 32, BF16, ct, order=order, pad=pad)
+
+
+@pytest.mark.parametrize("ct", [BF16, F16, E4M3])
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
+def test_many_rows_masked_places(qm, dev, bad, D, ct):
+    """NaN and infinities where no row sees them, and values of them that some of a tile's rows see and others do not."""
+    cache = K.Cache(40, 1, 16, D, ct, 7)
+    start, ln, table, rest = K.batch([137, 90], [70, 60], 16, 40, 7)
+    prefix = torch.tensor(rest[:5], dtype=torch.int32)
+    qt = BF16 if ct == E4M3 else ct
+    q = queries(130, 2, D, qt, 8)
+    want, bound = K.attention(q, cache, start, ln, table, qt, None, prefix, 77)
+    put = lambda t, at, val: t.view(torch.uint8).__setitem__(at, 0x7F) if ct == E4M3 else t.__setitem__(at, val)  # noqa: E731
+    for t in cache.data:
+        for b, n in enumerate(ln.tolist()):
+            put(t, (int(table[b, n // 16]), slice(None), slice(n % 16, 16)), bad)
+        put(t, (rest[4], slice(None), slice(77 - 64, 16)), bad)
+        for p in rest[5:]:
+            put(t, p, bad)
+    kv = cache.on(qm, dev)
+    more = dict(start=start.to(dev), prefix=prefix.to(dev), prefix_len=77)
+    both = (None, qm.attn_workspace(kv, 130, 2, 2, 77))
+    for ws in both:
+        K.check(qm.attn_prefix(q.to(dev), kv, ln.to(dev), table.to(dev), ws=ws, **more), want, bound, qt)
+    # values of the first sequence's tokens 100 and 118: its rows are tokens 67 to 136
+    for token, d in ((100, 5), (118, D - 1)):
+        put(cache.data[1], (int(table[0, token // 16]), 0, token % 16, d), bad)
+    kv = cache.on(qm, dev)
+    for ws in both:
+        got = qm.attn_prefix(q.to(dev), kv, ln.to(dev), table.to(dev), ws=ws, **more).cpu()
+        hit = torch.zeros((130, 2, D), dtype=torch.bool)
+        hit[100 - 67:70, :, 5] = True
+        hit[118 - 67:70, :, D - 1] = True
+        assert not torch.isfinite(got[hit].float()).any()
+        assert ct == E4M3 or torch.equal(got[hit], torch.full_like(got[hit], bad)) or math.isnan(bad)
+        K.check(torch.where(hit, want.to(qt), got), want, bound, qt)
+
+
+def test_many_rows_bad_pages(qm, dev):
+    cache = K.Cache(10, 2, 16, 128, BF16, 9)
+    table = torch.tensor([[1, -1, 3, 2 ** 31 - 1, 4, 5], [10, 4, -2 ** 31, 5, 6, 7]], dtype=torch.int32)
+    ln = torch.tensor([90, 2 ** 31 - 1], dtype=torch.int32)
+    start = torch.tensor([0, 100, 150], dtype=torch.int32)  # (ten rows of the first sequence see none of its keys)
+    prefix = torch.tensor([7, -1, 8, 10], dtype=torch.int32)
+    q = queries(152, 2, 128, BF16, 10)
+    kv = cache.on(qm, dev)
+    for ws in (None, qm.attn_workspace(kv, 152, 2, 2, 60)):
+        for n in (0, 60):
+            o = torch.full((152, 2, 128), 4.0, dtype=BF16, device=dev)
+            qm.attn_prefix(q.to(dev), kv, ln.to(dev), table.to(dev), start=start.to(dev), ws=ws, prefix=prefix.to(dev) if n else None, prefix_len=n, o=o)
+            want, bound = K.attention(q, cache, start, ln, table, BF16, None, prefix if n else (), n)
+            K.check(o[:150], want[:150], bound[:150], BF16)
+            assert bool((o[150:] == 4).all()) and (n or not o[:10].any())
+
+
+def test_many_rows_replayed(qm, dev):
+    """A captured prompt and a captured decode step of a large batch behind a prefix, replayed with other lengths."""
+    cache = K.Cache(90, 1, 16, 64, BF16, 11)
+    kv = cache.on(qm, dev)
+    pages = torch.randperm(89, generator=torch.Generator().manual_seed(3)).to(torch.int32)
+    table = pages[20:80].reshape(30, 2).contiguous()
+    start = torch.tensor([0, 70], dtype=torch.int32)
+    calls = []
+    for lens, st, n, tab, rows in ((torch.tensor([90]), start, 0, pages[:8].reshape(1, 8).contiguous(), 70), (torch.arange(30) % 20 + 1, None, 290, table, 30)):
+        q = queries(rows, 4, 64, BF16, n)
+        ld = lens.to(torch.int32).to(dev)
+        ws, o = qm.attn_workspace(kv, rows, len(lens), 4, n), torch.empty((rows, 4, 64), dtype=BF16, device=dev)
+        kw = dict(start=None if st is None else st.to(dev), prefix=pages[:19].to(dev) if n else None, prefix_len=n)
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        qd, td = q.to(dev), tab.to(dev)
+        with torch.cuda.graph(g):
+            qm.attn_prefix(qd, kv, ld, td, o=o, ws=ws, **kw)
+        calls.append((q, ld, tab, st, n, o, g, qd, td, kw, ws))
+    for step in range(3):
+        for q, ld, tab, st, n, o, g, qd, td, kw, ws in calls:
+            ld.add_(4)
+            g.replay()
+            eager = qm.attn_prefix(qd, kv, ld, td, ws=qm.attn_workspace(kv, q.shape[0], len(ld), 4, n), **kw)
+            torch.cuda.synchronize()
+            assert torch.equal(o, eager)
+            st = torch.arange(q.shape[0] + 1) if st is None else st
+            K.check(o, *K.attention(q, cache, st, ld.cpu(), tab, BF16, None, pages[:19] if n else (), n), BF16)
+
+
 # ---- chosen pages
 @pytest.mark.parametrize("ws", [True, False])
 @pytest.mark.parametrize("qt,ct", KINDS)
