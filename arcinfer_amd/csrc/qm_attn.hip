@@ -17,6 +17,14 @@ hipError_t attn_tile_f16_e4m3(const AttnArgs& a, int mt, unsigned grid, hipStrea
 // of a single piece are left as attn_kernel wrote them. What a row needs to know of the split stands in its tile's first slot.
 // Latency-bound: a launch, that slot's words, then the pieces' maxima and sums and kAhead results of each group at once.
 constexpr int kAhead = 8;
+__device__ __forceinline__ void store4(const AttnArgs& a, size_t to, const float (&y)[4]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if (a.otype == DT_F32) ((float*)a.o)[to + i] = y[i];
+    else if (a.otype == DT_F16) ((_Float16*)a.o)[to + i] = (_Float16)y[i];
+    else ((__bf16*)a.o)[to + i] = (__bf16)y[i];
+  }
+}
 template <int THREADS>
 __global__ __launch_bounds__(THREADS) void attn_join_kernel(AttnArgs a, int RT, int chosen) {
   constexpr int kWavesHere = THREADS / 64;
@@ -131,12 +139,48 @@ __global__ __launch_bounds__(THREADS) void attn_join_kernel(AttnArgs a, int RT, 
   }
   const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;  // (a row that sees no key is zeros)
   const float y[4] = {o.x * inv, o.y * inv, o.z * inv, o.w * inv};
-  const size_t to = (size_t)t * a.ldo + (size_t)hq * D + d;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    if (a.otype == DT_F32) ((float*)a.o)[to + i] = y[i];
-    else if (a.otype == DT_F16) ((_Float16*)a.o)[to + i] = (_Float16)y[i];
-    else ((__bf16*)a.o)[to + i] = (__bf16)y[i];
+  store4(a, (size_t)t * a.ldo + (size_t)hq * D + d, y);
+}
+
+// Joins the pieces of the row tiles that were cut behind the last whole round: 16 rows a work-group, D / 4 lanes of four elements a row. Pieces are
+// few (2 to 32): their maxima first, then results and sums.
+constexpr int kTailRows = 16;
+__global__ __launch_bounds__(256) void attn_tail_join_kernel(AttnArgs a, int RT) {
+  const int chunks = RT / kTailRows, j = blockIdx.x / chunks, D = a.kv.D;
+  const Tail t = tail_of(a, RT);
+  Item it;
+  if (j >= t.tail || !find_item(a, RT, t.whole + j, it)) return;
+  const int row0 = row_from(a.s, it.b), rows = rows_of(a.s, it.b), blocks = tile_blocks(a, RT, it.b, it.rt, rows);
+  const int size = part_blocks(blocks, t.parts), pieces = (blocks + size - 1) / size;
+  if (pieces <= 1) return;  // (attn_tile_kernel wrote the result)
+  const int lanes = D / 4, per = 256 / lanes, d = 4 * (threadIdx.x % lanes), from = blockIdx.x % chunks * kTailRows;
+  if ((int)threadIdx.x / lanes >= per) return;
+  const size_t floats = slot_floats(RT, D);
+  for (int r = from + threadIdx.x / lanes; r < from + kTailRows; r += per) {
+    const int row = it.rt * RT + r;
+    if (row >= rows * a.G) return;
+    const float* s = a.part + (size_t)j * floats + 4 + r;
+    const size_t step = (size_t)t.tail * floats;
+    float top = -__builtin_inff();
+    for (int p = 0; p < pieces; ++p)
+      if (s[p * step + RT] != 0.0f) top = fmaxf(top, s[p * step]);  // (a piece that the row sees nothing of has the sum 0)
+    float l = 0.0f;
+    float4 o = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (int p = 0; p < pieces; ++p) {
+      const float w = s[p * step + RT];
+      if (w == 0.0f) continue;
+      const float f = __builtin_amdgcn_exp2f(s[p * step] - top);
+      const float4 v = *(const float4*)(s + p * step - r + 2 * RT + (size_t)r * D + d);
+      l = fmaf(f, w, l);
+      o.x = fmaf(f, v.x, o.x);
+      o.y = fmaf(f, v.y, o.y);
+      o.z = fmaf(f, v.z, o.z);
+      o.w = fmaf(f, v.w, o.w);
+    }
+    const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
+    const float y[4] = {o.x * inv, o.y * inv, o.z * inv, o.w * inv};
+    const size_t to = (size_t)(row0 + row / a.G) * a.ldo + (size_t)(it.h * a.G + row % a.G) * D + d;
+    store4(a, to, y);
   }
 }
 
@@ -145,12 +189,17 @@ namespace {
 constexpr int kTarget = 512;         // pieces that a call is cut into: two work-groups a CU
 constexpr int kSharedTarget = 256;   // pieces of the shared prefix
 constexpr int kSharedFrom = 256;     // a shorter prefix is read with each sequence's own keys
+constexpr int kTailMost = 4;          // rounds of work-groups from which the last one is not worth cutting
 constexpr int kTileFrom = 64;        // rows of a key head from which attn_tile_kernel takes them
+// Products of a prefix (rows of all heads times keys times D) from which they are attn_tile_kernel's, in a launch of its own: below, attn_kernel's tiles in the
+// sequences' own launch take less. 8 heads of 128, rows of a head x keys, us: 192 x 2048 31 against 21, 192 x 16384 45.7 against 44.0, 384 x 16384
+// 65 against 85, 768 x 16384 106 against 158; D 256, 384 x 8192: 68 against 99. Behind 8-bit caches 192 x 16384 54 against 46, 512 x 16384 89 against 92.
+constexpr double kSharedTileFrom = 3.2e9, kSharedTileFrom8 = 8e9;
 
 long long div_up(long long a, long long b) { return (a + b - 1) / b; }
 // Rows of a tile, for `rows` of a sequence on average (or of the batch): what attn_kernel's registers hold, or 64 and 128 of attn_tile_kernel
-int tile_rows(long long rows, int D, int* tile) {
-  *tile = rows >= kTileFrom;
+int tile_rows(long long rows, long long from, int D, int* tile) {
+  *tile = rows >= from;
   if (*tile) return rows > 64 && D <= 128 ? 128 : 64;
   const int most = D <= 64 ? 64 : D <= 128 ? 32 : 16, want = rows <= 16 ? 16 : rows <= 32 ? 32 : 64;
   return want < most ? want : most;
@@ -168,15 +217,16 @@ static unsigned shared_grid(const AttnPlan& p, int HK) { return (unsigned)(div_u
 
 size_t attn_used_bytes(const AttnPlan& p, int HK, int D) { return shared_bytes(p, HK, D) + p.slots * slot_bytes(p.rt, D); }
 
-AttnPlan attn_plan(int T, int B, bool start, bool chosen, int HQ, int HK, int D, int prefix_len, size_t ws_bytes) {
+AttnPlan attn_plan(int T, int B, bool start, bool chosen, bool e8, int HQ, int HK, int D, int prefix_len, size_t ws_bytes) {
   const int G = HQ / HK;
   const long long rows = start ? div_up(T, B < T ? B : T) * G : G;  // of a sequence, on average
   const size_t have = ws_bytes / 256 * 256;
   AttnPlan p{};
-  p.rt = tile_rows(chosen && rows >= kTileFrom ? kTileFrom - 1 : rows, D, &p.tile);  // (chosen pages are a row's own: never many rows)
+  p.rt = tile_rows(rows, chosen ? rows + 1 : kTileFrom, D, &p.tile);  // (chosen pages are a row's own: never many rows)
   const AttnPlan alone = p;
   if (prefix_len >= kSharedFrom && B > 1 && T > 1 && !p.tile) {
-    p.shared_rt = tile_rows((long long)T * G, D, &p.shared_tile);
+    const bool many = (double)T * HQ * prefix_len * D >= (e8 ? kSharedTileFrom8 : kSharedTileFrom);
+    p.shared_rt = tile_rows((long long)T * G, many ? kTileFrom : (long long)T * G + 1, D, &p.shared_tile);
     if (!p.shared_tile) p.rt = p.shared_rt;  // (one launch for both: the batch's rows fill the tile, and a sequence's own keys take no longer for it)
     p.shared_tiles = (int)div_up((long long)T * G, p.shared_rt);
     const int blocks = (int)div_up(prefix_len, 128);
@@ -192,21 +242,22 @@ AttnPlan attn_plan(int T, int B, bool start, bool chosen, int HQ, int HK, int D,
   // (pieces of all row tiles are at most the target and one more for each of them; row tiles that fill the chip are left whole)
   if (left > 0 && items < (p.tile ? kTarget / 2 : 2 * kTarget)) p.target = (int)(left < kTarget ? left : kTarget);
   p.slots = p.target || p.shared ? (int)(items + p.target) : 0;
+  if (p.tile && !p.slots && items < kTailMost * kTarget && kTarget * slot_bytes(p.rt, D) <= have) p.slots = p.tail = kTarget;
   p.firsts = (int)(items / HK);
   return p;
 }
 
-size_t attn_workspace_bytes(int T, int B, int HQ, int HK, int D, int prefix_len) {
+size_t attn_workspace_bytes(int T, int B, bool e8, int HQ, int HK, int D, int prefix_len) {
   size_t most = 0;
   for (int mode = 0; mode < 3; ++mode) {  // a row a sequence, rows of the caller's, chosen pages
-    const size_t n = attn_used_bytes(attn_plan(T, mode == 2 ? T : B, mode == 1, mode == 2, HQ, HK, D, mode == 2 ? 0 : prefix_len, (size_t)1 << 60), HK, D);
+    const size_t n = attn_used_bytes(attn_plan(T, mode == 2 ? T : B, mode == 1, mode == 2, e8, HQ, HK, D, mode == 2 ? 0 : prefix_len, (size_t)1 << 60), HK, D);
     if (n > most) most = n;
   }
   return (most + 255) / 256 * 256;
 }
 
 long long attn_grid(const AttnPlan& p, int T, int B, bool start, int HQ, int HK) {
-  const long long own = p.slots ? p.slots : row_tiles(T, B, start, HQ / HK, p.rt) * HK;
+  const long long own = p.slots && !p.tail ? p.slots : row_tiles(T, B, start, HQ / HK, p.rt) * HK + p.tail;
   const long long grid = own + (p.shared ? shared_grid(p, HK) : 0), join = p.slots ? (long long)T * HQ : 0;
   const long long most = grid > join ? grid : join;
   return most * 256 <= kMostThreads ? most : 0;
@@ -235,7 +286,8 @@ hipError_t launch_attn(const AttnArgs& args, const AttnPlan& p, hipStream_t s) {
   a.shared_grid = a.shared = 0;
   a.shared_rt = p.rt;
   int tile = p.tile;
-  long long grid = p.slots ? p.slots : row_tiles(a.s.T, a.s.B, a.s.start != nullptr, a.G, p.rt) * a.kv.HK;
+  a.tail = p.tail;
+  long long grid = p.slots && !p.tail ? p.slots : row_tiles(a.s.T, a.s.B, a.s.start != nullptr, a.G, p.rt) * a.kv.HK + p.tail;
   if (a.sel) {  // as many pieces for every token: the target's, within the slots
     const long long items = (long long)a.s.T * div_up(a.G, p.rt) * a.kv.HK, blocks = div_up((long long)a.k * a.kv.page, 128);
     long long n = p.slots / items;
@@ -263,6 +315,10 @@ hipError_t launch_attn(const AttnArgs& args, const AttnPlan& p, hipStream_t s) {
   }
   const hipError_t e = attn_any(a, p.rt, tile, (unsigned)grid, s);
   if (e != hipSuccess || !a.slots) return e;
+  if (a.tail) {
+    attn_tail_join_kernel<<<(unsigned)(a.tail / 2 * (p.rt / kTailRows)), 256, 0, s>>>(a, p.rt);
+    return hipGetLastError();
+  }
   // (a wave a row where there are rows enough: work-groups of four waves, most of which have nothing to do, take longer to start than that)
   const long long rows = (long long)a.s.T * a.HQ;
   if (rows >= 1024) attn_join_kernel<64><<<(unsigned)rows, 64, 0, s>>>(a, p.rt, a.sel ? 1 : 0);

@@ -172,7 +172,7 @@ __global__ __launch_bounds__(256, 2) void attn_kernel(AttnArgs a) {
 
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 15, g = lane >> 4;
   const KvView& kv = a.kv;
-  int h, b = 0, rt, c = 0, blocks = 0x7fffff00, row0 = 0, rows, after = 0;  // (after: tokens of the sequence behind these rows)
+  int h, b = 0, rt, c = 0, blocks = kWhole, row0 = 0, rows, after = 0;  // (after: tokens of the sequence behind these rows)
   int rts = 1, more = 0;
   const bool shared = !CHOSEN && (int)blockIdx.x < a.shared_grid;
   if constexpr (CHOSEN) {

@@ -9,6 +9,7 @@ namespace qm {
 constexpr int kWaves = 4;   // of a work-group
 constexpr int kBlock = 32;  // keys of a wave's step
 constexpr int kLeast = 1;   // blocks of 128 keys of a piece at least
+constexpr int kWhole = 1 << 30;  // and of one that is not cut (a row tile sees fewer than 2^25)
 
 // Rows of a sequence, clamped to the call's (device lists are not trusted with memory)
 __device__ __forceinline__ int row_from(const Seqs& s, int b) {
@@ -51,7 +52,19 @@ struct Item {
   int b, h, rt, c, rts;
   int blocks;  // blocks of 128 keys of a piece
   int more;
+  int parts, slot;  // of a row tile behind the last whole round: its pieces at most, and the place of this one's result (-1: not such a one)
 };
+
+// Row tiles of attn_tile_kernel that fill the GPU more than once are whole, but for those behind the last whole round of a.tail work-groups: they
+// would leave most CUs idle, and are cut into as many pieces as there is room for, which fill up what the round before them leaves.
+struct Tail {
+  int whole, tail, parts;
+};
+constexpr int kMostParts = 32;
+constexpr int kLeastPart = 4;  // blocks of 128 keys of such a piece at least: it has its start and a result to be joined
+
+// The sequence's row tiles and those of all
+__device__ __forceinline__ int tiles_of(const AttnArgs& a, int RT, int b) { return b < a.s.B ? (rows_of(a.s, b) * a.G + RT - 1) / RT : 0; }
 
 // Inclusive sums over the lanes of a wave, by moves within rows of 16 and from one row's end to the next (no LDS)
 template <int CTRL, int ROWS>
@@ -76,18 +89,45 @@ __device__ __forceinline__ float sum64(float v) {
   return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), 63));
 }
 
+__device__ __forceinline__ Tail tail_of(const AttnArgs& a, int RT) {
+  float all = 0.0f;  // (below 2^24: exact)
+  for (int b = threadIdx.x & 63; b < a.s.B; b += 64) all += (float)tiles_of(a, RT, b);
+  const int n = (int)sum64(all) * a.kv.HK, left = n % a.tail;
+  Tail t{n, 0, 1};
+  if (left && a.tail / left > 1) t = {n - left, left, min(a.tail / left, kMostParts)};
+  return t;
+}
+// Blocks of 128 keys that a row tile's last row sees (the prefix's among them, if it reads them), and of a piece of them
+__device__ __forceinline__ int tile_blocks(const AttnArgs& a, int RT, int b, int rt, int rows) {
+  const int last = min((rt + 1) * RT, rows * a.G) - 1, most = (int)min((long long)a.s.W << a.kv.lg, 0x7fffffffLL);
+  const int seen = min(max(a.s.len[b] - rows + last / a.G + 1, 0), most);
+  return (int)(((unsigned)(seen + kBlock - 1) / kBlock + (a.shared ? 0u : (unsigned)(a.prefix_len + kBlock - 1) / kBlock) + kWaves - 1) / kWaves);
+}
+__device__ __forceinline__ int part_blocks(int blocks, int parts) { return parts > 1 ? max((blocks + parts - 1) / parts, kLeastPart) : kWhole; }
+
 // Sequences are looked at 64 at a time by each wave for itself (no wave waits for another): the sum over all of them, then the scan that says
 // whose unit number this is. (A call's units and row tiles are below 2^24, as its grid is; sums over lists that are none may wrap.)
 __device__ __forceinline__ bool find_item(const AttnArgs& a, int RT, int unit, Item& out) {
   const int lane = threadIdx.x & 63, HK = a.kv.HK;
-  const auto tiles_of = [&](int b) { return b < a.s.B ? (rows_of(a.s, b) * a.G + RT - 1) / RT : 0; };
   // (the first 64 sequences are held: most batches are no larger)
-  const int rts0 = tiles_of(lane), blocks0 = rts0 ? blocks_of(a, lane) : 0;
-  int blocks = 0x7fffff00;
-  if (a.target) {
+  const int rts0 = tiles_of(a, RT, lane), blocks0 = rts0 ? blocks_of(a, lane) : 0;
+  int blocks = kWhole, c = 0;
+  out.slot = -1;
+  out.parts = 1;
+  if (a.tail) {
+    const Tail t = tail_of(a, RT);
+    if (unit >= t.whole) {
+      const int u = unit - t.whole;
+      if (u >= t.tail * t.parts) return false;
+      c = u / t.tail;
+      unit = t.whole + u % t.tail;
+      out.slot = u;
+      out.parts = t.parts;
+    }
+  } else if (a.target) {
     float all = (float)rts0 * (float)blocks0;  // (a few parts in a million more or less do not matter)
     for (int b = lane + 64; b < a.s.B; b += 64) {
-      const int n = tiles_of(b);
+      const int n = tiles_of(a, RT, b);
       if (n) all += (float)n * (float)blocks_of(a, b);
     }
     all = sum64(all);
@@ -95,7 +135,7 @@ __device__ __forceinline__ bool find_item(const AttnArgs& a, int RT, int unit, I
   }
   int units0 = 0, tiles0 = 0;
   for (int b0 = 0; b0 < a.s.B; b0 += 64) {
-    const int rts = b0 ? tiles_of(b0 + lane) : rts0, n = b0 ? (rts ? blocks_of(a, b0 + lane) : 0) : blocks0;
+    const int rts = b0 ? tiles_of(a, RT, b0 + lane) : rts0, n = b0 ? (rts ? blocks_of(a, b0 + lane) : 0) : blocks0;
     const int pieces = max((n + blocks - 1) / blocks, 1), mine = rts * pieces * HK;
     const int units = scan64(mine), tiles = scan64(rts);
     const unsigned long long past = __ballot(units0 + units > unit);
@@ -122,7 +162,7 @@ __device__ __forceinline__ bool find_item(const AttnArgs& a, int RT, int unit, I
       }
       out.rt = out.rts - 1 - rt;
       out.h = pair % HK;
-      out.c = pair / HK;
+      out.c = c ? c : pair / HK;
       out.more = units0 / HK - tiles0;
       return true;
     }

@@ -48,6 +48,7 @@ struct AttnArgs {
   int target, slots;    // pieces that are aimed at (0: whole row tiles), and partial results that `part` holds, those of
   int firsts;           // first pieces (of a head) in front
   int pieces, blocks;   // chosen pages: pieces of a row tile, and blocks of 128 keys of one
+  int tail;             // work-groups at a time: the row tiles that are left behind the last whole round of them are cut (0: none)
   // The prefix for the rows of the whole batch (shared pieces; 0: it is read with each sequence's own keys), by shared_grid work-groups in front
   // of the launch's others: pieces of shared_blocks blocks of 128 keys for each of shared_tiles tiles of shared_rt rows of a key head; slot
   // (head * shared_tiles + tile) * shared + piece
@@ -57,12 +58,13 @@ struct AttnArgs {
 
 // How a call runs: tiles of rt rows (16 to 64: attn_kernel; more, or `tile`: attn_tile_kernel); pieces and blocks as in AttnArgs
 struct AttnPlan {
-  int rt, tile, target, slots, firsts;                              // target 0: nothing is split
+  int rt, tile, target, slots, firsts;                              // target 0: nothing is split,
+  int tail;                                                         // or (not 0) the last row tiles alone
   int shared, shared_rt, shared_tile, shared_tiles, shared_blocks;  // shared 0: the prefix is read with each sequence's own keys
 };
-AttnPlan attn_plan(int T, int B, bool start, bool chosen, int HQ, int HK, int D, int prefix_len, size_t ws_bytes);
+AttnPlan attn_plan(int T, int B, bool start, bool chosen, bool e8, int HQ, int HK, int D, int prefix_len, size_t ws_bytes);
 size_t attn_used_bytes(const AttnPlan& p, int HK, int D);
-size_t attn_workspace_bytes(int T, int B, int HQ, int HK, int D, int prefix_len);
+size_t attn_workspace_bytes(int T, int B, bool e8, int HQ, int HK, int D, int prefix_len);
 // Work-groups of the calls's launches at most (0: more than a grid holds)
 long long attn_grid(const AttnPlan& p, int T, int B, bool start, int HQ, int HK);
 hipError_t launch_attn(const AttnArgs& a, const AttnPlan& p, hipStream_t s);

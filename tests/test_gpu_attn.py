@@ -427,6 +427,37 @@ def test_many_rows_replayed(qm, dev):
             K.check(o, *K.attention(q, cache, st, ld.cpu(), tab, BF16, None, pages[:19] if n else (), n), BF16)
 
 
+@pytest.mark.parametrize("D,HK,G,rows,lens", [(64, 64, 1, [1100], [1100]), (16, 70, 2, [300, 200, 60], [300, 1500, 70]), (256, 33, 2, [520], [700]),
+                                              (128, 64, 1, [128, 1], [900, 5])])
+def test_last_round_of_tiles(qm, dev, D, HK, G, rows, lens):
+    """More row tiles than the GPU takes at once: those behind the last whole round are cut. Rows of many sequences, a few of whose results are
+    looked at; rows behind the last one stay; the workspace may hold anything, and any size of it serves."""
+    page, T = 32, max(sum(rows), 1100)
+    cache = K.Cache(sum((n + page - 1) // page for n in lens) + 2, HK, page, D, BF16, 21)
+    start, ln, table, rest = K.batch(lens, rows, page, cache.pages, 21)
+    q = queries(T, HK * G, D, BF16, 22)
+    kv = cache.on(qm, dev)
+    some, see, of = [], [], []
+    for b, n in enumerate(rows):
+        for t in {0, 1, n // 3, n // 2, n - 2, n - 1} & set(range(n)):
+            some.append(int(start[b]) + t)
+            see.append(lens[b] - n + t + 1)
+            of.append(b)
+    want, bound = K.attention(q[some], cache, torch.arange(len(some) + 1), torch.tensor(see), table[of], BF16)
+    full = qm.attn_workspace(kv, T, len(rows), HK * G).numel()
+    outs = []
+    for n in (full, 0, full // 2 // 256 * 256, full + 256):
+        ws = torch.full((max(n, 256),), 0xFF, dtype=torch.uint8, device=dev)
+        o = torch.full((T, HK * G, D), 3.0, dtype=BF16, device=dev)
+        qm.attn_prefix(q.to(dev), kv, ln.to(dev), table.to(dev), start=start.to(dev), o=o, ws=ws[:n] if n else None)
+        K.check(o[some], want, bound, BF16)
+        assert bool((o[sum(rows):] == 3).all())
+        outs.append(o)
+    # (cut or whole, every row is within two roundings of the other)
+    a, b = (outs[i][:sum(rows)].double() for i in (0, 1))
+    assert bool(((a - b).abs() <= 2.0 ** -7 * torch.maximum(a.abs(), b.abs()) + 2.0 ** -8).all())
+
+
 # ---- chosen pages
 @pytest.mark.parametrize("ws", [True, False])
 @pytest.mark.parametrize("qt,ct", KINDS)
