@@ -186,24 +186,31 @@ __global__ __launch_bounds__(256) void attn_tail_join_kernel(AttnArgs a, int RT)
 
 namespace {
 
-constexpr int kTarget = 512;         // pieces that a call is cut into: two work-groups a CU
-constexpr int kSharedTarget = 256;   // pieces of the shared prefix
-constexpr int kSharedFrom = 256;     // a shorter prefix is read with each sequence's own keys
-constexpr int kTailMost = 4;          // rounds of work-groups from which the last one is not worth cutting
-constexpr int kTileFrom = 64;        // rows of a key head from which attn_tile_kernel takes them
-// Products of a prefix (rows of all heads times keys times D) from which they are attn_tile_kernel's, in a launch of its own: below, attn_kernel's tiles in the
+// Pieces that a call is cut into: two work-groups a CU. attn_kernel's may be as many more as there are row tiles; attn_tile_kernel's, which take longer to
+// start and end, are kept to one round (12 sequences of 580 to 17200 tokens, 24 heads of 256 over 4: 64 us against 77; attn_kernel 74 against 71).
+constexpr int kTarget = 512;
+constexpr int kSharedTarget = 256;  // pieces of the shared prefix: one work-group a CU beside the sequences' own keys
+constexpr int kSharedFrom = 256;    // a shorter prefix is read with each sequence's own keys
+constexpr int kTailMost = 4;        // rounds of work-groups from which the last one is not worth cutting
+constexpr int kSharedRows = 64;     // rows of the batch from which attn_tile_kernel may take a prefix
+// Products of a prefix (rows of all heads times keys times D) from which it does, in a launch of its own: below, attn_kernel's tiles in the
 // sequences' own launch take less. 8 heads of 128, rows of a head x keys, us: 192 x 2048 31 against 21, 192 x 16384 45.7 against 44.0, 384 x 16384
 // 65 against 85, 768 x 16384 106 against 158; D 256, 384 x 8192: 68 against 99. Behind 8-bit caches 192 x 16384 54 against 46, 512 x 16384 89 against 92.
-constexpr double kSharedTileFrom = 3.2e9, kSharedTileFrom8 = 8e9;
+constexpr double kSharedFrom16 = 3.2e9, kSharedFrom8 = 8e9;
 
 long long div_up(long long a, long long b) { return (a + b - 1) / b; }
-// Rows of a tile, for `rows` of a sequence on average (or of the batch): what attn_kernel's registers hold, or 64 and 128 of attn_tile_kernel
-int tile_rows(long long rows, long long from, int D, int* tile) {
-  *tile = rows >= from;
-  if (*tile) return rows > 64 && D <= 128 ? 128 : 64;
+// Rows of attn_kernel's tile: what its registers hold
+int few_rows(long long rows, int D) {
   const int most = D <= 64 ? 64 : D <= 128 ? 32 : 16, want = rows <= 16 ? 16 : rows <= 32 ? 32 : 64;
   return want < most ? want : most;
 }
+// Rows of a sequence from which attn_tile_kernel takes them. 16 sequences of 4096 tokens, us: D 128, 8 heads: 48 rows 57 against 65, 20 rows 51.3
+// against 52.3 (but of 1000 tokens 18 against 16.7); D 256, 4 heads: 18 rows 53 against 64, 12 rows 51 against 53. Behind 8-bit caches, which
+// it widens on the way: D 128: 128 rows 72 against 77, 64 rows 56 against 54; D 256: 36 rows 52 against 65, 18 rows 49 against 44.
+int tile_from(int D, bool e8) { return e8 ? (D > 128 ? 33 : 65) : (D > 128 ? 17 : 33); }
+// Of its tile: 64 where that is all there is (64 rows of one sequence of 16384 tokens: 26.6 us against 30.5; 80 rows of 16 of 4096: 72 against 65), or all
+// that the registers hold
+int many_rows(long long rows, int D, bool e8) { return D <= 128 && (rows > 64 || e8) ? 128 : 64; }
 // Row tiles of all sequences at most
 long long row_tiles(int T, int B, bool start, int G, int rt) {
   return start ? (long long)T * G / rt + B : B * div_up(G, rt);  // (as first_slot counts them)
@@ -222,12 +229,18 @@ AttnPlan attn_plan(int T, int B, bool start, bool chosen, bool e8, int HQ, int H
   const long long rows = start ? div_up(T, B < T ? B : T) * G : G;  // of a sequence, on average
   const size_t have = ws_bytes / 256 * 256;
   AttnPlan p{};
-  p.rt = tile_rows(rows, chosen ? rows + 1 : kTileFrom, D, &p.tile);  // (chosen pages are a row's own: never many rows)
+  p.tile = !chosen && rows >= tile_from(D, e8);  // (chosen pages are a row's own: never many rows)
+  p.rt = p.tile ? many_rows(rows, D, e8) : few_rows(rows, D);
   const AttnPlan alone = p;
-  if (prefix_len >= kSharedFrom && B > 1 && T > 1 && !p.tile) {
-    const bool many = (double)T * HQ * prefix_len * D >= (e8 ? kSharedTileFrom8 : kSharedTileFrom);
-    p.shared_rt = tile_rows((long long)T * G, many ? kTileFrom : (long long)T * G + 1, D, &p.shared_tile);
-    if (!p.shared_tile) p.rt = p.shared_rt;  // (one launch for both: the batch's rows fill the tile, and a sequence's own keys take no longer for it)
+  if (prefix_len >= kSharedFrom && B > 1 && T > 1 && rows < kSharedRows) {
+    const long long all = (long long)T * G;
+    p.shared_tile = all >= kSharedRows && (double)T * HQ * prefix_len * D >= (e8 ? kSharedFrom8 : kSharedFrom16);
+    p.shared_rt = p.shared_tile ? many_rows(all, D, e8) : few_rows(all, D);
+    // (one launch for both: the batch's rows fill the tile, and a sequence's own keys take no longer for it)
+    if (!p.shared_tile) {
+      p.tile = 0;
+      p.rt = p.shared_rt;
+    }
     p.shared_tiles = (int)div_up((long long)T * G, p.shared_rt);
     const int blocks = (int)div_up(prefix_len, 128);
     long long n = kSharedTarget / ((long long)HK * p.shared_tiles);
@@ -240,7 +253,10 @@ AttnPlan attn_plan(int T, int B, bool start, bool chosen, bool e8, int HQ, int H
   const long long items = row_tiles(T, B, start, G, p.rt) * HK;
   const long long left = ((long long)have - (long long)shared_bytes(p, HK, D)) / (long long)slot_bytes(p.rt, D) - items;
   // (pieces of all row tiles are at most the target and one more for each of them; row tiles that fill the chip are left whole)
-  if (left > 0 && items < (p.tile ? kTarget / 2 : 2 * kTarget)) p.target = (int)(left < kTarget ? left : kTarget);
+  if (left > 0 && items < (p.tile ? kTarget / 2 : 2 * kTarget)) {
+    const long long want = p.tile ? kTarget - items : kTarget;
+    p.target = (int)(left < want ? left : want);
+  }
   p.slots = p.target || p.shared ? (int)(items + p.target) : 0;
   if (p.tile && !p.slots && items < kTailMost * kTarget && kTarget * slot_bytes(p.rt, D) <= have) p.slots = p.tail = kTarget;
   p.firsts = (int)(items / HK);

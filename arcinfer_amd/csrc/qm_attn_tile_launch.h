@@ -13,9 +13,16 @@ hipError_t tile_mode(const AttnArgs& a, unsigned grid, hipStream_t s) {
 
 template <typename TQ, typename TC, int PARTS>
 hipError_t tile_parts(const AttnArgs& a, int mt, unsigned grid, hipStream_t s) {
-  if (a.kv.D <= 64) return mt == 1 ? tile_mode<TQ, TC, 64, 1, PARTS>(a, grid, s) : tile_mode<TQ, TC, 64, 2, PARTS>(a, grid, s);
-  if (a.kv.D <= 128) return mt == 1 ? tile_mode<TQ, TC, 128, 1, PARTS>(a, grid, s) : tile_mode<TQ, TC, 128, 2, PARTS>(a, grid, s);
-  return tile_mode<TQ, TC, 256, 1, PARTS>(a, grid, s);
+  // (behind 8-bit caches, tiles of 64 rows are of heads beyond 128 only)
+  if constexpr (sizeof(TC) == 1) {
+    if (a.kv.D <= 64) return tile_mode<TQ, TC, 64, 2, PARTS>(a, grid, s);
+    if (a.kv.D <= 128) return tile_mode<TQ, TC, 128, 2, PARTS>(a, grid, s);
+    return tile_mode<TQ, TC, 256, 1, PARTS>(a, grid, s);
+  } else {
+    if (a.kv.D <= 64) return mt == 1 ? tile_mode<TQ, TC, 64, 1, PARTS>(a, grid, s) : tile_mode<TQ, TC, 64, 2, PARTS>(a, grid, s);
+    if (a.kv.D <= 128) return mt == 1 ? tile_mode<TQ, TC, 128, 1, PARTS>(a, grid, s) : tile_mode<TQ, TC, 128, 2, PARTS>(a, grid, s);
+    return tile_mode<TQ, TC, 256, 1, PARTS>(a, grid, s);
+  }
 }
 
 // Parts of P by the bits that the result keeps: f16 behind an 8-bit cache (P is bf16 there) two; f32 two of f16, three of bf16 (two would
