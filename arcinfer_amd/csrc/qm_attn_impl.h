@@ -347,11 +347,26 @@ __global__ __launch_bounds__(256, 2) void attn_kernel(AttnArgs a) {
     }
     if constexpr (E8) ks[s] = *(const v4f*)(kv.ksc + at.scale + 4 * g);
   };
+  // Elements of V vector vb of lane c of 16: of 8 bits two of a lane lie next to each other, one load of 16 bytes
+  constexpr bool PAIR = E8 && VB == 2;
+  const auto element = [&](int vb, int c) { return PAIR ? 2 * VE * c + VE * vb : vb * 128 + VE * c; };
   const auto load_v = [&](int vb, int s, const Place& at) {
-    const int d = vb * 128 + VE * col;
+    const int d = element(vb, col);
 #pragma unroll
-    for (int e = 0; e < 4; ++e)
-      vr[vb][s][e] = *(const vvec*)((const char*)kv.v + at.base + e * kv.ts * (long long)sizeof(TC) + (v_row + (FULL || d < kv.D ? d : 0) * (unsigned)sizeof(TC)));
+    for (int e = 0; e < 4; ++e) {
+      const char* p = (const char*)kv.v + at.base + e * kv.ts * (long long)sizeof(TC) + (v_row + (FULL || d < kv.D ? d : 0) * (unsigned)sizeof(TC));
+      if constexpr (PAIR) {
+        if (vb) continue;
+        const kvec w = *(const kvec*)p;
+#pragma unroll
+        for (int i = 0; i < VW; ++i) {
+          vr[0][s][e][i] = w[i];
+          vr[VB - 1][s][e][i] = w[VW + i];
+        }
+      } else {
+        vr[vb][s][e] = *(const vvec*)p;
+      }
+    }
     if (E8 && vb == 0) vs[s] = *(const v4f*)(kv.vsc + at.scale + 4 * g);
   };
   // Registers of K and of V are loaded for the next block as soon as this one's products have taken them: what a block waits for was asked
@@ -554,11 +569,11 @@ __global__ __launch_bounds__(256, 2) void attn_kernel(AttnArgs a) {
         v4i v[2];
         operands(vb, w, v[0], v[1]);
 #pragma unroll
-        for (int j = 0; j < 2; ++j)
+        for (int n = 0; n < PARTS; ++n)  // (parts outermost: no product waits for the one before)
 #pragma unroll
-          for (int m = 0; m < MT; ++m)
+          for (int j = 0; j < 2; ++j)
 #pragma unroll
-              for (int n = 0; n < PARTS; ++n) o[vb][2 * w + j][m] = mfma16<TP>(v[j], p[n][m], o[vb][2 * w + j][m]);
+            for (int m = 0; m < MT; ++m) o[vb][2 * w + j][m] = mfma16<TP>(v[j], p[n][m], o[vb][2 * w + j][m]);
       }
 #pragma unroll
     for (int vb = 0; vb < VB; ++vb)
@@ -650,7 +665,7 @@ __global__ __launch_bounds__(256, 2) void attn_kernel(AttnArgs a) {
       }
 #pragma unroll
       for (int vb = 0; vb < VB; ++vb) {
-        const int d = vb * 128 + VE * (4 * g + wave);
+        const int d = element(vb, 4 * g + wave);
         if (!FULL && d >= kv.D) continue;
 #pragma unroll
         for (int j = 0; j < VE; j += 4) *(v4f*)(slot + 2 * RT + (size_t)r * kv.D + d + j) = v4f{y[vb][j][m], y[vb][j + 1][m], y[vb][j + 2][m], y[vb][j + 3][m]};
@@ -666,7 +681,7 @@ __global__ __launch_bounds__(256, 2) void attn_kernel(AttnArgs a) {
     const size_t at = (size_t)(row0 + r / a.G) * a.ldo + (size_t)(h * a.G + r % a.G) * kv.D;
 #pragma unroll
     for (int vb = 0; vb < VB; ++vb) {
-      const int d = vb * 128 + VE * (4 * g + wave);
+      const int d = element(vb, 4 * g + wave);
       if (!FULL && d >= kv.D) continue;
       float z[VE];
 #pragma unroll
