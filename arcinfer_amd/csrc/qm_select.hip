@@ -106,16 +106,18 @@ __global__ __launch_bounds__(256) void page_score_kernel(SelectArgs a, int chunk
   }
 }
 
-// A work-group a token and key head. The k-th largest score, eight bits at a time from the first one that the scores differ in (by counts in LDS, whole
+// A work-group a token and key head. The k-th largest score, eleven bits at a time from the first one that the scores differ in (by counts in LDS, whole
 // numbers: their order does not matter); as soon as all that share the known bits are taken, it is found. Scores are held in registers (K a
 // thread; K = 0: read again each time, for tables beyond 256 kMostKept pages). Latency-bound.
 constexpr int kMostKept = 32;
+constexpr int kBits = 11, kBins = 1 << kBits;  // of scores that are told apart at a time: 3 times at most for most batches
 
 template <int K>
 __global__ __launch_bounds__(256) void page_pick_kernel(SelectArgs a) {
   typedef unsigned long long u64;
   constexpr int N = K ? K : 1;
-  __shared__ int hist[256], before[4], found[3];
+  __shared__ int hist[kBins], before[4], found[3];
+  __shared__ int counts[N][4];  // (K > 0) of each round and wave
   __shared__ u64 bits[2][4];
   const int item = blockIdx.x, t = item / a.kv.HK, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   int b;
@@ -163,15 +165,16 @@ __global__ __launch_bounds__(256) void page_pick_kernel(SelectArgs a) {
   all = bits[1][0] & bits[1][1] & bits[1][2] & bits[1][3];
   // (all: the bits that every score has, of those above the first one that they differ in)
   const u64 differ = any & ~all;
-  // The threshold: eight bits at a time, from the first one that they differ in, by how many scores have each value of them
+  // The threshold: kBits at a time, from the first one that they differ in, by how many scores have each value of them
   int top = differ ? 64 - __clzll(differ) : 0;  // bits that are not known yet
   u64 from = top == 64 ? 0 : all >> top << top;
   bool exact = false;  // whether those from `from` on are as many as are needed
   int left = need;     // of those that share the known bits
   while (top > 0 && !exact) {
-    const int low = top > 8 ? top - 8 : 0;
+    const int low = top > kBits ? top - kBits : 0;
     const u64 known = top == 64 ? 0 : ~0ull << top;
-    hist[tid] = 0;
+#pragma unroll
+    for (int i = 0; i < kBins; i += 256) hist[i + tid] = 0;
     __syncthreads();
     const auto count = [&](int r, u64 u) {
       if (lo + r * 256 + tid < hi && (u & known) == from) atomicAdd(&hist[(int)(u >> low) & ((1 << (top - low)) - 1)], 1);
@@ -184,8 +187,11 @@ __global__ __launch_bounds__(256) void page_pick_kernel(SelectArgs a) {
       for (int r = 0; r < rounds; ++r) count(r, key_of(lo + r * 256 + tid));
     }
     __syncthreads();
-    // how many have a larger value of these bits than thread tid's (255 - tid), or it
-    const int here = hist[255 - tid];
+    // how many have a larger value of these bits than the last of thread tid's bins (kBins / 256 from the top), or it
+    constexpr int B = kBins / 256;
+    int bin[B], here = 0;
+#pragma unroll
+    for (int i = 0; i < B; ++i) here += bin[i] = hist[kBins - 1 - B * tid - i];
     int up = here;
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) {
@@ -196,9 +202,18 @@ __global__ __launch_bounds__(256) void page_pick_kernel(SelectArgs a) {
     __syncthreads();
     for (int w = 0; w < wave; ++w) up += before[w];
     if (up >= left && up - here < left) {
-      found[0] = 255 - tid;
-      found[1] = left - (up - here);
-      found[2] = here;
+      int over = up - here;  // larger ones
+      bool is = false;
+#pragma unroll
+      for (int i = 0; i < B; ++i) {
+        if (!is && over + bin[i] >= left) {
+          is = true;
+          found[0] = kBins - 1 - B * tid - i;
+          found[1] = left - over;
+          found[2] = bin[i];
+        }
+        over += bin[i];
+      }
     }
     __syncthreads();
     from |= (u64)found[0] << low;
@@ -207,38 +222,63 @@ __global__ __launch_bounds__(256) void page_pick_kernel(SelectArgs a) {
     top = low;
   }
   // Those above `from`, and of those that are equal to it the first that are needed still; in their order
-  int equal = 0;
   const u64 below = (1ull << lane) - 1;
-  int out = a.first;
-  const auto put = [&](int r, u64 u) {
-    const int j = lo + r * 256 + tid;
-    bool take = j < hi && u >= from;
-    if (!exact) {
-      const bool eq = j < hi && u == from;
-      const u64 e = __ballot(eq);
-      __syncthreads();
-      if (lane == 0) before[wave] = __popcll(e);
-      __syncthreads();
-      int at = equal + __popcll(e & below);
-      for (int w = 0; w < wave; ++w) at += before[w];
-      equal += before[0] + before[1] + before[2] + before[3];
-      take = take && (!eq || at < left);
-    }
-    const u64 k = __ballot(take);
-    __syncthreads();
-    if (lane == 0) before[wave] = __popcll(k);
-    __syncthreads();
-    int at = out + __popcll(k & below);
-    for (int w = 0; w < wave; ++w) at += before[w];
-    if (take) sel[at] = j;
-    out += before[0] + before[1] + before[2] + before[3];
-  };
   if constexpr (K > 0) {
+    // (counts of all rounds at once: two barriers each for those of equals and of those taken)
+    const auto ranks = [&](auto is, int (&at)[N]) {
+#pragma unroll
+      for (int r = 0; r < K; ++r) {
+        const u64 m = r < rounds ? __ballot(is(r)) : 0;
+        at[r] = __popcll(m & below);
+        if (lane == 0) counts[r][wave] = __popcll(m);
+      }
+      __syncthreads();
+      int sum = 0;
+#pragma unroll
+      for (int r = 0; r < K; ++r) {
+        if (r >= rounds) break;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          if (w == wave) at[r] += sum;
+          sum += counts[r][w];
+        }
+      }
+      __syncthreads();
+    };
+    const auto in = [&](int r) { return lo + r * 256 + tid < hi; };
+    int equal[N], at[N];
+    if (!exact) ranks([&](int r) { return in(r) && key[r] == from; }, equal);
+    const auto take = [&](int r) { return in(r) && key[r] >= from && (exact || key[r] != from || equal[r] < left); };
+    ranks(take, at);
 #pragma unroll
     for (int r = 0; r < K; ++r)
-      if (r < rounds) put(r, key[r]);
+      if (r < rounds && take(r)) sel[a.first + at[r]] = lo + r * 256 + tid;
   } else {
-    for (int r = 0; r < rounds; ++r) put(r, key_of(lo + r * 256 + tid));
+    int equal = 0, out = a.first;
+    for (int r = 0; r < rounds; ++r) {
+      const int j = lo + r * 256 + tid;
+      const u64 u = key_of(j);
+      bool take = j < hi && u >= from;
+      if (!exact) {
+        const bool eq = j < hi && u == from;
+        const u64 e = __ballot(eq);
+        __syncthreads();
+        if (lane == 0) before[wave] = __popcll(e);
+        __syncthreads();
+        int at = equal + __popcll(e & below);
+        for (int w = 0; w < wave; ++w) at += before[w];
+        equal += before[0] + before[1] + before[2] + before[3];
+        take = take && (!eq || at < left);
+      }
+      const u64 k = __ballot(take);
+      __syncthreads();
+      if (lane == 0) before[wave] = __popcll(k);
+      __syncthreads();
+      int at = out + __popcll(k & below);
+      for (int w = 0; w < wave; ++w) at += before[w];
+      if (take) sel[at] = j;
+      out += before[0] + before[1] + before[2] + before[3];
+    }
   }
 }
 
