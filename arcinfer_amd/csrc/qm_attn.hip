@@ -188,10 +188,15 @@ namespace {
 
 // Pieces that a call is cut into: two work-groups a CU. attn_kernel's may be as many more as there are row tiles; attn_tile_kernel's, which take longer to
 // start and end, are kept to one round (12 sequences of 580 to 17200 tokens, 24 heads of 256 over 4: 64 us against 77; attn_kernel 74 against 71).
-constexpr int kTarget = 512;
-constexpr int kSharedTarget = 256;  // pieces of the shared prefix: one work-group a CU beside the sequences' own keys
-constexpr int kSharedFrom = 256;    // a shorter prefix is read with each sequence's own keys
-constexpr int kTailMost = 4;        // rounds of work-groups from which the last one is not worth cutting
+constexpr int kTarget = 512;  // (attn_tile_kernel's 64 us: 80 by 256 pieces, 78 by 1024)
+// Pieces of the shared prefix: one work-group a CU beside the sequences' own keys (48 sequences behind 8192 tokens 46 us, 16 behind 65000 60; 128 pieces
+// 59 and 96)
+constexpr int kSharedTarget = 256;
+// Bytes of a prefix, read once more for each further sequence, from which it is read once for all: below, the pieces' join takes longer than that.
+// 8 heads of 128, bf16, 500 tokens of their own, us: 8 sequences x 256 tokens 16.9 against 14.7, x 1024 17.3 against 16.9; 48 x 256 27.8 against 32.0,
+// x 1024 32 against 48; 2 x 1024 15.2 against 13.6.
+constexpr double kSharedBytes = 3.2e7;
+constexpr int kTailMost = 2;        // rounds of work-groups from which the last one is not cut (6656 tokens, 3.3 rounds: 362 us cut, 359 not)
 constexpr int kSharedRows = 64;     // rows of the batch from which attn_tile_kernel may take a prefix
 // Products of a prefix (rows of all heads times keys times D) from which it does, in a launch of its own: below, attn_kernel's tiles in the
 // sequences' own launch take less. 8 heads of 128, rows of a head x keys, us: 192 x 2048 31 against 21, 192 x 16384 45.7 against 44.0, 384 x 16384
@@ -232,7 +237,7 @@ AttnPlan attn_plan(int T, int B, bool start, bool chosen, bool e8, int HQ, int H
   p.tile = !chosen && rows >= tile_from(D, e8);  // (chosen pages are a row's own: never many rows)
   p.rt = p.tile ? many_rows(rows, D, e8) : few_rows(rows, D);
   const AttnPlan alone = p;
-  if (prefix_len >= kSharedFrom && B > 1 && T > 1 && rows < kSharedRows) {
+  if ((double)(B - 1) * prefix_len * HK * D * (e8 ? 2 : 4) >= kSharedBytes && T > 1 && rows < kSharedRows) {
     const long long all = (long long)T * G;
     p.shared_tile = all >= kSharedRows && (double)T * HQ * prefix_len * D >= (e8 ? kSharedFrom8 : kSharedFrom16);
     p.shared_rt = p.shared_tile ? many_rows(all, D, e8) : few_rows(all, D);

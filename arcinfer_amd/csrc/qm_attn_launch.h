@@ -19,7 +19,7 @@ hipError_t attn_mode(const AttnArgs& a, unsigned grid, hipStream_t s) {
 
 template <typename TQ, typename TC, int PARTS>
 hipError_t attn_parts(const AttnArgs& a, int mt, unsigned grid, hipStream_t s) {
-  // (row tiles: what the registers hold, as tiles_for has it)
+  // (row tiles: what the registers hold, as few_rows has it)
   if (a.kv.D <= 64) return mt == 1 ? attn_mode<TQ, TC, 64, 1, PARTS>(a, grid, s) : mt == 2 ? attn_mode<TQ, TC, 64, 2, PARTS>(a, grid, s) : attn_mode<TQ, TC, 64, 4, PARTS>(a, grid, s);
   if (a.kv.D <= 128) return mt == 1 ? attn_mode<TQ, TC, 128, 1, PARTS>(a, grid, s) : attn_mode<TQ, TC, 128, 2, PARTS>(a, grid, s);
   return attn_mode<TQ, TC, 256, 1, PARTS>(a, grid, s);

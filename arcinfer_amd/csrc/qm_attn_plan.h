@@ -61,7 +61,9 @@ struct Tail {
   int whole, tail, parts;
 };
 constexpr int kMostParts = 32;
-constexpr int kLeastPart = 4;  // blocks of 128 keys of such a piece at least: it has its start and a result to be joined
+// Blocks of 128 keys of such a piece at least: it has its start and a result to be joined (576 row tiles of 1300 to 2800 keys, 128 rows of 128 elements: 168 us;
+// by 8 blocks 173, by 16 191, uncut 186)
+constexpr int kLeastPart = 4;
 
 // The sequence's row tiles and those of all
 __device__ __forceinline__ int tiles_of(const AttnArgs& a, int RT, int b) { return b < a.s.B ? (rows_of(a.s, b) * a.G + RT - 1) / RT : 0; }

@@ -1,12 +1,19 @@
 // Attention of many rows over a paged cache: attn_kernel (qm_attn_impl.h) has four waves take keys in turn for the same few rows; here each of
 // the four has rows of its own, 16 MT of them, and all take the same keys, from LDS. A work-group's 64 MT rows then read a key once, where row tiles
-// of attn_kernel read it once for 16 or 32 rows: prompts, and a prefix's keys for the rows of a large batch.
+// of attn_kernel read it once for 16 or 32: prompts, drafted tokens, and a prefix's keys for the rows of a large batch.
 //
-// Keys and values go through registers into LDS in the order in which the matrix pipe takes them (8-bit ones widened, values transposed on
-// the way: once, for all rows), 64 keys a step (32 of heads beyond 128), two steps' places in turn: while a step is worked on the next one's
-// loads are on their way, and there is one barrier a step. Operands are read from LDS by 16 bytes a lane, 1 KB each without bank conflicts. What
-// bounds it: LDS reads (each wave reads every key and value: 16 KB for 32 keys of 128, 128 bytes a cycle for a CU's four waves) beside the matrix
-// pipe (32 instructions of 16 cycles a row tile and 32 keys) and the exponentials.
+// 64 keys a step (32 of heads beyond 128), two steps' places in turn: while a step is worked on the next one's loads are on their way, and there is one
+// barrier a step. A 16-bit cache's keys and values go straight to LDS, keys in operand order (a lane's 16 bytes are one operand), values as they lie, their
+// chunks exchanged within a row so that the reads, which transpose, meet no bank twice; what no row sees and what is behind the head is out of the
+// buffer's range, zeros. 8-bit ones go through registers, widened and transposed on the way: once, for all rows. A step's places in memory are worked out during
+// the step before (scalar instructions, between matrix instructions).
+//
+// The logits stay unscaled: e^(scale (s - m)) is one fma and one v_exp, the maximum is that of s (for a scale below zero -q is taken). What bounds it: the
+// matrix pipe (64 keys of 128 by a wave's 32 rows: 1024 cycles, of which 42 % of the time is made) with the vector instructions (160, and 32 exponentials of
+// four times an instruction's time) beside it, which two waves on a SIMD overlap in part. Measured, 32 heads of 128 over 8, bf16: the last 4096 of 16384 tokens
+// 907 us (1060 Tflop/s of what they see), 4096 of 4096 155 us; f32 results, three parts of each weight, 1533 us; a large library product reaches 1250.
+// Tried and not kept: the next scores' products between this block's exponentials (as fast with three parts, 5 % slower with one), values through
+// registers for 16-bit caches too (1016 us).
 #pragma once
 #include "qm_attn_impl.h"
 
@@ -132,7 +139,7 @@ __global__ __launch_bounds__(256, 2) void attn_tile_kernel(AttnArgs a) {
   }
 
   // Steps of keys that every row sees: blocks below seen_pre, and those from pre_blocks on below seen_own
-  const int seen_pre = a.prefix_len / kBlock, seen_own = pre_blocks + lo_lim / kBlock;
+  const int seen_pre = min(a.prefix_len / kBlock, pre_blocks), seen_own = pre_blocks + lo_lim / kBlock;
   // This wave's group of 16 keys of a step (NB 1: waves 0, 1 the first one, each half of its K operands and of its V vectors)
   const int mine = NB == 2 ? wave : wave >> 1, half = NB == 2 ? 0 : wave & 1;
   const int32_t* table = a.s.table + (size_t)b * a.s.W;

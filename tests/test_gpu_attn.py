@@ -458,6 +458,51 @@ def test_last_round_of_tiles(qm, dev, D, HK, G, rows, lens):
     assert bool(((a - b).abs() <= 2.0 ** -7 * torch.maximum(a.abs(), b.abs()) + 2.0 ** -8).all())
 
 
+def shared(qm, dev, qt, ct, D, B, HQ, HK, n, prefix_len, page, out=None, sizes=(1.0,)):
+    """A batch of n tokens a sequence behind a prefix: a few rows of the result against the plain form, all against the call without a workspace."""
+    lens = [n + 9 * i % 70 for i in range(B)]
+    cache = K.Cache(sum((m + page - 1) // page for m in lens) + (prefix_len + page - 1) // page, HK, page, D, ct, 31)
+    start, ln, table, rest = K.batch(lens, [n] * B, page, cache.pages, 31)
+    prefix = torch.tensor(rest, dtype=torch.int32)
+    q, out = queries(n * B, HQ, D, qt, 32), out or qt
+    kv = cache.on(qm, dev)
+    of = [0, B // 2, B - 1]
+    some, see = [n * b + (n - 1) * (b % 2) for b in of], [lens[b] - n + 1 + (n - 1) * (b % 2) for b in of]
+    want, bound = K.attention(q[some], cache, torch.arange(4), torch.tensor(see), table[of], out, None, prefix, prefix_len)
+    full = qm.attn_workspace(kv, n * B, B, HQ, prefix_len).numel()
+    args = (q.to(dev), kv, ln.to(dev), table.to(dev))
+    more = dict(start=None if n == 1 else start.to(dev), prefix=prefix.to(dev), prefix_len=prefix_len, out=out)
+    alone = qm.attn_prefix(*args, **more)
+    K.check(alone[some], want, bound, out)
+    for part in sizes:
+        ws = torch.full((int(full * part) // 256 * 256,), 0xFF, dtype=torch.uint8, device=dev)  # (NaN wherever it is read unwritten)
+        got = qm.attn_prefix(*args, **more, ws=ws)
+        K.check(got[some], want, bound, out)
+        a, b = got.double(), alone.double()
+        assert bool(((a - b).abs() <= (2.0 ** -6 if out != F32 else 2.0 ** -12) * (a.abs() + 1)).all())
+    return full
+
+
+@pytest.mark.parametrize("qt,ct", KINDS)
+@pytest.mark.parametrize("D,B,HQ,n", [(64, 20, 6, 1), (80, 9, 4, 2), (128, 11, 8, 1), (256, 6, 24, 2)])
+def test_shared_prefix(qm, dev, D, B, HQ, n, qt, ct):
+    """A prefix that is worth being read once (32 MB less), in the sequences' own launch."""
+    unit = (B - 1) * 2 * D * (2 if ct == E4M3 else 4)
+    prefix_len = int(3.2e7 / unit) + 45
+    for out in (None, F32):
+        full = shared(qm, dev, qt, ct, D, B, HQ, 2, n, prefix_len, 32, out, (1.0, 0.5, 0.1))
+    assert full != qm.attn_workspace(K.Cache(1, 2, 32, D, ct, 0).on(qm, dev), n * B, B, HQ, prefix_len - 46).numel()  # (below the bytes: another plan)
+
+
+@pytest.mark.parametrize("qt,ct", KINDS)
+@pytest.mark.parametrize("D,T", [(64, 256), (96, 192), (128, 128), (256, 64)])
+def test_shared_prefix_by_large_tiles(qm, dev, D, T, qt, ct):
+    """One of so many products that it has a launch of its own."""
+    prefix_len = int((8e9 if ct == E4M3 else 3.2e9) / (T * 32 * D)) + 77
+    shared(qm, dev, qt, ct, D, T, 32, 2, 1, prefix_len, 64, sizes=(1.0, 0.3))
+    shared(qm, dev, qt, ct, D, T // 3, 32, 2, 3, prefix_len, 64, F32)
+
+
 # ---- chosen pages
 @pytest.mark.parametrize("ws", [True, False])
 @pytest.mark.parametrize("qt,ct", KINDS)
