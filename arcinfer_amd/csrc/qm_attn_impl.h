@@ -218,7 +218,7 @@ __global__ __launch_bounds__(256, 2) void attn_kernel(AttnArgs a) {
   // (rows: tokens; a row of the tile is token r / G, query head h G + r % G)
   const int nrows = rows * a.G, first = rt * RT, last = min(first + RT, nrows) - 1;
   const int capacity = shared ? 0 : (int)min((long long)a.s.W << kv.lg, 0x7fffffffLL);
-  const int len = shared ? 0 : __builtin_amdgcn_readfirstlane(a.s.len[b]) - after;
+  const int len = shared ? 0 : __builtin_amdgcn_readfirstlane(length_of(a.s, b)) - after;
   // keys that the tile's first and last tokens see of their own
   const int lo_lim = min(max(len - rows + first / a.G + 1, 0), capacity);
   const int hi_lim = min(max(len - rows + last / a.G + 1, 0), capacity);

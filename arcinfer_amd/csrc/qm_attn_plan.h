@@ -34,9 +34,12 @@ __device__ __forceinline__ int sequence_of(const Seqs& s, int t) {
   return lo < s.B && t - row_from(s, lo) < rows_of(s, lo) && t >= row_from(s, lo) ? lo : -1;
 }
 
+// Tokens of a sequence (lengths below zero are zero: sums of them stay within 32 bits)
+__device__ __forceinline__ int length_of(const Seqs& s, int b) { return max(s.len[b], 0); }
+
 // Blocks of 128 keys of sequence b, the prefix in front of them (below 2^25: a prefix and a table hold 2^30 keys each)
 __device__ __forceinline__ int blocks_of(const AttnArgs& a, int b) {
-  const int most = a.s.W << a.kv.lg, n = min(max(a.s.len[b], 0), most);
+  const int most = a.s.W << a.kv.lg, n = min(length_of(a.s, b), most);
   return (int)(((unsigned)(n + 31) / 32 + (a.shared ? 0u : (unsigned)(a.prefix_len + 31) / 32) + 3) / 4);
 }
 
@@ -102,7 +105,7 @@ __device__ __forceinline__ Tail tail_of(const AttnArgs& a, int RT) {
 // Blocks of 128 keys that a row tile's last row sees (the prefix's among them, if it reads them), and of a piece of them
 __device__ __forceinline__ int tile_blocks(const AttnArgs& a, int RT, int b, int rt, int rows) {
   const int last = min((rt + 1) * RT, rows * a.G) - 1, most = (int)min((long long)a.s.W << a.kv.lg, 0x7fffffffLL);
-  const int seen = min(max(a.s.len[b] - rows + last / a.G + 1, 0), most);
+  const int seen = min(max(length_of(a.s, b) - rows + last / a.G + 1, 0), most);
   return (int)(((unsigned)(seen + kBlock - 1) / kBlock + (a.shared ? 0u : (unsigned)(a.prefix_len + kBlock - 1) / kBlock) + kWaves - 1) / kWaves);
 }
 __device__ __forceinline__ int part_blocks(int blocks, int parts) { return parts > 1 ? max((blocks + parts - 1) / parts, kLeastPart) : kWhole; }

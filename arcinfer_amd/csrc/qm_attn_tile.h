@@ -86,7 +86,7 @@ __global__ __launch_bounds__(256, 2) void attn_tile_kernel(AttnArgs a) {
   }
   const int nrows = rows * a.G, first = rt * RT, last = min(first + RT, nrows) - 1;
   const int capacity = shared ? 0 : (int)min((long long)a.s.W << kv.lg, 0x7fffffffLL);
-  const int len = shared ? 0 : __builtin_amdgcn_readfirstlane(a.s.len[b]);
+  const int len = shared ? 0 : __builtin_amdgcn_readfirstlane(length_of(a.s, b));
   const auto limit_of = [&](int r) { return min(max(len - rows + r / a.G + 1, 0), capacity); };  // keys that row r sees of its own
   const int lo_lim = limit_of(first), hi_lim = limit_of(last);
   int lim[MT];

@@ -14,7 +14,7 @@ namespace {
 __device__ __forceinline__ int pages_seen(const SelectArgs& a, int t, int& b) {
   b = sequence_of(a.s, t);
   if (b < 0) return 0;
-  const int at = a.s.len[b] - (row_from(a.s, b) + rows_of(a.s, b) - t);  // the token's place
+  const int at = length_of(a.s, b) - (row_from(a.s, b) + rows_of(a.s, b) - t);  // the token's place
   return at < 0 ? 0 : min((at >> a.kv.lg) + 1, a.s.W);
 }
 

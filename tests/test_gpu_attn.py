@@ -503,6 +503,55 @@ def test_shared_prefix_by_large_tiles(qm, dev, D, T, qt, ct):
     shared(qm, dev, qt, ct, D, T // 3, 32, 2, 3, prefix_len, 64, F32)
 
 
+def test_many_rows_scales(qm, dev):
+    for scale in (0.0, -0.3, 30.0):
+        for D in (64, 128, 256):
+            run(qm, dev, [130, 70], [60, 40], 2, 1, D, 16, F16, F16, scale=scale, out=F32)
+            run(qm, dev, [130, 70], [60, 40], 2, 1, D, 16, BF16, E4M3, scale=scale)
+
+
+def test_many_rows_q_and_o_strides(qm, dev):
+    """Rows of a wider matrix, at any element; nothing else is written."""
+    cache = K.Cache(20, 2, 16, 128, BF16, 3)
+    start, ln, table, _ = K.batch([90, 70], [66, 41], 16, 20, 3)
+    q = queries(107, 4, 128, BF16, 4)
+    kv = cache.on(qm, dev)
+    args = (kv, ln.to(dev), table.to(dev))
+    for out in (BF16, F32):
+        want = qm.attn_prefix(q.to(dev), *args, start=start.to(dev), out=out)
+        for off in (8, 3):
+            wide = torch.full((107, 700), 9.0, dtype=BF16, device=dev)
+            rows = wide.as_strided((107, 4, 128), (700, 128, 1), off)
+            rows.copy_(q)
+            got = torch.full((108, 601), -3.0, dtype=out, device=dev)
+            for ws in (None, qm.attn_workspace(kv, 107, 2, 4)):
+                o = qm.attn_prefix(rows, *args, start=start.to(dev), o=got.as_strided((107, 4, 128), (601, 128, 1), off), ws=ws)
+                if ws is None:
+                    assert torch.equal(o, want)
+            assert bool((got[107] == -3).all()) and bool((got[:, :off] == -3).all()) and bool((got[:, off + 512:] == -3).all())
+
+
+@pytest.mark.parametrize("rows", [1, 70])
+def test_lengths_of_any_value(qm, dev, rows):
+    """The least and the largest lengths: none of the keys, and all that the table holds."""
+    cache = K.Cache(10, 1, 16, 64, BF16, 5, mean=True)
+    kv = cache.on(qm, dev)
+    table = torch.tensor([[1, 2, 3], [4, 5, 6], [7, 8, 9]], dtype=torch.int32)
+    ln = torch.tensor([-2 ** 31, 2 ** 31 - 1, -2 ** 31 + 5], dtype=torch.int32)
+    start = torch.tensor([0, 1, 2, 3], dtype=torch.int32) * rows
+    q = queries(3 * rows, 2, 64, BF16, 6)
+    args = (q.to(dev), kv, ln.to(dev), table.to(dev))
+    want, bound = K.attention(q, cache, start, ln.clamp(min=0), table, BF16)
+    for ws in (None, qm.attn_workspace(kv, 3 * rows, 3, 2)):
+        o = qm.attn_prefix(*args, start=start.to(dev), ws=ws)
+        K.check(o, want, bound, BF16)
+        assert not o[:rows].any() and not o[2 * rows:].any() and o[rows:2 * rows].any(2).all()
+    sel = qm.select_pages(*args, 2, start=start.to(dev))
+    assert bool((sel[:rows] == -1).all()) and bool((sel[2 * rows:] == -1).all()) and bool((sel[rows:2 * rows] >= 0).all())
+    o = qm.attn_pages(*args, torch.tensor([0, 1, 2], dtype=torch.int32, device=dev).expand(3 * rows, 1, 3).contiguous(), start=start.to(dev))
+    K.check(o, want, bound, BF16)
+
+
 # ---- chosen pages
 @pytest.mark.parametrize("ws", [True, False])
 @pytest.mark.parametrize("qt,ct", KINDS)
