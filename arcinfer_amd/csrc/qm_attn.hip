@@ -190,7 +190,7 @@ namespace {
 // start and end, are kept to one round (12 sequences of 580 to 17200 tokens, 24 heads of 256 over 4: 64 us against 77; attn_kernel 74 against 71).
 constexpr int kTarget = 512;  // (attn_tile_kernel's 64 us: 80 by 256 pieces, 78 by 1024)
 // Pieces of the shared prefix: one work-group a CU beside the sequences' own keys (48 sequences behind 8192 tokens 46 us, 16 behind 65000 60; 128 pieces
-// 59 and 96)
+// 59 and 96; 512 51 and 59). In a launch of its own as many as any call's (768 rows behind 16384: 92 us, 105 by 256 pieces).
 constexpr int kSharedTarget = 256;
 // Bytes of a prefix, read once more for each further sequence, from which it is read once for all: below, the pieces' join takes longer than that.
 // 8 heads of 128, bf16, 500 tokens of their own, us: 8 sequences x 256 tokens 16.9 against 14.7, x 1024 17.3 against 16.9; 48 x 256 27.8 against 32.0,
@@ -199,9 +199,9 @@ constexpr double kSharedBytes = 3.2e7;
 constexpr int kTailMost = 2;        // rounds of work-groups from which the last one is not cut (6656 tokens, 3.3 rounds: 362 us cut, 359 not)
 constexpr int kSharedRows = 64;     // rows of the batch from which attn_tile_kernel may take a prefix
 // Products of a prefix (rows of all heads times keys times D) from which it does, in a launch of its own: below, attn_kernel's tiles in the
-// sequences' own launch take less. 8 heads of 128, rows of a head x keys, us: 192 x 2048 31 against 21, 192 x 16384 45.7 against 44.0, 384 x 16384
-// 65 against 85, 768 x 16384 106 against 158; D 256, 384 x 8192: 68 against 99. Behind 8-bit caches 192 x 16384 54 against 46, 512 x 16384 89 against 92.
-constexpr double kSharedFrom16 = 3.2e9, kSharedFrom8 = 8e9;
+// sequences' own launch take less. 8 heads of 128, rows of a head x keys, us: 192 x 2048 31 against 21, 192 x 16384 47 against 44, 384 x 16384
+// 63 against 85, 768 x 16384 92 against 158; D 256, 384 x 8192: 67 against 99. Behind 8-bit caches 192 x 16384 53 against 46, 512 x 16384 79 against 92.
+constexpr double kSharedFrom16 = 4e9, kSharedFrom8 = 6e9;
 
 long long div_up(long long a, long long b) { return (a + b - 1) / b; }
 // Rows of attn_kernel's tile: what its registers hold
@@ -248,7 +248,7 @@ AttnPlan attn_plan(int T, int B, bool start, bool chosen, bool e8, int HQ, int H
     }
     p.shared_tiles = (int)div_up((long long)T * G, p.shared_rt);
     const int blocks = (int)div_up(prefix_len, 128);
-    long long n = kSharedTarget / ((long long)HK * p.shared_tiles);
+    long long n = (p.shared_tile ? kTarget : kSharedTarget) / ((long long)HK * p.shared_tiles);
     if (n > blocks) n = blocks;
     if (n < 1) n = 1;
     p.shared_blocks = (int)div_up(blocks, n);

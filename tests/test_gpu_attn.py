@@ -498,7 +498,7 @@ def test_shared_prefix(qm, dev, D, B, HQ, n, qt, ct):
 @pytest.mark.parametrize("D,T", [(64, 256), (96, 192), (128, 128), (256, 64)])
 def test_shared_prefix_by_large_tiles(qm, dev, D, T, qt, ct):
     """One of so many products that it has a launch of its own."""
-    prefix_len = int((8e9 if ct == E4M3 else 3.2e9) / (T * 32 * D)) + 77
+    prefix_len = int((6e9 if ct == E4M3 else 4e9) / (T * 32 * D)) + 77
     shared(qm, dev, qt, ct, D, T, 32, 2, 1, prefix_len, 64, sizes=(1.0, 0.3))
     shared(qm, dev, qt, ct, D, T // 3, 32, 2, 3, prefix_len, 64, F32)
 
