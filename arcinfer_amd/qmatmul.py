@@ -742,48 +742,65 @@ def _check_cache(fn, kv, dev):
         _refuse(fn, "the cache is not on the current GPU")
 
 
+_rotations = {}  # QmRope by what it says
+
+
 def kv_append(x, HQ, kv, slots, pos, inv_freq, wq=None, wk=None, eps=1e-6, adjacent=False, sections=None, turns=False, scale=1.0,
               q_off=0, q_hs=None, k_off=None, k_hs=None, v_off=None, v_hs=None, q=None, out=None, stream=None):
     """qk_norm_rope of rows x [T, ldx] with the keys and the value heads (neither normed nor turned) to a KvCache: token t to its place
     slots[t] (int32 [T]: page * tokens of a page + place in it; one outside the cache, as a negative one, is not stored; no two the same).
     Value head h is at column v_off + h * v_hs (behind the key heads unless given). With kv.mean: the mean key of each page whose last
     token is among these. Returns q [T, HQ, D] of type out (that of a given q, else the cache's, bfloat16 for an 8-bit one), or the q given."""
+    # (Appending a few tokens takes the GPU 5 us: each check is made in the cheapest way, and only what fails it goes to the functions that say why.)
     fn = "qmatmul_kv_append"
     dev = _current_gpu()
     torch = _torch
-    f32 = torch.float32
     D, HK = kv.D, kv.heads
-    _check_cache(fn, kv, dev)
-    _check_rows(fn, "x", x, 2, dev)
+    if kv.device_index != dev:
+        _check_cache(fn, kv, dev)
+    sx, sp, one = x.stride(), pos.stride(), (1,)
+    if x.get_device() != dev or len(sx) != 2 or sx[1] != 1:
+        _check_rows(fn, "x", x, 2, dev)
     T, width = x.shape
-    _check_int32(fn, "slots", slots, 1, dev)
-    axes, half = 1 if pos.dim() == 1 else pos.size(0), inv_freq.numel()
-    _check_rows(fn, "pos", pos, None, dev)
-    _check_rows(fn, "inv_freq", inv_freq, 1, dev)
-    if pos.dtype != torch.int32 or pos.dim() not in (1, 2) or pos.shape[-1] != T or slots.numel() != T:
+    if slots.get_device() != dev or slots.dtype != torch.int32 or slots.stride() != one:
+        _check_int32(fn, "slots", slots, 1, dev)
+    axes, half = 1, inv_freq.numel()
+    if len(sp) != 1:
+        axes = pos.size(0)
+    if pos.get_device() != dev or sp[-1] != 1:
+        _check_rows(fn, "pos", pos, None, dev)
+    if inv_freq.get_device() != dev or inv_freq.stride() != one:
+        _check_rows(fn, "inv_freq", inv_freq, 1, dev)
+    if pos.dtype != torch.int32 or len(sp) > 2 or pos.shape[-1] != T or slots.numel() != T:
         _refuse(fn, f"pos {tuple(pos.shape)} {pos.dtype}, slots {tuple(slots.shape)}: int32, one column for each of {T} tokens")
+    f32 = torch.float32
     if inv_freq.dtype != f32:
         _refuse(fn, f"inv_freq {inv_freq.dtype}: float32")
     for w in (wq, wk):
         if w is not None:
-            _check_rows(fn, "wq or wk", w, 1, dev)
+            if w.get_device() != dev or w.stride() != one:
+                _check_rows(fn, "wq or wk", w, 1, dev)
             if w.dtype != f32 or w.numel() != D:
                 _refuse(fn, f"wq or wk {tuple(w.shape)} {w.dtype}: float32 [{D}]")
     if sections is None:
         sections = (half,)
     if len(sections) != axes or axes > 4 or sum(sections) != half:
         _refuse(fn, f"sections {sections}: one for each of {axes} axes (at most 4), their sum {half}")
-    q_hs, k_hs, v_hs = (D if hs is None else hs for hs in (q_hs, k_hs, v_hs))
+    if q_hs is None:
+        q_hs = D
+    if k_hs is None:
+        k_hs = D
+    if v_hs is None:
+        v_hs = D
     if k_off is None:
         k_off = q_off + HQ * q_hs
     if v_off is None:
         v_off = k_off + HK * k_hs
-    ldx, ps = x.stride(0) if T > 1 else _row_stride(x), pos.stride(0) if axes > 1 else T
+    ldx, ps = sx[0] if T > 1 else _row_stride(x), sp[0] if axes > 1 else T
     if (T | HQ | ldx | ps | q_off | q_hs | k_off | k_hs | v_off | v_hs | 2 * half) >> 31 or (axes > 1 and min(sections) < 0):
         _sizes(fn, T, HQ, ldx, ps, q_off, q_hs, k_off, k_hs, v_off, v_hs, 2 * half, *sections)
         if HQ < 0:
             _refuse(fn, f"HQ {HQ}")
-    rope = QmRope(2 * half, adjacent, axes, turns, tuple(sections), scale)
     if max(q_off + (HQ - 1) * q_hs if HQ else 0, k_off + (HK - 1) * k_hs, v_off + (HK - 1) * v_hs) + D > width:
         _refuse(fn, f"rows of {width} elements do not hold the heads")
     if out is None:
@@ -792,8 +809,14 @@ def kv_append(x, HQ, kv, slots, pos, inv_freq, wq=None, wk=None, eps=1e-6, adjac
         q, ldq = x.new_empty((T, HQ, D), dtype=out), HQ * D
     else:
         ldq = _head_rows(fn, "q", q, T, HQ, D, out, dev)
+    how = (2 * half, adjacent, turns, scale, *sections)
+    rope = _rotations.get(how)
+    if rope is None:
+        if len(_rotations) >= 64:
+            _rotations.clear()
+        rope = _rotations[how] = ctypes.pointer(QmRope(2 * half, adjacent, axes, turns, tuple(sections), scale))
     st = _function(fn)(x.data_ptr(), _dtype(x.dtype), ldx, T, q_off, q_hs, HQ, k_off, k_hs, v_off, v_hs,
-                       None if wq is None else wq.data_ptr(), None if wk is None else wk.data_ptr(), eps, ctypes.byref(rope),
+                       None if wq is None else wq.data_ptr(), None if wk is None else wk.data_ptr(), eps, rope,
                        pos.data_ptr(), ps, inv_freq.data_ptr(), slots.data_ptr(), kv.ref, q.data_ptr(), _dtype(out), ldq,
                        _current_stream(dev) if stream is None else stream)
     _done(fn, st)
