@@ -196,16 +196,24 @@ __global__ __launch_bounds__(256, 2) void attn_tile_kernel(AttnArgs a) {
   v4i kr[DIRECT ? 1 : KL];
   vvec vr[4];
   v4f ks, vs;
+  // (16-bit) the group's keys and values as buffers; nothing of them is in range where there is no such step
+  struct Aim {
+    __amdgpu_buffer_rsrc_t k, v;
+  };
+  const auto aim = [&](const Place& at, bool there) {
+    const unsigned range = !there ? 0 : at.edge < 16 ? (unsigned)at.edge * (unsigned)ts : 15u * (unsigned)ts + 2u * kv.D;
+    return Aim{buffer_at((const char*)kv.k + at.base, range), buffer_at((const char*)kv.v + at.base, range)};
+  };
+  const auto fetch = [&](const Aim& from, Step& to, int t) {  // t of KT loads of each
+    const int n = (mine * KS + half * KT + t) * 64;
+    to_lds(from.k, to.k + n, k_off[t]);
+    to_lds(from.v, to.v + n, v_off[t]);
+  };
   const auto load = [&](const Place& at, Step& to, Notes& note) {
     if constexpr (DIRECT) {
-      const unsigned range = at.edge < 16 ? (unsigned)at.edge * (unsigned)ts : 15u * (unsigned)ts + 2u * kv.D;
-      const __amdgpu_buffer_rsrc_t kb = buffer_at((const char*)kv.k + at.base, range), vb = buffer_at((const char*)kv.v + at.base, range);
+      const Aim from = aim(at, true);
 #pragma unroll
-      for (int t = 0; t < KT; ++t) {
-        const int n = (mine * KS + half * KT + t) * 64;
-        to_lds(kb, to.k + n, k_off[t]);
-        to_lds(vb, to.v + n, v_off[t]);
-      }
+      for (int t = 0; t < KT; ++t) fetch(from, to, t);
       if (lane == 0) note.flags[wave] = at.dead;
     } else {
 #pragma unroll
@@ -296,8 +304,15 @@ __global__ __launch_bounds__(256, 2) void attn_tile_kernel(AttnArgs a) {
   __builtin_amdgcn_s_waitcnt(kNoLoads);
   __syncthreads();
   const auto work = [&](int i, Step& cur, Step& other, const Notes& note, Notes& other_note) __attribute__((always_inline)) {
-    if (i + NB < end) load(next, other, other_note);
+    // (16-bit: between the first product's matrix instructions: a work-group's 32 KB at once would keep each wave for 580 cycles)
+    if constexpr (!DIRECT)
+      if (i + NB < end) load(next, other, other_note);
     const Place coming = next;
+    Aim from;
+    if constexpr (DIRECT) {
+      from = aim(next, i + NB < end);
+      if (lane == 0) other_note.flags[wave] = next.dead;
+    }
     // S^T. Operands are read from LDS four ahead of the products that take them (the compiler would read each and wait for it).
     v4i op[2][kAheadOps];
     constexpr int NK = NB * 2 * KS, NV = NB * VB * VE;
@@ -320,6 +335,11 @@ __global__ __launch_bounds__(256, 2) void attn_tile_kernel(AttnArgs a) {
 #pragma unroll
     for (int n = 0; n < NK / kAheadOps; ++n) {
       if ((n + 1) * kAheadOps < NK) read_k(n + 1);
+      if constexpr (DIRECT) {
+        static_assert(NK / kAheadOps == KT, "a load of each beside every four operands");
+        fetch(from, other, n);
+        __builtin_amdgcn_sched_barrier(kFree);
+      }
 #pragma unroll
       for (int u = 0; u < kAheadOps; ++u) {
         const int nb = (n * kAheadOps + u) / (2 * KS), t = (n * kAheadOps + u) % (2 * KS) / 2, s = u & 1;
