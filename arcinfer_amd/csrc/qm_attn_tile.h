@@ -9,9 +9,9 @@
 // the step before (scalar instructions, between matrix instructions).
 //
 // The logits stay unscaled: e^(scale (s - m)) is one fma and one v_exp, the maximum is that of s (for a scale below zero -q is taken). What bounds it: the
-// matrix pipe (64 keys of 128 by a wave's 32 rows: 1024 cycles, of which 42 % of the time is made) with the vector instructions (160, and 32 exponentials of
-// four times an instruction's time) beside it, which two waves on a SIMD overlap in part. Measured, 32 heads of 128 over 8, bf16: the last 4096 of 16384 tokens
-// 907 us (1060 Tflop/s of what they see), 4096 of 4096 155 us; f32 results, three parts of each weight, 1533 us; a large library product reaches 1250.
+// matrix pipe (64 keys of 128 by a wave's 32 rows: 1024 cycles, 46 % of the time at the full clock) with the vector instructions (160, and 32 exponentials of
+// four times an instruction's time) beside it. Measured, 32 heads of 128 over 8, bf16: the last 4096 of 16384 tokens 838 us (1150 Tflop/s of what they
+// see), 4096 of 4096 141 us; f32 results, three parts of each weight, 1405 us; a large library product reaches 1250.
 // Tried and not kept: the next scores' products between this block's exponentials (as fast with three parts, 5 % slower with one), values through
 // registers for 16-bit caches too (1016 us).
 #pragma once
@@ -28,6 +28,7 @@ __device__ __forceinline__ void to_lds(__amdgpu_buffer_rsrc_t from, v4i* to, uns
 typedef short v4s __attribute__((ext_vector_type(4)));
 typedef int v2i __attribute__((ext_vector_type(2)));
 __device__ __forceinline__ v2i transposed(const void* p) { return __builtin_bit_cast(v2i, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) v4s*)p)); }
+constexpr int kBetween = 4;  // vector instructions between two matrix instructions: as long as one takes
 constexpr int kNoLoads = 0x0F70;  // (s_waitcnt: no vector load under way)
 constexpr int kFree = 6;      // vector and scalar arithmetic, that the compiler may move past these reads
 
@@ -315,7 +316,7 @@ __global__ __launch_bounds__(256, 2) void attn_tile_kernel(AttnArgs a) {
     }
     // S^T. Operands are read from LDS four ahead of the products that take them (the compiler would read each and wait for it).
     v4i op[2][kAheadOps];
-    constexpr int NK = NB * 2 * KS, NV = NB * VB * VE;
+    constexpr int NK = NB * 2 * KS, NV = NB * VB * VE, VC = VB * VE / kAheadOps;
     const auto read_k = [&](int n) {
 #pragma unroll
       for (int u = 0; u < kAheadOps; ++u) {
@@ -327,7 +328,6 @@ __global__ __launch_bounds__(256, 2) void attn_tile_kernel(AttnArgs a) {
     const auto read_v = [&](int n) {
 #pragma unroll
       for (int u = 0; u < kAheadOps; ++u) op[n & 1][u] = value(cur, (n * kAheadOps + u) / (VB * VE), (n * kAheadOps + u) % (VB * VE));
-      __builtin_amdgcn_sched_barrier(kFree);
     };
     v4f x[NB][2][MT];
     read_k(0);
@@ -427,8 +427,7 @@ __global__ __launch_bounds__(256, 2) void attn_tile_kernel(AttnArgs a) {
       }
     }
     float w[NB][MT][8];
-#pragma unroll
-    for (int nb = 0; nb < NB; ++nb)
+    const auto weights = [&](int nb) {
 #pragma unroll
       for (int m = 0; m < MT; ++m) {
         const float from = (mx[m] == kMinusInf ? 0.0f : mx[m]) - kBias;
@@ -439,6 +438,8 @@ __global__ __launch_bounds__(256, 2) void attn_tile_kernel(AttnArgs a) {
           if constexpr (E8) w[nb][m][e] *= vsc[nb][e >> 2][e & 3];
         }
       }
+    };
+    weights(0);
     // Values that are not finite, of keys that some rows see and others do not: as in attn_kernel, counted apart, and zeros in the product (in LDS:
     // the work-group's waves all come here, or none does)
     if (__builtin_expect(odd, 0)) {
@@ -480,8 +481,8 @@ __global__ __launch_bounds__(256, 2) void attn_tile_kernel(AttnArgs a) {
       __syncthreads();
       read_v(0);
     }
-    // (of two waves on a SIMD, the one that has its weights goes first: the last 4096 of 16384 tokens 907 us against 943, f32 1533 against 1600; both
-    // products: 941)
+    // (of two waves on a SIMD, the one that has its weights goes first: the last 4096 of 16384 tokens 907 us against 943, f32 1533 against 1600, as
+    // this was then; both products: 941)
     __builtin_amdgcn_s_setprio(1);
     v4i p[PARTS][MT];
 #pragma unroll
@@ -496,7 +497,10 @@ __global__ __launch_bounds__(256, 2) void attn_tile_kernel(AttnArgs a) {
           }
       }
       if ((n + 1) * kAheadOps < NV) read_v(n + 1);
+      // (the second block's weights between the first one's products: 838 us against 843, f32 1405 against 1421)
+      if (NB == 2 && n == 0) weights(NB - 1);
       if (n == 0) next = place(asked);
+      if (NB == 1 || n >= VC) __builtin_amdgcn_sched_barrier(kFree);
 #pragma unroll
       for (int r = 0; r < PARTS; ++r)
 #pragma unroll
@@ -505,7 +509,19 @@ __global__ __launch_bounds__(256, 2) void attn_tile_kernel(AttnArgs a) {
 #pragma unroll
           for (int m = 0; m < MT; ++m) o[vb][j][m] = mfma16<TP>(op[n & 1][u], p[r][m], o[vb][j][m]);
         }
-      __builtin_amdgcn_sched_barrier(kFree);
+      if (NB == 1 || n >= VC) __builtin_amdgcn_sched_barrier(kFree);
+      if (NB == 2 && n == VC - 1) {
+#pragma unroll
+        for (int c = 0; c < VC; ++c) {
+          __builtin_amdgcn_sched_group_barrier(0x100, (DIRECT ? 2 : 1) * kAheadOps, 0);
+#pragma unroll
+          for (int u = 0; u < kAheadOps * MT * PARTS; ++u) {
+            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+            __builtin_amdgcn_sched_group_barrier(0x402, kBetween, 0);
+          }
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      }
     }
     __builtin_amdgcn_s_setprio(0);
     if (i + NB < end) keep(coming, other, other_note);
