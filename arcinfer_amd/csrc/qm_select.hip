@@ -27,7 +27,7 @@ __device__ __forceinline__ unsigned long long ordered(double s) {
 
 typedef double v4d __attribute__((ext_vector_type(4)));
 
-// Scores of 64 tiles pages of one token and key head a work-group, 16 at a time a wave: a product of 16 pages by 16 query heads on the f64 matrix
+// Scores of the pages of one token and key head, every chunks-th 64 of them a work-group, 16 at a time a wave: a product of 16 pages by 16 query heads on the f64 matrix
 // pipe, four elements of the heads at a time. Lane (c, g) holds elements g D / 4 .. of page c and of head c (the sum does not depend on which four
 // meet), four of them a load; the next pages' means are asked for before this product. The result's rows, in the order g + 4 i, are
 // the pages, its columns the heads. Few pages: latency-bound; many: bound by the pipe, 64 cycles an instruction (16 pages of 128 elements
@@ -49,15 +49,15 @@ __device__ __forceinline__ double max16(double v) {
 }
 
 template <typename TQ>
-__global__ __launch_bounds__(256) void page_score_kernel(SelectArgs a, int chunks, int tiles) {
+__global__ __launch_bounds__(256) void page_score_kernel(SelectArgs a, int chunks) {
   typedef __bf16 v4b __attribute__((ext_vector_type(4)));
   typedef TQ v4q __attribute__((ext_vector_type(4)));
   const int item = blockIdx.x / chunks, h = item % a.kv.HK, t = item / a.kv.HK, D = a.kv.D;
-  const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4, first = (int)(blockIdx.x % chunks) * 64 * tiles + 16 * (threadIdx.x >> 6);
+  const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4, first = (int)(blockIdx.x % chunks) * 64 + 16 * (threadIdx.x >> 6), step = 64 * chunks;
   int b;
   const int n = pages_seen(a, t, b);
   if (n <= a.k || first >= n) return;
-  const int steps = D / 16, end = min(n, first + 64 * (tiles - 1) + 1);
+  const int steps = D / 16;
   const bool qvec = ((uintptr_t)a.q & 7) == 0 && (a.ldq & 3) == 0;
   v4b m[kChunks];
   v4q q[kChunks];
@@ -77,11 +77,11 @@ __global__ __launch_bounds__(256) void page_score_kernel(SelectArgs a, int chunk
         else q[i] = v4q{p[4 * i], p[4 * i + 1], p[4 * i + 2], p[4 * i + 3]};
       }
   };
-  int page = page_of(first + c), next = page_of(first + 64 + c);
+  int page = page_of(first + c), next = page_of(first + step + c);
   load_heads(0);
   load_means(page);
-  for (int j0 = first; j0 < end; j0 += 64) {
-    const int after = page_of(j0 + 128 + c);
+  for (int j0 = first; j0 < n; j0 += step) {
+    const int after = page_of(j0 + 2 * step + c);
     v4d best = -__builtin_inf();
     for (int g0 = 0; g0 < a.G; g0 += 16) {
       if (g0 || (j0 > first && a.G > 16)) load_heads(g0);
@@ -282,20 +282,21 @@ __global__ __launch_bounds__(256) void page_pick_kernel(SelectArgs a) {
   }
 }
 
-// Pages of a wave: 16, and up to eight times as many where the chip has waves enough all the same (sequences of 60000 tokens, 8 heads of 128, us: 64 of them
-// 71 against 83 with 16 pages a wave, 128 127 against 148; 32 of 4000 to 60000, whose shorter ones leave waves idle, 28 against 38 with 112)
-static int score_tiles(long long items, int W) {
-  const long long n = items * ((W + 63) / 64) / 2048;
-  return n < 1 ? 1 : n > 8 ? 8 : (int)n;
+// Work-groups of all tokens and key heads, as many as the chip holds (four a CU) and some: each takes its pages in turn, as many as the sequence has (sequences of
+// 60000 tokens, 8 heads of 128: 32 of them 44 us, with a work-group for every 64 pages 51; 128 116 against 127; 64 of them with 4 heads of 256 69 against 95)
+constexpr int kScoreTarget = 1280;
+static int score_chunks(long long items, int W) {
+  const long long most = (W + 63) / 64, n = kScoreTarget / items;
+  return (int)(n < 1 ? 1 : n < most ? n : most);
 }
 long long select_grid(int T, int HK, int W) { return (long long)T * HK * ((W + 63) / 64); }
 
 hipError_t launch_select(const SelectArgs& a, hipStream_t s) {
   const unsigned items = (unsigned)(a.s.T * a.kv.HK);
   if (a.s.W > a.k) {
-    const int tiles = score_tiles(items, a.s.W), chunks = (a.s.W + 64 * tiles - 1) / (64 * tiles);
-    if (a.qtype == DT_F16) page_score_kernel<_Float16><<<items * chunks, 256, 0, s>>>(a, chunks, tiles);
-    else page_score_kernel<__bf16><<<items * chunks, 256, 0, s>>>(a, chunks, tiles);
+    const int chunks = score_chunks(items, a.s.W);
+    if (a.qtype == DT_F16) page_score_kernel<_Float16><<<items * chunks, 256, 0, s>>>(a, chunks);
+    else page_score_kernel<__bf16><<<items * chunks, 256, 0, s>>>(a, chunks);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
   }
