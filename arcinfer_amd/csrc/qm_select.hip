@@ -289,7 +289,7 @@ static int score_chunks(long long items, int W) {
   const long long most = (W + 63) / 64, n = kScoreTarget / items;
   return (int)(n < 1 ? 1 : n < most ? n : most);
 }
-long long select_grid(int T, int HK, int W) { return (long long)T * HK * ((W + 63) / 64); }
+long long select_grid(int T, int HK, int W) { return (long long)T * HK * score_chunks((long long)T * HK, W); }
 
 hipError_t launch_select(const SelectArgs& a, hipStream_t s) {
   const unsigned items = (unsigned)(a.s.T * a.kv.HK);

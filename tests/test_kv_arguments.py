@@ -125,7 +125,8 @@ def test_choice(qm, p):
                 dict(ws=p + 0x62000), dict(sel=p + 0x80000)):
         assert call(**bad) == ARG, bad
     assert call(ws=None) == WORKSPACE and call(wsb=2 * 2 * 4 * 8 - 1) == WORKSPACE
-    assert call(T=2 ** 22, B=2 ** 22, stride=2 ** 16) == SHAPE  # (more than a grid holds)
+    assert call(T=2 ** 24, B=2 ** 24, stride=2 ** 16) == SHAPE  # (more than a grid holds)
+    assert call(T=2 ** 22, B=2 ** 22, stride=2 ** 16) == WORKSPACE
 
 
 def test_appending(qm, p):
