@@ -43,6 +43,19 @@ def test_long_tables(qm, dev, n):
         assert torch.equal(got.cpu(), K.chosen(q, cache, start, ln, table, k, 0, 1)), k
 
 
+@pytest.mark.parametrize("new,HK,n", [([60, 40], 4, 700), ([900, 500], 1, 150), ([1, 1], 1, 2000)])
+def test_work_groups_that_take_several_pages(qm, dev, new, HK, n):
+    """More 64s of pages than work-groups of a token and key head: three, one, and all of them."""
+    D, page = 32, 16
+    lens = [n * page - 3, n * page // 3]
+    cache = K.Cache(n + n // 3 + 4, HK, page, D, BF16, n, mean=True)
+    start, ln, table, _ = K.batch(lens, new, page, cache.pages, n)
+    q = queries(sum(new), 2 * HK, D, BF16, 5)
+    kv = cache.on(qm, dev)
+    got = qm.select_pages(q.to(dev), kv, ln.to(dev), table.to(dev), 9, start=start.to(dev))
+    assert torch.equal(got.cpu(), K.chosen(q, cache, start, ln, table, 9, 1, 1))
+
+
 def test_ties_and_special_scores(qm, dev):
     """Equal scores go to the lower page, zeros of either sign are one; scores that differ in their last bits are told apart; NaN and pages that
     are none come last, minus infinity among them, plus infinity first."""
