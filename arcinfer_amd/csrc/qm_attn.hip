@@ -259,7 +259,9 @@ AttnPlan attn_plan(int T, int B, bool start, bool chosen, bool e8, int HQ, int H
   const long long left = ((long long)have - (long long)shared_bytes(p, HK, D)) / (long long)slot_bytes(p.rt, D) - items;
   // (pieces of all row tiles are at most the target and one more for each of them; row tiles that fill the chip are left whole)
   if (left > 0 && items < (p.tile ? kTarget / 2 : 2 * kTarget)) {
-    const long long want = p.tile ? kTarget - items : kTarget;
+    // (beside a prefix's work-groups half as many: 32 sequences of 300 tokens behind 4096 24 us against 31, 4 of 4000 behind 16384 31 against 36; 48 of 16 to 1500
+    // behind 8192 47 against 46)
+    const long long want = p.tile ? kTarget - items : p.shared && !p.shared_tile ? kTarget / 2 : kTarget;
     p.target = (int)(left < want ? left : want);
   }
   p.slots = p.target || p.shared ? (int)(items + p.target) : 0;
