@@ -552,6 +552,37 @@ def test_lengths_of_any_value(qm, dev, rows):
     K.check(o, want, bound, BF16)
 
 
+@pytest.mark.parametrize("B,HK,G,most,prefix_len", [(300, 4, 2, 1, 0), (1100, 1, 20, 1, 0), (400, 4, 3, 3, 0), (150, 8, 40, 2, 0), (300, 4, 4, 2, 700),
+                                                   (1100, 1, 2, 2, 300)])
+def test_batches_of_many_sequences(qm, dev, B, HK, G, most, prefix_len):
+    """More sequences than a wave adds up at once, some without rows; a few rows of the result are looked at, rows of no sequence stay."""
+    g = torch.Generator().manual_seed(B)
+    new = [1] * B if most == 1 else torch.randint(0, most + 1, (B,), generator=g).tolist()
+    lens = [max(n, 1) + i % 37 for i, n in enumerate(new)]
+    cache = K.Cache(4 * B + 60, HK, 16, 64, BF16, 1)
+    start, ln, table, rest = K.batch(lens, new, 16, cache.pages, 2)
+    prefix = torch.tensor(rest[:(prefix_len + 15) // 16], dtype=torch.int32)
+    T = int(start[-1])
+    q = queries(T + 3, HK * G, 64, BF16, 3)
+    kv = cache.on(qm, dev)
+    some = sorted({0, 1, T // 3, T // 2, T - 2, T - 1})
+    of = [int(torch.searchsorted(start[1:], t, right=True)) for t in some]
+    see = [lens[b] - (int(start[b + 1]) - t) + 1 for t, b in zip(some, of)]
+    want, bound = K.attention(q[some], cache, torch.arange(len(some) + 1), torch.tensor(see), table[of], BF16, None, prefix, prefix_len)
+    outs = []
+    for ws in (None, qm.attn_workspace(kv, T + 3, B, HK * G, prefix_len)):
+        if most == 1:
+            o = qm.attn_prefix(q[:T].to(dev), kv, ln.to(dev), table.to(dev), ws=ws)
+        else:
+            o = torch.full((T + 3, HK * G, 64), 5.0, dtype=BF16, device=dev)
+            qm.attn_prefix(q.to(dev), kv, ln.to(dev), table.to(dev), start=start.to(dev), ws=ws, o=o, prefix=prefix.to(dev), prefix_len=prefix_len)
+            assert bool((o[T:] == 5).all())
+        K.check(o[some], want, bound, BF16)
+        outs.append(o[:T].double())
+    a, b = outs
+    assert bool(((a - b).abs() <= 2.0 ** -6 * (a.abs() + 1)).all()) and bool(a.any(2).all())
+
+
 # ---- chosen pages
 @pytest.mark.parametrize("ws", [True, False])
 @pytest.mark.parametrize("qt,ct", KINDS)
