@@ -380,6 +380,58 @@ def test_many_rows_masked_places(qm, dev, bad, D, ct):
         K.check(torch.where(hit, want.to(qt), got), want, bound, qt)
 
 
+@pytest.mark.parametrize("rows", [5, 80])
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
+def test_scales_of_masked_places(qm, dev, bad, D, rows):
+    """An 8-bit cache's scales of NaN and infinities where no row sees them, and of a key and a value that the last rows see and the others do not."""
+    cache = K.Cache(20, 1, 16, D, E4M3, 7)
+    start, ln, table, rest = K.batch([150], [rows], 16, 20, 7)
+    prefix = torch.tensor(rest[:3], dtype=torch.int32)
+    q = queries(rows, 2, D, BF16, 8)
+    want, bound = K.attention(q, cache, start, ln, table, BF16, None, prefix, 37)
+    for s in cache.scales:
+        s[int(table[0, 150 // 16]), :, 150 % 16:] = bad
+        s[rest[2], :, 37 - 32:] = bad
+        s[rest[3:]] = bad
+    more = dict(start=start.to(dev), prefix=prefix.to(dev), prefix_len=37)
+    for which, token in ((None, 150), (1, 148), (0, 147)):
+        if which is not None:
+            cache.scales[which][int(table[0, token // 16]), 0, token % 16] = bad
+        kv = cache.on(qm, dev)
+        for ws in (None, qm.attn_workspace(kv, rows, 1, 2, 37)):
+            got = qm.attn_prefix(q.to(dev), kv, ln.to(dev), table.to(dev), ws=ws, **more).cpu()
+            n = rows - (150 - token)  # rows that do not see it
+            K.check(got[:n], want[:n], bound[:n], BF16)
+            if which == 1:
+                assert not torch.isfinite(got[n:].float()).any(2).any()
+
+
+@pytest.mark.parametrize("HK,G,new,lens,prefix_len", [(2, 4, [300, 70], [900, 2000], 0), (64, 1, [1100], [1100], 0), (2, 16, [1] * 100, [40 + i for i in range(100)], 20100)])
+def test_many_rows_on_two_streams(qm, dev, HK, G, new, lens, prefix_len):
+    """Pieces, tiles of a last round that are cut, and a prefix in a launch of its own: calls on two streams at once, a workspace each, and repeated: the
+    same bits."""
+    cache = K.Cache(sum((n + 63) // 64 for n in lens) + (prefix_len + 63) // 64, HK, 64, 128, BF16, 13)
+    start, ln, table, rest = K.batch(lens, new, 64, cache.pages, 13)
+    T = int(start[-1])
+    q = queries(T, HK * G, 128, BF16, 14).to(dev)
+    kv = cache.on(qm, dev)
+    prefix = torch.tensor(rest[:(prefix_len + 63) // 64], dtype=torch.int32).to(dev)
+    args, more = (q, kv, ln.to(dev), table.to(dev)), dict(start=start.to(dev), prefix=prefix if prefix_len else None, prefix_len=prefix_len)
+    space = lambda: qm.attn_workspace(kv, T, len(lens), HK * G, prefix_len)  # noqa: E731
+    want = qm.attn_prefix(*args, **more, ws=space())
+    torch.cuda.synchronize()
+    streams, got, kept = [torch.cuda.Stream() for _ in range(2)], [], []
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(s):
+            kept.append(space())
+            got += [qm.attn_prefix(*args, **more, ws=kept[-1]) for _ in range(4)]
+    for s in streams:
+        s.synchronize()
+    assert all(torch.equal(g, want) for g in got)
+
+
 def test_many_rows_bad_pages(qm, dev):
     cache = K.Cache(10, 2, 16, 128, BF16, 9)
     table = torch.tensor([[1, -1, 3, 2 ** 31 - 1, 4, 5], [10, 4, -2 ** 31, 5, 6, 7]], dtype=torch.int32)
