@@ -2,6 +2,9 @@
 
 The library is the product: this module only passes device pointers and sizes through the C ABI. It raises
 QMatmulError for any non-zero status, and refuses to run when the library is not built (there is no fallback).
+
+Calls run on torch's current stream, or on `stream`, the raw handle of another one. Inputs have to be ready there; results of the paged cache's calls that
+the caller does not give are made there too, as under torch.cuda.stream.
 """
 import ctypes
 import os
@@ -402,6 +405,16 @@ def _check_rows(fn, name, t, dim, dev):
         _refuse(fn, f"{name} has {t.dim()} dimensions, not {dim}")
     if t.numel() and t.shape[-1] != 1:
         _refuse(fn, f"the last dimension of {name} is not contiguous")
+
+
+def _made(stream, dev, make, *args, **more):
+    """make(*args, **more): a result, or a workspace that the call keeps to itself. With the stream that the caller names as the current one: a fill then comes
+    before the kernel, the memory is none that the current stream still works on, and nobody else gets it before that stream is done with it."""
+    if stream is None or stream == _current_stream(dev):
+        return make(*args, **more)
+    cuda = _torch.cuda
+    with cuda.stream(cuda.ExternalStream(stream, device=dev) if stream else cuda.default_stream(dev)):
+        return make(*args, **more)
 
 
 _INT_MAX = 0x7fffffff
@@ -806,7 +819,7 @@ def kv_append(x, HQ, kv, slots, pos, inv_freq, wq=None, wk=None, eps=1e-6, adjac
     if out is None:
         out = q.dtype if q is not None else kv.dtype if kv.dtype != torch.float8_e4m3fn else torch.bfloat16
     if q is None:
-        q, ldq = x.new_empty((T, HQ, D), dtype=out), HQ * D
+        q, ldq = _made(stream, dev, x.new_empty, (T, HQ, D), dtype=out), HQ * D
     else:
         ldq = _head_rows(fn, "q", q, T, HQ, D, out, dev)
     how = (2 * half, adjacent, turns, scale, *sections)
@@ -874,7 +887,7 @@ def _attention(fn, q, kv, lens, table, start, scale, o, out, ws, stream, *more):
         out = q.dtype if o is None else o.dtype
     if o is None:
         # (rows of no sequence are not written: without a list of rows there are none)
-        o, ldo = (q.new_empty if start is None else q.new_zeros)((T, HQ, kv.D), dtype=out), HQ * kv.D
+        o, ldo = _made(stream, dev, q.new_empty if start is None else q.new_zeros, (T, HQ, kv.D), dtype=out), HQ * kv.D
     else:
         ldo = _head_rows(fn, "o", o, T, HQ, kv.D, out, dev)
     ws_ptr, ws_bytes = _workspace(fn, ws, dev)
@@ -935,13 +948,13 @@ def select_pages(q, kv, lens, table, k, start=None, first=1, last=1, sel=None, w
         _refuse(fn, "the cache has no means")
     _sizes(fn, k, first, last)
     if sel is None:
-        sel = lens.new_empty((T, kv.heads, k)) if start is None else lens.new_full((T, kv.heads, k), -1)
+        sel = _made(stream, dev, lens.new_empty, (T, kv.heads, k)) if start is None else _made(stream, dev, lens.new_full, (T, kv.heads, k), -1)
     else:
         _check_int32(fn, "sel", sel, 3, dev)
         if tuple(sel.shape) != (T, kv.heads, k):
             _refuse(fn, f"sel {tuple(sel.shape)}: [{T}, {kv.heads}, {k}]")
     if ws is None and table.size(1) > k:
-        ws = select_workspace(kv, T, table.size(1))
+        ws = _made(stream, dev, select_workspace, kv, T, table.size(1))
     ws_ptr, ws_bytes = _workspace(fn, ws, dev)
     st = _function(fn)(q.data_ptr(), _dtype(q.dtype), ldq, HQ, ctypes.byref(seqs), kv.ref, k, first, last, sel.data_ptr(), ws_ptr, ws_bytes,
                        _current_stream(dev) if stream is None else stream)

@@ -1,0 +1,73 @@
+"""Calls that name a stream: what they make for themselves and for the caller is made on it (allocations and fills), not on torch's current one. Without a GPU:
+tensors of the meta device, streams that are recorded."""
+import contextlib
+from types import SimpleNamespace
+
+import pytest
+import torch
+
+F32, F16, BF16, I32, E4M3 = torch.float32, torch.float16, torch.bfloat16, torch.int32, torch.float8_e4m3fn
+
+
+@pytest.fixture()
+def made(qm, monkeypatch):
+    """Which streams are current at the allocations of a call (0: torch's current one)."""
+    at, seen = [0], []
+    monkeypatch.setattr(qm, "_torch", torch)
+    monkeypatch.setattr(qm, "_current_gpu", lambda: -1)  # (what get_device() says of a meta tensor)
+    monkeypatch.setattr(qm, "_current_stream", lambda dev: at[-1])
+    monkeypatch.setattr(qm, "_function", lambda name: lambda *a: 512 if name.endswith("_size") else 0)
+    monkeypatch.setattr(qm, "_call", lambda name, *a: 0)
+
+    @contextlib.contextmanager
+    def current(s):
+        at.append(s)
+        yield
+        at.pop()
+    monkeypatch.setattr(torch.cuda, "stream", current)
+    monkeypatch.setattr(torch.cuda, "ExternalStream", lambda handle, device=None: handle)
+    monkeypatch.setattr(torch.cuda, "default_stream", lambda device=None: "default")
+    for name in ("new_empty", "new_zeros", "new_full"):
+        real = getattr(torch.Tensor, name)
+        monkeypatch.setattr(torch.Tensor, name, lambda t, *a, real=real, **k: seen.append(at[-1]) or real(t, *a, **k))
+    empty = torch.empty
+
+    def on_meta(*a, **k):
+        seen.append(at[-1])
+        return empty(*a, **{**k, "device": "meta"})
+    monkeypatch.setattr(torch, "empty", on_meta)
+
+    def run(call, *a, **k):
+        seen.clear()
+        call(*a, **k)
+        return set(seen)
+    return SimpleNamespace(run=run, current=current)
+
+
+def meta(*shape, dtype=BF16):
+    return torch.zeros(shape, dtype=dtype, device="meta")
+
+
+def cached(qm):
+    kv = qm.KvCache(meta(8, 2, 16, 64), meta(8, 2, 16, 64), mean=meta(8, 2, 64))
+    q, lens, table, start = meta(5, 4, 64), meta(3, dtype=I32), meta(3, 6, dtype=I32), meta(4, dtype=I32)
+    return [(qm.kv_append, (meta(5, 512), 4, kv, meta(5, dtype=I32), meta(5, dtype=I32), meta(32, dtype=F32)), {}),
+            (qm.attn_prefix, (q, kv, lens, table), dict(start=start)),
+            (qm.attn_prefix, (q[:3], kv, lens, table), {}),
+            (qm.attn_pages, (q, kv, lens, table, meta(5, 2, 4, dtype=I32)), dict(start=start)),
+            (qm.select_pages, (q, kv, lens, table, 4), dict(start=start)),
+            (qm.select_pages, (q[:3], kv, lens, table, 4), {})]
+
+
+def check(made, calls):
+    for f, args, more in calls:
+        assert made.run(f, *args, **more) == {0}, f
+        assert made.run(f, *args, **more, stream=7) == {7}, f
+        with made.current(7):
+            assert made.run(f, *args, **more) == {7}, f
+            assert made.run(f, *args, **more, stream=7) == {7}, f
+            assert made.run(f, *args, **more, stream=0) == {"default"}, f
+
+
+def test_the_paged_cache(qm, made):
+    check(made, cached(qm))
