@@ -3,10 +3,11 @@
 The library is the product: this module only passes device pointers and sizes through the C ABI. It raises
 QMatmulError for any non-zero status, and refuses to run when the library is not built (there is no fallback).
 
-Calls run on torch's current stream, or on `stream`, the raw handle of another one. Inputs have to be ready there; results of the paged cache's calls that
-the caller does not give are made there too, as under torch.cuda.stream.
+Calls run on torch's current stream, or on `stream`, the raw handle of another one. Inputs have to be ready there; results that the caller does not
+give are made there too, as under torch.cuda.stream.
 """
 import ctypes
+import functools
 import os
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
@@ -149,6 +150,19 @@ def _stream(stream):
     return ctypes.c_void_p(_current_stream(torch.cuda.current_device()))
 
 
+def _on(stream, dev, make):
+    """What makes a call's results, and a workspace that it keeps to itself, where the caller names a stream: `make` with that stream as the current one. A fill
+    then comes before the kernel, the memory is none that the current stream still works on, and nobody else gets it before that stream is done with it."""
+    if stream is None or stream == _current_stream(dev):
+        return make
+    import torch
+
+    def made(*args, **more):
+        with torch.cuda.stream(torch.cuda.ExternalStream(stream, device=dev) if stream else torch.cuda.default_stream(dev)):
+            return make(*args, **more)
+    return made
+
+
 class QWeight:
     """A prepared weight (qm_weight*) from GGUF bytes: a uint8 tensor (device or CPU) or a numpy array. K is the raw
     row length; Q8_0 / Q4_0 / IQ4_NL / Q2_0 rows of K % 256 != 0 are padded with zero blocks, and self.K is then the
@@ -196,7 +210,7 @@ def quantize_act(x, M_stride=None, stream=None, act32=True):
     act32=False: per-256 scales, asc [K/256, M_stride] (qmatmul_quantize_act_ex)."""
     M, K = x.shape
     Ms = M if M_stride is None else M_stride
-    aq, asc, absum = _out_acts(Ms, K, x.device, act32)
+    aq, asc, absum = _on(stream, x.device.index, _out_acts)(Ms, K, x.device, act32)
     if act32:
         _call("qmatmul_quantize_act", _ptr(x), x.stride(0), M, Ms, K, _ptr(aq), _ptr(asc), _ptr(absum), _stream(stream))
     else:
@@ -209,7 +223,7 @@ def gemv(w, aq, asc, absum, T=1, C=None, ldc=None, c_off=0, accumulate=0, stream
     import torch
     Ms = aq.shape[0]
     if C is None:
-        C = torch.empty((T, w.rows), dtype=torch.float32, device=aq.device)
+        C = _on(stream, aq.device.index, torch.empty)((T, w.rows), dtype=torch.float32, device=aq.device)
         ldc = w.rows
     _call("qmatmul_gemv", w.handle, _ptr(aq), _ptr(asc), _ptr(absum), Ms, T, _ptr(C),
           w.rows if ldc is None else ldc, c_off, accumulate, _stream(stream))
@@ -223,7 +237,7 @@ def gemm(w, aq, asc, absum, M=None, C=None, ldc=None, c_off=0, accumulate=0, str
     Ms = aq.shape[0]
     M = Ms if M is None else M
     if C is None:
-        C = torch.empty((M, w.rows), dtype=torch.float32, device=aq.device)
+        C = _on(stream, aq.device.index, torch.empty)((M, w.rows), dtype=torch.float32, device=aq.device)
         ldc = w.rows
     if not act32:
         if noalloc:
@@ -247,7 +261,7 @@ def gemm_ws(w, aq, asc, absum, ws, M=None, C=None, ldc=None, c_off=0, accumulate
     Ms = aq.shape[0]
     M = Ms if M is None else M
     if C is None:
-        C = torch.empty((M, w.rows), dtype=torch.float32, device=aq.device)
+        C = _on(stream, aq.device.index, torch.empty)((M, w.rows), dtype=torch.float32, device=aq.device)
         ldc = w.rows
     _call("qmatmul_gemm_ws", w.handle, _ptr(aq), _ptr(asc), _ptr(absum), M, Ms, int(act32), _ptr(C),
           w.rows if ldc is None else ldc, c_off, accumulate, _ptr(ws), 0 if ws is None else ws.numel(),
@@ -258,8 +272,9 @@ def gemm_ws(w, aq, asc, absum, ws, M=None, C=None, ldc=None, c_off=0, accumulate
 def gemv_blocksums(w, aq, absum, T=1, stream=None):
     import torch
     nb = w.K // 32
-    isum = torch.empty((T, w.rows, nb), dtype=torch.int32, device=aq.device)
-    msum = torch.empty((T, w.rows, nb), dtype=torch.int32, device=aq.device) if w.qtype in (12, 13, 10) else None
+    empty = _on(stream, aq.device.index, torch.empty)
+    isum = empty((T, w.rows, nb), dtype=torch.int32, device=aq.device)
+    msum = empty((T, w.rows, nb), dtype=torch.int32, device=aq.device) if w.qtype in (12, 13, 10) else None
     _call("qmatmul_gemv_blocksums", w.handle, _ptr(aq), _ptr(absum), aq.shape[0], T, _ptr(isum), _ptr(msum),
           _stream(stream))
     return isum, msum
@@ -268,7 +283,7 @@ def gemv_blocksums(w, aq, absum, T=1, stream=None):
 def gemm_blocksums(w, aq, M=None, stream=None):
     import torch
     M = aq.shape[0] if M is None else M
-    isum = torch.empty((M, w.rows, w.K // 32), dtype=torch.int32, device=aq.device)
+    isum = _on(stream, aq.device.index, torch.empty)((M, w.rows, w.K // 32), dtype=torch.int32, device=aq.device)
     _call("qmatmul_gemm_blocksums", w.handle, _ptr(aq), M, aq.shape[0], _ptr(isum), _stream(stream))
     return isum
 
@@ -277,9 +292,10 @@ def moe_route(logits, NU, NE=None, stream=None):
     import torch
     T, ldl = logits.shape
     NE = ldl if NE is None else NE
-    ids = torch.empty((T, NU), dtype=torch.int32, device=logits.device)
-    wts = torch.empty((T, NU), dtype=torch.float32, device=logits.device)
-    counts = torch.empty((NE,), dtype=torch.int32, device=logits.device)
+    empty = _on(stream, logits.device.index, torch.empty)
+    ids = empty((T, NU), dtype=torch.int32, device=logits.device)
+    wts = empty((T, NU), dtype=torch.float32, device=logits.device)
+    counts = empty((NE,), dtype=torch.int32, device=logits.device)
     _call("qmatmul_moe_route", _ptr(logits), ldl, T, NE, NU, _ptr(ids), _ptr(wts), _ptr(counts), _stream(stream))
     return ids, wts, counts
 
@@ -323,8 +339,8 @@ def rmsnorm_quant(x, w, eps, M_stride=None, want_h=False, stream=None, act32=Tru
     import torch
     M, K = x.shape
     Ms = M if M_stride is None else M_stride
-    aq, asc, absum = _out_acts(Ms, K, x.device, act32)
-    h = torch.empty((Ms, K), dtype=torch.float32, device=x.device) if want_h else None
+    aq, asc, absum = _on(stream, x.device.index, _out_acts)(Ms, K, x.device, act32)
+    h = _on(stream, x.device.index, torch.empty)((Ms, K), dtype=torch.float32, device=x.device) if want_h else None
     _call("qmatmul_rmsnorm_quant_ex", _ptr(x), x.stride(0), _ptr(w), K, M, Ms, float(eps), int(act32), _ptr(aq),
           _ptr(asc), _ptr(absum), _ptr(h), K, _stream(stream))
     return aq, asc, absum, h
@@ -333,7 +349,7 @@ def rmsnorm_quant(x, w, eps, M_stride=None, want_h=False, stream=None, act32=Tru
 def swiglu_quant(gu, F, fused=False, gelu=False, M_stride=None, stream=None, act32=True):
     M = gu.shape[0]
     Ms = M if M_stride is None else M_stride
-    aq, asc, absum = _out_acts(Ms, F, gu.device, act32)
+    aq, asc, absum = _on(stream, gu.device.index, _out_acts)(Ms, F, gu.device, act32)
     _call("qmatmul_swiglu_quant_ex", _ptr(gu), gu.stride(0), F, M, Ms, int(fused), int(gelu), int(act32), _ptr(aq),
           _ptr(asc), _ptr(absum), _stream(stream))
     return aq, asc, absum
@@ -343,7 +359,7 @@ def add_norm_quant(x, t, w, eps, s, w2=None, M_stride=None, stream=None, act32=T
     """Updates x in place; returns (aq, asc, absum)."""
     M, K = x.shape
     Ms = M if M_stride is None else M_stride
-    aq, asc, absum = _out_acts(Ms, K, x.device, act32)
+    aq, asc, absum = _on(stream, x.device.index, _out_acts)(Ms, K, x.device, act32)
     _call("qmatmul_add_norm_quant_ex", _ptr(x), _ptr(t), _ptr(w), K, float(eps), float(s), _ptr(w2), M, Ms,
           int(act32), _ptr(aq), _ptr(asc), _ptr(absum), _stream(stream))
     return aq, asc, absum
@@ -405,16 +421,6 @@ def _check_rows(fn, name, t, dim, dev):
         _refuse(fn, f"{name} has {t.dim()} dimensions, not {dim}")
     if t.numel() and t.shape[-1] != 1:
         _refuse(fn, f"the last dimension of {name} is not contiguous")
-
-
-def _made(stream, dev, make, *args, **more):
-    """make(*args, **more): a result, or a workspace that the call keeps to itself. With the stream that the caller names as the current one: a fill then comes
-    before the kernel, the memory is none that the current stream still works on, and nobody else gets it before that stream is done with it."""
-    if stream is None or stream == _current_stream(dev):
-        return make(*args, **more)
-    cuda = _torch.cuda
-    with cuda.stream(cuda.ExternalStream(stream, device=dev) if stream else cuda.default_stream(dev)):
-        return make(*args, **more)
 
 
 _INT_MAX = 0x7fffffff
@@ -480,7 +486,7 @@ class Fp8Weight:
             pass
 
 
-def _out_fp8(fn, x, M, K, M_stride):
+def _out_fp8(fn, x, M, K, M_stride, stream, dev):
     """(M_stride, ldx, a8, asc) of a producer's rows x; where M_stride is 0 there is nothing to call for."""
     Ms, ldx = M if M_stride is None else M_stride, x.stride(0) if M > 1 else _row_stride(x)
     if (M | Ms | K | ldx) >> 31 or Ms == 0:
@@ -489,7 +495,8 @@ def _out_fp8(fn, x, M, K, M_stride):
         if Ms < M or K < 1:
             _refuse(fn, f"M {M}, M_stride {Ms}, K {K}")
     Kp = (K + 127) // 128 * 128
-    return (Ms, ldx, x.new_empty((Ms, Kp), dtype=_torch.float8_e4m3fn), x.new_empty((Kp // 128, Ms), dtype=_torch.float32))
+    empty = x.new_empty if stream is None else _on(stream, dev, x.new_empty)  # (the test here: a call that names none pays nothing)
+    return Ms, ldx, empty((Ms, Kp), dtype=_torch.float8_e4m3fn), empty((Kp // 128, Ms), dtype=_torch.float32)
 
 
 def quantize_fp8(x, M_stride=None, stream=None):
@@ -499,7 +506,7 @@ def quantize_fp8(x, M_stride=None, stream=None):
     dev = _current_gpu()
     _check_rows(fn, "x", x, 2, dev)
     M, K = x.shape
-    Ms, ldx, a8, asc = _out_fp8(fn, x, M, K, M_stride)
+    Ms, ldx, a8, asc = _out_fp8(fn, x, M, K, M_stride, stream, dev)
     if Ms == 0:
         return a8, asc
     st = _function(fn)(x.data_ptr(), _dtype(x.dtype), ldx, M, Ms, K, a8.data_ptr(), asc.data_ptr(),
@@ -518,8 +525,8 @@ def rmsnorm_fp8(x, w, eps, M_stride=None, want_h=False, stream=None):
     M, K = x.shape
     if w.dtype != torch.float32 or w.numel() != K:
         _refuse(fn, f"w {tuple(w.shape)} {w.dtype}: float32, one for each of {K} columns")
-    Ms, ldx, a8, asc = _out_fp8(fn, x, M, K, M_stride)
-    h = x.new_empty((M, K), dtype=torch.float32) if want_h else None
+    Ms, ldx, a8, asc = _out_fp8(fn, x, M, K, M_stride, stream, dev)
+    h = _on(stream, dev, x.new_empty)((M, K), dtype=torch.float32) if want_h else None
     if Ms == 0:
         return a8, asc, h
     st = _function(fn)(x.data_ptr(), _dtype(x.dtype), ldx, w.data_ptr(), K, M, Ms, eps, a8.data_ptr(),
@@ -537,7 +544,7 @@ def swiglu_fp8(gu, F, gelu=False, M_stride=None, stream=None):
     M = gu.size(0)
     if gu.size(1) < 2 * F:
         _refuse(fn, f"rows of {gu.shape[1]} elements hold no gate and up of {F}")
-    Ms, ldg, a8, asc = _out_fp8(fn, gu, M, F, M_stride)
+    Ms, ldg, a8, asc = _out_fp8(fn, gu, M, F, M_stride, stream, dev)
     if Ms == 0:
         return a8, asc
     st = _function(fn)(gu.data_ptr(), _dtype(gu.dtype), ldg, F, M, Ms, 1 if gelu else 0, a8.data_ptr(),
@@ -579,7 +586,7 @@ def gemm_fp8(w, a8, asc, M=None, C=None, ldc=None, c_off=0, accumulate=0, out=No
     if C is None:
         if accumulate or c_off or ldc is not None:
             _refuse(fn, "accumulate, c_off and ldc need a C")
-        C = asc.new_empty((M, w.rows), dtype=out)
+        C = (asc.new_empty if stream is None else _on(stream, dev, asc.new_empty))((M, w.rows), dtype=out)
         ldc = w.rows
     else:
         _check_rows(fn, "C", C, 2, dev)
@@ -662,12 +669,13 @@ def qk_norm_rope(x, HQ, HK, D, pos, inv_freq, wq=None, wk=None, eps=1e-6, adjace
         _refuse(fn, f"rows of {width} elements do not hold the heads")
     if out is None:
         out = q.dtype if q is not None else k.dtype if k is not None else x.dtype
+    empty = x.new_empty if stream is None else _on(stream, dev, x.new_empty)
     if q is None:
-        q, ldq = x.new_empty((T, HQ, D), dtype=out), HQ * D
+        q, ldq = empty((T, HQ, D), dtype=out), HQ * D
     else:
         ldq = _head_rows(fn, "q", q, T, HQ, D, out, dev)
     if k is None:
-        k, ldk = x.new_empty((T, HK, D), dtype=out), HK * D
+        k, ldk = empty((T, HK, D), dtype=out), HK * D
     else:
         ldk = _head_rows(fn, "k", k, T, HK, D, out, dev)
     st = _function(fn)(x.data_ptr(), _dtype(x.dtype), ldx, T, D, q_off, q_hs, HQ, k_off, k_hs, HK,
@@ -819,7 +827,7 @@ def kv_append(x, HQ, kv, slots, pos, inv_freq, wq=None, wk=None, eps=1e-6, adjac
     if out is None:
         out = q.dtype if q is not None else kv.dtype if kv.dtype != torch.float8_e4m3fn else torch.bfloat16
     if q is None:
-        q, ldq = _made(stream, dev, x.new_empty, (T, HQ, D), dtype=out), HQ * D
+        q, ldq = (x.new_empty if stream is None else _on(stream, dev, x.new_empty))((T, HQ, D), dtype=out), HQ * D
     else:
         ldq = _head_rows(fn, "q", q, T, HQ, D, out, dev)
     how = (2 * half, adjacent, turns, scale, *sections)
@@ -887,7 +895,8 @@ def _attention(fn, q, kv, lens, table, start, scale, o, out, ws, stream, *more):
         out = q.dtype if o is None else o.dtype
     if o is None:
         # (rows of no sequence are not written: without a list of rows there are none)
-        o, ldo = _made(stream, dev, q.new_empty if start is None else q.new_zeros, (T, HQ, kv.D), dtype=out), HQ * kv.D
+        make = q.new_empty if start is None else q.new_zeros
+        o, ldo = (make if stream is None else _on(stream, dev, make))((T, HQ, kv.D), dtype=out), HQ * kv.D
     else:
         ldo = _head_rows(fn, "o", o, T, HQ, kv.D, out, dev)
     ws_ptr, ws_bytes = _workspace(fn, ws, dev)
@@ -948,13 +957,14 @@ def select_pages(q, kv, lens, table, k, start=None, first=1, last=1, sel=None, w
         _refuse(fn, "the cache has no means")
     _sizes(fn, k, first, last)
     if sel is None:
-        sel = _made(stream, dev, lens.new_empty, (T, kv.heads, k)) if start is None else _made(stream, dev, lens.new_full, (T, kv.heads, k), -1)
+        make = lens.new_empty if start is None else functools.partial(lens.new_full, fill_value=-1)
+        sel = (make if stream is None else _on(stream, dev, make))((T, kv.heads, k))
     else:
         _check_int32(fn, "sel", sel, 3, dev)
         if tuple(sel.shape) != (T, kv.heads, k):
             _refuse(fn, f"sel {tuple(sel.shape)}: [{T}, {kv.heads}, {k}]")
     if ws is None and table.size(1) > k:
-        ws = _made(stream, dev, select_workspace, kv, T, table.size(1))
+        ws = _on(stream, dev, select_workspace)(kv, T, table.size(1))
     ws_ptr, ws_bytes = _workspace(fn, ws, dev)
     st = _function(fn)(q.data_ptr(), _dtype(q.dtype), ldq, HQ, ctypes.byref(seqs), kv.ref, k, first, last, sel.data_ptr(), ws_ptr, ws_bytes,
                        _current_stream(dev) if stream is None else stream)

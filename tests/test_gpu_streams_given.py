@@ -74,3 +74,12 @@ def test_appending(qm, dev, keep_busy):
     x = torch.randn((5, 8 * 64), generator=torch.Generator().manual_seed(5)).to(BF16).to(dev)
     kv, i, f = qm.KvCache.new(2, 2, 16, 64, BF16), torch.arange(5, dtype=torch.int32, device=dev), inv_freq(64).to(dev)
     both(keep_busy, lambda s: [qm.kv_append(x, 4, kv, i, i, f, stream=s), kv.k, kv.v], (5, 4, 64), BF16)
+
+
+def test_producers_and_the_rotation(qm, dev, keep_busy):
+    x = torch.randn((64, 512), generator=torch.Generator().manual_seed(6)).to(dev)
+    pos, f = torch.arange(64, dtype=torch.int32, device=dev), inv_freq(64).to(dev)
+    raw = lambda ts: [t.view(torch.uint8) if t.dtype == torch.float8_e4m3fn else t for t in ts]  # noqa: E731
+    both(keep_busy, lambda s: raw(qm.quantize_fp8(x, stream=s)), (64, 512), torch.uint8)
+    both(keep_busy, lambda s: qm.quantize_act(x, stream=s), (64, 512), torch.int8)
+    both(keep_busy, lambda s: qm.qk_norm_rope(x, 4, 4, 64, pos, f, stream=s), (64, 4, 64), F32)

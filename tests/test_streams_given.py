@@ -18,6 +18,7 @@ def made(qm, monkeypatch):
     monkeypatch.setattr(qm, "_current_stream", lambda dev: at[-1])
     monkeypatch.setattr(qm, "_function", lambda name: lambda *a: 512 if name.endswith("_size") else 0)
     monkeypatch.setattr(qm, "_call", lambda name, *a: 0)
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: -1)
 
     @contextlib.contextmanager
     def current(s):
@@ -71,3 +72,15 @@ def check(made, calls):
 
 def test_the_paged_cache(qm, made):
     check(made, cached(qm))
+
+
+def test_the_other_calls(qm, made):
+    """Producers, products, routing, the rotation."""
+    weight = SimpleNamespace(handle=1, rows=256, qtype=12, K=256, Kp=256)
+    x, w, acts = meta(5, 256, dtype=F32), meta(256, dtype=F32), (meta(5, 256, dtype=torch.int8), meta(8, 5, dtype=F32), meta(16, 5, dtype=torch.int16))
+    check(made, [(qm.quantize_act, (x,), {}), (qm.quantize_act, (x,), dict(act32=False)), (qm.gemv, (weight, *acts), {}), (qm.gemm, (weight, *acts), {}),
+                 (qm.gemm_ws, (weight, *acts, None), {}), (qm.gemv_blocksums, (weight, acts[0], acts[2]), {}), (qm.gemm_blocksums, (weight, acts[0]), {}),
+                 (qm.moe_route, (meta(5, 8, dtype=F32), 2), {}), (qm.rmsnorm_quant, (x, w, 1e-6), dict(want_h=True)), (qm.swiglu_quant, (meta(5, 512, dtype=F32), 256), {}),
+                 (qm.add_norm_quant, (x, x, w, 1e-6, 1.0), {}), (qm.quantize_fp8, (x,), {}), (qm.rmsnorm_fp8, (x, w, 1e-6), dict(want_h=True)),
+                 (qm.swiglu_fp8, (meta(5, 512, dtype=F32), 256), {}), (qm.gemm_fp8, (weight, meta(5, 256, dtype=E4M3), meta(2, 5, dtype=F32)), dict(out=BF16)),
+                 (qm.qk_norm_rope, (meta(5, 512), 4, 2, 64, meta(5, dtype=I32), meta(32, dtype=F32)), {})])
