@@ -412,13 +412,13 @@ def _current_gpu():
 
 
 def _check_rows(fn, name, t, dim, dev):
-    """t is on GPU `dev`, of `dim` dimensions where dim is given, its last one contiguous."""
-    if t.get_device() == dev and (not dim or t.dim() == dim) and t.stride(-1) == 1:
+    """t is on GPU `dev`, of `dim` dimensions where dim is given (one at least where it is not), its last one contiguous."""
+    if t.get_device() == dev and (t.dim() == dim if dim else t.dim()) and t.stride(-1) == 1:
         return
     if t.get_device() != dev:
         _refuse(fn, f"{name} is on {t.device}, not on the current GPU")
-    if dim and t.dim() != dim:
-        _refuse(fn, f"{name} has {t.dim()} dimensions, not {dim}")
+    if t.dim() != dim if dim else not t.dim():
+        _refuse(fn, f"{name} has {t.dim()} dimensions, not {dim or 'one or more'}")
     if t.numel() and t.shape[-1] != 1:
         _refuse(fn, f"the last dimension of {name} is not contiguous")
 
@@ -786,9 +786,9 @@ def kv_append(x, HQ, kv, slots, pos, inv_freq, wq=None, wk=None, eps=1e-6, adjac
     if slots.get_device() != dev or slots.dtype != torch.int32 or slots.stride() != one:
         _check_int32(fn, "slots", slots, 1, dev)
     axes, half = 1, inv_freq.numel()
-    if len(sp) != 1:
+    if len(sp) > 1:
         axes = pos.size(0)
-    if pos.get_device() != dev or sp[-1] != 1:
+    if pos.get_device() != dev or sp[-1:] != one:
         _check_rows(fn, "pos", pos, None, dev)
     if inv_freq.get_device() != dev or inv_freq.stride() != one:
         _check_rows(fn, "inv_freq", inv_freq, 1, dev)
@@ -930,8 +930,8 @@ def attn_pages(q, kv, lens, table, sel, start=None, scale=None, o=None, out=None
     head, others than those of the table none (-1). ws: of attn_workspace(kv, T, T, HQ)."""
     fn = "qmatmul_attn_pages"
     _check_int32(fn, "sel", sel, 3, _current_gpu())
-    if tuple(sel.shape[:2]) != (q.size(0), kv.heads):
-        _refuse(fn, f"sel {tuple(sel.shape)}: pages for each of {q.size(0)} rows and {kv.heads} key heads")
+    if tuple(sel.shape[:2]) != (*q.shape[:1], kv.heads):
+        _refuse(fn, f"sel {tuple(sel.shape)}, q {tuple(q.shape)}: pages for each row and each of {kv.heads} key heads")
     _sizes(fn, sel.size(2))
     return _attention(fn, q, kv, lens, table, start, scale, o, out, ws, stream, sel.data_ptr(), sel.size(2))
 

@@ -102,3 +102,15 @@ def test_refused(qm, calls):
         with pytest.raises(qm.QMatmulError):
             bad()
     assert not calls
+
+
+def test_tensors_without_dimensions_are_refused(qm, calls):
+    none = lambda dtype=BF16: meta(dtype=dtype)  # noqa: E731
+    for bad in (lambda: append(qm, pos=none(I32)), lambda: append(qm, x=none()), lambda: append(qm, slots=none(I32)), lambda: append(qm, f=none(F32)),
+                lambda: append(qm, wq=none(F32)), lambda: append(qm, wk=none(F32)), lambda: append(qm, q=none()), lambda: attn(qm, q=none()), lambda: attn(qm, o=none()),
+                lambda: attn(qm, lens=none(I32)), lambda: attn(qm, table=none(I32)), lambda: attn(qm, start=none(I32)), lambda: attn(qm, ws=none(torch.uint8)),
+                lambda: attn(qm, prefix=none(I32), prefix_len=1), lambda: chosen(qm, sel=none(I32)), lambda: choice(qm, sel=none(I32)),
+                lambda: qm.attn_pages(none(), cache(qm), meta(3, dtype=I32), meta(3, 5, dtype=I32), meta(3, 2, 4, dtype=I32)), lambda: qm.KvCache(none(), none())):
+        with pytest.raises(qm.QMatmulError):
+            bad()
+    assert not calls
