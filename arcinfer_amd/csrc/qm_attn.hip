@@ -38,7 +38,9 @@ __global__ __launch_bounds__(THREADS) void attn_join_kernel(AttnArgs a, int RT, 
   if (n0 >= a.slots) return;
   const size_t size = slot_floats(RT, D);
   const float* first = a.part + (size_t)n0 * size;
-  const int4 head = *(const int4*)first;
+  int4 head = *(const int4*)first;
+  // (lists that are no batch leave slots unwritten: their words may be anything, and stay within the slots)
+  head = {min(max(head.x, 1), a.slots), max(head.y, 0), max(head.z, 0), 0};
   const long long srow = (long long)t * a.G + g;
   // the partial result of piece p: of its row, the maximum; the sum lies a tile's rows behind it, the elements from two on. (The prefix's pieces and the
   // first one are known without the slot's words.)

@@ -1,0 +1,37 @@
+"""Attention over a paged cache with lists of rows that are no batch, and a workspace that holds anything: some rows' pieces are nobody's, and the join takes no
+word of such a slot unseen. (Which rows those are is worked out in tests/test_attn_split.py.)"""
+import pytest
+import torch
+
+from tests import kv_plain as K
+
+pytestmark = pytest.mark.gpu
+
+BF16 = torch.bfloat16
+
+
+@pytest.mark.parametrize("words", ["ones", "least", "largest", "random"])
+@pytest.mark.parametrize("prefix_len", [0, 1000])
+def test_descending_lists(qm, dev, words, prefix_len):
+    """Nothing outside o is written, and o is what the call's rows may be: the call ends."""
+    T, HQ, HK, D = 90, 8, 2, 128
+    cache = K.Cache(40, HK, 16, D, BF16, 1)
+    kv = cache.on(qm, dev)
+    q = torch.randn((T, HQ, D), generator=torch.Generator().manual_seed(2)).to(BF16).to(dev)
+    prefix = (torch.arange(63, dtype=torch.int32) % 40).to(dev)
+    for start in ([0, 90] * 8, [90, 0, 90, 0, 0], [-5, 90, 20, 2 ** 31 - 1, -2 ** 31, 7], [89, 0, 90] * 30):
+        B = len(start) - 1
+        ln = torch.full((B,), 3000, dtype=torch.int32, device=dev)
+        table = (torch.arange(B * 190, dtype=torch.int32).view(B, 190) % 40).to(dev)
+        n = qm.attn_workspace(kv, T, B, HQ, prefix_len).numel()
+        g = torch.Generator().manual_seed(3)
+        fill = {"ones": torch.full((n // 4,), -1), "least": torch.full((n // 4,), -2 ** 31), "largest": torch.full((n // 4,), 2 ** 31 - 1),
+                "random": torch.randint(-2 ** 31, 2 ** 31, (n // 4,), generator=g)}[words]
+        buf = torch.zeros((n + 512,), dtype=torch.uint8, device=dev)
+        buf[:n] = fill.to(torch.int32).to(dev).view(torch.uint8)
+        buf[n:] = 77
+        o = torch.full((T + 2, HQ, D), 3.0, dtype=BF16, device=dev)
+        qm.attn_prefix(q, kv, ln, table, start=torch.tensor(start, dtype=torch.int32, device=dev), prefix=prefix if prefix_len else None, prefix_len=prefix_len,
+                       o=o[1:T + 1], ws=buf[:n])
+        torch.cuda.synchronize()
+        assert bool((o[0] == 3).all()) and bool((o[T + 1] == 3).all()) and bool((buf[n:] == 77).all())
