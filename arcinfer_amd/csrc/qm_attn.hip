@@ -99,7 +99,7 @@ __global__ __launch_bounds__(THREADS) void attn_join_kernel(AttnArgs a, int RT, 
       top = most;
     }
     const float f = w != 0.0f ? __builtin_amdgcn_exp2f(m - top) : 0.0f;
-    weight[tid] = f;
+    weight[tid] = w != 0.0f ? f : -1.0f;  // (a weight that vanishes counts: its result may not be finite)
     if (w != 0.0f) l = fmaf(f, w, l);
     __syncthreads();
     if (group < groups) {
@@ -114,7 +114,7 @@ __global__ __launch_bounds__(THREADS) void attn_join_kernel(AttnArgs a, int RT, 
           const int p = group + (from + i) * groups;
           if (p >= n) continue;
           const float k = weight[p];
-          if (k == 0.0f) continue;  // (the slot may hold anything)
+          if (k < 0.0f) continue;  // (nothing seen: the slot may hold anything)
           o.x = fmaf(k, v[i].x, o.x);
           o.y = fmaf(k, v[i].y, o.y);
           o.z = fmaf(k, v[i].z, o.z);

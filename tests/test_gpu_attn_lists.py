@@ -35,3 +35,28 @@ def test_descending_lists(qm, dev, words, prefix_len):
                        o=o[1:T + 1], ws=buf[:n])
         torch.cuda.synchronize()
         assert bool((o[0] == 3).all()) and bool((o[T + 1] == 3).all()) and bool((buf[n:] == 77).all())
+
+
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), float("-inf")])
+@pytest.mark.parametrize("prefix_len,rows", [(0, 1), (0, 3), (2000, 1)])
+def test_values_of_vanishing_weight(qm, dev, bad, prefix_len, rows):
+    """A value that is not finite, of a key that rows see with a weight of e^-400: 0 times it in 32 bits, in the limit it itself, never a finite result. In
+    pieces as whole."""
+    D, B = 128, 40 if prefix_len else 1
+    own = 3000 if not prefix_len else 20
+    cache = K.Cache((own + 15) // 16 * B + (prefix_len + 15) // 16, 1, 16, D, BF16, 1)
+    start, ln, table, rest = K.batch([own] * B, [rows] * B, 16, cache.pages, 1, spare=0)
+    q = torch.zeros((rows * B, 2, D))
+    q[..., 0] = 8.0
+    cache.data[0][..., 0] = 0.0
+    pages = rest if prefix_len else table[0].tolist()
+    for p in pages[:20]:  # (the first keys: far below the others)
+        cache.data[0][p, :, :, 0] = -50.0
+    cache.data[1][pages[3], 0, 5, 7] = bad
+    kv, qd = cache.on(qm, dev), q.to(BF16).to(dev)
+    prefix = torch.tensor(rest, dtype=torch.int32).to(dev) if prefix_len else None
+    more = dict(start=start.to(dev), prefix=prefix, prefix_len=prefix_len, scale=1.0)
+    for ws in (None, qm.attn_workspace(kv, rows * B, B, 2, prefix_len)):
+        o = qm.attn_prefix(qd, kv, ln.to(dev), table.to(dev), ws=ws, **more).float()
+        odd = ~torch.isfinite(o)
+        assert bool(odd[..., 7].all()) and not odd[..., :7].any() and not odd[..., 8:].any()
