@@ -6,6 +6,7 @@
 #include <string.h>
 
 #include <atomic>
+#include <cmath>
 #include <mutex>
 
 #include "../../include/qmatmul.h"
@@ -1270,6 +1271,8 @@ static int attention(const char* fn, const void* q, int qtype, int ldq, int HQ, 
   if (kv->type != QM_E4M3 && kv->type != qtype) return fail(QM_ERR_TYPE, "%s: q of type %d, the cache of %d", fn, qtype, kv->type);
   if (otype != qtype && otype != QM_F32) return fail(QM_ERR_TYPE, "%s: output type %d (q's or QM_F32)", fn, otype);
   if (ldo < (long long)HQ * kv->D || prefix_len < 0 || prefix_len > 1 << 30) return fail(QM_ERR_SHAPE, "%s: ldo %d, prefix_len %d", fn, ldo, prefix_len);
+  a.c = scale * 1.44269504088896341f;
+  if (!std::isfinite(a.c)) return fail(QM_ERR_ARG, "%s: scale %g", fn, scale);
   if (none) return QM_OK;
   if (!o || (prefix_len && !prefix)) return fail(QM_ERR_ARG, "%s: null pointer", fn);
   const size_t so = dtype_size(otype);
@@ -1301,7 +1304,6 @@ static int attention(const char* fn, const void* q, int qtype, int ldq, int HQ, 
   a.prefix_len = prefix_len;
   a.sel = sel;
   a.k = k;
-  a.c = scale * 1.44269504088896341f;
   a.o = o;
   a.otype = otype;
   a.ldo = ldo;

@@ -389,7 +389,7 @@ int qmatmul_kv_append(const void* x, int xtype, int ldx, int T, int q_off, int q
  * which row i of n sees the first len - n + i + 1. A row that sees no key is zeros. What lies in masked places (behind a sequence, in
  * pages that are none, in later tokens) has no effect, whatever it holds.
  * q: qtype QM_F16 or QM_BF16, that of the cache unless it is QM_E4M3; head h of row t at t * ldq + h * D; HQ a multiple of
- * kv->heads. o: otype qtype or QM_F32, row stride ldo. Products are exact, sums f32; weights are rounded to 16 bits for the second product
+ * kv->heads. scale: finite, and scale * log2 e too. o: otype qtype or QM_F32, row stride ldo. Products are exact, sums f32; weights are rounded to 16 bits for the second product
  * where o is of a type with no more of them (bf16; f16 behind an f16 cache), and held in two or three parts of 16 bits elsewhere.
  * ws: device workspace, 256-byte aligned, of qmatmul_attn_workspace_size bytes (which grows with neither lengths nor the cache); NULL or a
  * smaller one: the prefix is read by each sequence for itself, and sequences are cut into fewer pieces or none, slower. Calls that may
