@@ -1280,7 +1280,7 @@ static int attention(const char* fn, const void* q, int qtype, int ldq, int HQ, 
   if (ws && !aligned(ws, 256)) return fail(QM_ERR_ARG, "%s: the workspace must be 256-byte aligned", fn);
   const int T = seqs->T, B = sel ? T : seqs->B;
   const bool start = !sel && seqs->start;
-  const qm::AttnPlan p = qm::attn_plan(T, B, start, sel != nullptr, kv->type == QM_E4M3, HQ, kv->heads, kv->D, prefix_len, ws ? ws_bytes : 0);
+  const qm::AttnPlan p = qm::attn_plan(T, B, start, sel || a.c == 0.0f, kv->type == QM_E4M3, HQ, kv->heads, kv->D, prefix_len, ws ? ws_bytes : 0);
   if (!qm::attn_grid(p, T, B, start, HQ, kv->heads)) return fail(QM_ERR_SHAPE, "%s: %d rows of %d heads are more than a grid holds", fn, T, HQ);
   const size_t used = qm::attn_used_bytes(p, kv->heads, kv->D);
   const HeadRows rq{q, T, kv->D, HQ, kv->D, ldq, 2}, ro{o, T, kv->D, HQ, kv->D, ldo, (long long)so};

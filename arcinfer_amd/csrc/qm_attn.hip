@@ -231,17 +231,17 @@ static unsigned shared_grid(const AttnPlan& p, int HK) { return (unsigned)(div_u
 
 size_t attn_used_bytes(const AttnPlan& p, int HK, int D) { return shared_bytes(p, HK, D) + p.slots * slot_bytes(p.rt, D); }
 
-AttnPlan attn_plan(int T, int B, bool start, bool chosen, bool e8, int HQ, int HK, int D, int prefix_len, size_t ws_bytes) {
+AttnPlan attn_plan(int T, int B, bool start, bool few, bool e8, int HQ, int HK, int D, int prefix_len, size_t ws_bytes) {
   const int G = HQ / HK;
   const long long rows = start ? div_up(T, B < T ? B : T) * G : G;  // of a sequence, on average
   const size_t have = ws_bytes / 256 * 256;
   AttnPlan p{};
-  p.tile = !chosen && rows >= tile_from(D, e8);  // (chosen pages are a row's own: never many rows)
+  p.tile = !few && rows >= tile_from(D, e8);
   p.rt = p.tile ? many_rows(rows, D, e8) : few_rows(rows, D);
   const AttnPlan alone = p;
   if ((double)(B - 1) * prefix_len * HK * D * (e8 ? 2 : 4) >= kSharedBytes && T > 1 && rows < kSharedRows) {
     const long long all = (long long)T * G;
-    p.shared_tile = all >= kSharedRows && (double)T * HQ * prefix_len * D >= (e8 ? kSharedFrom8 : kSharedFrom16);
+    p.shared_tile = !few && all >= kSharedRows && (double)T * HQ * prefix_len * D >= (e8 ? kSharedFrom8 : kSharedFrom16);
     p.shared_rt = p.shared_tile ? many_rows(all, D, e8) : few_rows(all, D);
     // (one launch for both: the batch's rows fill the tile, and a sequence's own keys take no longer for it)
     if (!p.shared_tile) {

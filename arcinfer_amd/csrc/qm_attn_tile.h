@@ -102,9 +102,9 @@ __global__ __launch_bounds__(256, 2) void attn_tile_kernel(AttnArgs a) {
   if (!shared && c > 0 && begin >= all_blocks) return;  // (a piece that this tile's rows do not see)
 
   // q as attn_kernel holds it
-  // (a scale below zero is its negative's with -q, one of zero any other's with zeros: maxima are those of the products then)
-  const float scale = a.c == 0.0f ? 1.0f : __builtin_fabsf(a.c);
-  const int q_and = a.c == 0.0f ? 0 : -1, q_xor = a.c < 0.0f ? 0x80008000 : 0;
+  // (a scale below zero is its negative's with -q: the maximum is that of the products then. None of zero comes here: masked logits would be NaN.)
+  const float scale = __builtin_fabsf(a.c);
+  const int q_xor = a.c < 0.0f ? 0x80008000 : 0;
   v4i q[MT][KS];
   const bool qvec = ((uintptr_t)a.q & 15) == 0 && (a.ldq & 7) == 0;
 #pragma unroll
@@ -123,7 +123,7 @@ __global__ __launch_bounds__(256, 2) void attn_tile_kernel(AttnArgs a) {
         for (int i = 0; i < 8; ++i) e[i] = p[at + i];
         q[m][t] = __builtin_bit_cast(v4i, e);
       }
-      q[m][t] = (q[m][t] & q_and) ^ q_xor;
+      q[m][t] ^= q_xor;
       if (!FULL && d >= kv.D) q[m][t] = v4i(0);
     }
   }

@@ -62,7 +62,8 @@ struct AttnPlan {
   int tail;                                                         // or (not 0) the last row tiles alone
   int shared, shared_rt, shared_tile, shared_tiles, shared_blocks;  // shared 0: the prefix is read with each sequence's own keys
 };
-AttnPlan attn_plan(int T, int B, bool start, bool chosen, bool e8, int HQ, int HK, int D, int prefix_len, size_t ws_bytes);
+// few: attn_kernel alone. Chosen pages are a row's own, never many rows; and a scale of zero, which attn_tile_kernel cannot have in front of its masks.
+AttnPlan attn_plan(int T, int B, bool start, bool few, bool e8, int HQ, int HK, int D, int prefix_len, size_t ws_bytes);
 size_t attn_used_bytes(const AttnPlan& p, int HK, int D);
 size_t attn_workspace_bytes(int T, int B, bool e8, int HQ, int HK, int D, int prefix_len);
 // Work-groups of the calls's launches at most (0: more than a grid holds)

@@ -60,3 +60,27 @@ def test_values_of_vanishing_weight(qm, dev, bad, prefix_len, rows):
         o = qm.attn_prefix(qd, kv, ln.to(dev), table.to(dev), ws=ws, **more).float()
         odd = ~torch.isfinite(o)
         assert bool(odd[..., 7].all()) and not odd[..., :7].any() and not odd[..., 8:].any()
+
+
+@pytest.mark.parametrize("qt,ct", [(BF16, BF16), (torch.float16, torch.float16), (BF16, torch.float8_e4m3fn)])
+@pytest.mark.parametrize("D", [64, 256])
+def test_scale_of_zero(qm, dev, D, qt, ct):
+    """Weights are equal whatever q holds; a q that is not finite makes its row NaN, as 0 times it. Rows of any number, and a prefix that a large batch shares."""
+    for rows, B, prefix_len in ((3, 1, 0), (100, 2, 50), (1, 140, 2100 if D == 256 else 8000)):
+        cache = K.Cache((120 + 15) // 16 * B + (prefix_len + 15) // 16, 2, 16, D, ct, 1)
+        start, ln, table, rest = K.batch([120] * B, [rows] * B, 16, cache.pages, 1)
+        q = torch.randn((rows * B, 8, D), generator=torch.Generator().manual_seed(2)).to(qt)
+        odd = torch.zeros((rows * B, 8), dtype=torch.bool)
+        for t, h, d, v in ((0, 1, 5, float("inf")), (rows * B - 1, 7, D - 1, float("-inf")), (rows * B // 2, 4, 0, float("nan"))):
+            q[t, h, d] = v
+            odd[t, h] = True
+        some = sorted({0, rows * B // 2, rows * B - 1, rows * B // 3})
+        of = [t // rows for t in some]
+        prefix = torch.tensor(rest[:(prefix_len + 15) // 16], dtype=torch.int32)
+        clean = torch.where(odd[..., None], torch.zeros_like(q), q)
+        want, bound = K.attention(clean[some], cache, torch.arange(len(some) + 1), torch.tensor([120 - rows + 1 + t % rows for t in some]), table[of], qt, 0.0, prefix, prefix_len)
+        kv = cache.on(qm, dev)
+        for ws in (None, qm.attn_workspace(kv, rows * B, B, 8, prefix_len)):
+            o = qm.attn_prefix(q.to(dev), kv, ln.to(dev), table.to(dev), start=start.to(dev), prefix=prefix.to(dev) if prefix_len else None, prefix_len=prefix_len, scale=0.0, ws=ws)
+            assert torch.equal(torch.isnan(o).all(2).cpu(), odd) and torch.equal(torch.isnan(o).any(2).cpu(), odd)
+            K.check(torch.where(odd[some][..., None].to(dev), want.to(qt).to(dev), o[some]), want, bound, qt)
