@@ -259,7 +259,8 @@ AttnPlan attn_plan(int T, int B, bool start, bool few, bool e8, int HQ, int HK, 
   }
   const long long items = row_tiles(T, B, start, G, p.rt) * HK;
   const long long left = ((long long)have - (long long)shared_bytes(p, HK, D)) / (long long)slot_bytes(p.rt, D) - items;
-  // (pieces of all row tiles are at most the target and one more for each of them; row tiles that fill the chip are left whole)
+  // (pieces of all row tiles are at most the target and one more for each of them; more row tiles than fill the chip are left whole. Lengths are not looked at for that, and are not known
+  // here: 43 sequences of 500 to 20000 tokens, five rows each, 24 heads of 256 over 4, take 228 us, 44 of them 443.)
   if (left > 0 && items < (p.tile ? kTarget / 2 : 2 * kTarget)) {
     // (beside a prefix's work-groups half as many: 32 sequences of 300 tokens behind 4096 24 us against 31, 4 of 4000 behind 16384 31 against 36; 48 of 16 to 1500
     // behind 8192 47 against 46)
@@ -345,7 +346,7 @@ hipError_t launch_attn(const AttnArgs& args, const AttnPlan& p, hipStream_t s) {
     return hipGetLastError();
   }
   // A wave a row where there are rows enough: work-groups of four waves, most of which have nothing to do, take longer to start than that (1536 rows:
-  // the call 57 us against 60). Sixteen waves where there are few rows, and so many pieces of each (24 rows of 128 pieces of D 256: 17.3 us
+  // the call 57 us against 60). Sixteen waves where there are few rows, and so many pieces of each (24 rows of 40 pieces of D 256: 17.3 us
   // against 17.9; 512 rows of 32: 67 against 59).
   const long long rows = (long long)a.s.T * a.HQ;
   if (rows >= 1024) attn_join_kernel<64><<<(unsigned)rows, 64, 0, s>>>(a, p.rt, a.sel ? 1 : 0);

@@ -10,8 +10,9 @@
 //
 // The logits stay unscaled: e^(scale (s - m)) is one fma and one v_exp, the maximum is that of s (for a scale below zero -q is taken). What bounds it: the
 // matrix pipe (64 keys of 128 by a wave's 32 rows: 1024 cycles, 46 % of the time at the full clock) with the vector instructions (160, and 32 exponentials of
-// four times an instruction's time) beside it. Measured, 32 heads of 128 over 8, bf16: the last 4096 of 16384 tokens 838 us (1150 Tflop/s of what they
-// see), 4096 of 4096 141 us; f32 results, three parts of each weight, 1405 us; a large library product reaches 1250.
+// four times an instruction's time) beside it. Measured, 32 heads of 128 over 8, bf16, at best and on average over a long run, whose clock is lower: the last 4096 of
+// 16384 tokens 838 and 907 us (1150 and 1060 Tflop/s of what they see), 4096 of 4096 141 and 161; f32 results, three parts of each weight, 1405 and 1508; a large
+// library product reaches 1250.
 // Tried and not kept: the next scores' products between this block's exponentials (as fast with three parts, 5 % slower with one), values through
 // registers for 16-bit caches too (1016 us).
 #pragma once
