@@ -153,7 +153,10 @@ def _stream(stream):
 def _on(stream, dev, make):
     """What makes a call's results, and a workspace that it keeps to itself, where the caller names a stream: `make` with that stream as the current one. A fill
     then comes before the kernel, the memory is none that the current stream still works on, and nobody else gets it before that stream is done with it."""
-    if stream is None or stream == _current_stream(dev):
+    if stream is None:
+        return make
+    stream = getattr(stream, "value", stream) or 0  # (of a ctypes pointer)
+    if stream == _current_stream(dev):
         return make
     import torch
 

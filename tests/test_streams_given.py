@@ -1,6 +1,7 @@
 """Calls that name a stream: what they make for themselves and for the caller is made on it (allocations and fills), not on torch's current one. Without a GPU:
 tensors of the meta device, streams that are recorded."""
 import contextlib
+import ctypes
 from types import SimpleNamespace
 
 import pytest
@@ -84,3 +85,10 @@ def test_the_other_calls(qm, made):
                  (qm.add_norm_quant, (x, x, w, 1e-6, 1.0), {}), (qm.quantize_fp8, (x,), {}), (qm.rmsnorm_fp8, (x, w, 1e-6), dict(want_h=True)),
                  (qm.swiglu_fp8, (meta(5, 512, dtype=F32), 256), {}), (qm.gemm_fp8, (weight, meta(5, 256, dtype=E4M3), meta(2, 5, dtype=F32)), dict(out=BF16)),
                  (qm.qk_norm_rope, (meta(5, 512), 4, 2, 64, meta(5, dtype=I32), meta(32, dtype=F32)), {})])
+
+
+def test_a_pointer_serves_as_a_number(qm, made):
+    for f, args, more in cached(qm) + [(qm.quantize_fp8, (meta(5, 256, dtype=F32),), {})]:
+        assert made.run(f, *args, **more, stream=ctypes.c_void_p(7)) == {7}, f
+        with made.current(7):
+            assert made.run(f, *args, **more, stream=ctypes.c_void_p(None)) == {"default"}, f
