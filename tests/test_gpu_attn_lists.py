@@ -84,3 +84,21 @@ def test_scale_of_zero(qm, dev, D, qt, ct):
             o = qm.attn_prefix(q.to(dev), kv, ln.to(dev), table.to(dev), start=start.to(dev), prefix=prefix.to(dev) if prefix_len else None, prefix_len=prefix_len, scale=0.0, ws=ws)
             assert torch.equal(torch.isnan(o).all(2).cpu(), odd) and torch.equal(torch.isnan(o).any(2).cpu(), odd)
             K.check(torch.where(odd[some][..., None].to(dev), want.to(qt).to(dev), o[some]), want, bound, qt)
+
+
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+def test_values_of_vanishing_weight_in_a_last_round(qm, dev, bad):
+    """The same by large tiles that are cut behind the last whole round of work-groups: rows that see the key have no finite result, the others have theirs."""
+    D, HK, T, at = 128, 64, 1100, 53
+    cache = K.Cache((T + 15) // 16, HK, 16, D, BF16, 1)
+    start, ln, table, _ = K.batch([T], [T], 16, cache.pages, 1, spare=0)
+    q = torch.zeros((T, HK, D))
+    q[..., 0] = 8.0
+    cache.data[0][..., 0] = 0.0
+    for p in table[0, :20].tolist():
+        cache.data[0][p, :, :, 0] = -50.0
+    cache.data[1][int(table[0, at // 16]), :, at % 16, 7] = bad
+    kv, qd = cache.on(qm, dev), q.to(BF16).to(dev)
+    for ws in (None, qm.attn_workspace(kv, T, 1, HK)):
+        odd = ~torch.isfinite(qm.attn_prefix(qd, kv, ln.to(dev), table.to(dev), start=start.to(dev), scale=1.0, ws=ws).float())
+        assert bool(odd[at:, :, 7].all()) and not odd[:at].any() and not odd[..., :7].any() and not odd[..., 8:].any()
