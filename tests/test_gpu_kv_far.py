@@ -65,3 +65,42 @@ def test_far_means(qm, dev):
     cache.ref = ctypes.byref(kv)
     got = qm.select_pages(q, cache, ln, torch.tensor([far], dtype=torch.int32, device=dev), 7)
     assert torch.equal(got, want)
+
+
+def test_far_rows(qm, dev):
+    """Rows of q, of the result and of the QKV product more than 2^31 elements behind the first one."""
+    T, HQ, HK, D, far = 4, 8, 2, 64, 2 ** 30
+    i32 = lambda t: torch.tensor(t, dtype=torch.int32, device=dev)  # noqa: E731
+    buf = torch.empty(((T - 1) * far + (HQ + 2 * HK) * D,), dtype=BF16, device=dev)
+    x = torch.randn((T, (HQ + 2 * HK) * D), generator=torch.Generator().manual_seed(1)).to(BF16).to(dev)
+    rows = buf.as_strided(x.shape, (far, 1))
+    rows.copy_(x)
+    near, kv = (qm.KvCache.new(2, HK, 16, D, BF16) for _ in range(2))
+    pos, f = i32([3, 4, 5, 6]), torch.rand(D // 2, generator=torch.Generator().manual_seed(2)).to(dev)
+    q = qm.kv_append(x, HQ, near, pos, pos, f)
+    got = qm.kv_append(rows, HQ, kv, pos, pos, f, q=rows[:, :HQ * D])  # (in place)
+    assert torch.equal(got, q.view(T, HQ * D)) and torch.equal(kv.k, near.k) and torch.equal(kv.v, near.v)
+    q4 = buf.as_strided((T, HQ, D), (far, D, 1))
+    out = torch.empty(((T - 1) * far + HQ * D,), dtype=BF16, device=dev)
+    o = out.as_strided((T, HQ, D), (far, D, 1))
+    for start, ln, table in ((None, i32([4, 5, 6, 7]), i32([[0]] * 4)), (i32([0, 4]), i32([7]), i32([[0]]))):
+        want = qm.attn_prefix(q, kv, ln, table, start=start)
+        qm.attn_prefix(q4, kv, ln, table, start=start, o=o)
+        assert torch.equal(o, want)
+        out.zero_()
+        qm.attn_pages(q4, kv, ln, table, i32([0]).expand(T, HK, 1).contiguous(), start=start, o=o)
+        assert torch.equal(o, qm.attn_pages(q, kv, ln, table, i32([0]).expand(T, HK, 1).contiguous(), start=start))
+
+
+def test_far_rows_of_large_tiles(qm, dev):
+    """The same for a prompt: 70 rows, the last of them more than 2^31 elements behind the first."""
+    T, HQ, HK, D, far = 70, 2, 1, 128, 2 ** 25
+    cache = K.Cache(8, HK, 16, D, BF16, 5)
+    kv, ln, table = cache.on(qm, dev), torch.tensor([100], dtype=torch.int32, device=dev), torch.arange(8, dtype=torch.int32, device=dev)[None]
+    start = torch.tensor([0, T], dtype=torch.int32, device=dev)
+    q = torch.randn((T, HQ, D), generator=torch.Generator().manual_seed(6)).to(BF16).to(dev)
+    bufs = [torch.empty(((T - 1) * far + HQ * D,), dtype=BF16, device=dev) for _ in range(2)]
+    rows, o = (b.as_strided((T, HQ, D), (far, D, 1)) for b in bufs)
+    rows.copy_(q)
+    qm.attn_prefix(rows, kv, ln, table, start=start, o=o)
+    assert torch.equal(o, qm.attn_prefix(q, kv, ln, table, start=start))
